@@ -23,6 +23,9 @@ SOURCES = {
     "kda_prefill_sp.cu": [],  # tensor-core prefill: agrees with the chain to rounding, so default FP flags
     "proj_gemm.cu": [],      # the projections: tcgen05 GEMM
     "proj_gemm_pair.cu": [], # the same on SM pairs (cta_group::2) for many rows
+    "lin_decode.cu": [],     # linear attention with one decay a head: row by row
+    "lin_prefill.cu": [],    # ... and chunked
+    "spec_accept.cu": [],    # verification of drafted tokens
     "kda_gather.cu": [],     # host code only: CUDA IPC handles for the full output buffers of a head-sharded prefill
     "fwd_rows.cu": [],       # row gather / scatter and the mark copy: data movement only
 }

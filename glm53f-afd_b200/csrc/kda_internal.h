@@ -135,6 +135,15 @@ int core_prefill_static_launch(int32_t heads, int32_t batch, const int32_t* cu_s
                                void* state_out, const int64_t* state_off, bool bf16_state, const glm53f_bf16* gate,
                                const glm53f_bf16* norm_w, float eps, glm53f_bf16* out, cudaStream_t stream);
 
+// Linear attention with one decay a head (lin_decode.cu): whether the common arguments are acceptable, and the row-by-row kernel.
+bool lin_args_ok(int32_t heads, int32_t qk_heads, int32_t batch, const void* cu, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                 const void* v, int64_t v_stride, const void* g, int64_t g_stride, const void* state_in, const void* state_off, const void* out,
+                 int64_t out_stride);
+int lin_rows_launch(int32_t heads, int32_t qk_heads, int32_t batch, const int32_t* cu, const int32_t* keep, const uint16_t* q, int64_t q_stride,
+                    const uint16_t* k, int64_t k_stride, const uint16_t* v, int64_t v_stride, const float* g, int64_t g_stride, const void* state_in,
+                    void* state_out, const int64_t* state_off, bool bf16_state, bool round_rows, float scale, uint16_t* out, int64_t out_stride,
+                    cudaStream_t stream);
+
 int sm_count();
 
 // Device address of the status word kernels record a timed-out wait in (current device).

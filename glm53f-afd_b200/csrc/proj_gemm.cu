@@ -84,6 +84,7 @@ struct GemmProblem {
 struct GemmParams {
     GemmProblem problem[2];    // the second: none, or (without clusters) another GEMM's tiles behind the first's
     long long tiles0, tiles;
+    ProjEpilogue epi;  // an instance with an epilogue: its one problem's
     int overlap;  // 0: alone; 1: the first of two independent launches; 2: the second (see glm53f_kda_proj_bf16_many)
     int* status;
 };
@@ -135,11 +136,13 @@ __device__ __forceinline__ GemmTile gemm_tile(const GemmParams& p, long long t) 
 }
 
 // KS = blocks per cluster = K splits of a tile (1: no cluster).  TWO: two problems, KS = 1 (an instance to itself: reading the parameters by a tile's problem
-// and the sums of a split k cost a launch of one 1 to 3 us).
-template <int NR, int KS, bool TWO>
+// and the sums of a split k cost a launch of one 1 to 3 us).  EPI: bias, activation and residual before the results leave; the residual's values
+// are on their way before the accumulator is waited for, sixteen rows ahead.
+template <int NR, int KS, bool TWO, bool EPI>
 __global__ void __launch_bounds__(kGemmThreads, kBlocksPerSm) proj_gemm_kernel(const __grid_constant__ GemmParams p) {
     constexpr bool SPLIT = KS > 1;
     static_assert(!SPLIT || !TWO, "");
+    static_assert(!EPI || !TWO, "");
     using C = Cfg<NR, SPLIT, TWO>;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -253,15 +256,35 @@ __global__ void __launch_bounds__(kGemmThreads, kBlocksPerSm) proj_gemm_kernel(c
         for (long long t = tile0; t < p.tiles; t += tile_step) {
             const GemmTile tile = gemm_tile<TWO>(p, t);
             const GemmProblem& x = tile.q;
-            if (!mbar_wait(&acc_full[buf], acc_ph[buf], ctx, kStatusGemmAccFull)) goto done;
-            acc_ph[buf] ^= 1u;
-            tc::fence_after_sync();
             const int fl = q * 32 + lane, f = tile.nt * kBM + fl;
             const bool f_ok = f < x.n;
             const long long row0 = (long long)tile.rt * NR;
             const long long ldo = x.ldo;
             const int rows = x.rows, out_f32 = x.out_f32;
             unsigned char* base = reinterpret_cast<unsigned char*>(x.out) + ((long long)tile.g * x.o_gstride + f) * (out_f32 ? 4 : 2);
+            // EPI: the bias of this thread's feature, and the residual's values of sixteen rows (of KS > 1: of the rows this block finishes).
+            constexpr int CW = NR / KS, kRes = SPLIT ? CW : 16;
+            float bias = 0.0f, res[EPI ? kRes : 1];
+            auto load_residual = [&](int c0) {
+                if constexpr (EPI) {
+                    const unsigned char* at = static_cast<const unsigned char*>(p.epi.residual) + ((long long)tile.g * p.epi.r_gstride + f) * (out_f32 ? 4 : 2);
+#pragma unroll
+                    for (int j = 0; j < kRes; ++j) {
+                        const long long row = row0 + c0 + j;
+                        res[j] = 0.0f;
+                        if (p.epi.residual != nullptr && f_ok && row < rows)
+                            res[j] = out_f32 ? *reinterpret_cast<const float*>(at + row * p.epi.ldr * 4)
+                                             : bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(at + row * p.epi.ldr * 2));
+                    }
+                }
+            };
+            if constexpr (EPI) {
+                if (p.epi.bias != nullptr && f_ok) bias = proj_bias(p.epi, tile.g, f);
+                load_residual(SPLIT ? (int)kr * CW : 0);
+            }
+            if (!mbar_wait(&acc_full[buf], acc_ph[buf], ctx, kStatusGemmAccFull)) goto done;
+            acc_ph[buf] ^= 1u;
+            tc::fence_after_sync();
             auto store = [&](int c, float v) {
                 const long long row = row0 + c;
                 if (f_ok && row < rows) {
@@ -281,8 +304,17 @@ __global__ void __launch_bounds__(kGemmThreads, kBlocksPerSm) proj_gemm_kernel(c
                         uint32_t r[16];
                         tc::tmem_ld16(tc::tmem_addr(tm, q, buf * C::kAcc + c0), r);
                         tc::tmem_ld_wait();
+                        if constexpr (EPI) {
+                            float y[16];
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) store(c0 + j, __uint_as_float(r[j]));
+                            for (int j = 0; j < 16; ++j) y[j] = res[j];
+                            if (c0 + 16 < NR) load_residual(c0 + 16);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) store(c0 + j, y[j] + proj_act(p.epi.act, __uint_as_float(r[j]) + bias));
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) store(c0 + j, __uint_as_float(r[j]));
+                        }
                     }
                     release();
                 } else {  // the parts of k, added in their order
@@ -320,7 +352,6 @@ __global__ void __launch_bounds__(kGemmThreads, kBlocksPerSm) proj_gemm_kernel(c
                 // memory and then finishes NR / KS of the tile's rows: it adds the blocks' partials in rank order (a fixed order:
                 // the same bits every time) through distributed shared memory, and stores.  (With rank 0 alone adding everything
                 // a launch of 64 rows of the 4096 -> 256 factor took 25 us.)
-                constexpr int CW = NR / KS;
                 float* red = reinterpret_cast<float*>(smem + C::oRed) + fl;  // [NR rows][128 features]
                 if (!opened) {  // the opening cluster barrier: every peer's barriers and buffers exist
                     cluster_wait();
@@ -355,6 +386,7 @@ __global__ void __launch_bounds__(kGemmThreads, kBlocksPerSm) proj_gemm_kernel(c
                     float sum = v[c][0];
 #pragma unroll
                     for (uint32_t r = 1; r < ks; ++r) sum = sum + v[c][r];
+                    if constexpr (EPI) sum = res[c] + proj_act(p.epi.act, sum + bias);
                     store((int)kr * CW + c, sum);
                 }
                 fence_cluster();
@@ -419,14 +451,14 @@ int pick_ksplit(long long tiles, int kblocks, long long resident) {
     return 1;
 }
 
-template <int NR, int KS, bool TWO = false>
+template <int NR, int KS, bool TWO, bool EPI>
 int launch_one(GemmParams& p, long long clusters, cudaStream_t stream) {
     using C = Cfg<NR, (KS > 1), TWO>;
     static int configured_dev = -1;
     int dev = 0;
     cudaGetDevice(&dev);
     if (configured_dev != dev) {
-        const cudaError_t e = cudaFuncSetAttribute(proj_gemm_kernel<NR, KS, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes);
+        const cudaError_t e = cudaFuncSetAttribute(proj_gemm_kernel<NR, KS, TWO, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes);
         if (e != cudaSuccess) return (int)e;
         configured_dev = dev;
     }
@@ -448,7 +480,7 @@ int launch_one(GemmParams& p, long long clusters, cudaStream_t stream) {
     }
     cfg.attrs = attr;
     cfg.numAttrs = na;
-    return (int)cudaLaunchKernelEx(&cfg, proj_gemm_kernel<NR, KS, TWO>, p);
+    return (int)cudaLaunchKernelEx(&cfg, proj_gemm_kernel<NR, KS, TWO, EPI>, p);
 }
 
 // The GEMM `j` as a launch's problem with tiles of nr rows; its tiles, 0 where it has no such form.
@@ -471,7 +503,7 @@ long long few_rows_problem(GemmProblem& q, const glm53f_proj_job& j, int nr) {
 }
 
 // One GEMM, or (b) two that share a launch without clusters.
-template <int NR>
+template <int NR, bool EPI>
 int launch_gemm(GemmParams& p, const glm53f_proj_job& a, const glm53f_proj_job* b, cudaStream_t stream) {
     p.tiles = p.tiles0 = few_rows_problem(p.problem[0], a, NR);
     if (p.tiles0 == 0) return (int)cudaErrorNotSupported;
@@ -480,17 +512,18 @@ int launch_gemm(GemmParams& p, const glm53f_proj_job& a, const glm53f_proj_job* 
         const long long more = few_rows_problem(p.problem[1], *b, NR);
         if (more == 0) return (int)cudaErrorNotSupported;
         p.tiles += more;
-        return launch_one<NR, 1, true>(p, p.tiles < cap ? p.tiles : cap, stream);
+        if constexpr (EPI) return kInvalid;
+        else return launch_one<NR, 1, true, false>(p, p.tiles < cap ? p.tiles : cap, stream);
     }
     const int ks = p.problem[0].segments;
     const long long fit = cap / ks;
     const long long clusters = p.tiles < fit ? p.tiles : fit;
     if constexpr (NR <= 64) {
-        if (ks == 8) return launch_one<NR, 8>(p, clusters, stream);
-        if (ks == 4) return launch_one<NR, 4>(p, clusters, stream);
-        if (ks == 2) return launch_one<NR, 2>(p, clusters, stream);
+        if (ks == 8) return launch_one<NR, 8, false, EPI>(p, clusters, stream);
+        if (ks == 4) return launch_one<NR, 4, false, EPI>(p, clusters, stream);
+        if (ks == 2) return launch_one<NR, 2, false, EPI>(p, clusters, stream);
     }
-    return launch_one<NR, 1>(p, clusters, stream);
+    return launch_one<NR, 1, false, EPI>(p, clusters, stream);
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -560,15 +593,17 @@ int check_job(const glm53f_proj_job& j) {
     return 0;
 }
 
-int few_rows(const glm53f_proj_job& a, const glm53f_proj_job* b, int overlap, int* status, cudaStream_t stream) {
+template <bool EPI>
+int few_rows(const glm53f_proj_job& a, const glm53f_proj_job* b, const ProjEpilogue& epi, int overlap, int* status, cudaStream_t stream) {
     GemmParams p{};
+    p.epi = epi;
     p.overlap = overlap;
     p.status = status;
     const int rows = b != nullptr && b->rows > a.rows ? b->rows : a.rows;
-    if (rows <= 16) return launch_gemm<16>(p, a, b, stream);
-    if (rows <= 32) return launch_gemm<32>(p, a, b, stream);
-    if (rows <= 64 || (b == nullptr && k_segments(a) > 1)) return launch_gemm<64>(p, a, b, stream);
-    return launch_gemm<96>(p, a, b, stream);
+    if (rows <= 16) return launch_gemm<16, EPI>(p, a, b, stream);
+    if (rows <= 32) return launch_gemm<32, EPI>(p, a, b, stream);
+    if (rows <= 64 || (b == nullptr && k_segments(a) > 1)) return launch_gemm<64, EPI>(p, a, b, stream);
+    return launch_gemm<96, EPI>(p, a, b, stream);
 }
 
 // Whether two GEMMs of few rows are one launch, the parts of a split k one after another in one block each: where one of them has tiles enough by itself
@@ -596,13 +631,13 @@ extern "C" int32_t glm53f_kda_proj_bf16_many(const glm53f_proj_job* jobs, int32_
         int rc = 0;
         if (j.rows <= kFewRows || (!two && j.rows <= kFewRowsSplit && k_segments(j) > 1)) {
             const bool share = two && share_launch(j, jobs[i + 1]);
-            rc = few_rows(j, share ? &jobs[i + 1] : nullptr, two && !share ? 1 : 0, status, stream);
-            if (rc == 0 && two && !share) rc = few_rows(jobs[i + 1], nullptr, 2, status, stream);
+            rc = few_rows<false>(j, share ? &jobs[i + 1] : nullptr, {}, two && !share ? 1 : 0, status, stream);
+            if (rc == 0 && two && !share) rc = few_rows<false>(jobs[i + 1], nullptr, {}, 2, status, stream);
             i += two ? 1 : 0;
         } else {
             PairProblem q[kPairProblems];
             if (!pair_problem(q[0], j) || (two && !pair_problem(q[1], jobs[i + 1]))) return (int)cudaErrorNotSupported;
-            rc = proj_gemm_pair_launch(q, two ? 2 : 1, status, stream);
+            rc = proj_gemm_pair_launch(q, two ? 2 : 1, false, status, stream);
             i += two ? 1 : 0;
         }
         if (rc != 0) return rc;
@@ -616,4 +651,23 @@ extern "C" int32_t glm53f_kda_proj_bf16(const uint16_t* x, int64_t ldx, int64_t 
     const glm53f_proj_job job{x, ldx, x_gstride, w, ldw, w_gstride, groups, rows, n, k, out, out_f32, ldo, o_gstride};
     const int rc = kda::check_job(job);
     return rc != 0 || rows == 0 ? rc : glm53f_kda_proj_bf16_many(&job, 1, stream);
+}
+
+extern "C" int32_t glm53f_kda_proj_bf16_fused(const glm53f_proj_job* job, const glm53f_proj_epilogue* epilogue, glm53f_stream_t stream) {
+    using namespace kda;
+    if (!job || !epilogue || check_job(*job) != 0) return kInvalid;
+    const glm53f_proj_job& j = *job;
+    const glm53f_proj_epilogue& e = *epilogue;
+    if (e.activation < GLM53F_PROJ_NONE || e.activation > GLM53F_PROJ_SIGMOID) return kInvalid;
+    if (e.bias && ((reinterpret_cast<uintptr_t>(e.bias) & (e.bias_f32 ? 3 : 1)) || (j.groups > 1 && e.bias_gstride < 0))) return kInvalid;
+    if (e.residual && ((reinterpret_cast<uintptr_t>(e.residual) & (j.out_f32 ? 3 : 1)) || e.ldr < j.n || (j.groups > 1 && e.r_gstride < 0))) return kInvalid;
+    if (j.rows == 0) return 0;
+    int* status = status_word();
+    if (status == nullptr) return (int)cudaErrorUnknown;
+    const ProjEpilogue epi{e.bias, e.residual, j.groups > 1 ? e.bias_gstride : 0, e.ldr, j.groups > 1 ? e.r_gstride : 0, e.bias_f32 != 0, e.activation};
+    if (j.rows <= kFewRows || (j.rows <= kFewRowsSplit && k_segments(j) > 1)) return few_rows<true>(j, nullptr, epi, 0, status, stream);
+    PairProblem q;
+    if (!pair_problem(q, j)) return (int)cudaErrorNotSupported;
+    q.epi = epi;
+    return proj_gemm_pair_launch(&q, 1, true, status, stream);
 }

@@ -129,8 +129,8 @@ __device__ __forceinline__ PairTile pair_tile(const PairParams& p, long long t) 
     return {q, i - u * q.r_tiles, u % q.n_tiles, u / q.n_tiles};
 }
 
-// SPLIT_ROWS: rows per tile at most where k runs in segments.
-template <int SPLIT_ROWS>
+// SPLIT_ROWS: rows per tile at most where k runs in segments.  EPI: bias, activation and residual before the results leave.
+template <int SPLIT_ROWS, bool EPI>
 __global__ void __launch_bounds__(kPairThreads, 1) proj_gemm_pair_kernel(const __grid_constant__ PairParams p) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -257,10 +257,32 @@ __global__ void __launch_bounds__(kPairThreads, 1) proj_gemm_pair_kernel(const _
             for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
         };
         // The tile's rows c0 .. c0 + 31 (those below row_tile) out, as load() gave them.
-        auto emit = [&](const PairTile& x, int c0, const float (&v)[kChunk]) {
+        // v[j]'s place in the chunk of 32 rows x 32 features, by load()'s layout.
+        auto feature_of = [&](const PairTile& x, int j) { return kFragments && x.q.tensor_out ? 16 * ((j >> 3) & 1) + 8 * ((j >> 1) & 1) + (lane >> 2) : lane; };
+        auto row_of = [&](const PairTile& x, int j) { return kFragments && x.q.tensor_out ? (j & 16) + 8 * ((j >> 2) & 1) + 2 * (lane & 3) + (j & 1) : j; };
+        auto finish = [&](const PairTile& x, int c0, float (&v)[kChunk]) {
+            const ProjEpilogue& e = x.q.epi;
+            const long long row0 = (long long)x.rt * x.q.row_tile + c0;
+            const int f0 = x.nt * 2 * kPM + (int)rank * kPM + q * 32;
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) {
+                const int f = f0 + feature_of(x, j);
+                const long long row = row0 + row_of(x, j);
+                const bool ok = f < x.q.n && row < x.q.rows;
+                const float bias = e.bias != nullptr && ok ? proj_bias(e, x.g, f) : 0.0f;
+                float res = 0.0f;
+                if (e.residual != nullptr && ok) {
+                    const long long at = (long long)x.g * e.r_gstride + row * e.ldr + f;
+                    res = x.q.out_f32 ? static_cast<const float*>(e.residual)[at] : bf16_bits_to_f32(static_cast<const uint16_t*>(e.residual)[at]);
+                }
+                v[j] = res + proj_act(e.act, v[j] + bias);
+            }
+        };
+        auto emit = [&](const PairTile& x, int c0, float (&v)[kChunk]) {
             const long long row0 = (long long)x.rt * x.q.row_tile + c0;
             const int f0 = x.nt * 2 * kPM + (int)rank * kPM + side * 64;
             if (row0 >= x.q.rows) return;  // the whole chunk is past the last row (the same for every thread)
+            if constexpr (EPI) finish(x, c0, v);
             if (x.q.tensor_out) {
                 unsigned char* box = boxes + out_buf * kOutBuf;
                 out_buf ^= 1;
@@ -399,17 +421,19 @@ done:
 
 }  // namespace
 
-int proj_gemm_pair_launch(const PairProblem* problems, int n, int* status, cudaStream_t stream) {
+int proj_gemm_pair_launch(const PairProblem* problems, int n, bool epilogue, int* status, cudaStream_t stream) {
     bool wide = false;  // tiles of more than 128 rows in segments: 7 % slower a tile than the narrow instance
     for (int i = 0; i < n; ++i) wide = wide || (problems[i].segments > 1 && problems[i].row_tile > 128);
-    auto* kernel = wide ? proj_gemm_pair_kernel<kPairSplitRows> : proj_gemm_pair_kernel<128>;
-    static int configured_dev[2] = {-1, -1};
+    auto* kernel = epilogue ? (wide ? proj_gemm_pair_kernel<kPairSplitRows, true> : proj_gemm_pair_kernel<128, true>)
+                            : (wide ? proj_gemm_pair_kernel<kPairSplitRows, false> : proj_gemm_pair_kernel<128, false>);
+    static int configured_dev[4] = {-1, -1, -1, -1};
+    const int which = 2 * epilogue + wide;
     int dev = 0;
     cudaGetDevice(&dev);
-    if (configured_dev[wide] != dev) {
+    if (configured_dev[which] != dev) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
         if (e != cudaSuccess) return (int)e;
-        configured_dev[wide] = dev;
+        configured_dev[which] = dev;
     }
     PairParams p{};
     for (int i = 0; i < n; ++i) p.problem[i] = problems[i];

@@ -16,6 +16,20 @@ _lib = None
 P = C.c_void_p
 I32, I64, F32 = C.c_int32, C.c_int64, C.c_float
 
+
+class ProjJob(C.Structure):
+    """glm53f_proj_job (include/glm53f_proj.h)."""
+
+    _fields_ = [("x", P), ("ldx", I64), ("x_gstride", I64), ("w", P), ("ldw", I64), ("w_gstride", I64), ("groups", I32), ("rows", I32), ("n", I32),
+                ("k", I32), ("out", P), ("out_f32", I32), ("ldo", I64), ("o_gstride", I64)]
+
+
+class ProjEpilogue(C.Structure):
+    """glm53f_proj_epilogue (include/glm53f_proj.h)."""
+
+    _fields_ = [("bias", P), ("bias_gstride", I64), ("residual", P), ("ldr", I64), ("r_gstride", I64), ("bias_f32", I32), ("activation", I32)]
+
+
 _CHAIN_TAIL = [P, I64, I64, P, I64, P, I64]  # p, p_stride, b_off, a, a_stride, g, g_stride
 
 SIGNATURES = {
@@ -60,19 +74,16 @@ SIGNATURES = {
     # include/glm53f_proj.h: the projections' GEMM (the arguments of glm53f_fwd_gemv_bf16 without its split-K scratch)
     "glm53f_kda_proj_bf16": (I32, [P, I64, I64, P, I64, I64, I32, I32, I32, I32, P, I32, I64, I64, P]),
     "glm53f_kda_proj_bf16_many": (I32, [P, I32, P]),
+    "glm53f_kda_proj_bf16_fused": (I32, [C.POINTER(ProjJob), C.POINTER(ProjEpilogue), P]),
+    # Parts 3 and 4 of include/glm53f_kda.h: linear attention with one decay a head, the verification of drafted tokens
+    "glm53f_kda_lin_decode_batch": (C.c_int, [I32, I32, I32, P, P, P, I64, P, I64, P, I64, P, I64, P, P, P, I32, F32, P, I64, P]),
+    "glm53f_kda_lin_prefill_workspace_bytes": (I64, [I32, I32, I32]),
+    "glm53f_kda_lin_prefill_varlen": (C.c_int, [I32, I32, I32, P, I32, I32, P, I64, P, I64, P, I64, P, I64, P, P, P, I32, F32, P, I64, P, I64, P]),
+    "glm53f_kda_accept_batch": (C.c_int, [I32, P, I32, P, I32, I64, P, P, I64, P, P, P, P, P]),
 }
 
-
-class ProjJob(C.Structure):
-    """glm53f_proj_job (include/glm53f_proj.h)."""
-
-    _fields_ = [("x", P), ("ldx", I64), ("x_gstride", I64), ("w", P), ("ldw", I64), ("w_gstride", I64), ("groups", I32), ("rows", I32), ("n", I32),
-                ("k", I32), ("out", P), ("out_f32", I32), ("ldo", I64), ("o_gstride", I64)]
-
-
-
 # The reference's thirteen (crates/glm53f-kda/tests/provenance.rs:41-69 asserts exactly these).
-REFERENCE_SYMBOLS = [n for n in SIGNATURES if n.startswith("glm53f_kda_") and "_core_" not in n and "_gather_" not in n and n not in ("glm53f_kda_device_status", "glm53f_kda_debug_wait_test", "glm53f_kda_prefill_mode", "glm53f_kda_verify_mode", "glm53f_kda_commit_mode", "glm53f_kda_mark_copy", "glm53f_kda_mark_copy_slots", "glm53f_kda_mark_copy_list", "glm53f_kda_store_words", "glm53f_kda_proj_bf16", "glm53f_kda_proj_bf16_many", "glm53f_kda_chain_commit_batch")]
+REFERENCE_SYMBOLS = [n for n in SIGNATURES if n.startswith("glm53f_kda_") and "_core_" not in n and "_gather_" not in n and "_lin_" not in n and n not in ("glm53f_kda_device_status", "glm53f_kda_debug_wait_test", "glm53f_kda_prefill_mode", "glm53f_kda_verify_mode", "glm53f_kda_commit_mode", "glm53f_kda_mark_copy", "glm53f_kda_mark_copy_slots", "glm53f_kda_mark_copy_list", "glm53f_kda_store_words", "glm53f_kda_proj_bf16", "glm53f_kda_proj_bf16_many", "glm53f_kda_proj_bf16_fused", "glm53f_kda_accept_batch", "glm53f_kda_chain_commit_batch")]
 
 
 def library_path() -> str:

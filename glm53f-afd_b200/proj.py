@@ -14,6 +14,7 @@ import torch
 from . import ffi
 from .core import CudaError, Invalid
 
+_BF = (torch.bfloat16, torch.int16, torch.uint16)
 HIDDEN = 4096
 KDA_HEADS, KDA_DIM = 64, 128
 KDA_WIDTH = KDA_HEADS * KDA_DIM          # 8192
@@ -60,9 +61,42 @@ def bf16(x: torch.Tensor, ldx: int, x_gstride: int, w: Bf16Mat, rows: int, out: 
     _launched(code, "glm53f_kda_proj_bf16")
 
 
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "sigmoid": 5}  # GLM53F_PROJ_*
+
+
+def fused(x: torch.Tensor, ldx: int, x_gstride: int, w: Bf16Mat, rows: int, out: torch.Tensor, ldo: int, o_gstride: int, out_f32: bool = False,
+          x_offset: int = 0, out_offset: int = 0, *, bias: torch.Tensor | None = None, activation: str = "none",
+          residual: torch.Tensor | None = None, ldr: int | None = None, r_gstride: int | None = None, residual_offset: int = 0) -> None:
+    """`bf16` with an epilogue in the same launch: out = residual + act(x w^T + bias), formed in f32 and rounded once.  bias [groups][n]
+    (bf16 or f32); residual of out's type, with out's strides unless others are given, `out` itself or memory of its own."""
+    if activation not in ACTIVATIONS:
+        raise Invalid(f"activation {activation!r}: one of {', '.join(ACTIVATIONS)}")
+    if rows == 0:
+        return
+    job = _job(x, ldx, x_gstride, w, rows, out, ldo, o_gstride, out_f32, x_offset, out_offset)
+    e = ffi.ProjEpilogue(activation=ACTIVATIONS[activation])
+    if bias is not None:
+        if bias.dtype not in (torch.float32, *_BF) or not bias.is_contiguous() or bias.numel() != w.groups * w.n:
+            raise Invalid(f"bias must be {w.groups} x {w.n} contiguous values, bf16 or f32")
+        e.bias, e.bias_gstride, e.bias_f32 = bias.data_ptr(), w.n, int(bias.dtype == torch.float32)
+    if residual is not None:
+        ldr, r_gstride = ldo if ldr is None else ldr, o_gstride if r_gstride is None else r_gstride
+        if (residual.dtype == torch.float32) != out_f32 or (not out_f32 and residual.dtype not in _BF):
+            raise Invalid("the residual has out's type")
+        if residual_offset < 0 or ldr < w.n or r_gstride < 0 or residual.numel() < residual_offset + (w.groups - 1) * r_gstride + (rows - 1) * ldr + w.n:
+            raise Invalid("the residual is smaller than the shapes named")
+        e.residual, e.ldr, e.r_gstride = residual.data_ptr() + residual_offset * residual.element_size(), ldr, r_gstride
+    here = torch.cuda.current_device()
+    for t in (x, w.t, out, bias, residual):
+        if t is not None and (not t.is_cuda or t.device.index != here):
+            raise Invalid(f"a tensor on {t.device}, the current device is cuda:{here}")
+    code = ffi.load().glm53f_kda_proj_bf16_fused(ffi.ProjJob(*job), e, torch.cuda.current_stream().cuda_stream)
+    _launched(code, "glm53f_kda_proj_bf16_fused")
+
+
 def _job(x, ldx, x_gstride, w: Bf16Mat, rows, out, ldo, o_gstride, out_f32=False, x_offset=0, out_offset=0) -> tuple:
     """The checked arguments of one GEMM: those of glm53f_kda_proj_bf16 before the stream, the fields of ffi.ProjJob."""
-    if x.dtype not in (torch.bfloat16, torch.int16, torch.uint16) or w.t.dtype not in (torch.bfloat16, torch.int16, torch.uint16):
+    if x.dtype not in _BF or w.t.dtype not in _BF:
         raise Invalid("x and the weight are bf16")
     if out.dtype != (torch.float32 if out_f32 else x.dtype) and not (not out_f32 and out.element_size() == 2):
         raise Invalid("out is f32 when out_f32, else bf16")

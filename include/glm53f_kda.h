@@ -445,6 +445,80 @@ int32_t glm53f_kda_commit_mode(int32_t mode);
  * Host-side settings, not thread safe; returns 0, or 1 for a limit outside the range. */
 int glm53f_kda_debug_wait_test(uint64_t wait_limit_ns, int32_t skip_first_state);
 
+/* ===================================================================================================
+ * Part 3: linear attention with one decay a head
+ *
+ * The recurrence that hybrid decoders use where the KDA layers have a delta rule and a decay for every key channel; not in
+ * the reference.  Per row t and head h, with S the state [128 (v)][128 (k)] in the layout of Parts 1 and 2:
+ *     S_t = exp(g_t) S_{t-1} + v_t k_t^T        y_t = scale * S_t q_t
+ *
+ * Common arguments:
+ *   heads, qk_heads   heads of v, g, the states and out (1..65535); heads of q and k, which divide them: heads
+ *                     [i * heads / qk_heads, (i + 1) * heads / qk_heads) read head i of q and k
+ *   cu_rows           device int32 [batch + 1]: request b owns rows [cu_rows[b], cu_rows[b + 1]); requests may have none
+ *   q, k, v           bf16, row r at + r * stride (elements): [qk_heads][128] of q and k, [heads][128] of v; 16-byte
+ *                     aligned, strides multiples of 8 and at least the row (parts of a fused projection's rows will do)
+ *   g, g_stride       f32 log decay of row r and head h at g[r * g_stride + h]; g_stride 0: one value a head for all rows.  -inf
+ *                     forgets everything before the row
+ *   state_in / state_out, state_off, state_bf16   as in Part 2; a request's state begins state_off[b] elements in.  Requests that
+ *                     write need regions of their own, in place or elsewhere
+ *   out               bf16, row r at + r * out_stride, [heads][128]; 16-byte aligned, the stride a multiple of 8; memory of
+ *                     its own.  Rows that belong to no request are left as they are
+ * =================================================================================================== */
+
+/* Row by row: single tokens and windows of drafted ones.  keep (device int32 [batch]; NULL: every row) limits request b to its
+ * first keep[b] rows.  state_out NULL leaves the states alone (a verify call), out NULL writes no outputs (a commit of
+ * kept rows); not both.  A bf16 state is rounded after every row, so that one call over several rows, or a verify and a
+ * commit of k rows, leave the bits of k single-row calls. */
+int glm53f_kda_lin_decode_batch(int32_t heads, int32_t qk_heads, int32_t batch, const int32_t* cu_rows, const int32_t* keep,
+                                const glm53f_bf16* q, int64_t q_stride, const glm53f_bf16* k, int64_t k_stride,
+                                const glm53f_bf16* v, int64_t v_stride, const float* g, int64_t g_stride,
+                                const void* state_in, void* state_out, const int64_t* state_off, int32_t state_bf16,
+                                float scale, glm53f_bf16* out, int64_t out_stride, glm53f_stream_t stream);
+
+/* Chunked prefill of packed sequences (chunks count from each sequence's first row).  max_len (host) >= the longest
+ * sequence; rows (host) >= cu_rows[batch]: the rows that q, k and v hold.  The state is FP32 from the first row to the last and rounded
+ * once; state_out must not be NULL, and equals state_in or has no byte in common with it.  `workspace` (16-byte aligned) of
+ * glm53f_kda_lin_prefill_workspace_bytes(heads, batch, max_len) bytes lets long sequences of few (sequence, head) chains run in
+ * several segments at once; with fewer bytes (0 and NULL among them) every chain is one walk.  Results depend on the number
+ * of segments to the order of the FP32 sums, and on nothing else in the batch. */
+int64_t glm53f_kda_lin_prefill_workspace_bytes(int32_t heads, int32_t batch, int32_t max_len);
+int glm53f_kda_lin_prefill_varlen(int32_t heads, int32_t qk_heads, int32_t batch, const int32_t* cu_rows, int32_t rows, int32_t max_len,
+                                  const glm53f_bf16* q, int64_t q_stride, const glm53f_bf16* k, int64_t k_stride,
+                                  const glm53f_bf16* v, int64_t v_stride, const float* g, int64_t g_stride,
+                                  const void* state_in, void* state_out, const int64_t* state_off, int32_t state_bf16,
+                                  float scale, glm53f_bf16* out, int64_t out_stride, void* workspace, int64_t workspace_bytes,
+                                  glm53f_stream_t stream);
+
+/* ===================================================================================================
+ * Part 4: verification of drafted tokens
+ * =================================================================================================== */
+
+/* How many rows of each window to keep, and the token that follows them: what stands between a verify and its commit
+ * (crates/glm53f-coordinator/src/scheduler.rs:765-875 keeps while a draft equals the target's choice; the greedy case here).
+ *
+ * Request b's window is rows [cu_rows[b], cu_rows[b + 1]) (device int32 [batch + 1]): its first row holds the last token
+ * that is certain, the others drafted ones.  Row i of `target` (+ i * ld elements, `vocab` long) is the target's distribution
+ * of the token BEHIND row i, so it judges tokens[i + 1]:
+ *   target_kind   GLM53F_KDA_PROBABILITIES   f32 probabilities p (negative, infinite or NaN entries count as 0)
+ *                 GLM53F_KDA_LOGITS_F32, _BF16   logits: p = softmax(logits / temperature[b]); -inf and NaN entries are never chosen
+ *   tokens        int32, one a row (a window's first is not read); one outside [0, vocab) is never kept
+ *   draft         f32 [rows][draft_ld]: row i the distribution that tokens[i] was drawn from (a window's first is not read);
+ *                 NULL: the drafter had one choice, q(tokens[i]) = 1
+ *   temperature   f32 [batch], logits only (NULL: 1 for all); 0 or less: greedy, the largest logit, the lowest index among equals
+ *   u             f32 [rows], uniform in [0, 1): u[i] judges tokens[i], a window's first draws the next token
+ * A token is kept while u q < p and all before it are (greedy: while it is the largest).  keep[b] = 1 + the tokens kept; next[b]
+ * is drawn from p behind a whole window, else from max(p - q, 0) of the first refused token's row -- without `draft`, from p
+ * without that token; from p where this leaves nothing: the lowest index whose running sum, divided by the whole, exceeds
+ * u.  Draws are made in 64 bits.  A row that leaves nothing gives next[b] = -1, a request without rows keep 0 and next -1.
+ * One launch; nothing is allocated.  vocab >= 1, ld and draft_ld >= vocab. */
+#define GLM53F_KDA_PROBABILITIES 0
+#define GLM53F_KDA_LOGITS_F32 1
+#define GLM53F_KDA_LOGITS_BF16 2
+int glm53f_kda_accept_batch(int32_t batch, const int32_t* cu_rows, int32_t vocab, const void* target, int32_t target_kind, int64_t ld,
+                            const int32_t* tokens, const float* draft, int64_t draft_ld, const float* temperature, const float* u,
+                            int32_t* keep, int32_t* next, glm53f_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

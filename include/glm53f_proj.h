@@ -55,6 +55,30 @@ typedef struct glm53f_proj_job {
 } glm53f_proj_job;
 int32_t glm53f_kda_proj_bf16_many(const glm53f_proj_job* jobs, int32_t count, glm53f_stream_t stream);
 
+/* glm53f_kda_proj_bf16 with an epilogue, one launch: out = residual + act(x w^T + bias), formed in f32 from the product's f32
+ * sum and rounded once; not in the reference.
+ *   bias        [groups][n], bf16 or (bias_f32 != 0) f32, group g at + g * bias_gstride (read only when groups > 1); NULL: none
+ *   activation  one of GLM53F_PROJ_*: relu max(y, 0), silu y / (1 + e^-y), gelu y (1 + erf(y / sqrt 2)) / 2, gelu_tanh the
+ *               same by tanh(sqrt(2 / pi) (y + 0.044715 y^3)), sigmoid 1 / (1 + e^-y)
+ *   residual    of out's type, row m of group g at + g * r_gstride + m * ldr (ldr >= n); NULL: none.  It may be `out` itself
+ *               (same address and strides), and otherwise has no element in common with it
+ * The job's fields, checks, row independence and status codes are glm53f_kda_proj_bf16's; bias and residual are aligned to
+ * their elements. */
+#define GLM53F_PROJ_NONE 0
+#define GLM53F_PROJ_RELU 1
+#define GLM53F_PROJ_SILU 2
+#define GLM53F_PROJ_GELU 3
+#define GLM53F_PROJ_GELU_TANH 4
+#define GLM53F_PROJ_SIGMOID 5
+typedef struct glm53f_proj_epilogue {
+    const void* bias;
+    int64_t bias_gstride;
+    const void* residual;
+    int64_t ldr, r_gstride;
+    int32_t bias_f32, activation;
+} glm53f_proj_epilogue;
+int32_t glm53f_kda_proj_bf16_fused(const glm53f_proj_job* job, const glm53f_proj_epilogue* epilogue, glm53f_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
