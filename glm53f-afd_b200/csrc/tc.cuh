@@ -140,6 +140,10 @@ __device__ __forceinline__ void tmem_st_frag(uint32_t taddr, const uint32_t (&r)
 __device__ __forceinline__ void stmatrix_t4(void* row, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(row)), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+// The same without transposing: row j of matrix m goes to the 16 bytes that lane 8 m + j names.
+__device__ __forceinline__ void stmatrix_4(void* row, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(row)), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
 // And back: the fragments of the four matrices that stmatrix_t4 with these addresses would have stored.
 __device__ __forceinline__ void ldmatrix_t4(const void* row, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(smem_u32(row)) : "memory");

@@ -57,3 +57,33 @@ def cu_of(lens, device):
     for n in lens:
         cu.append(cu[-1] + n)
     return torch.tensor(cu, dtype=torch.int32, device=device)
+
+
+def chunked(lens, q, k, v, g, state, scale, bf16_state):
+    """The same, with the bounds of the chunked form.  M, the recurrence of the magnitudes, is what every rounding is relative to: products of
+    bf16 are exact; a chunk's sums of up to 64 terms (and the scores' of 128) in the tensor core's f32 lose at most four half steps a term; a factor's
+    exponential and the sums of log decays eight; a chunk that passes over an older one's sums six.  w V is exact to f32 in three parts (24 bits), to 2^-16
+    in two; S and P as operands are, both, exact to 2^-16 (two roundings of bf16: 2^-8 of 2^-8)."""
+    rows, heads, d = v.shape
+    share = heads // q.shape[1]
+    q, k = (t.double().repeat_interleave(share, 1) for t in (q, k))
+    v, g = v.double(), g.double().expand(rows, heads)
+    y, yb = (torch.zeros(rows, heads, d, dtype=torch.float64, device=v.device) for _ in range(2))
+    ends, endb = [], []
+    first = 0
+    for b, n in enumerate(lens):
+        s = state[b].double()
+        m = s.abs()
+        part = (4 * 64 + 8 + 6 * ((n + 63) // 64)) * U32 + (UBF * UBF if bf16_state else 4 * U32)
+        for t in range(first, first + n):
+            decay = torch.exp(g[t])[:, None, None]
+            s = decay * s + v[t][:, :, None] * k[t][:, None, :]
+            m = decay * m + (v[t][:, :, None] * k[t][:, None, :]).abs()
+            y[t] = scale * (s * q[t][:, None, :]).sum(-1)
+            at = abs(scale) * (m * q[t][:, None, :].abs()).sum(-1) * (part + 2 * UBF * UBF + (4 * 128 + 4 * 64 + 16) * U32)
+            yb[t] = at + (UBF + U32) * (y[t].abs() + at) + 1e-38
+        e = part * m
+        ends.append(s)
+        endb.append(e + (UBF if bf16_state else U32) * (s.abs() + e) + 1e-38)
+        first += n
+    return y, torch.stack(ends), yb, torch.stack(endb)
