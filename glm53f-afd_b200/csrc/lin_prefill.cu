@@ -8,19 +8,21 @@
 // so a chunk is four products: Q K^T, S Q^T, V^T P^T and (w V)^T K, all on operands as the tensor copies bring them (128-byte
 // swizzle, K- or MN-major).  Bound by HBM where every SM has a chain (1 KiB a row and head); a chain's own pace is the tensor pipe's.
 //
-// Precision.  Sums are f32 in tensor memory, the state is f32 in registers.  What has to become a bf16 operand and is not one already goes
-// as a sum of several: P and S as two (16 bits: beside an output's rounding to bf16 nothing is left of their errors; as one each
-// they would add as much again), w V as three where the state is f32 (24 bits, all that f32 has) and as two where it is stored as
-// bf16.  Differences of G are of sums in 64 bits, held as two f32: a row that forgets everything (-inf, taken as -104 a row, which
-// is 0 in f32) must not blur those behind it.
+// Precision.  Sums and the state are f32 in tensor memory.  What has to become an operand and is not bf16 already keeps more bits than that: w V
+// goes as a sum of three bf16 parts where the state is f32 (24 bits, all that f32 has) and of two where it is stored as bf16, P as a sum of two (16 bits), S and
+// scale e^G Q as f32 operands of which the tensor core takes 11 bits: beside the outputs' rounding to bf16 little is left of their errors (as single bf16
+// operands P and S would add as much again).  Differences of G are of sums in 64 bits, held as two f32: a row that forgets everything (-inf, taken as
+// -104, which is 0 in f32) must not blur those behind it.
 //
 // Roles of a block, one (chain, segment) each, all meeting at mbarriers:
-//   warps 0-3    P of a chunk out of the accumulator into shared memory (hi and lo); the outputs of the one before: e^G_t and scale,
-//                transposing matrix stores, rows of 256 bytes to global memory
-//   warps 4-7    w V in parts, in V's own layout; the rows of a last, short chunk to zero (what lies there may be NaN)
-//   warps 8-15   the state: 64 key channels of a value channel a thread; scaled, added to, split and given to the tensor core as an operand in
-//                tensor memory
-//   warp 16      tensor copies of q, k, v, two chunks ahead       warp 17  the products       warp 18  sums and factors of the decays
+//   warps 0-3    P of a chunk out of the accumulator into shared memory (hi and lo)
+//   warps 4-7    the outputs through transposing matrix stores to rows of 256 bytes
+//   warps 8-11   scale e^G Q as f32
+//   warps 12-19  the parts of w V^T into tensor memory; the rows of a last, short chunk to zero (what lies there may be NaN)
+//   warps 20-27  the state, which is an operand of one product and the accumulator of the other: times e^G between the two
+//   warp 28      tensor copies of q, k, v, three chunks ahead     warp 29  the products       warp 30  sums and factors of the decays
+// A chunk's products take 1,920 cycles of the tensor pipe; what the other roles issue for it is the tighter bound, so their bodies are loops, their waits
+// sleep, and operands take the form that costs the fewest instructions.
 //
 // Few chains: a sequence is cut into segments that are walked at the same time, each from the state that the segments before it
 // leave.  That state comes from a pass over k and v alone (the state's product only), which writes what each segment adds from a zero
@@ -41,10 +43,10 @@ namespace {
 constexpr int CH = 64;                                  // rows a chunk
 constexpr int kTile = CH * DK * 2;                      // q, k or v of a chunk: two boxes of 64 rows x 128 bytes
 constexpr int kBox = CH * 128;
-constexpr int kStages = 2, kStage = 3 * kTile;
-constexpr int oWV = kStages * kStage;                   // w V: three parts in V's layout
-constexpr int oP = oWV + 3 * kTile;                     // P, two buffers of hi | lo
-constexpr int oY = oP + 2 * 2 * kBox;                   // a chunk's outputs on their way out
+constexpr int kStages = 3, kStage = 3 * kTile;
+constexpr int oQ = kStages * kStage;                    // scale e^G Q, f32: four boxes of 64 rows x 32 channels
+constexpr int oP = oQ + 2 * kTile;                      // P: hi | lo
+constexpr int oY = oP + 2 * kBox;                       // a chunk's outputs on their way out
 constexpr int kDecays = 4;                              // chunks of decay factors in flight
 struct Decays {
     float2 g[CH];     // G in powers of two: hi, lo
@@ -54,13 +56,17 @@ struct Decays {
 };
 constexpr int oDecays = oY + kTile;
 constexpr int oBars = oDecays + kDecays * (int)sizeof(Decays);
-enum : int { bFull = 0, bEmpty = bFull + kStages, bQK = bEmpty + kStages, bP = bQK + 2, bWV = bP + 2, bU, bUFree, bS, bO, bOFree, bDecay, bDecayFree = bDecay + kDecays, kBars = bDecayFree + kDecays };
-constexpr int oCtl = oBars + kBars * 8;
+enum : int {
+    bFull = 0, bEmpty = bFull + kStages, bQK = bEmpty + kStages, bPQ, bQS, bState, bAdd, bU = bAdd + 2, bO = bU + 2, bOFree = bO + 2, bDecay = bOFree + 2,
+    bDecayFree = bDecay + kDecays, kBars = bDecayFree + kDecays
+};
+constexpr int oCtl = oBars + (kBars + 1) / 2 * 16;
 constexpr int kSmem = oCtl + 16 + 1024;
 static_assert(kSmem <= 232448 && sizeof(Decays) % 16 == 0, "shared memory");
 
-constexpr int kPWarps = 4, kVWarps = 4, kSWarps = 8, kCopyWarp = 16, kMmaWarp = 17, kDecayWarp = 18, kThreads = 19 * 32;
-constexpr int cQK = 0, cO1 = 128, cO2 = 192, cU = 256, cSHi = 384, cSLo = 448, kCols = 512;  // tensor memory columns
+constexpr int kOWarp = 4, kQWarp = 8, kVWarp = 12, kSWarp = 20, kCopyWarp = 28, kMmaWarp = 29, kDecayWarp = 30, kThreads = 31 * 32;
+// Tensor memory columns: the state, the scores, two accumulators of outputs and two sets of w V^T in turn.
+constexpr int cS = 0, cQK = 128, cO = 192, cWV = 320, kCols = 512;
 
 enum : int { kStatusLinFull = 150, kStatusLinEmpty, kStatusLinQK, kStatusLinP, kStatusLinWV, kStatusLinU, kStatusLinS, kStatusLinO, kStatusLinDecay, kStatusLinFree };
 
@@ -102,14 +108,12 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < kStages; ++i) mbar_init(&bar[bFull + i], 1), mbar_init(&bar[bEmpty + i], 1);
-        for (int i = 0; i < 2; ++i) mbar_init(&bar[bQK + i], 1), mbar_init(&bar[bP + i], kPWarps);
-        mbar_init(&bar[bWV], kVWarps);
-        mbar_init(&bar[bU], 1);
-        mbar_init(&bar[bUFree], kSWarps);
-        mbar_init(&bar[bS], kSWarps);
-        mbar_init(&bar[bO], 1);
-        mbar_init(&bar[bOFree], kPWarps);
-        for (int i = 0; i < kDecays; ++i) mbar_init(&bar[bDecay + i], 1), mbar_init(&bar[bDecayFree + i], kVWarps + kSWarps + (STATE ? 0 : kPWarps));
+        mbar_init(&bar[bQK], 1);
+        mbar_init(&bar[bPQ], 8);
+        mbar_init(&bar[bQS], 1);
+        mbar_init(&bar[bState], 8);
+        for (int i = 0; i < 2; ++i) mbar_init(&bar[bAdd + i], 16), mbar_init(&bar[bU + i], 1), mbar_init(&bar[bO + i], 1), mbar_init(&bar[bOFree + i], 4);
+        for (int i = 0; i < kDecays; ++i) mbar_init(&bar[bDecay + i], 1), mbar_init(&bar[bDecayFree + i], STATE ? 16 : 24);
         ctl[0] = 0u;
         ctl[1] = 0u;
         mbar_init_fence();
@@ -135,8 +139,11 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar[i]);
     };
-    auto wait = [&](int i, uint32_t parity, int code) { return tc::warp_all(mbar_wait(&bar[i], parity & 1u, ctx, code)); };
-    auto decay_wait = [&](int c) { return wait(bDecay + c % kDecays, c / kDecays, kStatusLinDecay); };
+    // A wait that sleeps in hardware first: the polling of mbar_wait by thirty warps is a third of what the block would issue.
+    auto wait = [&](int i, uint32_t parity, int code) {
+        return tc::warp_all(mbar_try_wait_hint(&bar[i], parity & 1u, 200000u) || mbar_wait(&bar[i], parity & 1u, ctx, code));
+    };
+    auto wait_with_decays = [&](int c, int i, uint32_t parity, int code) { return wait(i, parity, code) && wait(bDecay + c % kDecays, c / kDecays, kStatusLinDecay); };
 
     if (idle) goto done;
     if (warp == kCopyWarp) {
@@ -155,48 +162,61 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
             }
         }
     } else if (warp == kMmaWarp) {
-        constexpr uint32_t id_qk = tc::idesc_bf16(64, 64, 0, 0, 0), id_u = tc::idesc_bf16(128, 128, 1, 1, 0), id_s = tc::idesc_bf16(128, 64, 0, 0, 0),
-                           id_pv = tc::idesc_bf16(128, 64, 1, 0, 0);
+        constexpr uint32_t id_qk = tc::idesc_bf16(64, 64, 0, 0, 0), id_u = tc::idesc_bf16(128, 128, 0, 1, 0), id_s = tc::idesc_tf32(128, 64), id_pv = tc::idesc_bf16(128, 64, 1, 0, 0);
         const uint32_t leader = tc::elect_one();
         const int parts = p.state_bf16 ? 2 : 3;
-        for (int c = 0; c < n; ++c) {
-            const unsigned char *q = smem + (c % kStages) * kStage, *k = q + kTile, *v = k + kTile;
-            if (!wait(bFull + c % kStages, c / kStages, kStatusLinFull)) goto done;
-            tc::fence_after_sync();
-            if (!STATE) {  // (its accumulator is free: P of the chunk two before was waited for)
+        // As values that the compiler knows to be the same in all lanes: loops over them stay converged and the products' operands in uniform
+        // registers.
+        const int n_all = (int)__reduce_max_sync(0xffffffffu, (unsigned)n);
+        const uint32_t tm_all = __reduce_max_sync(0xffffffffu, tm);
+        auto scores = [&](int c) {
+            const unsigned char *q = smem + (c % kStages) * kStage, *k = q + kTile;
 #pragma unroll
-                for (int i = 0; i < DK / 16; ++i)
-                    tc::mma_bf16_if(leader, tm + cQK + 64 * (c & 1), tc::desc_sw128_kmajor(q, CH, 16 * i), tc::desc_sw128_kmajor(k, CH, 16 * i), id_qk, i > 0);
-                tc::mma_commit_if(leader, &bar[bQK + (c & 1)]);
-            }
-            if (!wait(bWV, c, kStatusLinWV) || !wait(bUFree, c + 1, kStatusLinFree)) goto done;
+            for (int i = 0; i < DK / 16; ++i)
+                tc::mma_bf16_if(leader, tm_all + cQK, tc::desc_sw128_kmajor(q, CH, 16 * i), tc::desc_sw128_kmajor(k, CH, 16 * i), id_qk, i > 0);
+            tc::mma_commit_if(leader, &bar[bQK]);
+        };
+        if (!STATE && n_all > 0) {
+            if (!wait(bFull, 0, kStatusLinFull)) goto done;
             tc::fence_after_sync();
-            for (int part = 0; part < parts; ++part)
-#pragma unroll
-                for (int i = 0; i < CH / 16; ++i)
-                    tc::mma_bf16_if(leader, tm + cU, tc::desc_sw128_mnmajor(smem + oWV + part * kTile, CH, 16 * i), tc::desc_sw128_mnmajor(k, CH, 16 * i), id_u,
-                                    part > 0 || i > 0);
-            if (STATE) tc::mma_commit_if(leader, &bar[bEmpty + c % kStages]);
-            tc::mma_commit_if(leader, &bar[bU]);
+            scores(0);
+        }
+        for (int c = 0; c < n_all; ++c) {
+            const unsigned char *k = smem + (c % kStages) * kStage + kTile, *v = k + kTile;
+            if (STATE && !wait(bFull + c % kStages, c / kStages, kStatusLinFull)) goto done;
             if (!STATE) {
-                if (!wait(bS, c, kStatusLinS) || !wait(bOFree, c + 1, kStatusLinFree)) goto done;
+                const uint32_t o = tm_all + cO + 64 * (c & 1);
+                // (The state is there when its product with the chunk before has been waited for: one product's result as another's operand is not
+                // in the order of their issue.)
+                if (!wait(bPQ, c, kStatusLinP) || !wait(bOFree + (c & 1), c / 2 + 1, kStatusLinFree) ||
+                    !(c > 0 ? wait(bU + ((c - 1) & 1), (c - 1) / 2, kStatusLinU) : wait(bState, 0, kStatusLinS)))
+                    goto done;
                 tc::fence_after_sync();
 #pragma unroll
-                for (int part = 0; part < 2; ++part)
-#pragma unroll
-                    for (int i = 0; i < DK / 16; ++i)
-                        tc::mma_bf16_ts_if(leader, tm + cO1, tm + (part ? cSLo : cSHi) + 8 * i, tc::desc_sw128_kmajor(q, CH, 16 * i), id_s, part > 0 || i > 0);
-                if (!wait(bP + (c & 1), c / 2, kStatusLinP)) goto done;
-                tc::fence_after_sync();
-                const unsigned char* pt = smem + oP + (c & 1) * 2 * kBox;
-#pragma unroll
+                for (int i = 0; i < DK / 8; ++i) tc::mma_tf32_ts_if(leader, o, tm_all + cS + 8 * i, tc::desc_sw128_kmajor_f32(smem + oQ, CH, 8 * i), id_s, i > 0);
+                tc::mma_commit_if(leader, &bar[bQS]);
+                const unsigned char* pt = smem + oP;
+#pragma unroll 1
                 for (int part = 0; part < 2; ++part)
 #pragma unroll
                     for (int i = 0; i < CH / 16; ++i)
-                        tc::mma_bf16_if(leader, tm + cO2, tc::desc_sw128_mnmajor(v, CH, 16 * i), tc::desc_sw128_kmajor(pt + part * kBox, CH, 16 * i), id_pv, part > 0 || i > 0);
-                tc::mma_commit_if(leader, &bar[bEmpty + c % kStages]);
-                tc::mma_commit_if(leader, &bar[bO]);  // (the last one: whoever has seen it has seen the others)
+                        tc::mma_bf16_if(leader, o, tc::desc_sw128_mnmajor(v, CH, 16 * i), tc::desc_sw128_kmajor(pt + part * kBox, CH, 16 * i), id_pv, true);
+                tc::mma_commit_if(leader, &bar[bO + (c & 1)]);
+                if (c + 1 < n_all) {  // (P of this chunk has been read out of the scores' columns)
+                    if (!wait(bFull + (c + 1) % kStages, (c + 1) / kStages, kStatusLinFull)) goto done;
+                    tc::fence_after_sync();
+                    scores(c + 1);
+                }
             }
+            if (!wait(bAdd + (c & 1), c / 2, kStatusLinWV)) goto done;
+            tc::fence_after_sync();
+#pragma unroll 1
+            for (int part = 0; part < parts; ++part)
+#pragma unroll
+                for (int i = 0; i < CH / 16; ++i)
+                    tc::mma_bf16_ts_if(leader, tm_all + cS, tm_all + cWV + 96 * (c & 1) + 32 * part + 8 * i, tc::desc_sw128_mnmajor(k, CH, 16 * i), id_u, true);
+            tc::mma_commit_if(leader, &bar[bEmpty + c % kStages]);
+            tc::mma_commit_if(leader, &bar[bU + (c & 1)]);  // (the last one: whoever has seen it has seen the others)
             if (leader) ctl[0] = ctl[0] + 1u;
         }
     } else if (warp == kDecayWarp) {
@@ -238,232 +258,257 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
             arrive(bDecay + c % kDecays);
         }
         if (STATE && lane == 0) p.kept[(long long)chain * p.segments + seg] = exp2f((float)total);
-    } else if (warp < kPWarps) {
+    } else if (warp < kOWarp) {
         if (!STATE) {
-            const int w = warp;
-            bool ok = true;
-            // Chunk c's outputs: the accumulators' lanes are value channels, their columns rows.
-            auto outputs = [&](int c) {
-                ok = ok && wait(bO, c, kStatusLinO);
-                if (!named_bar_all(1, kPWarps * 32, ok)) return false;  // (and the rows of the chunk before have left the staging)
-                tc::fence_after_sync();
-                const Decays& x = decays[c % kDecays];
-                unsigned char* y = smem + oY;
-#pragma unroll
-                for (int half = 0; half < 2; ++half)
-#pragma unroll
-                    for (int t0 = 0; t0 < CH; t0 += 16) {
-                        uint32_t r1[8], r2[8];
-                        const uint32_t at = tc::tmem_addr(tm, w, t0) + ((uint32_t)(16 * half) << 16);
-                        tc::tmem_ld_frag(at + cO1, r1);
-                        tc::tmem_ld_frag(at + cO2, r2);
-                        tc::tmem_ld_wait();
-                        uint32_t z[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {  // (two rows of a value channel: 8 (i / 2) + 2 (lane % 4) and the next)
-                            const float2 e = *reinterpret_cast<const float2*>(&x.e[t0 + 8 * (i >> 1) + 2 * (lane & 3)]);
-                            const float2 inner = mul2(make_float2(p.scale, p.scale), make_float2(__uint_as_float(r2[2 * i]), __uint_as_float(r2[2 * i + 1])));
-                            const float2 v = fma2(e, make_float2(__uint_as_float(r1[2 * i]), __uint_as_float(r1[2 * i + 1])), inner);
-                            z[i] = tc::bf16x2(v.x, v.y);
-                        }
-                        const int t = t0 + 8 * (lane >> 4) + (lane & 7), piece = 4 * w + 2 * half + ((lane >> 3) & 1);
-                        tc::stmatrix_t4(y + t * 256 + ((piece ^ (t & 7)) << 4), z[0], z[1], z[2], z[3]);
-                    }
-                tc::fence_before_sync();
-                arrive(bOFree);
-                arrive(bDecayFree + c % kDecays);
-                named_bar_sync(2, kPWarps * 32);
-                uint16_t* out = p.out + (long long)(row0 + c * CH) * p.out_stride + h * DV;
-#pragma unroll
-                for (int i = 0; i < CH * 16 / (kPWarps * 32); ++i) {
-                    const int t = i * (kPWarps * 2) + (tid >> 4), piece = tid & 15;
-                    if (c * CH + t < rows)
-                        *reinterpret_cast<uint4*>(out + (long long)t * p.out_stride + piece * 8) = *reinterpret_cast<const uint4*>(y + t * 256 + ((piece ^ (t & 7)) << 4));
-                }
-                return true;
-            };
+            const int w = warp, t_lo = 16 * w + (lane >> 2);
+            const int row = 16 * w + 8 * ((lane >> 3) & 1) + (lane & 7);  // the matrix row that this lane names
+            unsigned char* pt = smem + oP + row * 128;
+            for (int j = w + 1; j < 4; ++j) {  // columns behind the warp's rows are all above the diagonal, in every chunk
+                unsigned char* at = pt + (((2 * j + (lane >> 4)) ^ (row & 7)) << 4);
+                tc::stmatrix_4(at, 0u, 0u, 0u, 0u);
+                tc::stmatrix_4(at + kBox, 0u, 0u, 0u, 0u);
+            }
             for (int c = 0; c < n; ++c) {
-                if (c > 0 && !outputs(c - 1)) goto done;
-                ok = ok && wait(bQK + (c & 1), c / 2, kStatusLinQK) && decay_wait(c);
-                if (!ok) continue;  // (the next vote ends it for all four warps)
+                if (!wait_with_decays(c, bQK, c, kStatusLinQK)) goto done;
                 tc::fence_after_sync();
                 const Decays& x = decays[c % kDecays];
-                unsigned char* pt = smem + oP + (c & 1) * 2 * kBox;
-                const int t_lo = 16 * w + (lane >> 2);
                 const float2 g_lo = x.g[t_lo], g_hi = x.g[t_lo + 8];
-                const int row = 16 * w + 8 * ((lane >> 3) & 1) + (lane & 7);  // the matrix row that this lane names
+                // (The products that read the last chunk's P were issued before this chunk's scores: they are through.)
+#pragma unroll 1
+                for (int j = 0; j <= w; ++j) {
+                    uint32_t r[8], hi[4], lo[4];
+                    tc::tmem_ld_frag(tc::tmem_addr(tm, w, cQK + 16 * j), r);
+                    tc::tmem_ld_wait();
 #pragma unroll
-                for (int s0 = 0; s0 < CH; s0 += 16) {
-                    uint32_t hi[4] = {0u, 0u, 0u, 0u}, lo[4] = {0u, 0u, 0u, 0u};
-                    if (s0 <= 16 * w) {  // (columns behind the warp's rows are all above the diagonal)
-                        uint32_t r[8];
-                        tc::tmem_ld_frag(tc::tmem_addr(tm, w, cQK + 64 * (c & 1) + s0), r);
-                        tc::tmem_ld_wait();
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {  // columns 8 (i / 2) + 2 (lane % 4) and the next, rows t_lo + 8 (i % 2)
-                            const int s = s0 + 8 * (i >> 1) + 2 * (lane & 3), t = t_lo + 8 * (i & 1);
-                            const float4 gs = *reinterpret_cast<const float4*>(&x.g[s]);
-                            const float2 gt = i & 1 ? g_hi : g_lo;
-                            const float2 d0 = sub2(gt, make_float2(gs.x, gs.y)), d1 = sub2(gt, make_float2(gs.z, gs.w));
-                            const float2 pv = mul2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), make_float2(ex2_ftz(d0.x + d0.y), ex2_ftz(d1.x + d1.y)));
-                            const float2 z = make_float2(s <= t ? pv.x : 0.0f, s + 1 <= t ? pv.y : 0.0f);
-                            hi[i] = tc::bf16x2(z.x, z.y);
-                            const float2 rest = lo_of(hi[i], z);
-                            lo[i] = tc::bf16x2(rest.x, rest.y);
-                        }
+                    for (int i = 0; i < 4; ++i) {  // columns 8 (i / 2) + 2 (lane % 4) and the next, rows t_lo + 8 (i % 2)
+                        const int s = 16 * j + 8 * (i >> 1) + 2 * (lane & 3), t = t_lo + 8 * (i & 1);
+                        const float4 gs = *reinterpret_cast<const float4*>(&x.g[s]);
+                        const float2 gt = i & 1 ? g_hi : g_lo;
+                        const float2 d0 = sub2(gt, make_float2(gs.x, gs.y)), d1 = sub2(gt, make_float2(gs.z, gs.w));
+                        const float2 pv = mul2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), make_float2(ex2_ftz(d0.x + d0.y), ex2_ftz(d1.x + d1.y)));
+                        const float2 z = mul2(make_float2(p.scale, p.scale), make_float2(s <= t ? pv.x : 0.0f, s + 1 <= t ? pv.y : 0.0f));
+                        hi[i] = tc::bf16x2(z.x, z.y);
+                        const float2 rest = lo_of(hi[i], z);
+                        lo[i] = tc::bf16x2(rest.x, rest.y);
                     }
-                    unsigned char* at = pt + row * 128 + (((s0 / 8 + (lane >> 4)) ^ (row & 7)) << 4);
+                    unsigned char* at = pt + (((2 * j + (lane >> 4)) ^ (row & 7)) << 4);
                     tc::stmatrix_4(at, hi[0], hi[1], hi[2], hi[3]);
                     tc::stmatrix_4(at + kBox, lo[0], lo[1], lo[2], lo[3]);
                 }
-                fence_proxy_async_smem();
                 tc::fence_before_sync();
-                arrive(bP + (c & 1));
+                fence_proxy_async_smem();
+                arrive(bPQ);
+                arrive(bDecayFree + c % kDecays);
             }
-            if (n > 0 && !outputs(n - 1)) goto done;
         }
-    } else if (warp < kPWarps + kVWarps) {
-        const int vt = tid - kPWarps * 32;
-        const bool three = !p.state_bf16;
-        for (int c = 0; c < n; ++c) {
-            if (!wait(bFull + c % kStages, c / kStages, kStatusLinFull) || !decay_wait(c)) goto done;
-            if (c > 0 && !wait(bU, c - 1, kStatusLinU)) goto done;
-            const Decays& x = decays[c % kDecays];
-            unsigned char *k = smem + (c % kStages) * kStage + kTile, *v = k + kTile, *wv = smem + oWV;
-            const int live = rows - c * CH;
+    } else if (warp < kQWarp) {
+        if (!STATE) {
+            const int w = warp - kOWarp, ot = tid - 32 * kOWarp, t8 = ot >> 4, piece = ot & 15;
+            unsigned char* y = smem + oY;
+            const unsigned char* from = y + t8 * 256 + ((piece ^ t8) << 4);  // rows t8 + 8 i
+            uint16_t* out = p.out + (long long)(row0 + t8) * p.out_stride + h * DV + piece * 8;
+            const long long step = 8 * p.out_stride;
+            for (int c = 0; c < n; ++c) {  // the accumulator's lanes are value channels, its columns rows
+                const bool ok = wait(bO + (c & 1), c / 2, kStatusLinO);
+                if (!named_bar_all(1, 128, ok)) goto done;  // (and the rows of the chunk before have left the staging)
+                tc::fence_after_sync();
 #pragma unroll 2
-            for (int i = 0; i < kTile / 16 / (kVWarps * 32); ++i) {
-                const int at = (i * kVWarps * 32 + vt) * 16, r = (at >> 7) & (CH - 1);
-                uint4 in = *reinterpret_cast<const uint4*>(v + at);
-                if (r >= live) {  // behind the sequence: another one's rows, or none
-                    in = make_uint4(0u, 0u, 0u, 0u);
-                    *reinterpret_cast<uint4*>(v + at) = in;
-                    *reinterpret_cast<uint4*>(k + at) = in;
-                }
-                const float w = x.w[r];
-                const uint32_t pair[4] = {in.x, in.y, in.z, in.w};
-                uint32_t part[3][4];
+                for (int i = 0; i < 8; ++i) {
+                    const int half = i >> 2, t0 = 16 * (i & 3);
+                    uint32_t r[8];
+                    tc::tmem_ld_frag(tc::tmem_addr(tm, w, cO + 64 * (c & 1) + t0) + ((uint32_t)(16 * half) << 16), r);
+                    tc::tmem_ld_wait();
+                    uint32_t z[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 z = mul2(make_float2(w, w), make_float2(__uint_as_float(pair[j] << 16), __uint_as_float(pair[j] & 0xffff0000u)));
-                    part[0][j] = tc::bf16x2(z.x, z.y);
-                    const float2 r1 = lo_of(part[0][j], z);
-                    part[1][j] = tc::bf16x2(r1.x, r1.y);
-                    const float2 r2 = lo_of(part[1][j], r1);
-                    part[2][j] = tc::bf16x2(r2.x, r2.y);
+                    for (int j = 0; j < 4; ++j) z[j] = tc::bf16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+                    const int t = t0 + 8 * (lane >> 4) + (lane & 7), to = 4 * w + 2 * half + ((lane >> 3) & 1);
+                    tc::stmatrix_t4(y + t * 256 + ((to ^ (t & 7)) << 4), z[0], z[1], z[2], z[3]);
                 }
-#pragma unroll
-                for (int j = 0; j < 3; ++j)
-                    if (j < 2 || three) *reinterpret_cast<uint4*>(wv + j * kTile + at) = make_uint4(part[j][0], part[j][1], part[j][2], part[j][3]);
+                tc::fence_before_sync();
+                arrive(bOFree + (c & 1));
+                named_bar_sync(2, 128);
+                const int live = rows - c * CH - t8;
+#pragma unroll 4
+                for (int i = 0; i < 8; ++i, out += step)
+                    if (8 * i < live) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(from + i * 2048);
             }
-            fence_proxy_async_smem();
-            arrive(bWV);
-            arrive(bDecayFree + c % kDecays);
         }
-    } else {  // the state: thread = value channel 32 (warp % 4) + lane, key channels 64 half ..
-        const int quad = warp & 3, half = (warp - kPWarps - kVWarps) >> 2, vc = 32 * quad + lane;
-        const int in_state = vc * DK + 64 * half;
-        float s[64];
-        const bool from_segments = !STATE && p.pass == 2;
-        float* mine = p.states + ((long long)chain * p.segments + seg) * (DK * DV) + in_state;
-        const long long off = p.state_off[b] + (long long)h * DK * DV + in_state;
-        if (STATE) {
-#pragma unroll
-            for (int i = 0; i < 64; ++i) s[i] = 0.0f;
-        } else if (from_segments || !p.state_bf16) {
-            const float* src = from_segments ? mine : static_cast<const float*>(p.state_in) + off;
-            if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float4 x = *reinterpret_cast<const float4*>(src + 4 * i);
-                    s[4 * i] = x.x, s[4 * i + 1] = x.y, s[4 * i + 2] = x.z, s[4 * i + 3] = x.w;
+    } else if (warp < kVWarp) {
+        if (!STATE) {
+            // Chunk c's q, times scale e^G, as f32; a thread takes a piece of eight channels of every sixteenth row.
+            const int qt = tid - 32 * kQWarp, r0 = qt >> 3, sw = r0 & 7, piece = (qt & 7) ^ sw;
+            unsigned char* to = smem + oQ + (piece >> 2) * kBox + r0 * 128;
+            const int to0 = ((2 * (piece & 3)) ^ sw) << 4, to1 = ((2 * (piece & 3) + 1) ^ sw) << 4;
+            for (int c = 0; c < n; ++c) {
+                if (!wait_with_decays(c, bFull + c % kStages, c / kStages, kStatusLinFull)) goto done;
+                if (c > 0 && !wait(bQS, c - 1, kStatusLinQK)) goto done;
+                const Decays& x = decays[c % kDecays];
+                const unsigned char* q = smem + (c % kStages) * kStage + qt * 16;
+#pragma unroll 4
+                for (int i = 0; i < 8; ++i) {
+                    const uint4 in = *reinterpret_cast<const uint4*>(q + i * 2048);
+                    const float f = x.e[16 * (i & 3) + r0];
+                    const float2 e = make_float2(f, f);
+                    unsigned char* at = to + 2 * (i >> 2) * kBox + (i & 3) * 2048;
+                    const float2 a0 = mul2(e, make_float2(__uint_as_float(in.x << 16), __uint_as_float(in.x & 0xffff0000u)));
+                    const float2 a1 = mul2(e, make_float2(__uint_as_float(in.y << 16), __uint_as_float(in.y & 0xffff0000u)));
+                    const float2 a2 = mul2(e, make_float2(__uint_as_float(in.z << 16), __uint_as_float(in.z & 0xffff0000u)));
+                    const float2 a3 = mul2(e, make_float2(__uint_as_float(in.w << 16), __uint_as_float(in.w & 0xffff0000u)));
+                    *reinterpret_cast<float4*>(at + to0) = make_float4(a0.x, a0.y, a1.x, a1.y);
+                    *reinterpret_cast<float4*>(at + to1) = make_float4(a2.x, a2.y, a3.x, a3.y);
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 64; ++i) s[i] = src[i];
+                fence_proxy_async_smem();
+                arrive(bPQ);
+                arrive(bDecayFree + c % kDecays);
             }
-        } else {
-            const uint16_t* src = static_cast<const uint16_t*>(p.state_in) + off;
-            if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+        }
+    } else if (warp < kSWarp) {
+        const int w = warp & 3, half = (warp - kVWarp) >> 2, vt = tid - 32 * kVWarp;
+        const int parts = p.state_bf16 ? 2 : 3;
+        for (int c = 0; c < n; ++c) {
+            if (!wait_with_decays(c, bFull + c % kStages, c / kStages, kStatusLinFull)) goto done;
+            const Decays& x = decays[c % kDecays];
+            unsigned char *k = smem + (c % kStages) * kStage + kTile, *v = k + kTile;
+            const int live = rows - c * CH;
+            if (live < CH) {  // behind the sequence: another one's rows, or none
+                for (int at = vt * 16; at < kTile; at += 256 * 16)
+                    if (((at >> 7) & (CH - 1)) >= live) *reinterpret_cast<uint4*>(k + at) = *reinterpret_cast<uint4*>(v + at) = make_uint4(0u, 0u, 0u, 0u);
+                fence_proxy_async_smem();
+            }
+            if (c > 1 && !wait(bU + (c & 1), c / 2 - 1, kStatusLinU)) goto done;  // the products with these columns' last parts are through
+            tc::fence_after_sync();
+#pragma unroll 1
+            for (int sh = 0; sh < 2; ++sh) {
+                uint32_t at = tc::tmem_addr(tm, w, cWV + 96 * (c & 1) + 16 * sh) + ((uint32_t)(16 * half) << 16), raw[8], part[8];
+                float2 z[8];
+                // V^T, value channels 32 w + 16 half + lane / 4 (+ 8): raw[2 i + 0 / 1] rows 32 sh + 8 i + 2 (lane % 4) and the next.
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int r = 32 * sh + 16 * i + 8 * (lane >> 4) + (lane & 7), piece = 4 * w + 2 * half + ((lane >> 3) & 1);
+                    tc::ldmatrix_t4(v + (piece >> 3) * kBox + r * 128 + (((piece & 7) ^ (r & 7)) << 4), raw[4 * i], raw[4 * i + 1], raw[4 * i + 2], raw[4 * i + 3]);
+                }
+                if (live < CH) {  // (whether or not the warp that clears these rows has been there)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = 32 * sh + 8 * i + 2 * (lane & 3);
+                        const uint32_t mask = (r < live ? 0xffffu : 0u) | (r + 1 < live ? 0xffff0000u : 0u);
+                        raw[2 * i] &= mask, raw[2 * i + 1] &= mask;
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(src + 8 * i);
-                    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) s[8 * i + 2 * j] = __uint_as_float(u[j] << 16), s[8 * i + 2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+                    const float2 f = *reinterpret_cast<const float2*>(&x.w[32 * sh + 8 * (i >> 1) + 2 * (lane & 3)]);
+                    z[i] = mul2(f, make_float2(__uint_as_float(raw[i] << 16), __uint_as_float(raw[i] & 0xffff0000u)));
                 }
-            } else {
+#pragma unroll 1
+                for (int j = 0; j < parts; ++j, at += 32) {
 #pragma unroll
-                for (int i = 0; i < 64; ++i) s[i] = bf16_bits_to_f32(src[i]);
-            }
-        }
-        auto give = [&]() {  // the state as an operand
-#pragma unroll
-            for (int i = 0; i < 64; i += 32) {
-                uint32_t hi[16], lo[16];
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const float2 z = make_float2(s[i + 2 * j], s[i + 2 * j + 1]);
-                    hi[j] = tc::bf16x2(z.x, z.y);
-                    const float2 rest = lo_of(hi[j], z);
-                    lo[j] = tc::bf16x2(rest.x, rest.y);
+                    for (int i = 0; i < 8; ++i) {
+                        part[i] = tc::bf16x2(z[i].x, z[i].y);
+                        z[i] = lo_of(part[i], z[i]);
+                    }
+                    tc::tmem_st_pairs(at, part);
                 }
-                tc::tmem_st16(tc::tmem_addr(tm, quad, cSHi + 32 * half + i / 2), hi);
-                tc::tmem_st16(tc::tmem_addr(tm, quad, cSLo + 32 * half + i / 2), lo);
             }
             tc::tmem_st_wait();
             tc::fence_before_sync();
-            arrive(bS);
-        };
-        if (!STATE && n > 0) give();
-        for (int c = 0; c < n; ++c) {
-            if (!decay_wait(c) || !wait(bU, c, kStatusLinU)) goto done;
-            tc::fence_after_sync();
-            const float all = decays[c % kDecays].all;
-#pragma unroll
-            for (int i = 0; i < 64; i += 16) {
-                uint32_t r[16];
-                tc::tmem_ld16(tc::tmem_addr(tm, quad, cU + 64 * half + i), r);
-                tc::tmem_ld_wait();
-#pragma unroll
-                for (int j = 0; j < 16; j += 2) {
-                    const float2 z = fma2(make_float2(all, all), make_float2(s[i + j], s[i + j + 1]), make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])));
-                    s[i + j] = z.x, s[i + j + 1] = z.y;
-                }
-            }
-            tc::fence_before_sync();
-            arrive(bUFree);
+            arrive(bAdd + (c & 1));
             arrive(bDecayFree + c % kDecays);
-            if (!STATE && c + 1 < n) {
-                if (!wait(bO, c, kStatusLinO)) goto done;  // the chunk's products have read the state before it
-                tc::fence_after_sync();
-                give();
-            }
-            if (warp == kPWarps + kVWarps && lane == 0) ctl[0] = ctl[0] + 1u;
         }
-        if (STATE) {
+    } else if (warp < kCopyWarp) {  // the state: thread = value channel 32 (warp % 4) + lane, key channels 64 half ..
+        const int quad = warp & 3, half = (warp - kSWarp) >> 2;
+        const uint32_t at = tc::tmem_addr(tm, quad, cS + 64 * half);
+        const int in_state = (32 * quad + lane) * DK + 64 * half;
+        const bool from_segments = !STATE && p.pass == 2;
+        float* mine = p.states + ((long long)chain * p.segments + seg) * (DK * DV) + in_state;
+        const long long off = p.state_off[b] + (long long)h * DK * DV + in_state;
+        const float* src32 = from_segments ? mine : static_cast<const float*>(p.state_in) + off;
+        const uint16_t* src16 = static_cast<const uint16_t*>(p.state_in) + off;
+        const bool wide = from_segments || !p.state_bf16, vec = ((wide ? reinterpret_cast<uintptr_t>(src32) : reinterpret_cast<uintptr_t>(src16)) & 15) == 0;
+#pragma unroll 1
+        for (int i = 0; i < 64; i += 16) {  // from memory
+            uint32_t x[16];
+            if (STATE) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) *reinterpret_cast<float4*>(mine + 4 * i) = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
-        } else if (last_seg && (n > 0 || seg == 0)) {
-            if (!p.state_bf16) {
-                float* dst = static_cast<float*>(p.state_out) + off;
-                if ((reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+                for (int j = 0; j < 16; ++j) x[j] = 0u;
+            } else if (vec && wide) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) *reinterpret_cast<float4*>(dst + 4 * i) = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
-                } else {
+                for (int j = 0; j < 4; ++j) {
+                    const uint4 y = *reinterpret_cast<const uint4*>(src32 + i + 4 * j);
+                    x[4 * j] = y.x, x[4 * j + 1] = y.y, x[4 * j + 2] = y.z, x[4 * j + 3] = y.w;
+                }
+            } else if (vec) {
 #pragma unroll
-                    for (int i = 0; i < 64; ++i) dst[i] = s[i];
+                for (int j = 0; j < 2; ++j) {
+                    const uint4 y = *reinterpret_cast<const uint4*>(src16 + i + 8 * j);
+                    const uint32_t u[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[8 * j + 2 * e] = u[e] << 16, x[8 * j + 2 * e + 1] = u[e] & 0xffff0000u;
                 }
             } else {
-                uint16_t* dst = static_cast<uint16_t*>(p.state_out) + off;
-                if ((reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        *reinterpret_cast<uint4*>(dst + 8 * i) = make_uint4(tc::bf16x2(s[8 * i], s[8 * i + 1]), tc::bf16x2(s[8 * i + 2], s[8 * i + 3]),
-                                                                           tc::bf16x2(s[8 * i + 4], s[8 * i + 5]), tc::bf16x2(s[8 * i + 6], s[8 * i + 7]));
+                for (int j = 0; j < 16; ++j) x[j] = wide ? __float_as_uint(src32[i + j]) : (uint32_t)src16[i + j] << 16;
+            }
+            tc::tmem_st16(at + i, x);
+        }
+        if (!STATE) {
+            tc::tmem_st_wait();
+            tc::fence_before_sync();
+            arrive(bState);
+        }
+        for (int c = 0; c < n; ++c) {
+            // The chunk's outputs have read the state (and the chunk before has been added).
+            if (STATE && c == 0 ? !wait(bDecay, 0, kStatusLinDecay)
+                                : !wait_with_decays(c, STATE ? bU + ((c - 1) & 1) : bQS, STATE ? (c - 1) / 2 : c, STATE ? kStatusLinU : kStatusLinS)) goto done;
+            const float all = decays[c % kDecays].all;
+            arrive(bDecayFree + c % kDecays);
+            tc::fence_after_sync();
+            if (!STATE || c > 0)
+#pragma unroll 1
+                for (int i = 0; i < 64; i += 32) {
+                    uint32_t x[32];
+                    tc::tmem_ld32(at + i, x);
+                    tc::tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        const float2 z = mul2(make_float2(all, all), make_float2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])));
+                        x[j] = __float_as_uint(z.x), x[j + 1] = __float_as_uint(z.y);
+                    }
+                    tc::tmem_st32(at + i, x);
+                }
+            tc::tmem_st_wait();
+            tc::fence_before_sync();
+            arrive(bAdd + (c & 1));
+            if (warp == kSWarp && lane == 0) ctl[0] = ctl[0] + 1u;
+        }
+        if (n > 0 && !wait(bU + ((n - 1) & 1), (n - 1) / 2, kStatusLinU)) goto done;  // (nobody leaves before the last product)
+        tc::fence_after_sync();
+        if (STATE || (last_seg && (n > 0 || seg == 0))) {
+            float* dst32 = STATE ? mine : static_cast<float*>(p.state_out) + off;
+            uint16_t* dst16 = static_cast<uint16_t*>(p.state_out) + off;
+            const bool wide_out = STATE || !p.state_bf16, vec_out = ((wide_out ? reinterpret_cast<uintptr_t>(dst32) : reinterpret_cast<uintptr_t>(dst16)) & 15) == 0;
+#pragma unroll 1
+            for (int i = 0; i < 64; i += 16) {
+                uint32_t x[16];
+                tc::tmem_ld16(at + i, x);
+                tc::tmem_ld_wait();
+                if (wide_out && vec_out) {
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) *reinterpret_cast<uint4*>(dst32 + i + j) = make_uint4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+                } else if (wide_out) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) dst32[i + j] = __uint_as_float(x[j]);
                 } else {
+                    uint32_t y[8];
 #pragma unroll
-                    for (int i = 0; i < 64; ++i) dst[i] = f32_to_bf16_bits(s[i]);
+                    for (int j = 0; j < 8; ++j) y[j] = tc::bf16x2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1]));
+                    if (vec_out) {
+                        *reinterpret_cast<uint4*>(dst16 + i) = make_uint4(y[0], y[1], y[2], y[3]);
+                        *reinterpret_cast<uint4*>(dst16 + i + 8) = make_uint4(y[4], y[5], y[6], y[7]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) dst16[i + j] = (uint16_t)(y[j >> 1] >> (16 * (j & 1)));
+                    }
                 }
             }
         }

@@ -94,6 +94,19 @@ __device__ __forceinline__ void mma_bf16_ts_if(uint32_t leader, uint32_t d_tmem,
         "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"((uint32_t)accumulate), "r"(leader)
         : "memory");
 }
+// The same on f32 operands of which the tensor core takes 11 bits (kind::tf32): 8 k an instruction, 8 columns of A in tensor memory.
+__device__ __forceinline__ constexpr uint32_t idesc_tf32(int M, int N) { return (1u << 4) | (2u << 7) | (2u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
+// Operand tile of R rows in boxes of 32 f32 along K, in the 128-byte swizzle.
+__device__ __forceinline__ uint64_t desc_sw128_kmajor_f32(const unsigned char* tile, int R, int k0) {
+    return smem_desc(tile + (size_t)(k0 / 32) * R * 128 + (k0 % 32) * 4, 16, 1024) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void mma_tf32_ts_if(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"((uint32_t)accumulate), "r"(leader)
+        : "memory");
+}
 __device__ __forceinline__ void mma_commit_if(uint32_t leader, uint64_t* bar) {
     asm volatile(
         "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
@@ -132,6 +145,13 @@ __device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[8]) {
 }
 __device__ __forceinline__ void tmem_st_frag(uint32_t taddr, const uint32_t (&r)[8]) {
     asm volatile("tcgen05.st.sync.aligned.16x256b.x2.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+                 "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+// 16 lanes x 16 columns, four columns at a time in the same manner: thread l holds column 4 i + l % 4 of lane l / 4 in r[2 i] and of lane l / 4 + 8 in
+// r[2 i + 1] -- of packed pairs of bf16, the fragments of 8 x 8 matrices.
+__device__ __forceinline__ void tmem_st_pairs(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
                  "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                  : "memory");
 }

@@ -63,7 +63,8 @@ def chunked(lens, q, k, v, g, state, scale, bf16_state):
     """The same, with the bounds of the chunked form.  M, the recurrence of the magnitudes, is what every rounding is relative to: products of
     bf16 are exact; a chunk's sums of up to 64 terms (and the scores' of 128) in the tensor core's f32 lose at most four half steps a term; a factor's
     exponential and the sums of log decays eight; a chunk that passes over an older one's sums six.  w V is exact to f32 in three parts (24 bits), to 2^-16
-    in two; S and P as operands are, both, exact to 2^-16 (two roundings of bf16: 2^-8 of 2^-8)."""
+    in two; P as an operand is exact to 2^-16 (two roundings of bf16: 2^-8 of 2^-8); of S and of the scaled q the tensor core takes 11 bits, cut off: 2^-10 of what
+    came into the chunk from before it, each."""
     rows, heads, d = v.shape
     share = heads // q.shape[1]
     q, k = (t.double().repeat_interleave(share, 1) for t in (q, k))
@@ -77,10 +78,13 @@ def chunked(lens, q, k, v, g, state, scale, bf16_state):
         part = (4 * 64 + 8 + 6 * ((n + 63) // 64)) * U32 + (UBF * UBF if bf16_state else 4 * U32)
         for t in range(first, first + n):
             decay = torch.exp(g[t])[:, None, None]
+            if (t - first) % 64 == 0:
+                before = m
+            before = decay * before
             s = decay * s + v[t][:, :, None] * k[t][:, None, :]
             m = decay * m + (v[t][:, :, None] * k[t][:, None, :]).abs()
             y[t] = scale * (s * q[t][:, None, :]).sum(-1)
-            at = abs(scale) * (m * q[t][:, None, :].abs()).sum(-1) * (part + 2 * UBF * UBF + (4 * 128 + 4 * 64 + 16) * U32)
+            at = abs(scale) * ((m * (part + UBF * UBF + (4 * 128 + 4 * 64 + 16) * U32) + before * 2.0 ** -9) * q[t][:, None, :].abs()).sum(-1)
             yb[t] = at + (UBF + U32) * (y[t].abs() + at) + 1e-38
         e = part * m
         ends.append(s)
