@@ -20,7 +20,8 @@
 //   warps 8-11   scale e^G Q as f32
 //   warps 12-19  the parts of w V^T into tensor memory; the rows of a last, short chunk to zero (what lies there may be NaN)
 //   warps 20-27  the state, which is an operand of one product and the accumulator of the other: times e^G between the two
-//   warp 28      tensor copies of q, k, v, three chunks ahead     warp 29  the products       warp 30  sums and factors of the decays
+//   warp 28      tensor copies of q, k, v, three chunks ahead     warp 31  sums and factors of the decays
+//   warp 29      the products with the state and to it            warp 30  the scores and their products with V
 // A chunk's products take 1,920 cycles of the tensor pipe; what the other roles issue for it is the tighter bound, so their bodies are loops, their waits
 // sleep, and operands take the form that costs the fewest instructions.
 //
@@ -45,8 +46,8 @@ constexpr int kTile = CH * DK * 2;                      // q, k or v of a chunk:
 constexpr int kBox = CH * 128;
 constexpr int kStages = 3, kStage = 3 * kTile;
 constexpr int oQ = kStages * kStage;                    // scale e^G Q, f32: four boxes of 64 rows x 32 channels
-constexpr int oP = oQ + 2 * kTile;                      // P: hi | lo
-constexpr int oY = oP + 2 * kBox;                       // a chunk's outputs on their way out
+constexpr int oP = oQ + 2 * kTile;                      // P: hi | lo, two buffers
+constexpr int oY = oP + 4 * kBox;                       // half a chunk's outputs on their way out
 constexpr int kDecays = 4;                              // chunks of decay factors in flight
 struct Decays {
     float2 g[CH];     // G in powers of two: hi, lo
@@ -54,17 +55,17 @@ struct Decays {
     float w[CH];
     float all, pad[3];  // e^G of the whole chunk
 };
-constexpr int oDecays = oY + kTile;
+constexpr int oDecays = oY + kTile / 2;
 constexpr int oBars = oDecays + kDecays * (int)sizeof(Decays);
 enum : int {
-    bFull = 0, bEmpty = bFull + kStages, bQK = bEmpty + kStages, bPQ, bQS, bState, bAdd, bU = bAdd + 2, bO = bU + 2, bOFree = bO + 2, bDecay = bOFree + 2,
+    bFull = 0, bEmpty = bFull + kStages, bQK = bEmpty + kStages, bP, bQ, bState, bQS, bAdd = bQS + 2, bU = bAdd + 2, bO = bU + 2, bOFree = bO + 2, bDecay = bOFree + 2,
     bDecayFree = bDecay + kDecays, kBars = bDecayFree + kDecays
 };
 constexpr int oCtl = oBars + (kBars + 1) / 2 * 16;
 constexpr int kSmem = oCtl + 16 + 1024;
 static_assert(kSmem <= 232448 && sizeof(Decays) % 16 == 0, "shared memory");
 
-constexpr int kOWarp = 4, kQWarp = 8, kVWarp = 12, kSWarp = 20, kCopyWarp = 28, kMmaWarp = 29, kDecayWarp = 30, kThreads = 31 * 32;
+constexpr int kOWarp = 4, kQWarp = 8, kVWarp = 12, kSWarp = 20, kCopyWarp = 28, kStateMmaWarp = 29, kScoreMmaWarp = 30, kDecayWarp = 31, kThreads = 32 * 32;
 // Tensor memory columns: the state, the scores, two accumulators of outputs and two sets of w V^T in turn.
 constexpr int cS = 0, cQK = 128, cO = 192, cWV = 320, kCols = 512;
 
@@ -96,6 +97,14 @@ __device__ __forceinline__ float2 lo_of(uint32_t hi, float2 x) {  // what a pair
     return sub2(x, make_float2(__uint_as_float(hi << 16), __uint_as_float(hi & 0xffff0000u)));
 }
 
+// Shared-memory descriptors in the 128-byte swizzle (8-row groups 1,024 bytes apart): the low word from an address and the leading byte offset, which the
+// products step through by adding to it.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t address, uint32_t leading) { return address >> 4 | leading >> 4 << 16; }
+__device__ __forceinline__ uint64_t desc(uint32_t lo) {
+    constexpr uint32_t hi = 1024 >> 4 | 1u << 14 | 2u << 29;
+    return (uint64_t)hi << 32 | lo;
+}
+
 // STATE: the pass that only sums up states.
 template <bool STATE>
 __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_constant__ PrefillParams p) {
@@ -107,18 +116,18 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
     uint32_t* tmem_slot = const_cast<uint32_t*>(ctl) + 2;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        for (int i = 0; i < kStages; ++i) mbar_init(&bar[bFull + i], 1), mbar_init(&bar[bEmpty + i], 1);
+        for (int i = 0; i < kStages; ++i) mbar_init(&bar[bFull + i], 1), mbar_init(&bar[bEmpty + i], STATE ? 1 : 2);
         mbar_init(&bar[bQK], 1);
-        mbar_init(&bar[bPQ], 8);
-        mbar_init(&bar[bQS], 1);
+        mbar_init(&bar[bP], 4);
+        mbar_init(&bar[bQ], 4);
         mbar_init(&bar[bState], 8);
-        for (int i = 0; i < 2; ++i) mbar_init(&bar[bAdd + i], 16), mbar_init(&bar[bU + i], 1), mbar_init(&bar[bO + i], 1), mbar_init(&bar[bOFree + i], 4);
+        for (int i = 0; i < 2; ++i) mbar_init(&bar[bQS + i], 1), mbar_init(&bar[bAdd + i], 16), mbar_init(&bar[bU + i], 1), mbar_init(&bar[bO + i], 1), mbar_init(&bar[bOFree + i], 4);
         for (int i = 0; i < kDecays; ++i) mbar_init(&bar[bDecay + i], 1), mbar_init(&bar[bDecayFree + i], STATE ? 16 : 24);
         ctl[0] = 0u;
         ctl[1] = 0u;
         mbar_init_fence();
     }
-    if (warp == kMmaWarp) tc::tmem_alloc(tmem_slot, kCols);
+    if (warp == kStateMmaWarp) tc::tmem_alloc(tmem_slot, kCols);
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
@@ -143,7 +152,7 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
     auto wait = [&](int i, uint32_t parity, int code) {
         return tc::warp_all(mbar_try_wait_hint(&bar[i], parity & 1u, 200000u) || mbar_wait(&bar[i], parity & 1u, ctx, code));
     };
-    auto wait_with_decays = [&](int c, int i, uint32_t parity, int code) { return wait(i, parity, code) && wait(bDecay + c % kDecays, c / kDecays, kStatusLinDecay); };
+    auto wait_with_decays = [&](int c, int i, uint32_t parity, int code) { return wait(bDecay + c % kDecays, c / kDecays, kStatusLinDecay) && wait(i, parity, code); };
 
     if (idle) goto done;
     if (warp == kCopyWarp) {
@@ -161,63 +170,75 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
                 }
             }
         }
-    } else if (warp == kMmaWarp) {
-        constexpr uint32_t id_qk = tc::idesc_bf16(64, 64, 0, 0, 0), id_u = tc::idesc_bf16(128, 128, 0, 1, 0), id_s = tc::idesc_tf32(128, 64), id_pv = tc::idesc_bf16(128, 64, 1, 0, 0);
+    } else if (warp == kStateMmaWarp) {
+        constexpr uint32_t id_u = tc::idesc_bf16(128, 128, 0, 1, 0), id_s = tc::idesc_tf32(128, 64);
         const uint32_t leader = tc::elect_one();
         const int parts = p.state_bf16 ? 2 : 3;
         // As values that the compiler knows to be the same in all lanes: loops over them stay converged and the products' operands in uniform
         // registers.
         const int n_all = (int)__reduce_max_sync(0xffffffffu, (unsigned)n);
-        const uint32_t tm_all = __reduce_max_sync(0xffffffffu, tm);
-        auto scores = [&](int c) {
-            const unsigned char *q = smem + (c % kStages) * kStage, *k = q + kTile;
-#pragma unroll
-            for (int i = 0; i < DK / 16; ++i)
-                tc::mma_bf16_if(leader, tm_all + cQK, tc::desc_sw128_kmajor(q, CH, 16 * i), tc::desc_sw128_kmajor(k, CH, 16 * i), id_qk, i > 0);
-            tc::mma_commit_if(leader, &bar[bQK]);
-        };
-        if (!STATE && n_all > 0) {
-            if (!wait(bFull, 0, kStatusLinFull)) goto done;
-            tc::fence_after_sync();
-            scores(0);
-        }
+        const uint32_t tm_all = __reduce_max_sync(0xffffffffu, tm), base = __reduce_max_sync(0xffffffffu, smem_u32(smem));
+        uint32_t stage = 0, phase = 0;
         for (int c = 0; c < n_all; ++c) {
-            const unsigned char *k = smem + (c % kStages) * kStage + kTile, *v = k + kTile;
-            if (STATE && !wait(bFull + c % kStages, c / kStages, kStatusLinFull)) goto done;
+            if (STATE && !wait(bFull + stage, phase, kStatusLinFull)) goto done;
             if (!STATE) {
                 const uint32_t o = tm_all + cO + 64 * (c & 1);
                 // (The state is there when its product with the chunk before has been waited for: one product's result as another's operand is not
                 // in the order of their issue.)
-                if (!wait(bPQ, c, kStatusLinP) || !wait(bOFree + (c & 1), c / 2 + 1, kStatusLinFree) ||
+                if (!wait(bOFree + (c & 1), c / 2 + 1, kStatusLinFree) || !wait(bQ, c, kStatusLinQK) ||
                     !(c > 0 ? wait(bU + ((c - 1) & 1), (c - 1) / 2, kStatusLinU) : wait(bState, 0, kStatusLinS)))
                     goto done;
                 tc::fence_after_sync();
+                const uint32_t q32 = desc_lo(base + oQ, 16);
 #pragma unroll
-                for (int i = 0; i < DK / 8; ++i) tc::mma_tf32_ts_if(leader, o, tm_all + cS + 8 * i, tc::desc_sw128_kmajor_f32(smem + oQ, CH, 8 * i), id_s, i > 0);
-                tc::mma_commit_if(leader, &bar[bQS]);
-                const unsigned char* pt = smem + oP;
-#pragma unroll 1
-                for (int part = 0; part < 2; ++part)
-#pragma unroll
-                    for (int i = 0; i < CH / 16; ++i)
-                        tc::mma_bf16_if(leader, o, tc::desc_sw128_mnmajor(v, CH, 16 * i), tc::desc_sw128_kmajor(pt + part * kBox, CH, 16 * i), id_pv, true);
-                tc::mma_commit_if(leader, &bar[bO + (c & 1)]);
-                if (c + 1 < n_all) {  // (P of this chunk has been read out of the scores' columns)
-                    if (!wait(bFull + (c + 1) % kStages, (c + 1) / kStages, kStatusLinFull)) goto done;
-                    tc::fence_after_sync();
-                    scores(c + 1);
-                }
+                for (int i = 0; i < DK / 8; ++i) tc::mma_tf32_ts_if(leader, o, tm_all + cS + 8 * i, desc(q32 + (i / 4) * (kBox >> 4) + 2 * (i % 4)), id_s, i > 0);
+                tc::mma_commit_if(leader, &bar[bQS + (c & 1)]);  // (two in turn: their waiters may be a chunk apart)
             }
             if (!wait(bAdd + (c & 1), c / 2, kStatusLinWV)) goto done;
             tc::fence_after_sync();
+            const uint32_t k = desc_lo(base + stage * kStage + kTile, kBox), wv = tm_all + cWV + 96 * (c & 1);
 #pragma unroll 1
             for (int part = 0; part < parts; ++part)
 #pragma unroll
-                for (int i = 0; i < CH / 16; ++i)
-                    tc::mma_bf16_ts_if(leader, tm_all + cS, tm_all + cWV + 96 * (c & 1) + 32 * part + 8 * i, tc::desc_sw128_mnmajor(k, CH, 16 * i), id_u, true);
-            tc::mma_commit_if(leader, &bar[bEmpty + c % kStages]);
+                for (int i = 0; i < CH / 16; ++i) tc::mma_bf16_ts_if(leader, tm_all + cS, wv + 32 * part + 8 * i, desc(k + 128 * i), id_u, true);
+            tc::mma_commit_if(leader, &bar[bEmpty + stage]);
             tc::mma_commit_if(leader, &bar[bU + (c & 1)]);  // (the last one: whoever has seen it has seen the others)
+            if (++stage == kStages) stage = 0, phase ^= 1u;
             if (leader) ctl[0] = ctl[0] + 1u;
+        }
+    } else if (warp == kScoreMmaWarp) {
+        constexpr uint32_t id_qk = tc::idesc_bf16(64, 64, 0, 0, 0), id_pv = tc::idesc_bf16(128, 64, 1, 0, 0);
+        const uint32_t leader = tc::elect_one();
+        const int n_all = STATE ? 0 : (int)__reduce_max_sync(0xffffffffu, (unsigned)n);
+        const uint32_t tm_all = __reduce_max_sync(0xffffffffu, tm), base = __reduce_max_sync(0xffffffffu, smem_u32(smem));
+        uint32_t stage = 0, phase = 0, before = 0;  // of the scores; of the products with V, a chunk behind
+        for (int c = 0; c <= n_all && n_all > 0; ++c) {
+            if (c > 0 && !wait(bP, c - 1, kStatusLinP)) goto done;  // the scores have been read, and P is there
+            if (c < n_all) {
+                if (!wait(bFull + stage, phase, kStatusLinFull)) goto done;
+                tc::fence_after_sync();
+                const uint32_t q = desc_lo(base + stage * kStage, 16), k = q + (kTile >> 4);
+#pragma unroll
+                for (int i = 0; i < DK / 16; ++i) {
+                    const uint32_t at = (i / 4) * (kBox >> 4) + 2 * (i % 4);
+                    tc::mma_bf16_if(leader, tm_all + cQK, desc(q + at), desc(k + at), id_qk, i > 0);
+                }
+                tc::mma_commit_if(leader, &bar[bQK]);
+            }
+            if (c > 0) {
+                if (!wait(bQS + ((c - 1) & 1), (c - 1) / 2, kStatusLinS)) goto done;  // which began the accumulator
+                tc::fence_after_sync();
+                const uint32_t v = desc_lo(base + before * kStage + 2 * kTile, kBox), o = tm_all + cO + 64 * ((c - 1) & 1);
+                uint32_t pt = desc_lo(base + oP + ((c - 1) & 1) * 2 * kBox, 16);
+#pragma unroll 1
+                for (int part = 0; part < 2; ++part, pt += kBox >> 4)
+#pragma unroll
+                    for (int i = 0; i < CH / 16; ++i) tc::mma_bf16_if(leader, o, desc(v + 128 * i), desc(pt + 2 * i), id_pv, true);
+                tc::mma_commit_if(leader, &bar[bEmpty + before]);
+                tc::mma_commit_if(leader, &bar[bO + ((c - 1) & 1)]);
+                before = before + 1 == kStages ? 0 : before + 1;
+            }
+            if (++stage == kStages) stage = 0, phase ^= 1u;
         }
     } else if (warp == kDecayWarp) {
         const float* g = p.g + (long long)row0 * p.g_stride + h;
@@ -265,16 +286,15 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
             unsigned char* pt = smem + oP + row * 128;
             for (int j = w + 1; j < 4; ++j) {  // columns behind the warp's rows are all above the diagonal, in every chunk
                 unsigned char* at = pt + (((2 * j + (lane >> 4)) ^ (row & 7)) << 4);
-                tc::stmatrix_4(at, 0u, 0u, 0u, 0u);
-                tc::stmatrix_4(at + kBox, 0u, 0u, 0u, 0u);
+                for (int i = 0; i < 4; ++i) tc::stmatrix_4(at + i * kBox, 0u, 0u, 0u, 0u);
             }
             for (int c = 0; c < n; ++c) {
                 if (!wait_with_decays(c, bQK, c, kStatusLinQK)) goto done;
                 tc::fence_after_sync();
                 const Decays& x = decays[c % kDecays];
                 const float2 g_lo = x.g[t_lo], g_hi = x.g[t_lo + 8];
-                // (The products that read the last chunk's P were issued before this chunk's scores: they are through.)
-#pragma unroll 1
+                unsigned char* mine = pt + (c & 1) * 2 * kBox;  // (the products that read this buffer last were issued before this chunk's scores: they are through)
+#pragma unroll 2
                 for (int j = 0; j <= w; ++j) {
                     uint32_t r[8], hi[4], lo[4];
                     tc::tmem_ld_frag(tc::tmem_addr(tm, w, cQK + 16 * j), r);
@@ -291,13 +311,13 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
                         const float2 rest = lo_of(hi[i], z);
                         lo[i] = tc::bf16x2(rest.x, rest.y);
                     }
-                    unsigned char* at = pt + (((2 * j + (lane >> 4)) ^ (row & 7)) << 4);
+                    unsigned char* at = mine + (((2 * j + (lane >> 4)) ^ (row & 7)) << 4);
                     tc::stmatrix_4(at, hi[0], hi[1], hi[2], hi[3]);
                     tc::stmatrix_4(at + kBox, lo[0], lo[1], lo[2], lo[3]);
                 }
                 tc::fence_before_sync();
                 fence_proxy_async_smem();
-                arrive(bPQ);
+                arrive(bP);
                 arrive(bDecayFree + c % kDecays);
             }
         }
@@ -309,28 +329,33 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
             uint16_t* out = p.out + (long long)(row0 + t8) * p.out_stride + h * DV + piece * 8;
             const long long step = 8 * p.out_stride;
             for (int c = 0; c < n; ++c) {  // the accumulator's lanes are value channels, its columns rows
-                const bool ok = wait(bO + (c & 1), c / 2, kStatusLinO);
-                if (!named_bar_all(1, 128, ok)) goto done;  // (and the rows of the chunk before have left the staging)
+                bool ok = wait(bO + (c & 1), c / 2, kStatusLinO);
                 tc::fence_after_sync();
+#pragma unroll 1
+                for (int rows32 = 0; rows32 < CH; rows32 += 32) {
+                    if (!named_bar_all(1, 128, ok)) goto done;  // (and the rows before have left the staging)
 #pragma unroll 2
-                for (int i = 0; i < 8; ++i) {
-                    const int half = i >> 2, t0 = 16 * (i & 3);
-                    uint32_t r[8];
-                    tc::tmem_ld_frag(tc::tmem_addr(tm, w, cO + 64 * (c & 1) + t0) + ((uint32_t)(16 * half) << 16), r);
-                    tc::tmem_ld_wait();
-                    uint32_t z[4];
+                    for (int i = 0; i < 4; ++i) {
+                        const int half = i >> 1, t0 = 16 * (i & 1);
+                        uint32_t r[8];
+                        tc::tmem_ld_frag(tc::tmem_addr(tm, w, cO + 64 * (c & 1) + rows32 + t0) + ((uint32_t)(16 * half) << 16), r);
+                        tc::tmem_ld_wait();
+                        uint32_t z[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) z[j] = tc::bf16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
-                    const int t = t0 + 8 * (lane >> 4) + (lane & 7), to = 4 * w + 2 * half + ((lane >> 3) & 1);
-                    tc::stmatrix_t4(y + t * 256 + ((to ^ (t & 7)) << 4), z[0], z[1], z[2], z[3]);
+                        for (int j = 0; j < 4; ++j) z[j] = tc::bf16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+                        const int t = t0 + 8 * (lane >> 4) + (lane & 7), to = 4 * w + 2 * half + ((lane >> 3) & 1);
+                        tc::stmatrix_t4(y + t * 256 + ((to ^ (t & 7)) << 4), z[0], z[1], z[2], z[3]);
+                    }
+                    if (rows32) {
+                        tc::fence_before_sync();
+                        arrive(bOFree + (c & 1));
+                    }
+                    named_bar_sync(2, 128);
+                    const int live = rows - c * CH - rows32 - t8;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i, out += step)
+                        if (8 * i < live) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(from + i * 2048);
                 }
-                tc::fence_before_sync();
-                arrive(bOFree + (c & 1));
-                named_bar_sync(2, 128);
-                const int live = rows - c * CH - t8;
-#pragma unroll 4
-                for (int i = 0; i < 8; ++i, out += step)
-                    if (8 * i < live) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(from + i * 2048);
             }
         }
     } else if (warp < kVWarp) {
@@ -339,9 +364,10 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
             const int qt = tid - 32 * kQWarp, r0 = qt >> 3, sw = r0 & 7, piece = (qt & 7) ^ sw;
             unsigned char* to = smem + oQ + (piece >> 2) * kBox + r0 * 128;
             const int to0 = ((2 * (piece & 3)) ^ sw) << 4, to1 = ((2 * (piece & 3) + 1) ^ sw) << 4;
+            const bool swap = piece & 4;  // (eight lanes' stores at a time: the four in one box take the even pieces while those in the other take the odd ones)
             for (int c = 0; c < n; ++c) {
                 if (!wait_with_decays(c, bFull + c % kStages, c / kStages, kStatusLinFull)) goto done;
-                if (c > 0 && !wait(bQS, c - 1, kStatusLinQK)) goto done;
+                if (c > 0 && !wait(bQS + ((c - 1) & 1), (c - 1) / 2, kStatusLinQK)) goto done;
                 const Decays& x = decays[c % kDecays];
                 const unsigned char* q = smem + (c % kStages) * kStage + qt * 16;
 #pragma unroll 4
@@ -354,11 +380,12 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
                     const float2 a1 = mul2(e, make_float2(__uint_as_float(in.y << 16), __uint_as_float(in.y & 0xffff0000u)));
                     const float2 a2 = mul2(e, make_float2(__uint_as_float(in.z << 16), __uint_as_float(in.z & 0xffff0000u)));
                     const float2 a3 = mul2(e, make_float2(__uint_as_float(in.w << 16), __uint_as_float(in.w & 0xffff0000u)));
-                    *reinterpret_cast<float4*>(at + to0) = make_float4(a0.x, a0.y, a1.x, a1.y);
-                    *reinterpret_cast<float4*>(at + to1) = make_float4(a2.x, a2.y, a3.x, a3.y);
+                    const float4 x0 = make_float4(a0.x, a0.y, a1.x, a1.y), x1 = make_float4(a2.x, a2.y, a3.x, a3.y);
+                    *reinterpret_cast<float4*>(at + (swap ? to1 : to0)) = swap ? x1 : x0;
+                    *reinterpret_cast<float4*>(at + (swap ? to0 : to1)) = swap ? x0 : x1;
                 }
                 fence_proxy_async_smem();
-                arrive(bPQ);
+                arrive(bQ);
                 arrive(bDecayFree + c % kDecays);
             }
         }
@@ -459,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
         for (int c = 0; c < n; ++c) {
             // The chunk's outputs have read the state (and the chunk before has been added).
             if (STATE && c == 0 ? !wait(bDecay, 0, kStatusLinDecay)
-                                : !wait_with_decays(c, STATE ? bU + ((c - 1) & 1) : bQS, STATE ? (c - 1) / 2 : c, STATE ? kStatusLinU : kStatusLinS)) goto done;
+                                : !wait_with_decays(c, STATE ? bU + ((c - 1) & 1) : bQS + (c & 1), STATE ? (c - 1) / 2 : c / 2, STATE ? kStatusLinU : kStatusLinS)) goto done;
             const float all = decays[c % kDecays].all;
             arrive(bDecayFree + c % kDecays);
             tc::fence_after_sync();
@@ -522,7 +549,7 @@ done:
     }
     tc::fence_before_sync();
     __syncthreads();
-    if (warp == kMmaWarp) tc::tmem_dealloc(tm, kCols);
+    if (warp == kStateMmaWarp) tc::tmem_dealloc(tm, kCols);
 }
 
 // The state before each segment of a chain, from what the segments add: one thread for four entries of a state.  Segments that the sequence does not reach are
