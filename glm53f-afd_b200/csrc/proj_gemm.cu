@@ -264,17 +264,17 @@ __global__ void __launch_bounds__(kGemmThreads, kBlocksPerSm) proj_gemm_kernel(c
             unsigned char* base = reinterpret_cast<unsigned char*>(x.out) + ((long long)tile.g * x.o_gstride + f) * (out_f32 ? 4 : 2);
             // EPI: the bias of this thread's feature, and the residual's values of sixteen rows (of KS > 1: of the rows this block finishes).
             constexpr int CW = NR / KS, kRes = SPLIT ? CW : 16;
-            float bias = 0.0f, res[EPI ? kRes : 1];
+            float bias = 0.0f, res[EPI ? kRes : 1] = {};
             auto load_residual = [&](int c0) {
-                if constexpr (EPI) {
-                    const unsigned char* at = static_cast<const unsigned char*>(p.epi.residual) + ((long long)tile.g * p.epi.r_gstride + f) * (out_f32 ? 4 : 2);
+                if constexpr (EPI) {  // (without a branch an element, so that all are in flight together; what lies past an extent is read from the last place within)
+                    if (p.epi.residual == nullptr) return;
+                    const long long at = (long long)tile.g * p.epi.r_gstride + min(f, x.n - 1), first = row0 + c0, most = rows - 1;
+                    if (out_f32) {
 #pragma unroll
-                    for (int j = 0; j < kRes; ++j) {
-                        const long long row = row0 + c0 + j;
-                        res[j] = 0.0f;
-                        if (p.epi.residual != nullptr && f_ok && row < rows)
-                            res[j] = out_f32 ? *reinterpret_cast<const float*>(at + row * p.epi.ldr * 4)
-                                             : bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(at + row * p.epi.ldr * 2));
+                        for (int j = 0; j < kRes; ++j) res[j] = static_cast<const float*>(p.epi.residual)[at + min(first + j, most) * p.epi.ldr];
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < kRes; ++j) res[j] = bf16_bits_to_f32(static_cast<const uint16_t*>(p.epi.residual)[at + min(first + j, most) * p.epi.ldr]);
                     }
                 }
             };
@@ -307,10 +307,11 @@ __global__ void __launch_bounds__(kGemmThreads, kBlocksPerSm) proj_gemm_kernel(c
                         if constexpr (EPI) {
                             float y[16];
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) y[j] = res[j];
+                            for (int j = 0; j < 16; ++j) y[j] = __uint_as_float(r[j]);
+                            proj_finish(p.epi.act, y, [&](int) { return bias; }, res);
                             if (c0 + 16 < NR) load_residual(c0 + 16);
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) store(c0 + j, y[j] + proj_act(p.epi.act, __uint_as_float(r[j]) + bias));
+                            for (int j = 0; j < 16; ++j) store(c0 + j, y[j]);
                         } else {
 #pragma unroll
                             for (int j = 0; j < 16; ++j) store(c0 + j, __uint_as_float(r[j]));
@@ -381,14 +382,16 @@ __global__ void __launch_bounds__(kGemmThreads, kBlocksPerSm) proj_gemm_kernel(c
 #pragma unroll
                     for (int c = 0; c < CW; ++c) v[c][r] = peer_load(remote + (uint32_t)(c * kBM * 4));
                 }
+                float sum[CW];
 #pragma unroll
                 for (int c = 0; c < CW; ++c) {
-                    float sum = v[c][0];
+                    sum[c] = v[c][0];
 #pragma unroll
-                    for (uint32_t r = 1; r < ks; ++r) sum = sum + v[c][r];
-                    if constexpr (EPI) sum = res[c] + proj_act(p.epi.act, sum + bias);
-                    store((int)kr * CW + c, sum);
+                    for (uint32_t r = 1; r < ks; ++r) sum[c] = sum[c] + v[c][r];
                 }
+                if constexpr (EPI) proj_finish(p.epi.act, sum, [&](int) { return bias; }, res);
+#pragma unroll
+                for (int c = 0; c < CW; ++c) store((int)kr * CW + c, sum[c]);
                 fence_cluster();
                 __syncwarp();
                 if (lane < KS) peer_mbar_arrive(peer_smem(red_empty, lane));
@@ -669,5 +672,7 @@ extern "C" int32_t glm53f_kda_proj_bf16_fused(const glm53f_proj_job* job, const 
     PairProblem q;
     if (!pair_problem(q, j)) return (int)cudaErrorNotSupported;
     q.epi = epi;
+    q.res_boxes = epi.residual && q.tensor_out && aligned16(epi.residual) && e.ldr % 8 == 0 && (j.groups == 1 || (e.r_gstride % 8 == 0 && e.r_gstride > 0)) &&
+                  matrix_map(&q.tm_res, &q.res_swapped, epi.residual, j.n, j.rows, j.groups, e.ldr, e.r_gstride, 16, 64);
     return proj_gemm_pair_launch(&q, 1, true, status, stream);
 }

@@ -45,20 +45,28 @@ constexpr int kPM = 128;           // features per block (256 per pair)
 constexpr int kPN = 256;           // rows per tile at most (half of them loaded by each block)
 constexpr int kPK = 64;
 constexpr int kPairThreads = 320;  // producer, MMA, eight epilogue warps
-constexpr int kPairStages = 6;
 constexpr int kPairABytes = kPM * 128, kPairBBytes = (kPN / 2) * 128;
 constexpr int kPairStageBytes = kPairABytes + kPairBBytes;  // 32 KiB
 constexpr int kPairTmemCols = 512;
 // Output staging: two buffers per pair of epilogue warps, each two boxes of 16 rows x 64 features in the 128-byte swizzle.
 // (NR is a multiple of 16, not of 32; a fence and two barriers per sixteen rows were most of the epilogue's time.)
 constexpr int kBoxRows = 16, kChunk = 2 * kBoxRows, kOutBuf = kChunk * 128;
-constexpr int oPairOut = kPairStages * kPairStageBytes;
-constexpr int oPairBars = oPairOut + 8 * kOutBuf;
-constexpr int oPairCtl = oPairBars + (2 * kPairStages + 4) * 8;
-constexpr int kPairSmem = oPairCtl + 16 + 1024;
-static_assert(kPairSmem <= 232448, "shared memory budget");
+// What an instance does with the results before they leave: nothing; bias and activation; a residual too, that comes by tensor copies, or straight into
+// registers (f32 results, rows that no tensor copy takes).  (As one instance the registers of all three spill.)
+enum PairEpilogue : int { kPlain, kNoResidual, kResidualBoxes, kResidualDirect };
+template <int EPI>
+struct PairSmem {
+    // An epilogue's residual arrives in boxes of its own, two buffers per pair of warps, in the last stage's place.
+    static constexpr int kAllStages = 6, kStages = kAllStages - (EPI == kResidualBoxes ? 1 : 0);
+    static constexpr int oOut = kAllStages * kPairStageBytes, oRes = oOut - 8 * kOutBuf;
+    static_assert(8 * kOutBuf <= kPairStageBytes, "a stage holds the residual's buffers");
+    static constexpr int oBars = oOut + 8 * kOutBuf;
+    static constexpr int kBars = 2 * kStages + 4 + (EPI == kResidualBoxes ? 8 : 0);
+    static constexpr int oCtl = oBars + kBars * 8, kBytes = oCtl + 16 + 1024;
+    static_assert(kBytes <= 232448, "shared memory budget");
+};
 
-enum : int { kStatusPairEmpty = 140, kStatusPairFull = 141, kStatusPairAccFull = 142, kStatusPairAccEmpty = 143 };
+enum : int { kStatusPairEmpty = 140, kStatusPairFull = 141, kStatusPairAccFull = 142, kStatusPairAccEmpty = 143, kStatusPairResidual = 144 };
 
 __device__ __forceinline__ uint32_t pair_rank() {
     uint32_t r;
@@ -129,22 +137,25 @@ __device__ __forceinline__ PairTile pair_tile(const PairParams& p, long long t) 
     return {q, i - u * q.r_tiles, u % q.n_tiles, u / q.n_tiles};
 }
 
-// SPLIT_ROWS: rows per tile at most where k runs in segments.  EPI: bias, activation and residual before the results leave.
-template <int SPLIT_ROWS, bool EPI>
+// SPLIT_ROWS: rows per tile at most where k runs in segments.  
+template <int SPLIT_ROWS, int EPI>
 __global__ void __launch_bounds__(kPairThreads, 1) proj_gemm_pair_kernel(const __grid_constant__ PairParams p) {
+    using L = PairSmem<EPI>;
+    constexpr int oPairOut = L::oOut, stages = L::kStages;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + oPairBars);   // used in the leader: both blocks' copies
-    uint64_t* empty = full + kPairStages;                            // in each block: the pair's MMAs are done with the stage
-    uint64_t* acc_full = empty + kPairStages;                        // in each block
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::oBars);   // used in the leader: both blocks' copies
+    uint64_t* empty = full + L::kStages;                            // in each block: the pair's MMAs are done with the stage
+    uint64_t* acc_full = empty + L::kStages;                        // in each block
     uint64_t* acc_empty = acc_full + 2;                              // used in the leader: both blocks' epilogues
-    volatile uint32_t* ctl = reinterpret_cast<volatile uint32_t*>(smem + oPairCtl);
+    uint64_t* res_full = acc_empty + 2;                              // EPI: in each block, two per pair of epilogue warps
+    volatile uint32_t* ctl = reinterpret_cast<volatile uint32_t*>(smem + L::oCtl);
     uint32_t* tmem_slot = const_cast<uint32_t*>(ctl) + 2;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = pair_rank();
     const long long tile0 = blockIdx.x >> 1, tile_step = gridDim.x >> 1;
     if (tid == 0) {
-        for (int i = 0; i < kPairStages; ++i) {
+        for (int i = 0; i < stages; ++i) {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
@@ -152,6 +163,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) proj_gemm_pair_kernel(const _
             mbar_init(&acc_full[i], 1);
             mbar_init(&acc_empty[i], 16);  // eight epilogue warps of each block
         }
+        if (EPI == kResidualBoxes)
+            for (int i = 0; i < 8; ++i) mbar_init(&res_full[i], 1);
         ctl[0] = 0u;
         ctl[1] = 0u;
         mbar_init_fence();
@@ -185,7 +198,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) proj_gemm_pair_kernel(const _
                     if (rank == 0) mbar_arrive_expect_tx(&full[s], tx);
                     pair_tensor_load(st, mw, kb * kPK, wy, wz, bar0 + 8 * s);
                     pair_tensor_load(st + kPairABytes, mx, kb * kPK, xy, xz, bar0 + 8 * s);
-                    if (++s == kPairStages) {
+                    if (++s == stages) {
                         s = 0;
                         ph ^= 1u;
                     }
@@ -213,7 +226,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) proj_gemm_pair_kernel(const _
                         for (int i = 0; i < kPK / 16; ++i)
                             pair_mma(leader, d, tc::desc_sw128_kmajor(st, kPM, 16 * i), tc::desc_sw128_kmajor(st + kPairABytes, kPN / 2, 16 * i), idesc, kb > 0 || i > 0);
                         pair_commit(leader, &empty[s]);
-                        if (++s == kPairStages) {
+                        if (++s == stages) {
                             s = 0;
                             ph ^= 1u;
                         }
@@ -239,10 +252,11 @@ __global__ void __launch_bounds__(kPairThreads, 1) proj_gemm_pair_kernel(const _
         // two-byte stores where four are enough now: the k = 128 gate factor at 512 rows
         // 13.8 -> 12.5 us, at 1,024 24.5 -> 21.3.)  Else lane = feature, v[j] = row c0 + j; and so in the instance that keeps the sums of more than 128 rows,
         // whose registers are full (o_proj at 513, 660 and 768 rows 40.6, 43.4 and 44.6 us, from fragments 45.9, 48.8 to 52.4 and 51.0 to 56.9).
-        constexpr bool kFragments = SPLIT_ROWS <= 128;
+        constexpr bool kFragments = SPLIT_ROWS <= 128 && EPI != kResidualDirect;
+        auto tensor_out = [&](const PairTile& x) { return EPI != kResidualDirect && x.q.tensor_out; };
         auto load = [&](const PairTile& x, int c0, float* v) {
             uint32_t r[16];
-            if (x.q.tensor_out) {
+            if (tensor_out(x)) {
                 uint32_t a[8], b[8];
                 tc::tmem_ld_frag(tc::tmem_addr(tm, q, buf * kPN + c0), a);
                 tc::tmem_ld_frag(tc::tmem_addr(tm, q, buf * kPN + c0) + (16u << 16), b);
@@ -257,37 +271,129 @@ __global__ void __launch_bounds__(kPairThreads, 1) proj_gemm_pair_kernel(const _
             for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
         };
         // The tile's rows c0 .. c0 + 31 (those below row_tile) out, as load() gave them.
-        // v[j]'s place in the chunk of 32 rows x 32 features, by load()'s layout.
-        auto feature_of = [&](const PairTile& x, int j) { return kFragments && x.q.tensor_out ? 16 * ((j >> 3) & 1) + 8 * ((j >> 1) & 1) + (lane >> 2) : lane; };
-        auto row_of = [&](const PairTile& x, int j) { return kFragments && x.q.tensor_out ? (j & 16) + 8 * ((j >> 2) & 1) + 2 * (lane & 3) + (j & 1) : j; };
-        auto finish = [&](const PairTile& x, int c0, float (&v)[kChunk]) {
-            const ProjEpilogue& e = x.q.epi;
-            const long long row0 = (long long)x.rt * x.q.row_tile + c0;
-            const int f0 = x.nt * 2 * kPM + (int)rank * kPM + q * 32;
+        // EPI.  v[j]'s place in the chunk of 32 rows x 32 features, by load()'s layout: feature place 2 ((j / 8) % 2) + (j / 2) % 2 of four, 8 apart, in
+        // fragments.
+        auto in_fragments = [&](const PairTile& x) { return kFragments && tensor_out(x); };
+        auto feature_of = [&](const PairTile& x, int j) { return in_fragments(x) ? 16 * ((j >> 3) & 1) + 8 * ((j >> 1) & 1) + (lane >> 2) : lane; };
+        float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f}, res[EPI >= kResidualBoxes ? kChunk : 1];
+        auto load_bias = [&](const PairTile& x) {
+            if (EPI != kPlain && x.q.epi.bias != nullptr)
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) {
-                const int f = f0 + feature_of(x, j);
-                const long long row = row0 + row_of(x, j);
-                const bool ok = f < x.q.n && row < x.q.rows;
-                const float bias = e.bias != nullptr && ok ? proj_bias(e, x.g, f) : 0.0f;
-                float res = 0.0f;
-                if (e.residual != nullptr && ok) {
-                    const long long at = (long long)x.g * e.r_gstride + row * e.ldr + f;
-                    res = x.q.out_f32 ? static_cast<const float*>(e.residual)[at] : bf16_bits_to_f32(static_cast<const uint16_t*>(e.residual)[at]);
+                for (int i = 0; i < 4; ++i) bias[i] = proj_bias(x.q.epi, x.g, min(x.nt * 2 * kPM + (int)rank * kPM + q * 32 + feature_of(x, 8 * (i >> 1) + 2 * (i & 1)), x.q.n - 1));
+        };
+        // The residual straight into registers (f32 results, or rows that no tensor copy takes): without a branch an element, so that all are in flight together;
+        // what lies past an extent is read from the last place within.
+        auto load_residual = [&](const PairTile& x, int c0) {
+            if constexpr (EPI == kResidualDirect) {
+                const ProjEpilogue& e = x.q.epi;
+                if (c0 >= x.q.row_tile) return;
+                const int row0 = x.rt * x.q.row_tile + c0, last = min(x.q.rows - 1 - row0, kChunk - 1);
+                if (last < 0) return;
+                long long at = (long long)x.g * e.r_gstride + row0 * e.ldr + min(x.nt * 2 * kPM + (int)rank * kPM + q * 32 + lane, x.q.n - 1);
+                if (x.q.out_f32) {
+                    const float* from = static_cast<const float*>(e.residual);
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j) {
+                        res[j] = from[at];
+                        at += j < last ? e.ldr : 0;
+                    }
+                } else {
+                    const uint16_t* from = static_cast<const uint16_t*>(e.residual);
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j) {
+                        res[j] = bf16_bits_to_f32(from[at]);
+                        at += j < last ? e.ldr : 0;
+                    }
                 }
-                v[j] = res + proj_act(e.act, v[j] + bias);
             }
         };
+        // ... or by tensor copies, two chunks ahead of the one that is being finished.  A place in the sequence of this pair's chunks:
+        struct Place {
+            long long t;
+            int c0;
+        };
+        unsigned char* res_boxes = smem + L::oRes + (set * 2 + side) * 2 * kOutBuf;
+        auto settle = [&](Place& at) {  // the chunk at this place, or the next one that has rows
+            while (at.t < p.tiles) {
+                const PairTile x = pair_tile(p, at.t);
+                if (at.c0 < x.q.row_tile && (long long)x.rt * x.q.row_tile + at.c0 < x.q.rows) return true;
+                at.t += tile_step;
+                at.c0 = set * kChunk;
+            }
+            return false;
+        };
+        int res_buf = 0;
+        uint32_t res_ph = 0;
+        Place ahead{tile0, set * kChunk};
+        auto copy_residual = [&](int b) {  // by the issuer
+            if (!settle(ahead)) return;
+            const PairTile x = pair_tile(p, ahead.t);
+            const int f0 = x.nt * 2 * kPM + (int)rank * kPM + side * 64, row0 = x.rt * x.q.row_tile + ahead.c0;
+            uint64_t* bar_b = &res_full[(set * 2 + side) * 2 + b];
+            if (f0 >= x.q.n) {  // (nothing to copy; the buffer's turn passes all the same)
+                mbar_arrive(bar_b);
+            } else {
+                const bool second = row0 + kBoxRows < x.q.rows && ahead.c0 + kBoxRows < x.q.row_tile;
+                mbar_arrive_expect_tx(bar_b, second ? kOutBuf : kOutBuf / 2);
+                for (int half = 0; half < (second ? 2 : 1); ++half)
+                    tensor_load_3d(res_boxes + b * kOutBuf + half * kBoxRows * 128, &x.q.tm_res, f0, x.q.res_swapped ? x.g : row0 + half * kBoxRows,
+                                   x.q.res_swapped ? row0 + half * kBoxRows : x.g, bar_b);
+            }
+            ahead.c0 += 2 * kChunk;
+        };
+        constexpr bool by_boxes = EPI == kResidualBoxes;
+        if (by_boxes && issuer) copy_residual(0), copy_residual(1);
+        auto finish = [&](const PairTile& x, int c0, float (&v)[kChunk]) {
+            const ProjEpilogue& e = x.q.epi;
+            const bool fragments = in_fragments(x);
+            float b[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) b[i] = fragments ? bias[i] : bias[0];
+            if constexpr (EPI >= kResidualBoxes) proj_finish(e.act, v, [&](int j) { return b[2 * ((j >> 3) & 1) + ((j >> 1) & 1)]; }, res);
+            else proj_finish(e.act, v, [&](int j) { return b[2 * ((j >> 3) & 1) + ((j >> 1) & 1)]; }, nullptr);
+        };
+        bool gone = false;  // a residual's copy did not come
         auto emit = [&](const PairTile& x, int c0, float (&v)[kChunk]) {
             const long long row0 = (long long)x.rt * x.q.row_tile + c0;
             const int f0 = x.nt * 2 * kPM + (int)rank * kPM + side * 64;
             if (row0 >= x.q.rows) return;  // the whole chunk is past the last row (the same for every thread)
-            if constexpr (EPI) finish(x, c0, v);
-            if (x.q.tensor_out) {
+            if constexpr (EPI != kPlain && !by_boxes) {
+                finish(x, c0, v);
+                load_residual(x, c0 + 2 * kChunk);
+            }
+            if (tensor_out(x)) {
                 unsigned char* box = boxes + out_buf * kOutBuf;
                 out_buf ^= 1;
                 if (issuer) bulk_wait_read<1>();  // this buffer's last stores have been read
-                named_bar_sync(bar, 64);
+                if constexpr (by_boxes) {
+                    // (The two warps go on together or not at all: the vote takes the place of the barrier.)
+                    const bool ok = mbar_wait(&res_full[(set * 2 + side) * 2 + res_buf], res_ph, ctx, kStatusPairResidual);
+                    gone = !named_bar_all(bar, 64, ok);
+                    if (gone) return;
+                    const unsigned char* from = res_boxes + res_buf * kOutBuf;
+                    if constexpr (kFragments) {
+                        const int row = (lane >> 4) * 8 + (lane & 7), piece = (q & 1) * 4 + ((lane >> 3) & 1);
+#pragma unroll
+                        for (int c = 0; c < 2; ++c)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                uint32_t r[4];
+                                tc::ldmatrix_t4(from + (16 * c + row) * 128 + (((piece + 2 * h) ^ (row & 7)) << 4), r[0], r[1], r[2], r[3]);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    res[16 * c + 8 * h + 2 * i] = __uint_as_float(r[i] << 16);
+                                    res[16 * c + 8 * h + 2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
+                                }
+                            }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < kChunk; ++j)
+                            res[j] = bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(from + j * 128 + (((fl >> 3) ^ (j & 7)) << 4) + (fl & 7) * 2));
+                    }
+                    finish(x, c0, v);
+                } else {
+                    named_bar_sync(bar, 64);
+                }
                 if constexpr (kFragments) {
                     // A lane names row lane % 8 of matrix lane / 8: features 8 ((lane / 8) % 2), rows 8 (lane / 16) of the sixteen by sixteen.
                     const int row = (lane >> 4) * 8 + (lane & 7), piece = (q & 1) * 4 + ((lane >> 3) & 1);
@@ -309,6 +415,11 @@ __global__ void __launch_bounds__(kPairThreads, 1) proj_gemm_pair_kernel(const _
                 }
                 fence_proxy_async_smem();
                 named_bar_sync(bar, 64);
+                if constexpr (by_boxes) {
+                    if (issuer) copy_residual(res_buf);  // (both warps have read it)
+                    res_buf ^= 1;
+                    if (res_buf == 0) res_ph ^= 1u;
+                }
                 if (issuer) {
                     if (f0 < x.q.n)  // features and rows past the extents are clipped by the copy
 #pragma unroll
@@ -352,6 +463,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) proj_gemm_pair_kernel(const _
                 tc::fence_after_sync();
                 return all;
             };
+            if constexpr (EPI != kPlain) {
+                load_bias(x);
+                load_residual(x, set * kChunk);
+            }
             if (x.q.segments == 1) {
                 if (!arrived()) goto done;
                 for (int c0 = set * kChunk; c0 < x.q.row_tile; c0 += 2 * kChunk) {
@@ -367,6 +482,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) proj_gemm_pair_kernel(const _
                         for (int j = 0; j < kChunk; ++j) v[j] = __uint_as_float(r[j]);
                     }
                     emit(x, c0, v);
+                    if (by_boxes && gone) goto done;
                 }
                 release();
             } else {
@@ -400,6 +516,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) proj_gemm_pair_kernel(const _
                     const int c0 = (2 * c + set) * kChunk;
                     if (c0 >= x.q.row_tile) break;
                     emit(x, c0, sum[c]);
+                    if (by_boxes && gone) goto done;
                 }
             }
         }
@@ -424,14 +541,20 @@ done:
 int proj_gemm_pair_launch(const PairProblem* problems, int n, bool epilogue, int* status, cudaStream_t stream) {
     bool wide = false;  // tiles of more than 128 rows in segments: 7 % slower a tile than the narrow instance
     for (int i = 0; i < n; ++i) wide = wide || (problems[i].segments > 1 && problems[i].row_tile > 128);
-    auto* kernel = epilogue ? (wide ? proj_gemm_pair_kernel<kPairSplitRows, true> : proj_gemm_pair_kernel<128, true>)
-                            : (wide ? proj_gemm_pair_kernel<kPairSplitRows, false> : proj_gemm_pair_kernel<128, false>);
-    static int configured_dev[4] = {-1, -1, -1, -1};
-    const int which = 2 * epilogue + wide;
+    using Kernel = void (*)(PairParams);
+    static constexpr Kernel kernels[8] = {proj_gemm_pair_kernel<128, kPlain>,         proj_gemm_pair_kernel<kPairSplitRows, kPlain>,
+                                          proj_gemm_pair_kernel<128, kNoResidual>,    proj_gemm_pair_kernel<kPairSplitRows, kNoResidual>,
+                                          proj_gemm_pair_kernel<128, kResidualBoxes>, proj_gemm_pair_kernel<kPairSplitRows, kResidualBoxes>,
+                                          proj_gemm_pair_kernel<128, kResidualDirect>, proj_gemm_pair_kernel<kPairSplitRows, kResidualDirect>};
+    static_assert(PairSmem<kResidualBoxes>::kBytes <= 232448, "shared memory budget");
+    const int epi = !epilogue ? kPlain : problems[0].epi.residual == nullptr ? kNoResidual : problems[0].res_boxes ? kResidualBoxes : kResidualDirect;
+    const int which = 2 * epi + wide, smem = epi == kResidualBoxes ? PairSmem<kResidualBoxes>::kBytes : PairSmem<kPlain>::kBytes;
+    const Kernel kernel = kernels[which];
+    static int configured_dev[8] = {-1, -1, -1, -1, -1, -1, -1, -1};
     int dev = 0;
     cudaGetDevice(&dev);
     if (configured_dev[which] != dev) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return (int)e;
         configured_dev[which] = dev;
     }
@@ -445,7 +568,7 @@ int proj_gemm_pair_launch(const PairProblem* problems, int n, bool epilogue, int
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(pairs * 2));
     cfg.blockDim = dim3(kPairThreads);
-    cfg.dynamicSmemBytes = kPairSmem;
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
