@@ -14,14 +14,17 @@
 // rounding moves one draw in a few hundred to the next token.  The maxima and sums that judge a token are 32-bit ones (a relative 1e-7
 // of a probability against u).
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "kda_internal.h"
 
 namespace kda {
 namespace {
 
-constexpr int kAccThreads = 512, kAccWarps = kAccThreads / 32, kAccBlocks = 8;  // blocks a request
-constexpr int kAccRows = 8;  // rows judged at a time
+constexpr int kAccMostWarps = 16;   // of a block: 8 or 16
+constexpr int kAccMostBlocks = 16;  // blocks a request, 8 or 16
+constexpr int kAccRows = 8;         // rows judged at a time
 
 struct AcceptParams {
     const int32_t* cu;
@@ -32,19 +35,22 @@ struct AcceptParams {
     const float* temperature;
     const float* u;
     int32_t *keep, *next;
+    int blocks;
 };
 
 struct AccShared {
+    double power[32];  // 2^(j / 32)
     // What this block's slice gives, read by the other blocks of the cluster.
     float max[kAccRows], sum[kAccRows];
     int best[kAccRows];
     double part;      // the slice's weights
     int last;         // the slice's last index with a weight, or -1
     // Within the block.
-    float wmax[kAccRows][kAccWarps], wsum[kAccRows][kAccWarps];
-    int wbest[kAccRows][kAccWarps];
-    double wpart[kAccWarps];
-    int wlast[kAccWarps];
+    float wmax[kAccRows][kAccMostWarps], wsum[kAccRows][kAccMostWarps];
+    int wbest[kAccRows][kAccMostWarps];
+    double wpart[kAccMostWarps];
+    double slot[kAccMostWarps][32];  // a warp's weights, its places in 32 parts
+    int wlast[kAccMostWarps];
     float row_max[kAccRows], row_sum[kAccRows];
     int row_best[kAccRows];
     int kept;
@@ -58,6 +64,9 @@ __device__ __forceinline__ uint32_t cluster_block() {
 __device__ __forceinline__ void cluster_meet() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The two halves of it, for what need not be waited for at once.
+__device__ __forceinline__ void cluster_said() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_heard() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t at_block(const void* local, uint32_t block) {
     uint32_t r;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(local)), "r"(block));
@@ -85,52 +94,126 @@ __device__ __forceinline__ float target_at(const void* row, long long i) {
     if constexpr (KIND == GLM53F_KDA_LOGITS_BF16) return bf16_bits_to_f32(__ldg(static_cast<const uint16_t*>(row) + i));
     else return __ldg(static_cast<const float*>(row) + i);
 }
-// Eight consecutive entries from i on, those at `end` and beyond as `fill`.
+// Eight consecutive entries from i on as they lie in memory (vector loads; or, where the row's end or its alignment rules those out, one at a
+// time, those at `end` and beyond as `fill`), and as floats.  Apart, so that several loads are in flight before the first is looked at.
 template <int KIND>
-__device__ __forceinline__ void target_8(const void* row, long long i, long long end, bool vec, float fill, float (&x)[8]) {
-    if (vec && i + 8 <= end) {
-        if constexpr (KIND == GLM53F_KDA_LOGITS_BF16) {
-            const uint4 r = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + i));
-            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+struct Eight {
+    static constexpr int kWords = KIND == GLM53F_KDA_LOGITS_BF16 ? 4 : 8;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void load_whole(const void* row, long long i) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[2 * j] = __uint_as_float(w[j] << 16);
-                x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-            }
-        } else {
-            const float4* r = reinterpret_cast<const float4*>(static_cast<const float*>(row) + i);
-            const float4 a = __ldg(r), b = __ldg(r + 1);
-            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+        for (int j = 0; j < kWords; j += 4) {
+            const uint4 r = __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(row) + i * (kWords / 2)) + j / 4);
+            w[j] = r.x, w[j + 1] = r.y, w[j + 2] = r.z, w[j + 3] = r.w;
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = i + j < end ? target_at<KIND>(row, i + j) : fill;
     }
-}
+    __device__ __forceinline__ void load_some(const void* row, long long i, long long end, float fill) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t u = __float_as_uint(i + j < end ? target_at<KIND>(row, i + j) : fill);
+            if constexpr (kWords == 8) w[j] = u;
+            else w[j >> 1] = j & 1 ? w[j >> 1] | (u & 0xffff0000u) : u >> 16;
+        }
+    }
+    __device__ __forceinline__ void load(const void* row, long long i, long long end, bool vec, float fill) {
+        if (vec && i + 8 <= end) load_whole(row, i);
+        else load_some(row, i, end, fill);
+    }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if constexpr (kWords == 8) x[j] = __uint_as_float(w[j]);
+            else x[j] = __uint_as_float(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
+        }
+    }
+};
 
+// e^x for x <= 0 to a few units of 2^-52: x = (32 e + j) ln 2 / 32 + r, so e^x = 2^e 2^(j/32) e^r with |r| < 0.011, of which Taylor's series to
+// the fifth power leaves 3e-15.  (Half the double-precision operations of the general function, which were what a draw spent its time on.)
+__device__ __forceinline__ double exp_below(double x, const double* power) {
+    const double magic = 6755399441055744.0;  // 1.5 2^52: adding it rounds to an integer, which the low word then holds
+    const double shifted = fma(x, 46.166241308446828384, magic);
+    const int n = __double2loint(shifted);
+    const double whole = shifted - magic;
+    double r = fma(whole, -0.021660849390173098, x);
+    r = fma(whole, -2.325192846878874e-12, r);
+    double y = fma(r, 1.0 / 120, 1.0 / 24);
+    y = fma(r, y, 1.0 / 6);
+    y = fma(r, y, 0.5);
+    y = fma(r, y, 1.0);
+    y = fma(r, y, 1.0);
+    const double base = power[n & 31];
+    return x < -690.0 ? 0.0 : y * __hiloint2double(__double2hiint(base) + ((n >> 5) << 20), __double2loint(base));
+}
 // e^((l - max) / t) with the largest logits at exactly 1 (an infinite one too) and NaN at 0.
-__device__ __forceinline__ double logit_weight(float l, float max, double inv_t) {
+__device__ __forceinline__ double logit_weight(float l, float max, double inv_t, const double* power) {
     if (l == max) return 1.0;
-    const double e = exp(((double)l - (double)max) * inv_t);
+    const double e = exp_below(((double)l - (double)max) * inv_t, power);
     return l < max ? e : 0.0;
 }
 __device__ __forceinline__ float finite_weight(float p) { return p > 0.0f && p < INFINITY ? p : 0.0f; }
 
-// The larger of two (value, lowest index) pairs; an index of -1 is none.
-__device__ __forceinline__ void take_best(float& m, int& i, float om, int oi) {
-    if (oi >= 0 && (i < 0 || om > m || (om == m && oi < i))) m = om, i = oi;
+// A row's statistics: its largest logit m, the sum of 2^((l - m) scale) over it, the lowest index of the largest (greedy).  A sum at a maximum of -inf is 0.
+struct Stats {
+    float m = kNoLogit, s = 0.0f;
+    int best = -1;
+};
+template <bool GREEDY>
+__device__ __forceinline__ void take(Stats& a, const float (&x)[8], int at, long long vocab, float scale) {
+    float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    if constexpr (GREEDY) {
+        if (top > a.m || a.best < 0) {
+            a.m = fmaxf(top, a.m);
+#pragma unroll
+            for (int j = 7; j >= 0; --j)
+                if (x[j] == top && at + j < vocab) a.best = at + j;
+        }
+    } else {
+        if (top > a.m) {
+            a.s *= a.m == kNoLogit ? 0.0f : ex2_approx((a.m - top) * scale);
+            a.m = top;
+        }
+        float e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = ex2_ftz((x[j] - a.m) * scale);
+        float sum = ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+        if (!(sum < INFINITY)) {  // a NaN among them, or infinities: seldom, so one at a time
+            sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum += x[j] == a.m ? (a.m == kNoLogit ? 0.0f : 1.0f) : x[j] < a.m ? ex2_ftz((x[j] - a.m) * scale) : 0.0f;
+        }
+        a.s += sum;
+    }
+}
+// Over the lanes of a warp.
+template <bool GREEDY>
+__device__ __forceinline__ void join_lanes(Stats& a, float scale) {
+    float m = a.m;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    if constexpr (GREEDY) {
+        a.best = (int)__reduce_min_sync(0xffffffffu, a.best >= 0 && a.m == m ? (unsigned)a.best : 0xffffffffu);  // (none is -1)
+    } else {
+        float s = a.m == m ? a.s : a.s * ex2_ftz((a.m - m) * scale);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+        a.s = s;
+    }
+    a.m = m;
 }
 
 // What a draw weighs: the row's distribution p, less the drafter's, or without the refused token.
 enum : int { kWhole = 0, kLessDraft = 1, kWithout = 2 };
 
-template <int KIND>
-__global__ void __launch_bounds__(kAccThreads) accept_kernel(const __grid_constant__ AcceptParams p) {
+template <int KIND, int kAccWarps>
+__global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept_kernel(const __grid_constant__ AcceptParams p) {
+    constexpr int kAccThreads = kAccWarps * 32, kAccDeep = KIND == GLM53F_KDA_LOGITS_BF16 ? 4 : 2;  // (rows read side by side)
     constexpr bool LOGITS = KIND != GLM53F_KDA_PROBABILITIES;
     constexpr int kSize = KIND == GLM53F_KDA_LOGITS_BF16 ? 2 : 4;
     __shared__ AccShared sh;
+    if (threadIdx.x < 32) sh.power[threadIdx.x] = exp2((double)threadIdx.x / 32);
     grid_ready();
-    const int b = blockIdx.x / kAccBlocks, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int blocks = p.blocks, b = blockIdx.x / blocks, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t block = cluster_block();
     const int first = p.cu[b], n = p.cu[b + 1] - first;
     if (n <= 0) {  // the same for the whole cluster
@@ -148,103 +231,93 @@ __global__ void __launch_bounds__(kAccThreads) accept_kernel(const __grid_consta
     const float scale = greedy ? 0.0f : kLog2e / temperature;
     const double inv_t = greedy ? 0.0 : 1.0 / (double)temperature;
     // This block's slice, in runs of eight.
-    const long long runs = (p.vocab + 7) / 8, run0 = runs * block / kAccBlocks, run1 = runs * (block + 1) / kAccBlocks;
+    const long long runs = (p.vocab + 7) / 8, run0 = runs * block / blocks, run1 = runs * (block + 1) / blocks;
 
+    __syncthreads();  // the powers
     int kept = 1;  // rows kept so far
     float stop_max = 0.0f;
     int stop_best = -1;
     for (int g0 = 0;; g0 += kAccRows) {
         const int rows_here = min(n - g0, kAccRows);
+        // What the first warp's lanes judge, a row each, on its way meanwhile.
+        int token = -1;
+        float token_target = 0.0f;
+        double token_left = 0.0;
+        if (warp == 0 && lane < rows_here && g0 + lane + 1 < n) {
+            const int i = g0 + lane;
+            token = p.tokens[first + i + 1];
+            if (token < 0 || token >= p.vocab) token = -1;
+            if (token >= 0 && !greedy) {
+                token_target = target_at<KIND>(row_at(i), token);
+                token_left = (double)p.u[first + i + 1] * (p.draft == nullptr ? 1.0 : (double)finite_weight(draft_at(i + 1)[token]));
+            }
+        }
         if constexpr (LOGITS) {
-            for (int i = 0; i < rows_here; ++i) {
-                const void* row = row_at(g0 + i);
-                float m = kNoLogit, s = 0.0f;
-                int best = -1;
-                for (long long r = run0 + tid; r < run1; r += kAccThreads) {
-                    float x[8];
-                    target_8<KIND>(row, 8 * r, p.vocab, vec, kNoLogit, x);
-                    if (greedy) {
+            auto read = [&](auto is_greedy) {
+                constexpr bool GREEDY = decltype(is_greedy)::value;
+                for (int i0 = 0; i0 < rows_here; i0 += kAccDeep) {
+                    Stats st[kAccDeep];
+                    const int deep = min(rows_here - i0, kAccDeep);
+                    // All rows' entries at a place side by side, the next place's on their way while these are looked at.
+                    Eight<KIND> now[kAccDeep], ahead[kAccDeep];
+                    auto load = [&](long long r, Eight<KIND>(&to)[kAccDeep]) {
+                        if (vec && 8 * r + 8 <= p.vocab) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            if (x[j] > m || (best < 0 && x[j] == m && 8 * r + j < p.vocab)) m = x[j], best = (int)(8 * r + j);
-                    } else {
-                        float top = x[0];
+                            for (int d = 0; d < kAccDeep; ++d) to[d].load_whole(row_at(g0 + i0 + min(d, deep - 1)), 8 * r);
+                        } else {
 #pragma unroll
-                        for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
-                        if (top > m) {
-                            s *= m == kNoLogit ? 0.0f : ex2_approx((m - top) * scale);
-                            m = top;
+                            for (int d = 0; d < kAccDeep; ++d) to[d].load_some(row_at(g0 + i0 + min(d, deep - 1)), 8 * r, p.vocab, kNoLogit);
                         }
+                    };
+                    if (run0 + tid < run1) load(run0 + tid, now);
+                    for (long long r = run0 + tid; r < run1; r += kAccThreads) {
+                        if (r + kAccThreads < run1) load(r + kAccThreads, ahead);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) s += x[j] == m ? (m == kNoLogit ? 0.0f : 1.0f) : x[j] < m ? ex2_approx((x[j] - m) * scale) : 0.0f;
+                        for (int d = 0; d < kAccDeep; ++d) {
+                            float x[8];
+                            now[d].get(x);
+                            take<GREEDY>(st[d], x, (int)(8 * r), p.vocab, scale);
+                            now[d] = ahead[d];
+                        }
                     }
-                }
-                // (Sums at a maximum of -inf are 0, and so are their factors.)
 #pragma unroll
-                for (int d = 16; d > 0; d >>= 1) {
-                    const float om = __shfl_xor_sync(0xffffffffu, m, d), os = __shfl_xor_sync(0xffffffffu, s, d);
-                    const int ob = __shfl_xor_sync(0xffffffffu, best, d);
-                    if (greedy) {
-                        take_best(m, best, om, ob);
-                    } else {
-                        const float top = fmaxf(m, om);
-                        s = (m == top ? s : s * ex2_approx((m - top) * scale)) + (om == top ? os : os * ex2_approx((om - top) * scale));
-                        m = top;
+                    for (int d = 0; d < kAccDeep; ++d) {
+                        join_lanes<GREEDY>(st[d], scale);
+                        if (lane == 0 && d < deep) sh.wmax[i0 + d][warp] = st[d].m, sh.wsum[i0 + d][warp] = st[d].s, sh.wbest[i0 + d][warp] = st[d].best;
                     }
                 }
-                if (lane == 0) sh.wmax[i][warp] = m, sh.wsum[i][warp] = s, sh.wbest[i][warp] = best;
-            }
-            __syncthreads();
-            if (tid < rows_here) {
-                float m = sh.wmax[tid][0], s = sh.wsum[tid][0];
-                int best = sh.wbest[tid][0];
-                for (int w = 1; w < kAccWarps; ++w) {
-                    const float om = sh.wmax[tid][w], os = sh.wsum[tid][w];
-                    if (greedy) {
-                        take_best(m, best, om, sh.wbest[tid][w]);
-                    } else {
-                        const float top = fmaxf(m, om);
-                        s = (m == top ? s : s * ex2_approx((m - top) * scale)) + (om == top ? os : os * ex2_approx((om - top) * scale));
-                        m = top;
-                    }
+                // A warp to a row: over the block's warps, then over the cluster's blocks.
+                __syncthreads();
+                if (warp < rows_here) {
+                    Stats a;
+                    if (lane < kAccWarps) a.m = sh.wmax[warp][lane], a.s = sh.wsum[warp][lane], a.best = sh.wbest[warp][lane];
+                    join_lanes<GREEDY>(a, scale);
+                    if (lane == 0) sh.max[warp] = a.m, sh.sum[warp] = a.s, sh.best[warp] = a.best;
                 }
-                sh.max[tid] = m, sh.sum[tid] = s, sh.best[tid] = best;
-            }
-            cluster_meet();
-            if (tid < rows_here) {
-                float m = peer_f32(&sh.max[tid], 0), s = peer_f32(&sh.sum[tid], 0);
-                int best = peer_i32(&sh.best[tid], 0);
-                for (uint32_t c = 1; c < kAccBlocks; ++c) {
-                    const float om = peer_f32(&sh.max[tid], c), os = peer_f32(&sh.sum[tid], c);
-                    if (greedy) {
-                        take_best(m, best, om, peer_i32(&sh.best[tid], c));
-                    } else {
-                        const float top = fmaxf(m, om);
-                        s = (m == top ? s : s * ex2_approx((m - top) * scale)) + (om == top ? os : os * ex2_approx((om - top) * scale));
-                        m = top;
+                cluster_meet();
+                if (warp < rows_here) {
+                    Stats a;
+                    if (lane < blocks) {
+                        a.m = peer_f32(&sh.max[warp], lane);
+                        if constexpr (GREEDY) a.best = peer_i32(&sh.best[warp], lane);
+                        else a.s = peer_f32(&sh.sum[warp], lane);
                     }
+                    join_lanes<GREEDY>(a, scale);
+                    if (lane == 0) sh.row_max[warp] = a.m, sh.row_sum[warp] = a.s, sh.row_best[warp] = a.best;
                 }
-                sh.row_max[tid] = m, sh.row_sum[tid] = s, sh.row_best[tid] = best;
-            }
-            __syncthreads();
+                __syncthreads();
+            };
+            if (greedy) read(std::true_type{});
+            else read(std::false_type{});
         }
         // Each lane of the first warp judges one row's token.
         if (warp == 0) {
             bool keep = false;
-            const int i = g0 + lane;
-            if (lane < rows_here && i + 1 < n) {
-                const int token = p.tokens[first + i + 1];
-                if (token >= 0 && token < p.vocab) {
-                    if (greedy) {
-                        keep = token == sh.row_best[lane] && sh.row_max[lane] != kNoLogit;
-                    } else {
-                        const double q = p.draft == nullptr ? 1.0 : (double)finite_weight(draft_at(i + 1)[token]);
-                        const float x = target_at<KIND>(row_at(i), token);
-                        const double left = (double)p.u[first + i + 1] * q;
-                        if constexpr (LOGITS) keep = left * (double)sh.row_sum[lane] < logit_weight(x, sh.row_max[lane], inv_t) && sh.row_max[lane] != kNoLogit;
-                        else keep = left < (double)finite_weight(x);
-                    }
-                }
+            if (token >= 0) {
+                if (greedy) keep = token == sh.row_best[lane] && sh.row_max[lane] != kNoLogit;
+                else if constexpr (LOGITS)
+                    keep = token_left * (double)sh.row_sum[lane] < logit_weight(token_target, sh.row_max[lane], inv_t, sh.power) && sh.row_max[lane] != kNoLogit;
+                else keep = token_left < (double)finite_weight(token_target);
             }
             const unsigned all = __ballot_sync(0xffffffffu, keep);
             if (lane == 0) sh.kept = __ffs(~all) - 1;  // (lanes from rows_here on keep nothing)
@@ -272,17 +345,25 @@ __global__ void __launch_bounds__(kAccThreads) accept_kernel(const __grid_consta
         int mode = whole ? kWhole : less != nullptr ? kLessDraft : kWithout;
         const double x01 = fmax((double)p.u[first], 0.0);
         double norm = 1.0;  // the weights' sum, by which the drafter's probabilities are multiplied instead of dividing each of p's
-        auto weights = [&](long long i, double (&w)[8]) {
+        struct Place {
+            Eight<KIND> x;
+            Eight<GLM53F_KDA_PROBABILITIES> y;
+        };
+        auto fetch = [&](long long i, Place& a) {
+            a.x.load(row, i, p.vocab, vec, LOGITS ? kNoLogit : 0.0f);
+            if (mode == kLessDraft) a.y.load(less, i, p.vocab, vec_draft, 0.0f);
+        };
+        auto weights = [&](long long i, const Place& a, double (&w)[8]) {
             float x[8];
-            target_8<KIND>(row, i, p.vocab, vec, LOGITS ? kNoLogit : 0.0f, x);
+            a.x.get(x);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                if constexpr (LOGITS) w[j] = stop_max == kNoLogit ? 0.0 : logit_weight(x[j], stop_max, inv_t);
+                if constexpr (LOGITS) w[j] = stop_max == kNoLogit ? 0.0 : logit_weight(x[j], stop_max, inv_t, sh.power);
                 else w[j] = (double)finite_weight(x[j]);
             }
             if (mode == kLessDraft) {
                 float y[8];
-                target_8<GLM53F_KDA_PROBABILITIES>(less, i, p.vocab, vec_draft, 0.0f, y);
+                a.y.get(y);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const double rest = w[j] - (double)finite_weight(y[j]) * norm;
@@ -294,28 +375,48 @@ __global__ void __launch_bounds__(kAccThreads) accept_kernel(const __grid_consta
                     if (i + j == token) w[j] = 0.0;
             }
         };
-        // A warp's runs of the slice, consecutive ones.
+        // A warp's runs of the slice, consecutive ones, in up to 32 slots of `group` steps of 32 runs.
         const long long mine0 = run0 + (run1 - run0) * warp / kAccWarps, mine1 = run0 + (run1 - run0) * (warp + 1) / kAccWarps;
-        // The slice's sum into sh.part; returns all slices', and the sum before this block's.
-        auto sum_up = [&](double& before, int& last_of_all) {
-            double s = 0.0;
-            int last = -1;
-            for (long long r = mine0 + lane; r < mine1; r += 32) {
-                double w[8];
-                weights(8 * r, w);
+        const int steps = (int)((mine1 - mine0 + 31) / 32), group = (steps + 31) / 32;
+        double before = 0.0, total = 0.0;
+        int last = -1;
+        // Passes over the row, one body of code: of logits with the drafter's probabilities first the weights' sum, then what is drawn from, and
+        // once more where that leaves nothing.
+        const int drawn_from = mode;
+        if (LOGITS && drawn_from == kLessDraft) mode = kWhole;
+        for (bool said = false;; said = true) {
+            int seen = -1, in_slot = 0, slot = 0;
+            double part = 0.0, s = 0.0;
+            Place now, ahead;
+            if (mine0 + lane < mine1) fetch(8 * (mine0 + lane), now);
+#pragma unroll 1
+            for (int k = 0; k < steps; ++k) {
+                const long long r = mine0 + 32 * k + lane;
+                if (r + 32 < mine1) fetch(8 * (r + 32), ahead);
+                if (r < mine1) {
+                    double w[8];
+                    weights(8 * r, now, w);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    s += w[j];
-                    if (w[j] > 0.0) last = (int)(8 * r + j);
+                    for (int j = 0; j < 8; ++j) {
+                        s += w[j];
+                        if (w[j] > 0.0) seen = (int)(8 * r + j);
+                    }
+                }
+                now = ahead;
+                if (++in_slot == group || k + 1 == steps) {
+#pragma unroll
+                    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+                    if (lane == 0) sh.slot[warp][slot] = s;
+                    part += s;
+                    s = 0.0;
+                    in_slot = 0;
+                    ++slot;
                 }
             }
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) {
-                s += __shfl_xor_sync(0xffffffffu, s, d);
-                last = max(last, __shfl_xor_sync(0xffffffffu, last, d));
-            }
-            if (lane == 0) sh.wpart[warp] = s, sh.wlast[warp] = last;
+            seen = __reduce_max_sync(0xffffffffu, seen);
+            if (lane == 0) sh.wpart[warp] = part, sh.wlast[warp] = seen;
             __syncthreads();
+            if (said) cluster_heard();  // (the last pass's sums have been read everywhere)
             if (tid == 0) {
                 double t = 0.0;
                 int l = -1;
@@ -323,72 +424,72 @@ __global__ void __launch_bounds__(kAccThreads) accept_kernel(const __grid_consta
                 sh.part = t, sh.last = l;
             }
             cluster_meet();
-            double all = 0.0;
-            last_of_all = -1;
-            for (uint32_t c = 0; c < kAccBlocks; ++c) {
-                if (c == block) before = all;
-                all += peer_f64(&sh.part, c);
-                last_of_all = max(last_of_all, peer_i32(&sh.last, c));
+            // Every warp adds the blocks' sums in the same order; each lane has fetched one.
+            const double theirs = lane < blocks ? peer_f64(&sh.part, lane) : 0.0;
+            last = __reduce_max_sync(0xffffffffu, lane < blocks ? peer_i32(&sh.last, lane) : -1);
+            total = 0.0;
+            for (int c = 0; c < blocks; ++c) {
+                if (c == (int)block) before = total;
+                total += __shfl_sync(0xffffffffu, theirs, c);
             }
-            cluster_meet();  // read everywhere before it is written again, and before a block leaves
-            return all;
-        };
-        double before = 0.0;
-        int last = -1;
-        if (LOGITS && mode == kLessDraft) {
-            mode = kWhole;
-            norm = sum_up(before, last);
-            mode = kLessDraft;
-        }
-        double total = sum_up(before, last);
-        if (!(total > 0.0) && mode != kWhole) {
-            mode = kWhole;
-            total = sum_up(before, last);
+            cluster_said();
+            if (mode == kWhole && drawn_from == kLessDraft && LOGITS && !said) {
+                norm = total;
+                mode = kLessDraft;
+            } else if (!(total > 0.0) && mode != kWhole) {
+                mode = kWhole;
+            } else {
+                break;
+            }
         }
         const double point = x01 * total;
         if (!(total > 0.0)) {
             if (block == 0 && tid == 0) p.next[b] = -1;
-        } else if (block == 0 && tid == 0 && !(point < total)) {
-            p.next[b] = last;  // (u at its largest, rounded up to the whole)
-        } else if (point < total) {
-            // The warp whose run holds the point; the sums are those that made the total, added in the same order.
-            double lo = before, own = 0.0;
+        } else if (!(point < total)) {
+            if (block == 0 && tid == 0) p.next[b] = last;  // (u at its largest, rounded up to the whole)
+        } else {
+            // The warp whose runs hold the point, and the slot; the sums are those that made the total, added in the same order.
+            double lo = before, s = 0.0;
             bool here = false;
-            {
-                double s = 0.0;
-                for (int w = 0; w < kAccWarps; ++w) {
-                    const double to = s + sh.wpart[w];
-                    if (w == warp) lo = before + s, own = before + to;
-                    s = to;
-                }
-                here = lo <= point && point < own;
+            for (int w = 0; w < kAccWarps; ++w) {
+                const double to = s + sh.wpart[w];
+                if (w == warp) lo = before + s, here = before + s <= point && point < before + to;
+                s = to;
             }
             if (here) {
-                double sum = lo;
+                int slot = 0;
+                double at_slot = 0.0;  // (lo + the slots before: the warp's sum was added up in this order)
+                const int slots = (steps + group - 1) / group;
+                while (slot + 1 < slots && !(point < lo + (at_slot + sh.slot[warp][slot]))) at_slot += sh.slot[warp][slot++];
+                double sum = lo + at_slot;
                 int found = -1, seen = -1;
-                for (long long r = mine0; r < mine1 && found < 0; r += 32) {
-                    double w[8], s = 0.0;
-                    if (r + lane < mine1) {
-                        weights(8 * (r + lane), w);
-                    } else {
+                // (Through to the warp's last step: should the sums' rounding leave the point behind the slot, it is the first weight behind it.)
+#pragma unroll 1
+                for (int k = slot * group; k < steps && found < 0; ++k) {
+                    const long long r = mine0 + 32 * k + lane;
+                    double w[8], s8 = 0.0;
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) w[j] = 0.0;
+                    for (int j = 0; j < 8; ++j) w[j] = 0.0;
+                    if (r < mine1) {
+                        Place a;
+                        fetch(8 * r, a);
+                        weights(8 * r, a, w);
                     }
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) s += w[j];
-                    double upto = s;
+                    for (int j = 0; j < 8; ++j) s8 += w[j];
+                    double upto = s8;
 #pragma unroll
                     for (int d = 1; d < 32; d <<= 1) {
                         const double o = __shfl_up_sync(0xffffffffu, upto, d);
                         if (lane >= d) upto += o;
                     }
-                    double at = sum + (upto - s);
+                    double at = sum + (upto - s8);
                     int hit = 0x7fffffff;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         at += w[j];
                         if (w[j] > 0.0) {
-                            seen = (int)(8 * (r + lane) + j);
+                            seen = (int)(8 * r + j);
                             if (at > point && hit == 0x7fffffff) hit = seen;
                         }
                     }
@@ -400,25 +501,44 @@ __global__ void __launch_bounds__(kAccThreads) accept_kernel(const __grid_consta
                 if (lane == 0) p.next[b] = found >= 0 ? found : seen;  // (seen: the last of the run, should the sums' order leave the point behind it)
             }
         }
+        cluster_heard();  // no block leaves while another may still read its sums
     } else {
-        cluster_meet();  // no block leaves while another may still read its sums
+        cluster_meet();
     }
 }
 
-template <int KIND>
-int accept_launch(const AcceptParams& p, int batch, cudaStream_t stream) {
+template <int KIND, int WARPS>
+int accept_launch(AcceptParams p, int batch, int blocks, cudaStream_t stream) {
+    p.blocks = blocks;
+    static int configured_dev = -1;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (configured_dev != dev) {
+        const cudaError_t e = cudaFuncSetAttribute(accept_kernel<KIND, WARPS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return (int)e;
+        configured_dev = dev;
+    }
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)batch * kAccBlocks);
-    cfg.blockDim = dim3(kAccThreads);
+    cfg.gridDim = dim3((unsigned)batch * p.blocks);
+    cfg.blockDim = dim3(WARPS * 32);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = kAccBlocks;
+    attr[0].val.clusterDim.x = (unsigned)p.blocks;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1 + early_attribute(attr[1]);
-    return (int)cudaLaunchKernelEx(&cfg, accept_kernel<KIND>, p);
+    return (int)cudaLaunchKernelEx(&cfg, accept_kernel<KIND, WARPS>, p);
+}
+
+// Few requests: as many threads each as a cluster can have, while every block has an SM.  Many: blocks of which an SM holds two.
+template <int KIND>
+int accept_launch(const AcceptParams& p, int batch, cudaStream_t stream) {
+    const long long sms = sm_count();
+    if (batch * (long long)kAccMostBlocks <= sms) return accept_launch<KIND, kAccMostWarps>(p, batch, kAccMostBlocks, stream);
+    if (batch * 8ll <= sms) return accept_launch<KIND, kAccMostWarps>(p, batch, 8, stream);
+    return accept_launch<KIND, 8>(p, batch, 8, stream);
 }
 
 }  // namespace
@@ -435,7 +555,7 @@ extern "C" int glm53f_kda_accept_batch(int32_t batch, const int32_t* cu_rows, in
     if (batch == 0) return 0;
     if (!cu_rows || !target || !tokens || !u || !keep || !next) return kInvalid;
     if ((reinterpret_cast<uintptr_t>(target) & (target_kind == GLM53F_KDA_LOGITS_BF16 ? 1 : 3)) != 0 || (reinterpret_cast<uintptr_t>(draft) & 3) != 0) return kInvalid;
-    const AcceptParams p{cu_rows, vocab, ld, draft_ld, target, tokens, draft, temperature, u, keep, next};
+    const AcceptParams p{cu_rows, vocab, ld, draft_ld, target, tokens, draft, temperature, u, keep, next, 8};
     cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
     if (target_kind == GLM53F_KDA_LOGITS_F32) return accept_launch<GLM53F_KDA_LOGITS_F32>(p, batch, stream);
     if (target_kind == GLM53F_KDA_LOGITS_BF16) return accept_launch<GLM53F_KDA_LOGITS_BF16>(p, batch, stream);
