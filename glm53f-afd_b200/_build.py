@@ -72,7 +72,7 @@ def host_built_for() -> str:
 
 
 def _host_stale(src: str) -> bool:
-    if _stale(HOST, [src, LIB, os.path.join(INCLUDE, "glm53f_kda.h")]):
+    if _stale(HOST, [src, LIB, os.path.join(INCLUDE, "glm53f_kda.h"), os.path.join(INCLUDE, "glm53f_proj.h")]):
         return True
     with open(HOST, "rb") as f:
         return host_built_for().encode() + b"\0" not in f.read()

@@ -12,10 +12,12 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "glm53f_kda.h"
+#include "glm53f_proj.h"
 
 namespace {
 
@@ -275,6 +277,185 @@ int core_decode(PyObject* const* a) {
     });
 }
 
+// ---- linear.py, spec.py and proj.fused: the modules hold the same checks, with their errors ---------------------------------------
+inline int here() { return c10::cuda::current_device(); }
+inline const at::Tensor& on_device(PyObject* o, int dev) {
+    const at::Tensor& t = tensor(o);
+    if (!t.is_cuda() || t.get_device() != dev) throw Miss{};
+    return t;
+}
+template <typename T>
+T* need_here(PyObject* o, Kind kind, int64_t n, int dev) {
+    on_device(o, dev);
+    return need<T>(o, kind, n);
+}
+inline bool is_bf16(const at::Tensor& t) {
+    const auto d = t.scalar_type();
+    return d == at::kBFloat16 || d == at::kShort || d == at::kUInt16;
+}
+// `rows` rows of heads x 128 bf16 values: [rows][heads x 128] or [rows][heads][128], rows any multiple of eight elements apart.
+inline Rows head_rows(PyObject* o, int64_t rows, int64_t heads, int dev) {
+    const at::Tensor& t = on_device(o, dev);
+    const int64_t width = heads * kD;
+    if (!is_bf16(t) || t.dim() < 2 || t.dim() > 3 || t.size(0) < rows) throw Miss{};
+    if (t.dim() == 2 ? t.size(1) != width || t.stride(1) != 1 : t.size(1) != heads || t.size(2) != kD || t.stride(2) != 1 || (heads > 1 && t.stride(1) != kD)) throw Miss{};
+    const int64_t stride = t.size(0) > 1 ? t.stride(0) : width;
+    auto* at = static_cast<glm53f_bf16*>(t.data_ptr());
+    if (stride % 8 || stride < width || (reinterpret_cast<uintptr_t>(at) & 15)) throw Miss{};
+    return {at, stride};
+}
+
+// lin(prefill, heads, qk_heads, rows, max_len, cu_rows, q, k, v, g, state, state_off, keep, state_out, scale, out, workspace, max_state_off)
+int lin(PyObject* const* a) {
+    const bool prefill = a[0] == Py_True;
+    const int64_t heads = to_i64(a[1]), qk = to_i64(a[2]), rows = to_i64(a[3]), max_len = to_i64(a[4]);
+    if (heads < 1 || heads > 65535 || qk < 1 || heads % qk || rows < 1 || rows > 0x7fffffff || max_len < 0 || max_len > rows) throw Miss{};
+    const int dev = here();
+    const auto* cu = need_here<const int32_t>(a[5], kI32, 2, dev);
+    const int64_t batch = tensor(a[5]).numel() - 1;
+    if (batch > 65535) throw Miss{};
+    const Rows q = head_rows(a[6], rows, qk, dev), k = head_rows(a[7], rows, qk, dev), v = head_rows(a[8], rows, heads, dev);
+    const at::Tensor& g = on_device(a[9], dev);
+    if (g.scalar_type() != at::kFloat || g.numel() == 0) throw Miss{};
+    int64_t g_stride = 0;
+    if (g.dim() == 1) {
+        if (g.size(0) != heads || (heads > 1 && g.stride(0) != 1)) throw Miss{};
+    } else {
+        if (g.dim() != 2 || g.size(0) < rows || g.size(1) != heads || (heads > 1 && g.stride(1) != 1)) throw Miss{};
+        g_stride = g.size(0) > 1 ? g.stride(0) : heads;
+        if (g_stride < heads) throw Miss{};
+    }
+    const at::Tensor& state = on_device(a[10], dev);
+    const bool f32 = state.scalar_type() == at::kFloat;
+    if ((!f32 && !is_bf16(state)) || !state.is_contiguous()) throw Miss{};
+    const auto* off = need_here<const int64_t>(a[11], kI64, batch, dev);
+    const auto* keep = a[12] == Py_None ? nullptr : need_here<const int32_t>(a[12], kI32, batch, dev);
+    if (a[17] != Py_None) {
+        const int64_t most = to_i64(a[17]);
+        if (most < 0 || state.numel() < mul_add(most, 1, heads * kD * kD)) throw Miss{};
+    }
+    void *si = state.data_ptr(), *so = nullptr;
+    if (PyUnicode_Check(a[13])) {
+        so = si;
+    } else if (a[13] != Py_None) {
+        const at::Tensor& t = on_device(a[13], dev);
+        if (t.scalar_type() != state.scalar_type() || t.numel() < state.numel() || !t.is_contiguous()) throw Miss{};
+        so = t.data_ptr();
+        const auto x = reinterpret_cast<uintptr_t>(si), y = reinterpret_cast<uintptr_t>(so);
+        if (x != y && y < x + state.nbytes() && x < y + t.nbytes()) throw Miss{};
+    }
+    double scale = 0.08838834764831845;
+    if (a[14] != Py_None) {
+        if (!PyFloat_CheckExact(a[14])) throw Miss{};
+        scale = PyFloat_AS_DOUBLE(a[14]);
+    }
+    const Rows out = a[15] == Py_None ? Rows{nullptr, 0} : head_rows(a[15], rows, heads, dev);
+    const auto st = reinterpret_cast<glm53f_stream_t>(c10::cuda::getCurrentCUDAStream().stream());
+    const auto* gp = static_cast<const float*>(g.data_ptr());
+    if (!prefill) {
+        if (so == nullptr && out.ptr == nullptr) throw Miss{};
+        return unlocked([&] {
+            return glm53f_kda_lin_decode_batch((int32_t)heads, (int32_t)qk, (int32_t)batch, cu, keep, q.ptr, q.stride, k.ptr, k.stride, v.ptr, v.stride, gp, g_stride,
+                                               si, so, off, f32 ? 0 : 1, (float)scale, out.ptr, out.stride, st);
+        });
+    }
+    if (so == nullptr || out.ptr == nullptr) throw Miss{};
+    void* ws = nullptr;
+    int64_t bytes = 0;
+    if (a[16] != Py_None) {
+        const at::Tensor& w = on_device(a[16], dev);
+        if (!w.is_contiguous()) throw Miss{};
+        bytes = (int64_t)w.nbytes();
+        ws = bytes != 0 ? w.data_ptr() : nullptr;
+    }
+    return unlocked([&] {
+        return glm53f_kda_lin_prefill_varlen((int32_t)heads, (int32_t)qk, (int32_t)batch, cu, (int32_t)rows, (int32_t)max_len, q.ptr, q.stride, k.ptr, k.stride, v.ptr,
+                                             v.stride, gp, g_stride, si, so, off, f32 ? 0 : 1, (float)scale, out.ptr, out.stride, ws, bytes, st);
+    });
+}
+
+// accept(cu_rows, tokens, target, u, keep, next, probabilities, draft, temperature)
+int accept(PyObject* const* a) {
+    const int dev = here();
+    const auto* cu = need_here<const int32_t>(a[0], kI32, 2, dev);
+    const int64_t batch = tensor(a[0]).numel() - 1;
+    const auto* tokens = need_here<const int32_t>(a[1], kI32, 1, dev);
+    const int64_t rows = tensor(a[1]).numel();
+    if (batch > 0xffffff || (a[6] != Py_True && a[6] != Py_False)) throw Miss{};
+    const bool probabilities = a[6] == Py_True;
+    auto matrix = [&](PyObject* o, int64_t vocab, int64_t& ld) -> const at::Tensor& {
+        const at::Tensor& t = on_device(o, dev);
+        if (t.dim() != 2 || t.size(0) < rows || t.size(1) < 1 || t.size(1) > 0x7fffffff || (vocab > 0 && t.size(1) != vocab) || (t.size(1) > 1 && t.stride(1) != 1))
+            throw Miss{};
+        ld = t.size(0) > 1 ? t.stride(0) : t.size(1);
+        if (ld < t.size(1)) throw Miss{};
+        return t;
+    };
+    int64_t ld = 0, draft_ld = 0;
+    const at::Tensor& target = matrix(a[2], 0, ld);
+    const int64_t vocab = target.size(1);
+    const bool f32 = target.scalar_type() == at::kFloat;
+    if (!f32 && (probabilities || target.scalar_type() != at::kBFloat16)) throw Miss{};
+    const float *draft = nullptr, *temperature = nullptr;
+    if (a[7] != Py_None) {
+        const at::Tensor& d = matrix(a[7], vocab, draft_ld);
+        if (d.scalar_type() != at::kFloat) throw Miss{};
+        draft = static_cast<const float*>(d.data_ptr());
+    }
+    if (a[8] != Py_None) {
+        if (probabilities) throw Miss{};
+        temperature = need_here<const float>(a[8], kF32, batch, dev);
+    }
+    const auto* u = need_here<const float>(a[3], kF32, rows, dev);
+    auto *keep = need_here<int32_t>(a[4], kI32, batch, dev), *next = need_here<int32_t>(a[5], kI32, batch, dev);
+    const auto st = reinterpret_cast<glm53f_stream_t>(c10::cuda::getCurrentCUDAStream().stream());
+    const void* tp = target.data_ptr();
+    const int32_t kind = probabilities ? GLM53F_KDA_PROBABILITIES : f32 ? GLM53F_KDA_LOGITS_F32 : GLM53F_KDA_LOGITS_BF16;
+    return unlocked([&] { return glm53f_kda_accept_batch((int32_t)batch, cu, (int32_t)vocab, tp, kind, ld, tokens, draft, draft_ld, temperature, u, keep, next, st); });
+}
+
+// proj_fused(x, ldx, x_gstride, w, n, k, ldw, groups, w_gstride, rows, out, ldo, o_gstride, out_f32, x_offset, out_offset, bias, activation, residual, ldr, r_gstride,
+// residual_offset)
+int proj_fused(PyObject* const* a) {
+    const int dev = here();
+    const at::Tensor &x = on_device(a[0], dev), &w = on_device(a[3], dev), &out = on_device(a[10], dev);
+    const int64_t ldx = to_i64(a[1]), xg = to_i64(a[2]), n = to_i64(a[4]), k = to_i64(a[5]), ldw = to_i64(a[6]), groups = to_i64(a[7]), wg = to_i64(a[8]),
+                  rows = to_i64(a[9]), ldo = to_i64(a[11]), og = to_i64(a[12]), x_offset = to_i64(a[14]), o_offset = to_i64(a[15]), act = to_i64(a[17]);
+    const bool f32 = a[13] == Py_True;
+    if (!f32 && a[13] != Py_False) throw Miss{};
+    for (int64_t v : {ldx, xg, n, k, ldw, groups, wg, rows, ldo, og, x_offset, o_offset})
+        if (v < 0 || v > 0x3fffffffffll) throw Miss{};
+    if (groups < 1 || rows < 1 || n < 1 || k < 1 || groups > 0xffff || rows > 0x7fffffff || n > 0x7fffffff || k > 0x7fffffff) throw Miss{};
+    auto fits = [&](const at::Tensor& t, int64_t offset, int64_t gs, int64_t r, int64_t ld, int64_t width) {
+        return mul_add(groups - 1, gs, mul_add(r - 1, ld, mul_add(offset, 1, width))) <= t.numel();
+    };
+    if (!is_bf16(x) || !is_bf16(w) || (f32 ? out.scalar_type() != at::kFloat : out.element_size() != 2)) throw Miss{};
+    if (!fits(x, x_offset, xg, rows, ldx, k) || !fits(w, 0, wg, n, ldw, k) || !fits(out, o_offset, og, rows, ldo, n)) throw Miss{};
+    glm53f_proj_epilogue e{};
+    if (act < GLM53F_PROJ_NONE || act > GLM53F_PROJ_SIGMOID) throw Miss{};
+    e.activation = (int32_t)act;
+    if (a[16] != Py_None) {
+        const at::Tensor& b = on_device(a[16], dev);
+        e.bias_f32 = b.scalar_type() == at::kFloat;
+        if ((!e.bias_f32 && !is_bf16(b)) || !b.is_contiguous() || b.numel() != groups * n) throw Miss{};
+        e.bias = b.data_ptr();
+        e.bias_gstride = n;
+    }
+    if (a[18] != Py_None) {
+        const at::Tensor& r = on_device(a[18], dev);
+        e.ldr = a[19] == Py_None ? ldo : to_i64(a[19]);
+        e.r_gstride = a[20] == Py_None ? og : to_i64(a[20]);
+        const int64_t offset = to_i64(a[21]);
+        if (f32 ? r.scalar_type() != at::kFloat : !is_bf16(r)) throw Miss{};
+        if (offset < 0 || e.ldr < n || e.r_gstride < 0 || !fits(r, offset, e.r_gstride, rows, e.ldr, n)) throw Miss{};
+        e.residual = static_cast<const unsigned char*>(r.data_ptr()) + offset * r.element_size();
+    }
+    const glm53f_proj_job job{static_cast<const uint16_t*>(x.data_ptr()) + x_offset, ldx, xg, static_cast<const uint16_t*>(w.data_ptr()), ldw, wg, (int32_t)groups,
+                              (int32_t)rows, (int32_t)n, (int32_t)k, static_cast<unsigned char*>(out.data_ptr()) + o_offset * out.element_size(), f32 ? 1 : 0, ldo, og};
+    const auto st = reinterpret_cast<glm53f_stream_t>(c10::cuda::getCurrentCUDAStream().stream());
+    return unlocked([&] { return glm53f_kda_proj_bf16_fused(&job, &e, st); });
+}
+
 template <typename F>
 PyObject* answer(F&& f) {
     long code = -1;
@@ -295,6 +476,15 @@ PyObject* py_chain_batch(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 PyObject* py_core_decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return answer([&] { return n == 18 ? core_decode(args) : -1; });
+}
+PyObject* py_lin(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return answer([&] { return n == 18 ? lin(args) : -1; });
+}
+PyObject* py_accept(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return answer([&] { return n == 9 ? accept(args) : -1; });
+}
+PyObject* py_proj_fused(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return answer([&] { return n == 22 ? proj_fused(args) : -1; });
 }
 // raw_stream(Stream) -> the CUDA stream's address, or None for a stream it does not know.
 PyObject* py_raw_stream(PyObject*, PyObject* s) {
@@ -326,6 +516,9 @@ PyMethodDef methods[] = {
     {"chain_batch", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_chain_batch)), METH_FASTCALL, nullptr},
     {"raw_stream", py_raw_stream, METH_O, nullptr},
     {"core_decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_core_decode)), METH_FASTCALL, nullptr},
+    {"lin", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_lin)), METH_FASTCALL, nullptr},
+    {"accept", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_accept)), METH_FASTCALL, nullptr},
+    {"proj_fused", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_proj_fused)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Native host path of the per-layer launches.", -1, methods, nullptr, nullptr, nullptr, nullptr};

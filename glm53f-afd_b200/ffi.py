@@ -116,7 +116,7 @@ _native = None
 class _PythonPath:
     """Stands in for the native host path: it takes no call, so every launch goes through the Python checks and ctypes."""
 
-    core_decode = chain_batch = staticmethod(lambda *_: -1)
+    core_decode = chain_batch = lin = accept = proj_fused = staticmethod(lambda *_: -1)
     raw_stream = staticmethod(lambda _: None)
 
 

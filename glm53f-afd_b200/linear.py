@@ -96,6 +96,10 @@ def decode_batch(heads, rows, cu_rows, q, k, v, g, state, state_off, *, qk_heads
     on the device.  state_out: "in_place", None (a verify: not written) or a tensor; out=None writes no outputs (a commit of kept
     rows).  A verify and a commit of k rows leave the bits of k single-row calls."""
     qk_heads = heads if qk_heads is None else qk_heads
+    code = ffi.host().lin(False, heads, qk_heads, rows, 0, cu_rows, q, k, v, g, state, state_off, keep, state_out, scale, out, None, max_state_off)
+    if code >= 0:
+        return _launched(code, "glm53f_kda_lin_decode_batch")
+    # Not the plain accepted call: the same checks here, with their errors.
     batch, args, kind, o, o_stride = _tokens(heads, qk_heads, rows, cu_rows, q, k, v, g, state, state_off, out)
     if keep is not None:
         _need(keep, "keep", (torch.int32,), batch)
@@ -116,6 +120,9 @@ def prefill_varlen(heads, rows, cu_rows, max_len, q, k, v, g, state, state_off, 
     """glm53f_kda_lin_prefill_varlen: chunked prefill of packed sequences, the longest of at most max_len rows.  `workspace`: a CUDA uint8
     tensor of `prefill_workspace_bytes` bytes, or None."""
     qk_heads = heads if qk_heads is None else qk_heads
+    code = ffi.host().lin(True, heads, qk_heads, rows, max_len, cu_rows, q, k, v, g, state, state_off, None, state_out, scale, out, workspace, max_state_off)
+    if code >= 0:
+        return _launched(code, "glm53f_kda_lin_prefill_varlen")
     if not 0 <= max_len <= rows:
         raise Invalid(f"max_len {max_len} of {rows} rows")
     if out is None:

@@ -73,6 +73,11 @@ def fused(x: torch.Tensor, ldx: int, x_gstride: int, w: Bf16Mat, rows: int, out:
         raise Invalid(f"activation {activation!r}: one of {', '.join(ACTIVATIONS)}")
     if rows == 0:
         return
+    code = ffi.host().proj_fused(x, ldx, x_gstride, w.t, w.n, w.k, w.ld, w.groups, w.gstride, rows, out, ldo, o_gstride, out_f32, x_offset, out_offset, bias,
+                                 ACTIVATIONS[activation], residual, ldr, r_gstride, residual_offset)
+    if code >= 0:
+        return _launched(code, "glm53f_kda_proj_bf16_fused")
+    # Not the plain accepted call: the same checks here, with their errors.
     job = _job(x, ldx, x_gstride, w, rows, out, ldo, o_gstride, out_f32, x_offset, out_offset)
     e = ffi.ProjEpilogue(activation=ACTIVATIONS[activation])
     if bias is not None:

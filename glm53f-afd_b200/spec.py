@@ -31,6 +31,10 @@ def accept_batch(cu_rows, tokens, target, u, keep, next, *, probabilities=False,
     0: greedy; None: 1), or f32 probabilities.  `draft` f32 [rows][vocab]: row i is what tokens[i] was drawn from (None: the
     drafter had one choice).  u f32 [rows] in [0, 1): u[i] judges tokens[i], a window's first draws the next token.  Writes
     int32 keep[b], the rows to commit (1 .. the window's), and next[b], the token behind them (-1: the row left nothing)."""
+    code = ffi.host().accept(cu_rows, tokens, target, u, keep, next, probabilities, draft, temperature)
+    if code >= 0:
+        return _launched(code, "glm53f_kda_accept_batch")
+    # Not the plain accepted call: the same checks here, with their errors.
     _need(cu_rows, "cu_rows", (torch.int32,), 1)
     batch = cu_rows.numel() - 1
     _need(tokens, "tokens", (torch.int32,), 0)
