@@ -3,7 +3,7 @@
 //     S_t = e^g_t S_{t-1} + v_t k_t^T        y_t = scale S_t q_t        (S: [128 (v)][128 (k)] per request and head)
 //
 // Bound by HBM: a unit (request, head) reads and writes its state once, 64 or 32 KiB each way, beside 1 KiB a row.  The value rows of
-// a state do not depend on one another, so a block of four warps takes half of a unit and nothing is shared: a thread keeps four value rows x sixteen
+// a state do not depend on one another, so a block of two warps takes a quarter of a unit and nothing is shared: a thread keeps four value rows x sixteen
 // key channels in registers from the load to the store, all of its loads in flight at once, and walks the rows of the
 // window.  Eight lanes make a value row's sum: the thread adds its sixteen products in order, then a halving exchange over the eight lanes adds the
 // four rows' partial sums at once (four shuffles for four rows).  The arithmetic of a row does not depend on the call it
@@ -15,7 +15,7 @@
 namespace kda {
 namespace {
 
-constexpr int kLinThreads = 128, kLinSplit = 2;  // blocks a unit
+constexpr int kLinThreads = 64, kLinSplit = 4;  // blocks a unit (of 128 threads, two a unit: 48 windows of 16 rows of f32 states 234 us, so 188; single rows the same)
 
 struct LinStepParams {
     int heads, share;  // share: heads to a head of q and k
@@ -47,6 +47,13 @@ __device__ __forceinline__ void widen8(const uint4& u, float* x) {
         x[2 * i] = __uint_as_float(w[i] << 16);
         x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
+}
+
+// Two values rounded at once: one by one the conversions go through the unit of the transcendental functions, a quarter as fast (windows of 16 slots 36.6 us so, of which
+// that unit was busy two thirds).
+__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 // A thread's four rows x (two runs of eight channels, 64 apart).  The vector forms need the state on 16 bytes.
@@ -100,7 +107,7 @@ __device__ __forceinline__ void store_state(void* base, long long at, bool vec, 
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float *x = &s[i][8 * j + 2 * e];
-                    w[e] = (uint32_t)f32_to_bf16_bits(x[0]) | (uint32_t)f32_to_bf16_bits(x[1]) << 16;
+                    w[e] = bf16x2(x[0], x[1]);
                 }
                 if (vec) {
                     *reinterpret_cast<uint4*>(p + i * DK + 64 * j) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -128,7 +135,7 @@ __device__ __forceinline__ void store_state(void* base, long long at, bool vec, 
 
 // ROUND: a bf16 state is rounded after every row (the prefill rounds once, when it stores).
 template <bool BF16, bool ROUND>
-__global__ void __launch_bounds__(kLinThreads) lin_step_kernel(const __grid_constant__ LinStepParams p) {
+__global__ void __launch_bounds__(kLinThreads, 8) lin_step_kernel(const __grid_constant__ LinStepParams p) {
     grid_ready();
     const long long unit = blockIdx.x / kLinSplit;
     const int b = (int)(unit / p.heads), h = (int)(unit % p.heads);
@@ -183,7 +190,10 @@ __global__ void __launch_bounds__(kLinThreads) lin_step_kernel(const __grid_cons
             for (int j = 0; j < 16; j += 2) {
                 const float2 add = mul2(v2, make_float2(kk[j], kk[j + 1]));  // exact: two bf16 factors
                 float2 z = fma2(make_float2(s[i][j], s[i][j + 1]), d2, add);
-                if constexpr (BF16 && ROUND) z = make_float2(bf16_round(z.x), bf16_round(z.y));
+                if constexpr (BF16 && ROUND) {
+                    const uint32_t two = bf16x2(z.x, z.y);
+                    z = make_float2(__uint_as_float(two << 16), __uint_as_float(two & 0xffff0000u));
+                }
                 s[i][j] = z.x, s[i][j + 1] = z.y;
                 sum = fma2(z, make_float2(qq[j], qq[j + 1]), sum);
             }
