@@ -44,13 +44,11 @@ struct AccShared {
     float max[kAccRows], sum[kAccRows];
     int best[kAccRows];
     double part;      // the slice's weights
-    int last;         // the slice's last index with a weight, or -1
     // Within the block.
     float wmax[kAccRows][kAccMostWarps], wsum[kAccRows][kAccMostWarps];
     int wbest[kAccRows][kAccMostWarps];
     double wpart[kAccMostWarps];
     double slot[kAccMostWarps][32];  // a warp's weights, its places in 32 parts
-    int wlast[kAccMostWarps];
     float row_max[kAccRows], row_sum[kAccRows];
     int row_best[kAccRows];
     int kept;
@@ -119,6 +117,17 @@ struct Eight {
         if (vec && i + 8 <= end) load_whole(row, i);
         else load_some(row, i, end, fill);
     }
+    // The largest of them (NaN only where all are).
+    __device__ __forceinline__ float top() const {
+        if constexpr (kWords == 8) {
+            const float* x = reinterpret_cast<const float*>(w);
+            return fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        } else {
+            const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(w);
+            const __nv_bfloat162 m = __hmax2(__hmax2(x[0], x[1]), __hmax2(x[2], x[3]));
+            return fmaxf(__low2float(m), __high2float(m));
+        }
+    }
     __device__ __forceinline__ void get(float (&x)[8]) const {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -128,28 +137,27 @@ struct Eight {
     }
 };
 
-// e^x for x <= 0 to a few units of 2^-52: x = (32 e + j) ln 2 / 32 + r, so e^x = 2^e 2^(j/32) e^r with |r| < 0.011, of which Taylor's series to
-// the fifth power leaves 3e-15.  (Half the double-precision operations of the general function, which were what a draw spent its time on.)
-__device__ __forceinline__ double exp_below(double x, const double* power) {
+// A row's weights in 64 bits: e^x of x = (l - max) / t <= 0.  x = (32 e + j) ln 2 / 32 + r, so e^x = 2^e 2^(j/32) e^r with |r| < 0.011, of which
+// Taylor's series to the fourth power leaves 1.3e-12: a draw among 131,072 moves by it once in ten million.  (With the general exponential, and every
+// special case looked at for every entry, a draw's pass took four times as many instructions.)  NaN and what is below e^-690 is 0.  Rows whose
+// largest is infinite: see weights() in the kernel.
+constexpr double kTurns = 46.166241308446828384;  // 32 / ln 2
+struct RowScale {
+    double max, inv_t, turns;  // turns: inv_t 32 / ln 2
+};
+__device__ __forceinline__ double logit_weight(float l, const RowScale& a, const double* power) {
     const double magic = 6755399441055744.0;  // 1.5 2^52: adding it rounds to an integer, which the low word then holds
-    const double shifted = fma(x, 46.166241308446828384, magic);
+    const double d = (double)l - a.max, x = d * a.inv_t, shifted = fma(d, a.turns, magic);
     const int n = __double2loint(shifted);
     const double whole = shifted - magic;
     double r = fma(whole, -0.021660849390173098, x);
     r = fma(whole, -2.325192846878874e-12, r);
-    double y = fma(r, 1.0 / 120, 1.0 / 24);
-    y = fma(r, y, 1.0 / 6);
+    double y = fma(r, 1.0 / 24, 1.0 / 6);
     y = fma(r, y, 0.5);
     y = fma(r, y, 1.0);
     y = fma(r, y, 1.0);
     const double base = power[n & 31];
-    return x < -690.0 ? 0.0 : y * __hiloint2double(__double2hiint(base) + ((n >> 5) << 20), __double2loint(base));
-}
-// e^((l - max) / t) with the largest logits at exactly 1 (an infinite one too) and NaN at 0.
-__device__ __forceinline__ double logit_weight(float l, float max, double inv_t, const double* power) {
-    if (l == max) return 1.0;
-    const double e = exp_below(((double)l - (double)max) * inv_t, power);
-    return l < max ? e : 0.0;
+    return x > -690.0 ? y * __hiloint2double(__double2hiint(base) + ((n >> 5) << 20), __double2loint(base)) : 0.0;
 }
 __device__ __forceinline__ float finite_weight(float p) { return p > 0.0f && p < INFINITY ? p : 0.0f; }
 
@@ -158,11 +166,13 @@ struct Stats {
     float m = kNoLogit, s = 0.0f;
     int best = -1;
 };
-template <bool GREEDY>
-__device__ __forceinline__ void take(Stats& a, const float (&x)[8], int at, long long vocab, float scale) {
-    float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+template <bool GREEDY, int KIND>
+__device__ __forceinline__ void take(Stats& a, const Eight<KIND>& in, int at, long long vocab, float scale) {
+    const float top = in.top();
+    float x[8];
     if constexpr (GREEDY) {
         if (top > a.m || a.best < 0) {
+            in.get(x);
             a.m = fmaxf(top, a.m);
 #pragma unroll
             for (int j = 7; j >= 0; --j)
@@ -173,16 +183,20 @@ __device__ __forceinline__ void take(Stats& a, const float (&x)[8], int at, long
             a.s *= a.m == kNoLogit ? 0.0f : ex2_approx((a.m - top) * scale);
             a.m = top;
         }
-        float e[8];
+        in.get(x);
+        float2 sum[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = ex2_ftz((x[j] - a.m) * scale);
-        float sum = ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-        if (!(sum < INFINITY)) {  // a NaN among them, or infinities: seldom, so one at a time
-            sum = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sum += x[j] == a.m ? (a.m == kNoLogit ? 0.0f : 1.0f) : x[j] < a.m ? ex2_ftz((x[j] - a.m) * scale) : 0.0f;
+        for (int j = 0; j < 4; ++j) {
+            const float2 t = mul2(fma2(make_float2(a.m, a.m), make_float2(-1.0f, -1.0f), make_float2(x[2 * j], x[2 * j + 1])), make_float2(scale, scale));
+            sum[j] = make_float2(ex2_ftz(t.x), ex2_ftz(t.y));
         }
-        a.s += sum;
+        float all = ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) + ((sum[2].x + sum[2].y) + (sum[3].x + sum[3].y));
+        if (!(all < INFINITY)) {  // a NaN among them, or infinities: seldom, so one at a time
+            all = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) all += x[j] == a.m ? (a.m == kNoLogit ? 0.0f : 1.0f) : x[j] < a.m ? ex2_ftz((x[j] - a.m) * scale) : 0.0f;
+        }
+        a.s += all;
     }
 }
 // Over the lanes of a warp.
@@ -249,7 +263,7 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
             if (token < 0 || token >= p.vocab) token = -1;
             if (token >= 0 && !greedy) {
                 token_target = target_at<KIND>(row_at(i), token);
-                token_left = (double)p.u[first + i + 1] * (p.draft == nullptr ? 1.0 : (double)finite_weight(draft_at(i + 1)[token]));
+                token_left = (double)p.u[first + i + 1] * (p.draft == nullptr ? 1.0 : (double)fmaxf(draft_at(i + 1)[token], 0.0f));
             }
         }
         if constexpr (LOGITS) {
@@ -274,9 +288,7 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
                         if (r + kAccThreads < run1) load(r + kAccThreads, ahead);
 #pragma unroll
                         for (int d = 0; d < kAccDeep; ++d) {
-                            float x[8];
-                            now[d].get(x);
-                            take<GREEDY>(st[d], x, (int)(8 * r), p.vocab, scale);
+                            take<GREEDY>(st[d], now[d], (int)(8 * r), p.vocab, scale);
                             now[d] = ahead[d];
                         }
                     }
@@ -316,7 +328,11 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
             if (token >= 0) {
                 if (greedy) keep = token == sh.row_best[lane] && sh.row_max[lane] != kNoLogit;
                 else if constexpr (LOGITS)
-                    keep = token_left * (double)sh.row_sum[lane] < logit_weight(token_target, sh.row_max[lane], inv_t, sh.power) && sh.row_max[lane] != kNoLogit;
+                {
+                    const float m = sh.row_max[lane];
+                    const double e = token_target == m ? 1.0 : m < INFINITY ? logit_weight(token_target, {(double)m, inv_t, inv_t * kTurns}, sh.power) : 0.0;
+                    keep = token_left * (double)sh.row_sum[lane] < e && m != kNoLogit;
+                }
                 else keep = token_left < (double)finite_weight(token_target);
             }
             const unsigned all = __ballot_sync(0xffffffffu, keep);
@@ -343,7 +359,9 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
         const float* less = whole || p.draft == nullptr ? nullptr : draft_at(stop + 1);
         const int token = whole ? -1 : p.tokens[first + stop + 1];
         int mode = whole ? kWhole : less != nullptr ? kLessDraft : kWithout;
-        const double x01 = fmax((double)p.u[first], 0.0);
+        // (Short of 1, whatever is given: the drawn point then lies before the whole.)
+        const double x01 = fmin(fmax((double)p.u[first], 0.0), 1.0 - 0x1p-53);
+        const RowScale row_scale{(double)stop_max, inv_t, inv_t * kTurns};
         double norm = 1.0;  // the weights' sum, by which the drafter's probabilities are multiplied instead of dividing each of p's
         struct Place {
             Eight<KIND> x;
@@ -356,20 +374,25 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
         auto weights = [&](long long i, const Place& a, double (&w)[8]) {
             float x[8];
             a.x.get(x);
+            if constexpr (!LOGITS) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if constexpr (LOGITS) w[j] = stop_max == kNoLogit ? 0.0 : logit_weight(x[j], stop_max, inv_t, sh.power);
-                else w[j] = (double)finite_weight(x[j]);
+                for (int j = 0; j < 8; ++j) w[j] = (double)finite_weight(x[j]);
+            } else if (fabsf(stop_max) < INFINITY) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j] = logit_weight(x[j], row_scale, sh.power);
+            } else {  // infinite logits share everything; of -inf alone nothing is left
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j] = x[j] == INFINITY ? 1.0 : 0.0;
             }
             if (mode == kLessDraft) {
                 float y[8];
                 a.y.get(y);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const double rest = w[j] - (double)finite_weight(y[j]) * norm;
+                    const double rest = fma((double)fmaxf(y[j], 0.0f), -norm, w[j]);
                     w[j] = rest > 0.0 ? rest : 0.0;
                 }
-            } else if (mode == kWithout) {
+            } else if (mode == kWithout && token >= i && token < i + 8) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     if (i + j == token) w[j] = 0.0;
@@ -379,13 +402,12 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
         const long long mine0 = run0 + (run1 - run0) * warp / kAccWarps, mine1 = run0 + (run1 - run0) * (warp + 1) / kAccWarps;
         const int steps = (int)((mine1 - mine0 + 31) / 32), group = (steps + 31) / 32;
         double before = 0.0, total = 0.0;
-        int last = -1;
         // Passes over the row, one body of code: of logits with the drafter's probabilities first the weights' sum, then what is drawn from, and
         // once more where that leaves nothing.
         const int drawn_from = mode;
         if (LOGITS && drawn_from == kLessDraft) mode = kWhole;
         for (bool said = false;; said = true) {
-            int seen = -1, in_slot = 0, slot = 0;
+            int in_slot = 0, slot = 0;
             double part = 0.0, s = 0.0;
             Place now, ahead;
             if (mine0 + lane < mine1) fetch(8 * (mine0 + lane), now);
@@ -396,11 +418,7 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
                 if (r < mine1) {
                     double w[8];
                     weights(8 * r, now, w);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        s += w[j];
-                        if (w[j] > 0.0) seen = (int)(8 * r + j);
-                    }
+                    s += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
                 }
                 now = ahead;
                 if (++in_slot == group || k + 1 == steps) {
@@ -413,20 +431,17 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
                     ++slot;
                 }
             }
-            seen = __reduce_max_sync(0xffffffffu, seen);
-            if (lane == 0) sh.wpart[warp] = part, sh.wlast[warp] = seen;
+            if (lane == 0) sh.wpart[warp] = part;
             __syncthreads();
             if (said) cluster_heard();  // (the last pass's sums have been read everywhere)
             if (tid == 0) {
                 double t = 0.0;
-                int l = -1;
-                for (int w = 0; w < kAccWarps; ++w) t += sh.wpart[w], l = max(l, sh.wlast[w]);
-                sh.part = t, sh.last = l;
+                for (int w = 0; w < kAccWarps; ++w) t += sh.wpart[w];
+                sh.part = t;
             }
             cluster_meet();
             // Every warp adds the blocks' sums in the same order; each lane has fetched one.
             const double theirs = lane < blocks ? peer_f64(&sh.part, lane) : 0.0;
-            last = __reduce_max_sync(0xffffffffu, lane < blocks ? peer_i32(&sh.last, lane) : -1);
             total = 0.0;
             for (int c = 0; c < blocks; ++c) {
                 if (c == (int)block) before = total;
@@ -445,8 +460,6 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
         const double point = x01 * total;
         if (!(total > 0.0)) {
             if (block == 0 && tid == 0) p.next[b] = -1;
-        } else if (!(point < total)) {
-            if (block == 0 && tid == 0) p.next[b] = last;  // (u at its largest, rounded up to the whole)
         } else {
             // The warp whose runs hold the point, and the slot; the sums are those that made the total, added in the same order.
             double lo = before, s = 0.0;
