@@ -48,7 +48,6 @@ constexpr int kStages = 3, kStage = 3 * kTile;
 constexpr int oQ = kStages * kStage;                    // scale e^G Q, f32: four boxes of 64 rows x 32 channels
 constexpr int oP = oQ + 2 * kTile;                      // P: hi | lo, two buffers
 constexpr int oY = oP + 4 * kBox;                       // half a chunk's outputs on their way out
-constexpr int kDecays = 4;                              // chunks of decay factors in flight
 struct Decays {
     float2 g[CH];     // G in powers of two: hi, lo
     float e[CH];      // scale e^G
@@ -56,10 +55,9 @@ struct Decays {
     float all, pad[3];  // e^G of the whole chunk
 };
 constexpr int oDecays = oY + kTile / 2;
-constexpr int oBars = oDecays + kDecays * (int)sizeof(Decays);
+constexpr int oBars = oDecays + kStages * (int)sizeof(Decays);  // (a chunk's factors come and go with its rows)
 enum : int {
-    bFull = 0, bEmpty = bFull + kStages, bQK = bEmpty + kStages, bP, bQ, bState, bQS, bAdd = bQS + 2, bU = bAdd + 2, bO = bU + 2, bOFree = bO + 2, bDecay = bOFree + 2,
-    bDecayFree = bDecay + kDecays, kBars = bDecayFree + kDecays
+    bFull = 0, bEmpty = bFull + kStages, bQK = bEmpty + kStages, bP, bReady, bState, bQS, bAdd = bQS + 2, bU = bAdd + 2, bO = bU + 2, bOFree = bO + 2, kBars = bOFree + 2
 };
 constexpr int oCtl = oBars + (kBars + 1) / 2 * 16;
 constexpr int kSmem = oCtl + 16 + 1024;
@@ -116,13 +114,12 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
     uint32_t* tmem_slot = const_cast<uint32_t*>(ctl) + 2;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        for (int i = 0; i < kStages; ++i) mbar_init(&bar[bFull + i], 1), mbar_init(&bar[bEmpty + i], STATE ? 1 : 2);
+        for (int i = 0; i < kStages; ++i) mbar_init(&bar[bFull + i], 2), mbar_init(&bar[bEmpty + i], STATE ? 1 : 2);  // (full: the copies and the decays)
         mbar_init(&bar[bQK], 1);
         mbar_init(&bar[bP], 4);
-        mbar_init(&bar[bQ], 4);
+        mbar_init(&bar[bReady], 5);  // q of a chunk (four warps), and the chunk before added to the state
         mbar_init(&bar[bState], 8);
         for (int i = 0; i < 2; ++i) mbar_init(&bar[bQS + i], 1), mbar_init(&bar[bAdd + i], 16), mbar_init(&bar[bU + i], 1), mbar_init(&bar[bO + i], 1), mbar_init(&bar[bOFree + i], 4);
-        for (int i = 0; i < kDecays; ++i) mbar_init(&bar[bDecay + i], 1), mbar_init(&bar[bDecayFree + i], STATE ? 16 : 24);
         ctl[0] = 0u;
         ctl[1] = 0u;
         mbar_init_fence();
@@ -152,7 +149,6 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
     auto wait = [&](int i, uint32_t parity, int code) {
         return tc::warp_all(mbar_try_wait_hint(&bar[i], parity & 1u, 200000u) || mbar_wait(&bar[i], parity & 1u, ctx, code));
     };
-    auto wait_with_decays = [&](int c, int i, uint32_t parity, int code) { return wait(bDecay + c % kDecays, c / kDecays, kStatusLinDecay) && wait(i, parity, code); };
 
     if (idle) goto done;
     if (warp == kCopyWarp) {
@@ -185,9 +181,12 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
                 const uint32_t o = tm_all + cO + 64 * (c & 1);
                 // (The state is there when its product with the chunk before has been waited for: one product's result as another's operand is not
                 // in the order of their issue.)
-                if (!wait(bOFree + (c & 1), c / 2 + 1, kStatusLinFree) || !wait(bQ, c, kStatusLinQK) ||
-                    !(c > 0 ? wait(bU + ((c - 1) & 1), (c - 1) / 2, kStatusLinU) : wait(bState, 0, kStatusLinS)))
-                    goto done;
+                // (One barrier for all that this product waits for: each wait that is passed costs 200 cycles here.)
+                if (c == 0) {
+                    if (!wait(bState, 0, kStatusLinS)) goto done;
+                    if (leader) mbar_arrive(&bar[bReady]);
+                }
+                if (!wait(bReady, c, kStatusLinQK)) goto done;
                 tc::fence_after_sync();
                 const uint32_t q32 = desc_lo(base + oQ, 16);
 #pragma unroll
@@ -202,6 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
 #pragma unroll
                 for (int i = 0; i < CH / 16; ++i) tc::mma_bf16_ts_if(leader, tm_all + cS, wv + 32 * part + 8 * i, desc(k + 128 * i), id_u, true);
             tc::mma_commit_if(leader, &bar[bEmpty + stage]);
+            if (!STATE && c + 1 < n_all) tc::mma_commit_if(leader, &bar[bReady]);
             tc::mma_commit_if(leader, &bar[bU + (c & 1)]);  // (the last one: whoever has seen it has seen the others)
             if (++stage == kStages) stage = 0, phase ^= 1u;
             if (leader) ctl[0] = ctl[0] + 1u;
@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
         double total = 0.0;  // of the whole segment (pass 1)
         if (n > 0) fetch(0);
         for (int c = 0; c < n; ++c) {
-            if (!wait(bDecayFree + c % kDecays, c / kDecays + 1, kStatusLinDecay)) goto done;
+            if (!wait(bEmpty + c % kStages, c / kStages + 1, kStatusLinDecay)) goto done;
             double a[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) a[j] = (double)(next[j] < -104.0f ? -104.0f : next[j]) * 1.4426950408889634;
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
                 if (lane >= d) upto += o;
             }
             const double all = __shfl_sync(0xffffffffu, upto, 31), sum[2] = {upto - a[1], upto};
-            Decays& x = decays[c % kDecays];
+            Decays& x = decays[c % kStages];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int r = 2 * lane + j;
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
             }
             if (lane == 0) x.all = exp2f((float)all);
             total += all;
-            arrive(bDecay + c % kDecays);
+            arrive(bFull + c % kStages);
         }
         if (STATE && lane == 0) p.kept[(long long)chain * p.segments + seg] = exp2f((float)total);
     } else if (warp < kOWarp) {
@@ -289,9 +289,9 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
                 for (int i = 0; i < 4; ++i) tc::stmatrix_4(at + i * kBox, 0u, 0u, 0u, 0u);
             }
             for (int c = 0; c < n; ++c) {
-                if (!wait_with_decays(c, bQK, c, kStatusLinQK)) goto done;
+                if (!wait(bQK, c, kStatusLinQK)) goto done;  // (whoever issued the scores has seen the chunk's rows and decays arrive)
                 tc::fence_after_sync();
-                const Decays& x = decays[c % kDecays];
+                const Decays& x = decays[c % kStages];
                 const float2 g_lo = x.g[t_lo], g_hi = x.g[t_lo + 8];
                 unsigned char* mine = pt + (c & 1) * 2 * kBox;  // (the products that read this buffer last were issued before this chunk's scores: they are through)
 #pragma unroll 2
@@ -318,7 +318,6 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
                 tc::fence_before_sync();
                 fence_proxy_async_smem();
                 arrive(bP);
-                arrive(bDecayFree + c % kDecays);
             }
         }
     } else if (warp < kQWarp) {
@@ -361,15 +360,16 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
     } else if (warp < kVWarp) {
         if (!STATE) {
             // Chunk c's q, times scale e^G, as f32; a thread takes a piece of eight channels of every sixteenth row.
-            const int qt = tid - 32 * kQWarp, r0 = qt >> 3, sw = r0 & 7, piece = (qt & 7) ^ sw;
+            // Eight lanes take four pieces each of two neighbouring rows, the halves crosswise, so that neither their loads nor their stores meet in a bank.
+            const int qt = tid - 32 * kQWarp, l = qt & 7, r0 = 2 * (qt >> 4) + (l >> 2), sw = r0 & 7, piece = (l & 3) + 4 * ((l >> 2) ^ ((qt >> 3) & 1));
             unsigned char* to = smem + oQ + (piece >> 2) * kBox + r0 * 128;
-            const int to0 = ((2 * (piece & 3)) ^ sw) << 4, to1 = ((2 * (piece & 3) + 1) ^ sw) << 4;
-            const bool swap = piece & 4;  // (eight lanes' stores at a time: the four in one box take the even pieces while those in the other take the odd ones)
+            const int to0 = ((2 * (piece & 3)) ^ sw) << 4, to1 = ((2 * (piece & 3) + 1) ^ sw) << 4, from = r0 * 128 + ((piece ^ sw) << 4);
             for (int c = 0; c < n; ++c) {
-                if (!wait_with_decays(c, bFull + c % kStages, c / kStages, kStatusLinFull)) goto done;
+                if (!wait(bFull + c % kStages, c / kStages, kStatusLinFull)) goto done;
+                if (!wait(bOFree + (c & 1), c / 2 + 1, kStatusLinFree)) goto done;  // (the accumulator of the product that will wait for this)
                 if (c > 0 && !wait(bQS + ((c - 1) & 1), (c - 1) / 2, kStatusLinQK)) goto done;
-                const Decays& x = decays[c % kDecays];
-                const unsigned char* q = smem + (c % kStages) * kStage + qt * 16;
+                const Decays& x = decays[c % kStages];
+                const unsigned char* q = smem + (c % kStages) * kStage + from;
 #pragma unroll 4
                 for (int i = 0; i < 8; ++i) {
                     const uint4 in = *reinterpret_cast<const uint4*>(q + i * 2048);
@@ -380,21 +380,19 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
                     const float2 a1 = mul2(e, make_float2(__uint_as_float(in.y << 16), __uint_as_float(in.y & 0xffff0000u)));
                     const float2 a2 = mul2(e, make_float2(__uint_as_float(in.z << 16), __uint_as_float(in.z & 0xffff0000u)));
                     const float2 a3 = mul2(e, make_float2(__uint_as_float(in.w << 16), __uint_as_float(in.w & 0xffff0000u)));
-                    const float4 x0 = make_float4(a0.x, a0.y, a1.x, a1.y), x1 = make_float4(a2.x, a2.y, a3.x, a3.y);
-                    *reinterpret_cast<float4*>(at + (swap ? to1 : to0)) = swap ? x1 : x0;
-                    *reinterpret_cast<float4*>(at + (swap ? to0 : to1)) = swap ? x0 : x1;
+                    *reinterpret_cast<float4*>(at + to0) = make_float4(a0.x, a0.y, a1.x, a1.y);
+                    *reinterpret_cast<float4*>(at + to1) = make_float4(a2.x, a2.y, a3.x, a3.y);
                 }
                 fence_proxy_async_smem();
-                arrive(bQ);
-                arrive(bDecayFree + c % kDecays);
+                arrive(bReady);
             }
         }
     } else if (warp < kSWarp) {
         const int w = warp & 3, half = (warp - kVWarp) >> 2, vt = tid - 32 * kVWarp;
         const int parts = p.state_bf16 ? 2 : 3;
         for (int c = 0; c < n; ++c) {
-            if (!wait_with_decays(c, bFull + c % kStages, c / kStages, kStatusLinFull)) goto done;
-            const Decays& x = decays[c % kDecays];
+            if (!wait(bFull + c % kStages, c / kStages, kStatusLinFull)) goto done;
+            const Decays& x = decays[c % kStages];
             unsigned char *k = smem + (c % kStages) * kStage + kTile, *v = k + kTile;
             const int live = rows - c * CH;
             if (live < CH) {  // behind the sequence: another one's rows, or none
@@ -440,7 +438,6 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
             tc::tmem_st_wait();
             tc::fence_before_sync();
             arrive(bAdd + (c & 1));
-            arrive(bDecayFree + c % kDecays);
         }
     } else if (warp < kCopyWarp) {  // the state: thread = value channel 32 (warp % 4) + lane, key channels 64 half ..
         const int quad = warp & 3, half = (warp - kSWarp) >> 2;
@@ -485,10 +482,10 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
         }
         for (int c = 0; c < n; ++c) {
             // The chunk's outputs have read the state (and the chunk before has been added).
-            if (STATE && c == 0 ? !wait(bDecay, 0, kStatusLinDecay)
-                                : !wait_with_decays(c, STATE ? bU + ((c - 1) & 1) : bQS + (c & 1), STATE ? (c - 1) / 2 : c / 2, STATE ? kStatusLinU : kStatusLinS)) goto done;
-            const float all = decays[c % kDecays].all;
-            arrive(bDecayFree + c % kDecays);
+            if (STATE ? !wait(bFull + c % kStages, c / kStages, kStatusLinFull) || (c > 0 && !wait(bU + ((c - 1) & 1), (c - 1) / 2, kStatusLinU))
+                      : !wait(bQS + (c & 1), c / 2, kStatusLinS))
+                goto done;
+            const float all = decays[c % kStages].all;
             tc::fence_after_sync();
             if (!STATE || c > 0)
 #pragma unroll 1
