@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
         mbar_init(&bar[bP], 4);
         mbar_init(&bar[bReady], 5);  // q of a chunk (four warps), and the chunk before added to the state
         mbar_init(&bar[bState], 8);
-        for (int i = 0; i < 2; ++i) mbar_init(&bar[bQS + i], 1), mbar_init(&bar[bAdd + i], 16), mbar_init(&bar[bU + i], 1), mbar_init(&bar[bO + i], 1), mbar_init(&bar[bOFree + i], 4);
+        for (int i = 0; i < 2; ++i) mbar_init(&bar[bQS + i], 1), mbar_init(&bar[bAdd + i], STATE ? 8 : 16), mbar_init(&bar[bU + i], 1), mbar_init(&bar[bO + i], 1), mbar_init(&bar[bOFree + i], 4);
         ctl[0] = 0u;
         ctl[1] = 0u;
         mbar_init_fence();
@@ -150,11 +150,75 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
         return tc::warp_all(mbar_try_wait_hint(&bar[i], parity & 1u, 200000u) || mbar_wait(&bar[i], parity & 1u, ctx, code));
     };
 
+    // The pass that only sums up states goes backwards: rows are then weighed by all that comes behind them in the segment, and nothing that has been
+    // added is scaled again.  Its segments are whole ones.
+    auto chunk_at = [&](int c) { return STATE ? n - 1 - c : c; };
+
+    // The parts of w V^T, by eight warps: all chunks, or in the pass that only sums up states every other one (the warps that have no outputs to work on take the rest).
+    auto weigh_values = [&](int vt, int first_chunk) {
+        const int w = (vt >> 5) & 3, half = vt >> 7;
+        const int parts = p.state_bf16 ? 2 : 3;
+        for (int c = first_chunk; c < n; c += STATE ? 2 : 1) {
+            // The products with these columns' last parts are through -- first, so that a chunk which this side skips is never the one the next barrier tells of.
+            if (c > 1 && !wait(bU + (c & 1), c / 2 - 1, kStatusLinU)) return false;
+            if (!wait(bFull + c % kStages, c / kStages, kStatusLinFull)) return false;
+            const Decays& x = decays[c % kStages];
+            unsigned char *k = smem + (c % kStages) * kStage + kTile, *v = k + kTile;
+            const int live = rows - chunk_at(c) * CH;
+            if (live < CH) {  // behind the sequence: another one's rows, or none
+                for (int at = vt * 16; at < kTile; at += 256 * 16)
+                    if (((at >> 7) & (CH - 1)) >= live) *reinterpret_cast<uint4*>(k + at) = *reinterpret_cast<uint4*>(v + at) = make_uint4(0u, 0u, 0u, 0u);
+                fence_proxy_async_smem();
+            }
+            tc::fence_after_sync();
+#pragma unroll 1
+            for (int sh = 0; sh < 2; ++sh) {
+                uint32_t at = tc::tmem_addr(tm, w, cWV + 96 * (c & 1) + 16 * sh) + ((uint32_t)(16 * half) << 16), raw[8], part[8];
+                float2 z[8];
+                // V^T, value channels 32 w + 16 half + lane / 4 (+ 8): raw[2 i + 0 / 1] rows 32 sh + 8 i + 2 (lane % 4) and the next.
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int r = 32 * sh + 16 * i + 8 * (lane >> 4) + (lane & 7), piece = 4 * w + 2 * half + ((lane >> 3) & 1);
+                    tc::ldmatrix_t4(v + (piece >> 3) * kBox + r * 128 + (((piece & 7) ^ (r & 7)) << 4), raw[4 * i], raw[4 * i + 1], raw[4 * i + 2], raw[4 * i + 3]);
+                }
+                if (live < CH) {  // (whether or not the warp that clears these rows has been there)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = 32 * sh + 8 * i + 2 * (lane & 3);
+                        const uint32_t mask = (r < live ? 0xffffu : 0u) | (r + 1 < live ? 0xffff0000u : 0u);
+                        raw[2 * i] &= mask, raw[2 * i + 1] &= mask;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float2 f = *reinterpret_cast<const float2*>(&x.w[32 * sh + 8 * (i >> 1) + 2 * (lane & 3)]);
+                    z[i] = mul2(f, make_float2(__uint_as_float(raw[i] << 16), __uint_as_float(raw[i] & 0xffff0000u)));
+                }
+#pragma unroll 1
+                for (int j = 1; j < parts; ++j, at += 32) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        part[i] = tc::bf16x2(z[i].x, z[i].y);
+                        z[i] = lo_of(part[i], z[i]);
+                    }
+                    tc::tmem_st_pairs(at, part);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) part[i] = tc::bf16x2(z[i].x, z[i].y);
+                tc::tmem_st_pairs(at, part);
+            }
+            tc::tmem_st_wait();
+            tc::fence_before_sync();
+            arrive(bAdd + (c & 1));
+        }
+        return true;
+    };
+
     if (idle) goto done;
     if (warp == kCopyWarp) {
         if (lane == 0) {
             for (int c = 0; c < n; ++c) {
-                const int s = c % kStages, row = row0 + c * CH, hq = h / p.share;
+                const int s = c % kStages, row = row0 + chunk_at(c) * CH, hq = h / p.share;
                 if (!mbar_wait(&bar[bEmpty + s], ((c / kStages) & 1) ^ 1u, ctx, kStatusLinEmpty)) goto done;
                 unsigned char* st = smem + s * kStage;
                 mbar_arrive_expect_tx(&bar[bFull + s], STATE ? 2 * kTile : 3 * kTile);
@@ -177,6 +241,7 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
         uint32_t stage = 0, phase = 0;
         for (int c = 0; c < n_all; ++c) {
             if (STATE && !wait(bFull + stage, phase, kStatusLinFull)) goto done;
+            if (STATE && c == 0 && !wait(bState, 0, kStatusLinS)) goto done;  // (zeros)
             if (!STATE) {
                 const uint32_t o = tm_all + cO + 64 * (c & 1);
                 // (The state is there when its product with the chunk before has been waited for: one product's result as another's operand is not
@@ -202,6 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
                 for (int i = 0; i < CH / 16; ++i) tc::mma_bf16_ts_if(leader, tm_all + cS, wv + 32 * part + 8 * i, desc(k + 128 * i), id_u, true);
             tc::mma_commit_if(leader, &bar[bEmpty + stage]);
             if (!STATE && c + 1 < n_all) tc::mma_commit_if(leader, &bar[bReady]);
+            if (STATE && c + 1 == n_all) tc::mma_commit_if(leader, &bar[bQS]);  // (for the state's warps, which follow no chunk but the last)
             tc::mma_commit_if(leader, &bar[bU + (c & 1)]);  // (the last one: whoever has seen it has seen the others)
             if (++stage == kStages) stage = 0, phase ^= 1u;
             if (leader) ctl[0] = ctl[0] + 1u;
@@ -246,11 +312,11 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
         auto fetch = [&](int c) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const int r = c * CH + 2 * lane + j;
+                const int r = chunk_at(c) * CH + 2 * lane + j;
                 next[j] = r < rows ? __ldg(g + (long long)r * p.g_stride) : 0.0f;
             }
         };
-        double total = 0.0;  // of the whole segment (pass 1)
+        double total = 0.0;  // pass 1: of the segment's rows behind the chunk
         if (n > 0) fetch(0);
         for (int c = 0; c < n; ++c) {
             if (!wait(bEmpty + c % kStages, c / kStages + 1, kStatusLinDecay)) goto done;
@@ -272,13 +338,15 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
                 const float hi = (float)sum[j];
                 x.g[r] = make_float2(hi, (float)(sum[j] - (double)hi));
                 x.e[r] = p.scale * exp2f(hi);
-                x.w[r] = exp2f((float)(all - sum[j]));
+                x.w[r] = exp2f((float)(STATE ? total + (all - sum[j]) : all - sum[j]));
             }
             if (lane == 0) x.all = exp2f((float)all);
             total += all;
             arrive(bFull + c % kStages);
         }
         if (STATE && lane == 0) p.kept[(long long)chain * p.segments + seg] = exp2f((float)total);
+    } else if (STATE && warp < kQWarp) {
+        if (!weigh_values(tid, 1)) goto done;
     } else if (warp < kOWarp) {
         if (!STATE) {
             const int w = warp, t_lo = 16 * w + (lane >> 2);
@@ -388,57 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
             }
         }
     } else if (warp < kSWarp) {
-        const int w = warp & 3, half = (warp - kVWarp) >> 2, vt = tid - 32 * kVWarp;
-        const int parts = p.state_bf16 ? 2 : 3;
-        for (int c = 0; c < n; ++c) {
-            if (!wait(bFull + c % kStages, c / kStages, kStatusLinFull)) goto done;
-            const Decays& x = decays[c % kStages];
-            unsigned char *k = smem + (c % kStages) * kStage + kTile, *v = k + kTile;
-            const int live = rows - c * CH;
-            if (live < CH) {  // behind the sequence: another one's rows, or none
-                for (int at = vt * 16; at < kTile; at += 256 * 16)
-                    if (((at >> 7) & (CH - 1)) >= live) *reinterpret_cast<uint4*>(k + at) = *reinterpret_cast<uint4*>(v + at) = make_uint4(0u, 0u, 0u, 0u);
-                fence_proxy_async_smem();
-            }
-            if (c > 1 && !wait(bU + (c & 1), c / 2 - 1, kStatusLinU)) goto done;  // the products with these columns' last parts are through
-            tc::fence_after_sync();
-#pragma unroll 1
-            for (int sh = 0; sh < 2; ++sh) {
-                uint32_t at = tc::tmem_addr(tm, w, cWV + 96 * (c & 1) + 16 * sh) + ((uint32_t)(16 * half) << 16), raw[8], part[8];
-                float2 z[8];
-                // V^T, value channels 32 w + 16 half + lane / 4 (+ 8): raw[2 i + 0 / 1] rows 32 sh + 8 i + 2 (lane % 4) and the next.
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int r = 32 * sh + 16 * i + 8 * (lane >> 4) + (lane & 7), piece = 4 * w + 2 * half + ((lane >> 3) & 1);
-                    tc::ldmatrix_t4(v + (piece >> 3) * kBox + r * 128 + (((piece & 7) ^ (r & 7)) << 4), raw[4 * i], raw[4 * i + 1], raw[4 * i + 2], raw[4 * i + 3]);
-                }
-                if (live < CH) {  // (whether or not the warp that clears these rows has been there)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = 32 * sh + 8 * i + 2 * (lane & 3);
-                        const uint32_t mask = (r < live ? 0xffffu : 0u) | (r + 1 < live ? 0xffff0000u : 0u);
-                        raw[2 * i] &= mask, raw[2 * i + 1] &= mask;
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float2 f = *reinterpret_cast<const float2*>(&x.w[32 * sh + 8 * (i >> 1) + 2 * (lane & 3)]);
-                    z[i] = mul2(f, make_float2(__uint_as_float(raw[i] << 16), __uint_as_float(raw[i] & 0xffff0000u)));
-                }
-#pragma unroll 1
-                for (int j = 0; j < parts; ++j, at += 32) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        part[i] = tc::bf16x2(z[i].x, z[i].y);
-                        z[i] = lo_of(part[i], z[i]);
-                    }
-                    tc::tmem_st_pairs(at, part);
-                }
-            }
-            tc::tmem_st_wait();
-            tc::fence_before_sync();
-            arrive(bAdd + (c & 1));
-        }
+        if (!weigh_values(tid - 32 * kVWarp, 0)) goto done;
     } else if (warp < kCopyWarp) {  // the state: thread = value channel 32 (warp % 4) + lane, key channels 64 half ..
         const int quad = warp & 3, half = (warp - kSWarp) >> 2;
         const uint32_t at = tc::tmem_addr(tm, quad, cS + 64 * half);
@@ -475,19 +493,14 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
             }
             tc::tmem_st16(at + i, x);
         }
-        if (!STATE) {
-            tc::tmem_st_wait();
-            tc::fence_before_sync();
-            arrive(bState);
-        }
-        for (int c = 0; c < n; ++c) {
+        tc::tmem_st_wait();
+        tc::fence_before_sync();
+        arrive(bState);
+        for (int c = 0; c < n && !STATE; ++c) {
             // The chunk's outputs have read the state (and the chunk before has been added).
-            if (STATE ? !wait(bFull + c % kStages, c / kStages, kStatusLinFull) || (c > 0 && !wait(bU + ((c - 1) & 1), (c - 1) / 2, kStatusLinU))
-                      : !wait(bQS + (c & 1), c / 2, kStatusLinS))
-                goto done;
+            if (!wait(bQS + (c & 1), c / 2, kStatusLinS)) goto done;
             const float all = decays[c % kStages].all;
             tc::fence_after_sync();
-            if (!STATE || c > 0)
 #pragma unroll 1
                 for (int i = 0; i < 64; i += 32) {
                     uint32_t x[32];
@@ -505,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
             arrive(bAdd + (c & 1));
             if (warp == kSWarp && lane == 0) ctl[0] = ctl[0] + 1u;
         }
-        if (n > 0 && !wait(bU + ((n - 1) & 1), (n - 1) / 2, kStatusLinU)) goto done;  // (nobody leaves before the last product)
+        if (n > 0 && !(STATE ? wait(bQS, 0, kStatusLinU) : wait(bU + ((n - 1) & 1), (n - 1) / 2, kStatusLinU))) goto done;  // (nobody leaves before the last product)
         tc::fence_after_sync();
         if (STATE || (last_seg && (n > 0 || seg == 0))) {
             float* dst32 = STATE ? mine : static_cast<float*>(p.state_out) + off;
