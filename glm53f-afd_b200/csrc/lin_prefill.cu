@@ -6,7 +6,7 @@
 //     y_t  = scale (e^G_t S q_t + sum over s <= t of P_ts v_s),   P_ts = (q_t . k_s) e^(G_t - G_s)
 //     S'   = e^G_63 S + sum over s of w_s v_s k_s^T,              w_s = e^(G_63 - G_s)
 // so a chunk is four products: Q K^T, S Q^T, V^T P^T and (w V)^T K, all on operands as the tensor copies bring them (128-byte
-// swizzle, K- or MN-major).  Bound by HBM where every SM has a chain (1 KiB a row and head); a chain's own pace is the tensor pipe's.
+// swizzle, K- or MN-major).  Bound by HBM where every SM has a chain, a sequence's head (1 KiB a row and head); a chain's own pace is the tensor pipe's.
 //
 // Precision.  Sums and the state are f32 in tensor memory.  What has to become an operand and is not bf16 already keeps more bits than that: w V
 // goes as a sum of three bf16 parts where the state is f32 (24 bits, all that f32 has) and of two where it is stored as bf16, P as a sum of two (16 bits), S and
@@ -14,7 +14,7 @@
 // operands P and S would add as much again).  Differences of G are of sums in 64 bits, held as two f32: a row that forgets everything (-inf, taken as
 // -104, which is 0 in f32) must not blur those behind it.
 //
-// Roles of a block, one (chain, segment) each, all meeting at mbarriers:
+// Roles of a block, one (sequence, head, segment) each, all meeting at mbarriers:
 //   warps 0-3    P of a chunk out of the accumulator into shared memory (hi and lo)
 //   warps 4-7    the outputs through transposing matrix stores to rows of 256 bytes
 //   warps 8-11   scale e^G Q as f32
@@ -82,13 +82,62 @@ struct PrefillParams {
     float scale;
     uint16_t* out;
     long long out_stride;
-    // Segments: `segments` of seg_chunks chunks a chain, one block each.  pass 0: a walk of the whole chain; 1: what a segment adds, for all but the last;
-    // 2: with outputs, from the states that the segments before leave.
-    int pass, segments, seg_chunks;
-    float* states;  // [chain][segments][128 x 128]: pass 1 writes segment s's sum at s, lin_join_kernel makes it the state before segment s
-    float* kept;    // [chain][segments]: how much of the state before it a segment leaves
+    // Segments of seg_chunks chunks, one block each; in the pass that sums up states parts of part_chunks, one or two a segment.  What a part adds lies in a slot
+    // of `states`, and how much of the state before it it leaves in `kept`; lin_join_kernel makes of a sequence's slots the states before its segments.
+    int seg_chunks, part_chunks;
+    int slots;  // of a head; 0: every sequence is one segment
+    float *states, *kept;
     int* status;
 };
+
+// The block's work, r counting those of one head: (b, seg), found by each warp for itself.  Whole segments come first and then the sequences' rest, the longest
+// first (within 32 sequences): blocks start in this order, and a long one that starts last would run alone.
+template <bool STATE>
+__device__ bool pick_work(const PrefillParams& p, int r, int lane, int& b, int& seg) {
+    const int sub = p.seg_chunks / p.part_chunks;
+    auto chunks_of = [&](int i) { return i < p.batch ? (p.cu[i + 1] - p.cu[i] + CH - 1) / CH : 0; };
+    for (int g0 = 0; p.slots > 0 && g0 < p.batch; g0 += 32) {
+        const int chunks = chunks_of(g0 + lane), mine = STATE ? max(chunks - 1, 0) / p.seg_chunks * sub : chunks / p.seg_chunks;
+        int upto = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += o;
+        }
+        const int all = __shfl_sync(0xffffffffu, upto, 31);
+        if (r < all) {
+            const int l = __ffs(__ballot_sync(0xffffffffu, upto > r)) - 1;
+            b = g0 + l;
+            seg = r - __shfl_sync(0xffffffffu, upto - mine, l);
+            return true;
+        }
+        r -= all;
+    }
+    if (!STATE && p.slots == 0 && p.batch == 1) return true;
+    for (int g0 = 0; !STATE && g0 < p.batch; g0 += 32) {
+        const int chunks = chunks_of(g0 + lane), rest = chunks % p.seg_chunks;
+        const int size = g0 + lane < p.batch && (rest > 0 || chunks == 0) ? rest : -1;  // (an empty sequence's state is handed on)
+        const int all = __popc(__ballot_sync(0xffffffffu, size >= 0));
+        if (r < all) {
+            int rank = 0;
+#pragma unroll 4
+            for (int j = 0; j < 32; ++j) {
+                const int other = __shfl_sync(0xffffffffu, size, j);
+                rank += other > size || (other == size && j < lane);
+            }
+            const int l = __ffs(__ballot_sync(0xffffffffu, rank == r)) - 1;
+            b = g0 + l;
+            seg = __shfl_sync(0xffffffffu, chunks / p.seg_chunks, l);
+            return true;
+        }
+        r -= all;
+    }
+    return false;
+}
+// A sequence's first slot: of a head's 2 (rows / segment's rows), enough for its segments' states and for two parts of each but the last.
+__device__ __forceinline__ long long first_slot(const PrefillParams& p, int h, int first) {
+    return (long long)h * p.slots + 2 * (first / (p.seg_chunks * CH));
+}
 
 __device__ __forceinline__ float2 sub2(float2 a, float2 b) { return fma2(b, make_float2(-1.0f, -1.0f), a); }
 __device__ __forceinline__ float2 lo_of(uint32_t hi, float2 x) {  // what a pair's hi parts leave
@@ -132,15 +181,17 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
     const WaitCtx ctx{ctl, ctl + 1, p.status};
     grid_ready();
 
-    // The block's chain and its chunks [c0, c0 + n).
-    const int chain = (int)blockIdx.x / p.segments, seg = (int)blockIdx.x - chain * p.segments;
-    const int b = chain / p.heads, h = chain - b * p.heads;
-    const int first = p.cu[b], len = p.cu[b + 1] - first;
-    const int chunks = (len + CH - 1) / CH, c0 = seg * p.seg_chunks;
-    const int n = max(0, min(p.seg_chunks, chunks - c0));
+    // The block's sequence and head and its chunks [c0, c0 + n).
+    const int h = (int)blockIdx.x % p.heads;
+    int b = 0, seg = 0;
+    const bool idle = !pick_work<STATE>(p, (int)blockIdx.x / p.heads, lane, b, seg);
+    b = (int)__reduce_max_sync(0xffffffffu, (unsigned)b);
+    seg = (int)__reduce_max_sync(0xffffffffu, (unsigned)seg);
+    const int first = p.cu[b], len = p.cu[b + 1] - first, seg_chunks = STATE ? p.part_chunks : p.seg_chunks;
+    const int chunks = (len + CH - 1) / CH, c0 = seg * seg_chunks;
+    const int n = max(0, min(seg_chunks, chunks - c0));
     const bool last_seg = c0 + n >= chunks;
     const int row0 = first + c0 * CH, rows = min(len - c0 * CH, n * CH);  // this block's rows
-    const bool idle = STATE ? last_seg : (n == 0 && seg > 0);
     auto arrive = [&](int i) {  // one arrival a warp, behind what its lanes have done
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar[i]);
@@ -344,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
             total += all;
             arrive(bFull + c % kStages);
         }
-        if (STATE && lane == 0) p.kept[(long long)chain * p.segments + seg] = exp2f((float)total);
+        if (STATE && lane == 0) p.kept[first_slot(p, h, first) + seg] = exp2f((float)total);
     } else if (STATE && warp < kQWarp) {
         if (!weigh_values(tid, 1)) goto done;
     } else if (warp < kOWarp) {
@@ -461,8 +512,8 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
         const int quad = warp & 3, half = (warp - kSWarp) >> 2;
         const uint32_t at = tc::tmem_addr(tm, quad, cS + 64 * half);
         const int in_state = (32 * quad + lane) * DK + 64 * half;
-        const bool from_segments = !STATE && p.pass == 2;
-        float* mine = p.states + ((long long)chain * p.segments + seg) * (DK * DV) + in_state;
+        const bool from_segments = !STATE && p.slots > 0 && chunks > p.seg_chunks;
+        float* mine = p.states + (first_slot(p, h, first) + seg) * (DK * DV) + in_state;
         const long long off = p.state_off[b] + (long long)h * DK * DV + in_state;
         const float* src32 = from_segments ? mine : static_cast<const float*>(p.state_in) + off;
         const uint16_t* src16 = static_cast<const uint16_t*>(p.state_in) + off;
@@ -520,7 +571,7 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
         }
         if (n > 0 && !(STATE ? wait(bQS, 0, kStatusLinU) : wait(bU + ((n - 1) & 1), (n - 1) / 2, kStatusLinU))) goto done;  // (nobody leaves before the last product)
         tc::fence_after_sync();
-        if (STATE || (last_seg && (n > 0 || seg == 0))) {
+        if (STATE || last_seg) {
             float* dst32 = STATE ? mine : static_cast<float*>(p.state_out) + off;
             uint16_t* dst16 = static_cast<uint16_t*>(p.state_out) + off;
             const bool wide_out = STATE || !p.state_bf16, vec_out = ((wide_out ? reinterpret_cast<uintptr_t>(dst32) : reinterpret_cast<uintptr_t>(dst16)) & 15) == 0;
@@ -562,14 +613,26 @@ done:
     if (warp == kStateMmaWarp) tc::tmem_dealloc(tm, kCols);
 }
 
-// The state before each segment of a chain, from what the segments add: one thread for four entries of a state.  Segments that the sequence does not reach are
-// left alone.
-constexpr int kJoinThreads = 128, kJoinBlocks = DK * DV / 4 / kJoinThreads;
+// The state before each segment of the sequences that have more than one, from what their parts add: one thread for four entries of a state.
+constexpr int kJoinThreads = 128, kJoinBlocks = DK * DV / 4 / kJoinThreads, kJoinAhead = 8;
 __global__ void __launch_bounds__(kJoinThreads) lin_join_kernel(const __grid_constant__ PrefillParams p) {
     grid_ready();
-    const int chain = blockIdx.x / kJoinBlocks, b = chain / p.heads, h = chain - b * p.heads;
+    const int work = blockIdx.x / kJoinBlocks, h = work % p.heads, lane = threadIdx.x & 31;
+    int r = work / p.heads, b = -1;
+    for (int g0 = 0; g0 < p.batch; g0 += 32) {
+        const int i = g0 + lane;
+        const unsigned cut = __ballot_sync(0xffffffffu, i < p.batch && p.cu[i + 1] - p.cu[i] > p.seg_chunks * CH);
+        const int all = __popc(cut);
+        if (r < all) {
+            b = g0 + (int)__fns(cut, 0, r + 1);
+            break;
+        }
+        r -= all;
+    }
+    if (b < 0) return;
     const int at = ((int)(blockIdx.x % kJoinBlocks) * kJoinThreads + threadIdx.x) * 4;
-    const int len = p.cu[b + 1] - p.cu[b], chunks = (len + CH - 1) / CH, used = max(1, (chunks + p.seg_chunks - 1) / p.seg_chunks);
+    const int first = p.cu[b], chunks = (p.cu[b + 1] - first + CH - 1) / CH, sub = p.seg_chunks / p.part_chunks, parts = (chunks - 1) / p.seg_chunks * sub;
+    const long long slot = first_slot(p, h, first);
     const long long off = p.state_off[b] + (long long)h * DK * DV + at;
     float4 s;
     if (p.state_bf16) {
@@ -579,15 +642,25 @@ __global__ void __launch_bounds__(kJoinThreads) lin_join_kernel(const __grid_con
         const float* src = static_cast<const float*>(p.state_in) + off;
         s = make_float4(src[0], src[1], src[2], src[3]);
     }
-    float4* states = reinterpret_cast<float4*>(p.states + (long long)chain * p.segments * (DK * DV) + at);
-    const float* kept = p.kept + (long long)chain * p.segments;
-    for (int i = 0; i < used; ++i) {
-        float4 add = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const float d = i + 1 < used ? kept[i] : 0.0f;
-        if (i + 1 < used) add = states[(long long)i * (DK * DV / 4)];
-        states[(long long)i * (DK * DV / 4)] = s;
-        s = make_float4(fmaf(d, s.x, add.x), fmaf(d, s.y, add.y), fmaf(d, s.z, add.z), fmaf(d, s.w, add.w));
+    float4* states = reinterpret_cast<float4*>(p.states + slot * (DK * DV) + at);
+    const float* kept = p.kept + slot;
+    // A segment's state takes a slot whose part has been read: segment i's comes behind the loads of parts up to i * sub at least.
+    int seg = 0, in_seg = 0;
+    for (int i = 0; i < parts; i += kJoinAhead) {
+        float4 add[kJoinAhead];
+        float d[kJoinAhead];
+#pragma unroll
+        for (int j = 0; j < kJoinAhead; ++j)
+            if (i + j < parts) add[j] = states[(long long)(i + j) * (DK * DV / 4)], d[j] = kept[i + j];
+#pragma unroll
+        for (int j = 0; j < kJoinAhead; ++j) {
+            if (i + j >= parts) break;
+            if (in_seg == 0) states[(long long)seg * (DK * DV / 4)] = s, ++seg;
+            if (++in_seg == sub) in_seg = 0;
+            s = make_float4(fmaf(d[j], s.x, add[j].x), fmaf(d[j], s.y, add[j].y), fmaf(d[j], s.z, add[j].z), fmaf(d[j], s.w, add[j].w));
+        }
     }
+    states[(long long)seg * (DK * DV / 4)] = s;
 }
 
 bool rows_map(CUtensorMap* tm, const void* base, int heads, long long rows, long long stride) {
@@ -601,7 +674,7 @@ bool rows_map(CUtensorMap* tm, const void* base, int heads, long long rows, long
 }
 
 template <bool STATE>
-int walk_launch(const PrefillParams& p, cudaStream_t stream) {
+int walk_launch(const PrefillParams& p, long long blocks, cudaStream_t stream) {
     static int configured_dev = -1;
     int dev = 0;
     cudaGetDevice(&dev);
@@ -610,16 +683,32 @@ int walk_launch(const PrefillParams& p, cudaStream_t stream) {
         if (e != cudaSuccess) return (int)e;
         configured_dev = dev;
     }
-    return launch_early(lin_prefill_kernel<STATE>, dim3((unsigned)(p.heads * (long long)p.batch * p.segments)), kThreads, kSmem, stream, p);
+    return launch_early(lin_prefill_kernel<STATE>, dim3((unsigned)blocks), kThreads, kSmem, stream, p);
 }
 
-// Segments of a chain: as many as give every SM a block, of eight chunks at least (a pass over fewer costs more than it saves).
-int pick_segments(long long chains, int max_len) {
-    const long long fit = sm_count() / (chains > 0 ? chains : 1), chunks = (max_len + CH - 1) / CH;
-    long long n = chunks / 8 < fit ? chunks / 8 : fit;
-    return n < 2 ? 1 : (int)n;
+// Segments.  Were all sequences one block, the longest sequence's chunks would be the time where they are more than an SM's share of all chunks.  So the longest is
+// cut into as many segments as there are SMs for it by that share, of kMinChunks chunks at least (a pass over fewer costs more than it saves).
+constexpr int kMinChunks = 8;
+struct Segments {
+    int seg_chunks, part_chunks;
+    long long slots;  // of a head
+};
+Segments pick_segments(int heads, long long rows, int max_len, long long workspace_bytes) {
+    const int chunks = (max_len + CH - 1) / CH;
+    long long n = (long long)sm_count() * max_len / (heads * rows);
+    n = n < chunks / kMinChunks ? n : chunks / kMinChunks;
+    for (; n > 1; --n) {
+        Segments x{};
+        x.seg_chunks = (int)((chunks + n - 1) / n);
+        const long long cuts = (rows - 1) / (x.seg_chunks * CH);  // segments that another one follows
+        const int sub = cuts > 0 && heads * cuts * 2 <= sm_count() && x.seg_chunks >= 2 * kMinChunks ? 2 : 1;
+        x.part_chunks = (x.seg_chunks + sub - 1) / sub;
+        x.seg_chunks = x.part_chunks * sub;
+        x.slots = 2 * (rows / (x.seg_chunks * CH));
+        if (x.seg_chunks < chunks && heads * x.slots * (4ll * DK * DV + 4) <= workspace_bytes) return x;
+    }
+    return {(1 << 25) - 1, (1 << 25) - 1, 0};  // (every sequence whole, however long)
 }
-long long segment_bytes(long long chains, int segments) { return chains * segments * (4ll * DK * DV) + (chains * segments * 4 + 15) / 16 * 16; }
 
 }  // namespace
 }  // namespace kda
@@ -627,9 +716,9 @@ long long segment_bytes(long long chains, int segments) { return chains * segmen
 extern "C" int64_t glm53f_kda_lin_prefill_workspace_bytes(int32_t heads, int32_t batch, int32_t max_len) {
     using namespace kda;
     if (heads < 1 || heads > 65535 || batch < 1 || max_len < 1) return 0;
-    const long long chains = (long long)heads * batch;
-    const int n = pick_segments(chains, max_len);
-    return n > 1 ? segment_bytes(chains, n) : 0;
+    // However many rows there are, a head's slots are twice the segments that SMs were counted for.
+    const Segments x = pick_segments(heads, max_len, max_len, INT64_MAX);
+    return x.slots > 0 ? 2ll * sm_count() * (4ll * DK * DV + 4) : 0;
 }
 
 extern "C" int glm53f_kda_lin_prefill_varlen(int32_t heads, int32_t qk_heads, int32_t batch, const int32_t* cu_rows, int32_t rows, int32_t max_len,
@@ -665,21 +754,17 @@ extern "C" int glm53f_kda_lin_prefill_varlen(int32_t heads, int32_t qk_heads, in
     p.out_stride = out_stride;
     p.status = status_word();
     if (p.status == nullptr) return (int)cudaErrorUnknown;
-    const long long chains = (long long)heads * batch;
-    const int chunks = (max_len + CH - 1) / CH;
-    int n = pick_segments(chains, max_len);
-    while (n > 1 && segment_bytes(chains, n) > workspace_bytes) --n;
-    p.segments = n;
-    p.seg_chunks = (chunks + n - 1) / n;
-    p.segments = (chunks + p.seg_chunks - 1) / p.seg_chunks;
-    if (p.segments <= 1) return walk_launch<false>(p, stream);
+    const Segments x = pick_segments(heads, rows, max_len, workspace_bytes);
+    p.seg_chunks = x.seg_chunks;
+    p.part_chunks = x.part_chunks;
+    p.slots = (int)x.slots;
+    if (x.slots == 0) return walk_launch<false>(p, (long long)heads * batch, stream);
     p.states = static_cast<float*>(workspace);
-    p.kept = p.states + chains * p.segments * (DK * DV);
-    p.pass = 1;
-    int rc = walk_launch<true>(p, stream);
+    p.kept = p.states + heads * x.slots * (DK * DV);
+    const long long cuts = (rows - 1) / (x.seg_chunks * CH);
+    int rc = walk_launch<true>(p, heads * cuts * (x.seg_chunks / x.part_chunks), stream);
     if (rc != 0) return rc;
-    rc = launch_early(lin_join_kernel, dim3((unsigned)(chains * kJoinBlocks)), kJoinThreads, 0, stream, p);
+    rc = launch_early(lin_join_kernel, dim3((unsigned)(heads * (cuts < batch ? cuts : batch) * kJoinBlocks)), kJoinThreads, 0, stream, p);
     if (rc != 0) return rc;
-    p.pass = 2;
-    return walk_launch<false>(p, stream);
+    return walk_launch<false>(p, heads * (cuts + batch), stream);
 }
