@@ -687,8 +687,11 @@ int walk_launch(const PrefillParams& p, long long blocks, cudaStream_t stream) {
 }
 
 // Segments.  Were all sequences one block, the longest sequence's chunks would be the time where they are more than an SM's share of all chunks.  So the longest is
-// cut into as many segments as there are SMs for it by that share, of kMinChunks chunks at least (a pass over fewer costs more than it saves).
-constexpr int kMinChunks = 8;
+// cut into as many segments as there are SMs for it by that share, of kMinChunks chunks at least -- where that pays: a walk takes 2.0 us a chunk, the pass before it
+// half that a chunk, and two more launches with the join as much as kExtraChunks chunks.  (Measured over an evicted L2: 8 heads x 1,024 rows 36 us in four segments
+// and 41 whole; 8 x 512 rows 36 and 29, so whole; 64 x 1,024 rows 52 and 45, so whole; 8 x 2,048 rows 38 and 67.  Segments of two chunks
+// take 4 us from 1,024 rows of one head and add 4 to 4,096 rows of four.)
+constexpr int kMinChunks = 4, kExtraChunks = 7;
 struct Segments {
     int seg_chunks, part_chunks;
     long long slots;  // of a head
@@ -705,7 +708,7 @@ Segments pick_segments(int heads, long long rows, int max_len, long long workspa
         x.part_chunks = (x.seg_chunks + sub - 1) / sub;
         x.seg_chunks = x.part_chunks * sub;
         x.slots = 2 * (rows / (x.seg_chunks * CH));
-        if (x.seg_chunks < chunks && heads * x.slots * (4ll * DK * DV + 4) <= workspace_bytes) return x;
+        if (x.seg_chunks + x.part_chunks / 2 + kExtraChunks < chunks && heads * x.slots * (4ll * DK * DV + 4) <= workspace_bytes) return x;
     }
     return {(1 << 25) - 1, (1 << 25) - 1, 0};  // (every sequence whole, however long)
 }
@@ -733,7 +736,10 @@ extern "C" int glm53f_kda_lin_prefill_varlen(int32_t heads, int32_t qk_heads, in
     if (batch == 0) return 0;
     if (state_out == nullptr || out == nullptr) return kInvalid;
     cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
-    if (max_len <= 8)
+    // A handful of rows a sequence: row by row, which is memory-bound over many chains and a row's latency over few.  (Measured over an evicted L2, rows against chunks:
+    // 16 chains of 8 rows 14 and 16 us, of 16 rows 18 and 16; 512 chains of 32 rows 55 and 57 us, of 64 rows 117 and 59.)
+    const long long waves = ((long long)heads * batch + sm_count() - 1) / sm_count();
+    if (max_len <= 8 * (waves < 4 ? waves : 4))
         return lin_rows_launch(heads, qk_heads, batch, cu_rows, nullptr, q, q_stride, k, k_stride, v, v_stride, g, g_stride, state_in, state_out, state_off,
                                state_bf16 != 0, false, scale, out, out_stride, stream);
     PrefillParams p{};
