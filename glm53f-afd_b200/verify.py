@@ -6,22 +6,26 @@ of `VerifyScratch` (forward.rs:777-815), over the slots of `marks.KvPool`:
 
   verify   every KDA layer runs its chain over the windows' rows with the states read but not written, and keeps the
            layer's projection rows and replay inputs in the scratch (forward.rs:3484-3560 in Mode::Verify);
+  accept   the rows to keep, from the target's distribution behind every row (spec.py; the reference decides on the host,
+           crates/glm53f-coordinator/src/scheduler.rs:765-875);
   commit   with the rows each slot keeps, one launch replays every layer's saves into the states and one moves every
            layer's conv window past the kept rows (forward.rs:1958-2031); the slots' token counts advance.
 
 The checks and their messages are the reference's: windows of 1..=8 rows, no verify while one is pending, a commit
-must name the slots of the pending verify in its order with 1..=rows kept rows.  The attention (DSA) layers, the MLPs
-and the sampling between `verify` and `commit` belong to the rest of the forward and are not built: the caller hands
+must name the slots of the pending verify in its order with 1..=rows kept rows.  The attention (DSA) layers and the MLPs
+between `verify` and `commit` belong to the rest of the forward and are not built: the caller hands
 each KDA layer its projected rows (`KdaVerify.layer`).
 """
 from __future__ import annotations
 
+import contextlib
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
 from . import ffi
 from . import kernel as K
 from . import marks
+from . import spec
 from .core import Invalid
 
 KDA_HEADS, KDA_DIM = marks.KDA_HEADS, marks.KDA_DIM
@@ -148,6 +152,21 @@ class KdaVerify:
             cb.launch_bf16_state(self.meta, stream)
         else:
             cb.launch(self.meta, stream)
+
+    # ---- accept -----------------------------------------------------------------------------------------------
+    def accept(self, tokens, target, u, keep, next, *, probabilities=False, draft=None, temperature=None, stream: Optional[K.Stream] = None) -> None:
+        """How many rows of each window of the open round to keep, and the token behind them: `spec.accept_batch` over the round's
+        windows, in its order.  Writes int32 keep[i] and next[i] on the device; `commit(slots, keep[:n].tolist())` follows."""
+        if self.pending is None:
+            raise Invalid("no verify is open")
+        rows, n = self.meta.total_rows(), self.meta.batch()
+        if tokens.numel() != rows or target.shape[0] != rows:
+            raise Invalid(f"{tokens.numel()} tokens and {target.shape[0]} rows of the target for {rows} rows of the round")
+        stream = stream or self.pool.stream
+        self._order(stream)
+        cu_rows = self.meta.cu_rows.t[:(n + 1) * 4].view(K._torch().int32)
+        with contextlib.nullcontext() if stream.stream is None else K._torch().cuda.stream(stream.stream):
+            spec.accept_batch(cu_rows, tokens, target, u, keep, next, probabilities=probabilities, draft=draft, temperature=temperature)
 
     # ---- commit -----------------------------------------------------------------------------------------------
     def commit(self, slots: Sequence[marks.GlmKv], keep: Sequence[int], stream: Optional[K.Stream] = None) -> None:
