@@ -138,6 +138,30 @@ __device__ __forceinline__ PairTile pair_tile(const PairParams& p, long long t) 
 }
 
 // SPLIT_ROWS: rows per tile at most where k runs in segments.  
+// A lane's feature of a chunk's rows, one after the other: a whole chunk's as straight stores or loads (with the extents looked at for every row and the address
+// multiplied out, 26 instructions a value were the time: two groups of 333 rows x 8,192 f32 results 33 us, so 16).  Of a residual's rows
+// past the last the last is read again.
+constexpr int kRowsAChunk = kChunk;
+template <typename T, typename Value>
+__device__ __forceinline__ void put_rows(T* to, long long stride, int live, Value value) {
+    if (live == kRowsAChunk) {
+#pragma unroll
+        for (int j = 0; j < kRowsAChunk; ++j, to += stride) *to = value(j);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kRowsAChunk; ++j, to += stride)
+            if (j < live) *to = value(j);
+    }
+}
+template <typename T, typename Take>
+__device__ __forceinline__ void get_rows(const T* from, long long stride, int live, Take take) {
+#pragma unroll
+    for (int j = 0; j < kRowsAChunk; ++j) {
+        take(j, *from);
+        from += j + 1 < live ? stride : 0;
+    }
+}
+
 template <int SPLIT_ROWS, int EPI>
 __global__ void __launch_bounds__(kPairThreads, 1) proj_gemm_pair_kernel(const __grid_constant__ PairParams p) {
     using L = PairSmem<EPI>;
@@ -287,24 +311,11 @@ __global__ void __launch_bounds__(kPairThreads, 1) proj_gemm_pair_kernel(const _
             if constexpr (EPI == kResidualDirect) {
                 const ProjEpilogue& e = x.q.epi;
                 if (c0 >= x.q.row_tile) return;
-                const int row0 = x.rt * x.q.row_tile + c0, last = min(x.q.rows - 1 - row0, kChunk - 1);
-                if (last < 0) return;
-                long long at = (long long)x.g * e.r_gstride + row0 * e.ldr + min(x.nt * 2 * kPM + (int)rank * kPM + q * 32 + lane, x.q.n - 1);
-                if (x.q.out_f32) {
-                    const float* from = static_cast<const float*>(e.residual);
-#pragma unroll
-                    for (int j = 0; j < kChunk; ++j) {
-                        res[j] = from[at];
-                        at += j < last ? e.ldr : 0;
-                    }
-                } else {
-                    const uint16_t* from = static_cast<const uint16_t*>(e.residual);
-#pragma unroll
-                    for (int j = 0; j < kChunk; ++j) {
-                        res[j] = bf16_bits_to_f32(from[at]);
-                        at += j < last ? e.ldr : 0;
-                    }
-                }
+                const int row0 = x.rt * x.q.row_tile + c0, live = min(x.q.rows - row0, kChunk);
+                if (live <= 0) return;
+                const long long at = (long long)x.g * e.r_gstride + row0 * e.ldr + min(x.nt * 2 * kPM + (int)rank * kPM + q * 32 + lane, x.q.n - 1);
+                if (x.q.out_f32) get_rows(static_cast<const float*>(e.residual) + at, e.ldr, live, [&](int j, float r) { res[j] = r; });
+                else get_rows(static_cast<const uint16_t*>(e.residual) + at, e.ldr, live, [&](int j, uint16_t r) { res[j] = bf16_bits_to_f32(r); });
             }
         };
         // ... or by tensor copies, two chunks ahead of the one that is being finished.  A place in the sequence of this pair's chunks:
@@ -432,15 +443,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) proj_gemm_pair_kernel(const _
                     bulk_commit();
                 }
             } else if (f0 + fl < x.q.n) {
-                unsigned char* base = reinterpret_cast<unsigned char*>(x.q.out) + ((long long)x.g * x.q.o_gstride + f0 + fl) * (x.q.out_f32 ? 4 : 2);
-#pragma unroll
-                for (int j = 0; j < kChunk; ++j) {
-                    const long long row = row0 + j;
-                    if (row < x.q.rows && c0 + j < x.q.row_tile) {
-                        if (x.q.out_f32) *reinterpret_cast<float*>(base + row * x.q.ldo * 4) = v[j];
-                        else *reinterpret_cast<uint16_t*>(base + row * x.q.ldo * 2) = f32_to_bf16_bits(v[j]);
-                    }
-                }
+                const int live = (int)min(min((long long)kChunk, x.q.rows - row0), (long long)(x.q.row_tile - c0));
+                const long long at = (long long)x.g * x.q.o_gstride + f0 + fl + row0 * x.q.ldo;
+                if (x.q.out_f32) put_rows(static_cast<float*>(x.q.out) + at, x.q.ldo, live, [&](int j) { return v[j]; });
+                else put_rows(static_cast<uint16_t*>(x.q.out) + at, x.q.ldo, live, [&](int j) { return f32_to_bf16_bits(v[j]); });
             }
         };
         auto release = [&] {
