@@ -4,11 +4,14 @@
 // kept while u_{i+1} q_{i+1}(token) < p_i(token); the next token is drawn by a running sum from max(p - q, 0) of the first refused
 // token's row, or from p behind a whole window.
 //
-// Bound by HBM for many requests (logits are read once for a row's maximum and sum; the row that is drawn from comes from L2 the
-// second time) and by latency for one.  A request is a thread-block cluster: each block takes a slice of the vocabulary, all rows of the
-// window; the slices' maxima and sums meet in distributed shared memory, every block makes the same decision, and all of
-// them draw together: a warp sums a run of consecutive weights, the one whose run holds the drawn point looks for it.  One launch,
-// no scratch in global memory, no atomics: the same result every time.
+// Bound by HBM for many requests' windows, by the instructions of the draws next to it, and by latency for one.  A request is a thread-block cluster: each block
+// takes a slice of the vocabulary, all rows of the window; the slices' maxima and sums meet in distributed shared memory, every block makes the same
+// decision, and all of them draw together: a warp sums a run of consecutive weights, the one whose run holds the drawn point looks for it.  One launch, no
+// scratch in global memory, no atomics: the same result every time.
+//
+// Rows are read between their 16-byte boundaries, wherever those lie, through a ring of asynchronous copies for each warp (48 greedy windows of eight rows of
+// 131,072 bf16 logits, 101 MB: 30 us, 3.4 TB/s; with eight loads a lane in registers, which the compiler spills, 47, with two times four 39).  The row that is drawn
+// from comes from L2 the second time; a draw of all 48 adds 20 us, another 16 with a drafter's distributions to read and a second pass.
 //
 // A draw decides between neighbours of a sum over the whole vocabulary, so weights and sums are formed in 64 bits there: in 32, the sums'
 // rounding moves one draw in a few hundred to the next token.  The maxima and sums that judge a token are 32-bit ones (a relative 1e-7
@@ -38,17 +41,20 @@ struct AcceptParams {
     int blocks;
 };
 
+constexpr int kCopies = 16;  // of the table of powers
+constexpr int kSlots = 4;
+
 struct AccShared {
-    double power[32];  // 2^(j / 32)
+    double power[32][kCopies];  // 2^(j / 32)
     // What this block's slice gives, read by the other blocks of the cluster.
     float max[kAccRows], sum[kAccRows];
     int best[kAccRows];
     double part;      // the slice's weights
     // Within the block.
-    float wmax[kAccRows][kAccMostWarps], wsum[kAccRows][kAccMostWarps];
-    int wbest[kAccRows][kAccMostWarps];
+    float wmax[kAccRows][kAccMostWarps + 1], wsum[kAccRows][kAccMostWarps + 1];  // (the last place: the row's two ends)
+    int wbest[kAccRows][kAccMostWarps + 1];
     double wpart[kAccMostWarps];
-    double slot[kAccMostWarps][32];  // a warp's weights, its places in 32 parts
+    double slot[kAccMostWarps][kSlots];  // a warp's weights, its places in so many parts
     float row_max[kAccRows], row_sum[kAccRows];
     int row_best[kAccRows];
     int kept;
@@ -86,47 +92,46 @@ __device__ __forceinline__ double peer_f64(const void* local, uint32_t block) {
     return v;
 }
 
+// Copies into a lane's own places of its warp's ring.
+__device__ __forceinline__ void copy_16(void* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_sent() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LATER>
+__device__ __forceinline__ void copies_here() { asm volatile("cp.async.wait_group %0;" ::"n"(LATER) : "memory"); }  // all but the last LATER groups
+
 constexpr float kNoLogit = -INFINITY;
 template <int KIND>
 __device__ __forceinline__ float target_at(const void* row, long long i) {
     if constexpr (KIND == GLM53F_KDA_LOGITS_BF16) return bf16_bits_to_f32(__ldg(static_cast<const uint16_t*>(row) + i));
     else return __ldg(static_cast<const float*>(row) + i);
 }
-// Eight consecutive entries from i on as they lie in memory (vector loads; or, where the row's end or its alignment rules those out, one at a
-// time, those at `end` and beyond as `fill`), and as floats.  Apart, so that several loads are in flight before the first is looked at.
+// Eight consecutive entries from i on as they lie in memory (vector loads; or, where a row's end rules those out, one at a time, those before the row and behind it as
+// `fill`), and as floats.  Apart, so that several loads are in flight before the first is looked at.
 template <int KIND>
 struct Eight {
     static constexpr int kWords = KIND == GLM53F_KDA_LOGITS_BF16 ? 4 : 8;
     uint32_t w[kWords];
-    __device__ __forceinline__ void load_whole(const void* row, long long i) {
+    // How many entries lie between a 16-byte boundary and the row: runs of eight begin that much before a multiple of eight.
+    static __device__ __forceinline__ int shift(const void* row) { return (int)(reinterpret_cast<uintptr_t>(row) & 15) / (kWords / 2); }
+    __device__ __forceinline__ void load_whole(const void* row, int i) {
 #pragma unroll
         for (int j = 0; j < kWords; j += 4) {
-            const uint4 r = __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(row) + i * (kWords / 2)) + j / 4);
+            const uint4 r = __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(row) + (long long)i * (kWords / 2)) + j / 4);
             w[j] = r.x, w[j + 1] = r.y, w[j + 2] = r.z, w[j + 3] = r.w;
         }
     }
-    __device__ __forceinline__ void load_some(const void* row, long long i, long long end, float fill) {
+    __device__ __forceinline__ void load_some(const void* row, int i, int end, float fill) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const uint32_t u = __float_as_uint(i + j < end ? target_at<KIND>(row, i + j) : fill);
+            const uint32_t u = __float_as_uint(i + j >= 0 && i + j < end ? target_at<KIND>(row, i + j) : fill);
             if constexpr (kWords == 8) w[j] = u;
             else w[j >> 1] = j & 1 ? w[j >> 1] | (u & 0xffff0000u) : u >> 16;
         }
     }
-    __device__ __forceinline__ void load(const void* row, long long i, long long end, bool vec, float fill) {
-        if (vec && i + 8 <= end) load_whole(row, i);
+    __device__ __forceinline__ void load(const void* row, int i, int end, bool aligned, float fill) {
+        if (aligned && i >= 0 && i <= end - 8) load_whole(row, i);
         else load_some(row, i, end, fill);
-    }
-    // The largest of them (NaN only where all are).
-    __device__ __forceinline__ float top() const {
-        if constexpr (kWords == 8) {
-            const float* x = reinterpret_cast<const float*>(w);
-            return fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-        } else {
-            const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(w);
-            const __nv_bfloat162 m = __hmax2(__hmax2(x[0], x[1]), __hmax2(x[2], x[3]));
-            return fmaxf(__low2float(m), __high2float(m));
-        }
     }
     __device__ __forceinline__ void get(float (&x)[8]) const {
 #pragma unroll
@@ -137,27 +142,29 @@ struct Eight {
     }
 };
 
-// A row's weights in 64 bits: e^x of x = (l - max) / t <= 0.  x = (32 e + j) ln 2 / 32 + r, so e^x = 2^e 2^(j/32) e^r with |r| < 0.011, of which
+// A row's weights in 64 bits: e^x of x = (l - max) / t <= 0.  With z = 32 x / ln 2 = 32 e + j + f, |f| <= 1/2: e^x = 2^e 2^(j/32) e^(f ln 2 / 32), of which
 // Taylor's series to the fourth power leaves 1.3e-12: a draw among 131,072 moves by it once in ten million.  (With the general exponential, and every
 // special case looked at for every entry, a draw's pass took four times as many instructions.)  NaN and what is below e^-690 is 0.  Rows whose
-// largest is infinite: see weights() in the kernel.
+// largest is infinite: see weights() in the kernel.  The pass waits for instructions, of which this is 20 an entry; the table lies in sixteen copies, two banks each.
 constexpr double kTurns = 46.166241308446828384;  // 32 / ln 2
 struct RowScale {
-    double max, inv_t, turns;  // turns: inv_t 32 / ln 2
+    double max, turns;  // turns: 32 / (t ln 2)
+    float lowest;       // max - 690 t: what counts as 0 lies below
 };
-__device__ __forceinline__ double logit_weight(float l, const RowScale& a, const double* power) {
+__device__ __forceinline__ RowScale row_scale_of(float max, float t) { return {(double)max, kTurns / (double)t, fmaf(-690.0f, t, max)}; }
+__device__ __forceinline__ double logit_weight(float l, const RowScale& a, const double* power) {  // power: the lane's copy
+    constexpr double c = 1.0 / kTurns;
     const double magic = 6755399441055744.0;  // 1.5 2^52: adding it rounds to an integer, which the low word then holds
-    const double d = (double)l - a.max, x = d * a.inv_t, shifted = fma(d, a.turns, magic);
+    const double z = ((double)l - a.max) * a.turns, shifted = z + magic;
     const int n = __double2loint(shifted);
-    const double whole = shifted - magic;
-    double r = fma(whole, -0.021660849390173098, x);
-    r = fma(whole, -2.325192846878874e-12, r);
-    double y = fma(r, 1.0 / 24, 1.0 / 6);
-    y = fma(r, y, 0.5);
-    y = fma(r, y, 1.0);
-    y = fma(r, y, 1.0);
-    const double base = power[n & 31];
-    return x > -690.0 ? y * __hiloint2double(__double2hiint(base) + ((n >> 5) << 20), __double2loint(base)) : 0.0;
+    const double f = z - (shifted - magic);
+    double y = fma(f, c * c * c * c / 24, c * c * c / 6);
+    y = fma(f, y, c * c / 2);
+    y = fma(f, y, c);
+    y = fma(f, y, 1.0);
+    const double base = power[(n & 31) * kCopies];
+    y *= __hiloint2double(((n & ~31) << 15) + __double2hiint(base), __double2loint(base));
+    return l >= a.lowest ? y : 0.0;
 }
 __device__ __forceinline__ float finite_weight(float p) { return p > 0.0f && p < INFINITY ? p : 0.0f; }
 
@@ -166,35 +173,77 @@ struct Stats {
     float m = kNoLogit, s = 0.0f;
     int best = -1;
 };
-template <bool GREEDY, int KIND>
-__device__ __forceinline__ void take(Stats& a, const Eight<KIND>& in, int at, long long vocab, float scale) {
-    const float top = in.top();
-    float x[8];
-    if constexpr (GREEDY) {
-        if (top > a.m || a.best < 0) {
-            in.get(x);
-            a.m = fmaxf(top, a.m);
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return fma2(a, make_float2(1.0f, 1.0f), b); }
+// A chunk: four pieces of 16 bytes a lane, a piece's lanes next to one another; the lane's first entry is entry `at` of the row.
+constexpr int kPieces = 4, kPiece = 512, kChunk = 32 * kPieces;  // (a chunk in pieces of one lane)
+template <int KIND>
+constexpr int kEach = KIND == GLM53F_KDA_LOGITS_BF16 ? 8 : 4;  // entries of a piece
+template <int KIND>
+__device__ __forceinline__ void entries(const uint4& piece, float (&x)[kEach<KIND>]) {
+    const uint32_t w[4] = {piece.x, piece.y, piece.z, piece.w};
 #pragma unroll
-            for (int j = 7; j >= 0; --j)
-                if (x[j] == top && at + j < vocab) a.best = at + j;
+    for (int j = 0; j < kEach<KIND>; ++j) {
+        if constexpr (kEach<KIND> == 4) x[j] = __uint_as_float(w[j]);
+        else x[j] = __uint_as_float(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
+    }
+}
+template <int KIND>
+__device__ __forceinline__ float largest(const uint4 (&in)[kPieces]) {  // (NaN only where all are)
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(in);
+    if constexpr (kEach<KIND> == 4) {
+        float m = __uint_as_float(w[0]);
+#pragma unroll
+        for (int j = 1; j < 4 * kPieces; ++j) m = fmaxf(m, __uint_as_float(w[j]));
+        return m;
+    } else {
+        const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(w);
+        __nv_bfloat162 m[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+        for (int j = 4; j < 4 * kPieces; ++j) m[j & 3] = __hmax2(m[j & 3], x[j]);
+        m[0] = __hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3]));
+        return fmaxf(__low2float(m[0]), __high2float(m[0]));
+    }
+}
+template <bool GREEDY, int KIND>
+__device__ __forceinline__ void take(Stats& a, const uint4 (&in)[kPieces], int at, float scale) {
+    const float top = largest<KIND>(in);
+    float x[kEach<KIND>];
+    if constexpr (GREEDY) {
+        if (top > a.m) {
+            a.m = top;
+#pragma unroll
+            for (int i = kPieces - 1; i >= 0; --i) {
+                entries<KIND>(in[i], x);
+#pragma unroll
+                for (int j = kEach<KIND> - 1; j >= 0; --j)
+                    if (x[j] == top) a.best = at + i * 32 * kEach<KIND> + j;
+            }
         }
     } else {
         if (top > a.m) {
             a.s *= a.m == kNoLogit ? 0.0f : ex2_approx((a.m - top) * scale);
             a.m = top;
         }
-        in.get(x);
-        float2 sum[4];
+        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        const float2 less = make_float2(-a.m, -a.m), times = make_float2(scale, scale);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 t = mul2(fma2(make_float2(a.m, a.m), make_float2(-1.0f, -1.0f), make_float2(x[2 * j], x[2 * j + 1])), make_float2(scale, scale));
-            sum[j] = make_float2(ex2_ftz(t.x), ex2_ftz(t.y));
+        for (int i = 0; i < kPieces; ++i) {
+            entries<KIND>(in[i], x);
+#pragma unroll
+            for (int j = 0; j < kEach<KIND>; j += 2) {
+                const float2 t = mul2(add2(make_float2(x[j], x[j + 1]), less), times);
+                sum[j / 2 & 1] = add2(sum[j / 2 & 1], make_float2(ex2_ftz(t.x), ex2_ftz(t.y)));
+            }
         }
-        float all = ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) + ((sum[2].x + sum[2].y) + (sum[3].x + sum[3].y));
+        float all = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         if (!(all < INFINITY)) {  // a NaN among them, or infinities: seldom, so one at a time
             all = 0.0f;
+#pragma unroll 1
+            for (int i = 0; i < kPieces; ++i) {
+                entries<KIND>(i == 0 ? in[0] : i == 1 ? in[1] : i == 2 ? in[2] : in[3], x);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) all += x[j] == a.m ? (a.m == kNoLogit ? 0.0f : 1.0f) : x[j] < a.m ? ex2_ftz((x[j] - a.m) * scale) : 0.0f;
+                for (int j = 0; j < kEach<KIND>; ++j) all += x[j] == a.m ? (a.m == kNoLogit ? 0.0f : 1.0f) : x[j] < a.m ? ex2_ftz((x[j] - a.m) * scale) : 0.0f;
+            }
         }
         a.s += all;
     }
@@ -216,19 +265,28 @@ __device__ __forceinline__ void join_lanes(Stats& a, float scale) {
     a.m = m;
 }
 
+// Chunks of a warp on their way.
+template <int WARPS>
+constexpr int kRingChunks = WARPS == 8 ? 4 : 2;
+
 // What a draw weighs: the row's distribution p, less the drafter's, or without the refused token.
 enum : int { kWhole = 0, kLessDraft = 1, kWithout = 2 };
 
 template <int KIND, int kAccWarps>
 __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept_kernel(const __grid_constant__ AcceptParams p) {
-    constexpr int kAccThreads = kAccWarps * 32, kAccDeep = KIND == GLM53F_KDA_LOGITS_BF16 ? 4 : 2;  // (rows read side by side)
+    constexpr int kDeep = kRingChunks<kAccWarps>;
+    extern __shared__ __align__(16) unsigned char rings[];
     constexpr bool LOGITS = KIND != GLM53F_KDA_PROBABILITIES;
     constexpr int kSize = KIND == GLM53F_KDA_LOGITS_BF16 ? 2 : 4;
     __shared__ AccShared sh;
-    if (threadIdx.x < 32) sh.power[threadIdx.x] = exp2((double)threadIdx.x / 32);
+    if (threadIdx.x < 32) {
+        const double power = exp2((double)threadIdx.x / 32);
+        for (int i = 0; i < kCopies; ++i) sh.power[threadIdx.x][i] = power;
+    }
     grid_ready();
-    const int blocks = p.blocks, b = blockIdx.x / blocks, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int blocks = p.blocks, b = blockIdx.x >> (__ffs(blocks) - 1), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t block = cluster_block();
+    unsigned char* ring = rings + warp * (kDeep * kPieces * kPiece) + lane * 16;
     const int first = p.cu[b], n = p.cu[b + 1] - first;
     if (n <= 0) {  // the same for the whole cluster
         if (block == 0 && tid == 0) p.keep[b] = 0, p.next[b] = -1;
@@ -237,15 +295,14 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
     const unsigned char* rows = static_cast<const unsigned char*>(p.target) + (long long)first * p.ld * kSize;
     auto row_at = [&](int i) { return static_cast<const void*>(rows + (long long)i * p.ld * kSize); };
     auto draft_at = [&](int i) { return p.draft + (long long)(first + i) * p.draft_ld; };
-    const bool vec = (reinterpret_cast<uintptr_t>(p.target) & 15) == 0 && (p.ld * kSize) % 16 == 0;
-    const bool vec_draft = (reinterpret_cast<uintptr_t>(p.draft) & 15) == 0 && p.draft_ld % 4 == 0;
     // (Capped: an infinite one would make 0 times infinity of a logit of -inf.)
     const float temperature = LOGITS && p.temperature != nullptr ? (p.temperature[b] < 1e30f ? p.temperature[b] : 1e30f) : 1.0f;
     const bool greedy = LOGITS && !(temperature > 0.0f);
     const float scale = greedy ? 0.0f : kLog2e / temperature;
-    const double inv_t = greedy ? 0.0 : 1.0 / (double)temperature;
-    // This block's slice, in runs of eight.
-    const long long runs = (p.vocab + 7) / 8, run0 = runs * block / blocks, run1 = runs * (block + 1) / blocks;
+    const double* power = &sh.power[0][lane % kCopies];
+    const int block_bits = __ffs(blocks) - 1;  // (a power of two)
+    // This block's slice [run0, run1) of `runs` runs of eight.
+    auto slice = [&](long long runs, long long& run0, long long& run1) { run0 = runs * block >> block_bits, run1 = runs * (block + 1) >> block_bits; };
 
     __syncthreads();  // the powers
     int kept = 1;  // rows kept so far
@@ -269,40 +326,83 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
         if constexpr (LOGITS) {
             auto read = [&](auto is_greedy) {
                 constexpr bool GREEDY = decltype(is_greedy)::value;
-                for (int i0 = 0; i0 < rows_here; i0 += kAccDeep) {
-                    Stats st[kAccDeep];
-                    const int deep = min(rows_here - i0, kAccDeep);
-                    // All rows' entries at a place side by side, the next place's on their way while these are looked at.
-                    Eight<KIND> now[kAccDeep], ahead[kAccDeep];
-                    auto load = [&](long long r, Eight<KIND>(&to)[kAccDeep]) {
-                        if (vec && 8 * r + 8 <= p.vocab) {
+                // The pieces of a row between its 16-byte boundaries, this warp's share of them: address (of the lane's first), number, first entry.
+                constexpr int kWarpBits = kAccWarps == 16 ? 4 : 3;
+                static_assert(1 << kWarpBits == kAccWarps, "warps");
+                auto share = [&](int i, const unsigned char*& from, int& pieces, int& at) {
+                    const unsigned char* row = static_cast<const unsigned char*>(row_at(g0 + i));
+                    const int lead = (int)(0 - reinterpret_cast<uintptr_t>(row) & 15);
+                    const long long inside = (p.vocab - lead / kSize) / kEach<KIND>, w = (long long)block * kAccWarps + warp;  // (fewer than none: none)
+                    const int first_piece = (int)(max(inside, 0ll) * w >> (block_bits + kWarpBits));
+                    pieces = (int)(max(inside, 0ll) * (w + 1) >> (block_bits + kWarpBits)) - first_piece;
+                    from = row + lead + (long long)first_piece * 16 + lane * 16;
+                    at = lead / kSize + (first_piece + lane) * kEach<KIND>;
+                };
+                const unsigned char* from = nullptr;
+                int to_row = -1, left = 0, unused, to_slot = 0, slot = 0;
+                auto send = [&] {  // the next chunk's copies; behind the last row's, none
+                    while (left <= 0 && ++to_row < rows_here) share(to_row, from, left, unused);
+                    if (to_row < rows_here) {
+                        unsigned char* to = ring + to_slot * (kPieces * kPiece);
+                        if (left >= kChunk) {
 #pragma unroll
-                            for (int d = 0; d < kAccDeep; ++d) to[d].load_whole(row_at(g0 + i0 + min(d, deep - 1)), 8 * r);
+                            for (int i = 0; i < kPieces; ++i) copy_16(to + i * kPiece, from + i * kPiece);
                         } else {
 #pragma unroll
-                            for (int d = 0; d < kAccDeep; ++d) to[d].load_some(row_at(g0 + i0 + min(d, deep - 1)), 8 * r, p.vocab, kNoLogit);
+                            for (int i = 0; i < kPieces; ++i)
+                                if (32 * i + lane < left) copy_16(to + i * kPiece, from + i * kPiece);
                         }
-                    };
-                    if (run0 + tid < run1) load(run0 + tid, now);
-                    for (long long r = run0 + tid; r < run1; r += kAccThreads) {
-                        if (r + kAccThreads < run1) load(r + kAccThreads, ahead);
+                        from += kPieces * kPiece;
+                        left -= kChunk;
+                    }
+                    copies_sent();
+                    to_slot = to_slot + 1 == kDeep ? 0 : to_slot + 1;
+                };
+#pragma unroll 1
+                for (int j = 0; j < kDeep; ++j) send();
+#pragma unroll 1
+                for (int i = 0; i < rows_here; ++i) {
+                    Stats st;
+                    const unsigned char* unread;
+                    int pieces, at;
+                    share(i, unread, pieces, at);
+#pragma unroll 1
+                    for (; pieces > 0; pieces -= kChunk, at += kChunk * kEach<KIND>) {
+                        copies_here<kDeep - 1>();
+                        const unsigned char* here = ring + slot * (kPieces * kPiece);
+                        uint4 x[kPieces];
+                        const uint32_t fill = KIND == GLM53F_KDA_LOGITS_BF16 ? 0xff80ff80u : 0xff800000u;  // -inf
 #pragma unroll
-                        for (int d = 0; d < kAccDeep; ++d) {
-                            take<GREEDY>(st[d], now[d], (int)(8 * r), p.vocab, scale);
-                            now[d] = ahead[d];
+                        for (int j = 0; j < kPieces; ++j) {
+                            x[j] = make_uint4(fill, fill, fill, fill);
+                            if (32 * j + lane < pieces) x[j] = *reinterpret_cast<const uint4*>(here + j * kPiece);
                         }
+                        take<GREEDY, KIND>(st, x, at, scale);
+                        slot = slot + 1 == kDeep ? 0 : slot + 1;
+                        send();
                     }
-#pragma unroll
-                    for (int d = 0; d < kAccDeep; ++d) {
-                        join_lanes<GREEDY>(st[d], scale);
-                        if (lane == 0 && d < deep) sh.wmax[i0 + d][warp] = st[d].m, sh.wsum[i0 + d][warp] = st[d].s, sh.wbest[i0 + d][warp] = st[d].best;
-                    }
+                    join_lanes<GREEDY>(st, scale);
+                    if (lane == 0) sh.wmax[i][warp] = st.m, sh.wsum[i][warp] = st.s, sh.wbest[i][warp] = st.best;
                 }
+                // What lies before the first boundary and behind the last, 14 entries at most: a row to a warp of the first block.
+                if (warp < rows_here) {
+                    const void* row = row_at(g0 + warp);
+                    const int lead = (int)(0 - reinterpret_cast<uintptr_t>(row) & 15) / kSize;
+                    const long long inside = max((p.vocab - lead) / kEach<KIND>, 0ll) * kEach<KIND>, at = lane < lead ? lane : inside + lane;
+                    Stats a;
+                    if (block == 0 && at < p.vocab && lane < 16) {
+                        const float x = target_at<KIND>(row, at);
+                        if (x > kNoLogit) a.m = x, a.s = 1.0f, a.best = (int)at;
+                    }
+                    join_lanes<GREEDY>(a, scale);
+                    if (lane == 0) sh.wmax[warp][kAccWarps] = a.m, sh.wsum[warp][kAccWarps] = a.s, sh.wbest[warp][kAccWarps] = a.best;
+                }
+                __syncthreads();
                 // A warp to a row: over the block's warps, then over the cluster's blocks.
                 __syncthreads();
                 if (warp < rows_here) {
                     Stats a;
-                    if (lane < kAccWarps) a.m = sh.wmax[warp][lane], a.s = sh.wsum[warp][lane], a.best = sh.wbest[warp][lane];
+                    if (lane <= kAccWarps) a.m = sh.wmax[warp][lane], a.s = sh.wsum[warp][lane], a.best = sh.wbest[warp][lane];
                     join_lanes<GREEDY>(a, scale);
                     if (lane == 0) sh.max[warp] = a.m, sh.sum[warp] = a.s, sh.best[warp] = a.best;
                 }
@@ -330,7 +430,7 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
                 else if constexpr (LOGITS)
                 {
                     const float m = sh.row_max[lane];
-                    const double e = token_target == m ? 1.0 : m < INFINITY ? logit_weight(token_target, {(double)m, inv_t, inv_t * kTurns}, sh.power) : 0.0;
+                    const double e = token_target == m ? 1.0 : m < INFINITY ? logit_weight(token_target, row_scale_of(m, temperature), power) : 0.0;
                     keep = token_left * (double)sh.row_sum[lane] < e && m != kNoLogit;
                 }
                 else keep = token_left < (double)finite_weight(token_target);
@@ -361,17 +461,19 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
         int mode = whole ? kWhole : less != nullptr ? kLessDraft : kWithout;
         // (Short of 1, whatever is given: the drawn point then lies before the whole.)
         const double x01 = fmin(fmax((double)p.u[first], 0.0), 1.0 - 0x1p-53);
-        const RowScale row_scale{(double)stop_max, inv_t, inv_t * kTurns};
+        const RowScale row_scale = row_scale_of(stop_max, temperature);
         double norm = 1.0;  // the weights' sum, by which the drafter's probabilities are multiplied instead of dividing each of p's
         struct Place {
             Eight<KIND> x;
             Eight<GLM53F_KDA_PROBABILITIES> y;
         };
-        auto fetch = [&](long long i, Place& a) {
-            a.x.load(row, i, p.vocab, vec, LOGITS ? kNoLogit : 0.0f);
-            if (mode == kLessDraft) a.y.load(less, i, p.vocab, vec_draft, 0.0f);
+        const int shift = Eight<KIND>::shift(row), vocab = (int)p.vocab;
+        const bool draft_too = less != nullptr && (Eight<GLM53F_KDA_PROBABILITIES>::shift(less) - shift) % 4 == 0;  // (16-byte boundaries at the same entries)
+        auto fetch = [&](int i, Place& a) {
+            a.x.load(row, i, vocab, true, LOGITS ? kNoLogit : 0.0f);
+            if (mode == kLessDraft) a.y.load(less, i, vocab, draft_too, 0.0f);
         };
-        auto weights = [&](long long i, const Place& a, double (&w)[8]) {
+        auto weights = [&](int i, const Place& a, double (&w)[8]) {
             float x[8];
             a.x.get(x);
             if constexpr (!LOGITS) {
@@ -379,7 +481,7 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
                 for (int j = 0; j < 8; ++j) w[j] = (double)finite_weight(x[j]);
             } else if (fabsf(stop_max) < INFINITY) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) w[j] = logit_weight(x[j], row_scale, sh.power);
+                for (int j = 0; j < 8; ++j) w[j] = logit_weight(x[j], row_scale, power);
             } else {  // infinite logits share everything; of -inf alone nothing is left
 #pragma unroll
                 for (int j = 0; j < 8; ++j) w[j] = x[j] == INFINITY ? 1.0 : 0.0;
@@ -392,15 +494,17 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
                     const double rest = fma((double)fmaxf(y[j], 0.0f), -norm, w[j]);
                     w[j] = rest > 0.0 ? rest : 0.0;
                 }
-            } else if (mode == kWithout && token >= i && token < i + 8) {
+            } else if (mode == kWithout && (unsigned)(token - i) < 8u) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     if (i + j == token) w[j] = 0.0;
             }
         };
-        // A warp's runs of the slice, consecutive ones, in up to 32 slots of `group` steps of 32 runs.
-        const long long mine0 = run0 + (run1 - run0) * warp / kAccWarps, mine1 = run0 + (run1 - run0) * (warp + 1) / kAccWarps;
-        const int steps = (int)((mine1 - mine0 + 31) / 32), group = (steps + 31) / 32;
+        long long run0, run1;
+        slice((p.vocab + shift + 7) / 8, run0, run1);
+        // A warp's runs of the slice, consecutive ones, in slots of `group` steps of 32 runs.
+        const int mine0 = (int)(run0 + (run1 - run0) * warp / kAccWarps), mine1 = (int)(run0 + (run1 - run0) * (warp + 1) / kAccWarps);
+        const int steps = (mine1 - mine0 + 31) / 32, group = (steps + kSlots - 1) / kSlots;
         double before = 0.0, total = 0.0;
         // Passes over the row, one body of code: of logits with the drafter's probabilities first the weights' sum, then what is drawn from, and
         // once more where that leaves nothing.
@@ -410,14 +514,14 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
             int in_slot = 0, slot = 0;
             double part = 0.0, s = 0.0;
             Place now, ahead;
-            if (mine0 + lane < mine1) fetch(8 * (mine0 + lane), now);
+            if (mine0 + lane < mine1) fetch(8 * (mine0 + lane) - shift, now);
 #pragma unroll 1
             for (int k = 0; k < steps; ++k) {
-                const long long r = mine0 + 32 * k + lane;
-                if (r + 32 < mine1) fetch(8 * (r + 32), ahead);
+                const int r = mine0 + 32 * k + lane;
+                if (r + 32 < mine1) fetch(8 * (r + 32) - shift, ahead);
                 if (r < mine1) {
                     double w[8];
-                    weights(8 * r, now, w);
+                    weights(8 * r - shift, now, w);
                     s += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
                 }
                 now = ahead;
@@ -479,14 +583,14 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
                 // (Through to the warp's last step: should the sums' rounding leave the point behind the slot, it is the first weight behind it.)
 #pragma unroll 1
                 for (int k = slot * group; k < steps && found < 0; ++k) {
-                    const long long r = mine0 + 32 * k + lane;
+                    const int r = mine0 + 32 * k + lane;
                     double w[8], s8 = 0.0;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) w[j] = 0.0;
                     if (r < mine1) {
                         Place a;
-                        fetch(8 * r, a);
-                        weights(8 * r, a, w);
+                        fetch(8 * r - shift, a);
+                        weights(8 * r - shift, a, w);
                     }
 #pragma unroll
                     for (int j = 0; j < 8; ++j) s8 += w[j];
@@ -502,7 +606,7 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
                     for (int j = 0; j < 8; ++j) {
                         at += w[j];
                         if (w[j] > 0.0) {
-                            seen = (int)(8 * r + j);
+                            seen = 8 * r - shift + j;
                             if (at > point && hit == 0x7fffffff) hit = seen;
                         }
                     }
@@ -520,38 +624,59 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
     }
 }
 
+// The launch of a configuration, and how many of its clusters the device holds at a time (asked for once; 0 where it cannot be told).
 template <int KIND, int WARPS>
-int accept_launch(AcceptParams p, int batch, int blocks, cudaStream_t stream) {
-    p.blocks = blocks;
-    static int configured_dev = -1;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (configured_dev != dev) {
-        const cudaError_t e = cudaFuncSetAttribute(accept_kernel<KIND, WARPS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) return (int)e;
-        configured_dev = dev;
-    }
+struct AcceptLaunch {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)batch * p.blocks);
-    cfg.blockDim = dim3(WARPS * 32);
-    cfg.stream = stream;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)p.blocks;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1 + early_attribute(attr[1]);
-    return (int)cudaLaunchKernelEx(&cfg, accept_kernel<KIND, WARPS>, p);
-}
+    AcceptLaunch(int batch, int blocks, cudaStream_t stream) {
+        cfg.gridDim = dim3((unsigned)batch * blocks);
+        cfg.blockDim = dim3(WARPS * 32);
+        cfg.dynamicSmemBytes = KIND == GLM53F_KDA_PROBABILITIES ? 0 : WARPS * kRingChunks<WARPS> * kPieces * kPiece;  // (probabilities have no statistics)
+        cfg.stream = stream;
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)blocks;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+    }
+    cudaError_t configure() {
+        static int configured_dev = -1;
+        int dev = 0;
+        cudaGetDevice(&dev);
+        if (configured_dev == dev) return cudaSuccess;
+        cudaError_t e = cudaFuncSetAttribute(accept_kernel<KIND, WARPS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(accept_kernel<KIND, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes);
+        if (e == cudaSuccess) configured_dev = dev;
+        return e;
+    }
+    int fit() {
+        static int counted[2] = {-1, -1};
+        int& n = counted[attr[0].val.clusterDim.x == kAccMostBlocks];
+        if (n < 0) {
+            n = 0;
+            if (configure() != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, accept_kernel<KIND, WARPS>, &cfg) != cudaSuccess) cudaGetLastError(), n = 0;
+        }
+        return n;
+    }
+    int run(AcceptParams p) {
+        const cudaError_t e = configure();
+        if (e != cudaSuccess) return (int)e;
+        p.blocks = (int)attr[0].val.clusterDim.x;
+        cfg.numAttrs = 1 + early_attribute(attr[1]);
+        return (int)cudaLaunchKernelEx(&cfg, accept_kernel<KIND, WARPS>, p);
+    }
+};
 
-// Few requests: as many threads each as a cluster can have, while every block has an SM.  Many: blocks of which an SM holds two.
+// Few requests: as many threads each as a cluster can have, while all of them run at once.  (Eight windows of eight rows: 14 us in clusters of eight blocks of
+// sixteen warps, which fit, 24 in clusters of sixteen, of which one would have to wait.)  Many: smaller blocks, of which an SM holds three.
 template <int KIND>
 int accept_launch(const AcceptParams& p, int batch, cudaStream_t stream) {
-    const long long sms = sm_count();
-    if (batch * (long long)kAccMostBlocks <= sms) return accept_launch<KIND, kAccMostWarps>(p, batch, kAccMostBlocks, stream);
-    if (batch * 8ll <= sms) return accept_launch<KIND, kAccMostWarps>(p, batch, 8, stream);
-    return accept_launch<KIND, 8>(p, batch, 8, stream);
+    AcceptLaunch<KIND, kAccMostWarps> most(batch, kAccMostBlocks, stream), many(batch, 8, stream);
+    if (batch <= most.fit()) return most.run(p);
+    if (batch <= many.fit()) return many.run(p);
+    return AcceptLaunch<KIND, 8>(batch, 8, stream).run(p);
 }
 
 }  // namespace
@@ -561,7 +686,7 @@ extern "C" int glm53f_kda_accept_batch(int32_t batch, const int32_t* cu_rows, in
                                        const int32_t* tokens, const float* draft, int64_t draft_ld, const float* temperature, const float* u,
                                        int32_t* keep, int32_t* next, glm53f_stream_t stream_) {
     using namespace kda;
-    if (batch < 0 || batch > 0xfffffff || vocab < 1 || ld < vocab) return kInvalid;
+    if (batch < 0 || batch > 0xfffffff || vocab < 1 || vocab > 0x7fffffc0 || ld < vocab) return kInvalid;
     if (target_kind < GLM53F_KDA_PROBABILITIES || target_kind > GLM53F_KDA_LOGITS_BF16) return kInvalid;
     if (target_kind == GLM53F_KDA_PROBABILITIES && temperature != nullptr) return kInvalid;
     if (draft != nullptr && draft_ld < vocab) return kInvalid;
