@@ -22,8 +22,11 @@
 //   warps 20-27  the state, which is an operand of one product and the accumulator of the other: times e^G between the two
 //   warp 28      tensor copies of q, k, v, three chunks ahead     warp 31  sums and factors of the decays
 //   warp 29      the products with the state and to it            warp 30  the scores and their products with V
-// A chunk's products take 1,920 cycles of the tensor pipe; what the other roles issue for it is the tighter bound, so their bodies are loops, their waits
-// sleep, and operands take the form that costs the fewest instructions.
+// A chunk's products take 1,920 cycles of the tensor pipe and, where every SM works, its rows 2,900 of a share of HBM; it takes 3,300 to 4,000.  What bounds it is what
+// the other roles issue (2,200 instructions a scheduler) and the round of the state: its product with Q, its scaling, the sum of w V K, each of which waits
+// for the one before.  So bodies are loops, waits sleep, and operands take the form that costs the fewest instructions.  148 heads x 4,096 rows take 150 us
+// (69 of HBM's time), 64 heads x 8,192 rows in two segments 190 us (84), 8 heads x 65,536 in eighteen 206 us (82).  What was measured and is not here: w V^T through shared
+// memory, the state's scaling in registers, registers moved between the roles, polling waits, a second buffer of q, half of q ahead, tiles brought to L2 before.
 //
 // Few chains: a sequence is cut into segments that are walked at the same time, each from the state that the segments before it
 // leave.  That state comes from a pass over k and v alone (the state's product only), which writes what each segment adds from a zero
@@ -553,17 +556,17 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
             const float all = decays[c % kStages].all;
             tc::fence_after_sync();
 #pragma unroll 1
-                for (int i = 0; i < 64; i += 32) {
-                    uint32_t x[32];
-                    tc::tmem_ld32(at + i, x);
-                    tc::tmem_ld_wait();
+            for (int i = 0; i < 64; i += 32) {
+                uint32_t x[32];
+                tc::tmem_ld32(at + i, x);
+                tc::tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        const float2 z = mul2(make_float2(all, all), make_float2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])));
-                        x[j] = __float_as_uint(z.x), x[j + 1] = __float_as_uint(z.y);
-                    }
-                    tc::tmem_st32(at + i, x);
+                for (int j = 0; j < 32; j += 2) {
+                    const float2 z = mul2(make_float2(all, all), make_float2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])));
+                    x[j] = __float_as_uint(z.x), x[j + 1] = __float_as_uint(z.y);
                 }
+                tc::tmem_st32(at + i, x);
+            }
             tc::tmem_st_wait();
             tc::fence_before_sync();
             arrive(bAdd + (c & 1));

@@ -96,10 +96,6 @@ __device__ __forceinline__ void mma_bf16_ts_if(uint32_t leader, uint32_t d_tmem,
 }
 // The same on f32 operands of which the tensor core takes 11 bits (kind::tf32): 8 k an instruction, 8 columns of A in tensor memory.
 __device__ __forceinline__ constexpr uint32_t idesc_tf32(int M, int N) { return (1u << 4) | (2u << 7) | (2u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
-// Operand tile of R rows in boxes of 32 f32 along K, in the 128-byte swizzle.
-__device__ __forceinline__ uint64_t desc_sw128_kmajor_f32(const unsigned char* tile, int R, int k0) {
-    return smem_desc(tile + (size_t)(k0 / 32) * R * 128 + (k0 % 32) * 4, 16, 1024) | ((uint64_t)2 << 61);
-}
 __device__ __forceinline__ void mma_tf32_ts_if(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, bool accumulate) {
     asm volatile(
         "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
