@@ -4,7 +4,8 @@
  * (crates/glm53f-kda/kernels/glm53f_kda.h:73-270, bound by crates/glm53f-kda/src/ffi.rs:16-287) with the
  * same names, argument order, types and meaning, so the reference's Rust `ffi` module links against this
  * library unchanged.  Part 2 adds the "core" entry points the benchmark configurations use (inputs after
- * the short convolution: q, k, v, log decay, beta).
+ * the short convolution: q, k, v, log decay, beta), Part 3 linear attention with one decay a head and Part 4 the
+ * verification of drafted tokens, which the reference does not have.
  *
  * Conventions shared by every entry point (reference header lines 5-9, 43-47):
  *   - raw device pointers, strides and offsets in ELEMENTS of the pointed-to type, a CUDA stream;
@@ -480,8 +481,9 @@ int glm53f_kda_lin_decode_batch(int32_t heads, int32_t qk_heads, int32_t batch, 
  * sequence; rows (host) >= cu_rows[batch]: the rows that q, k and v hold.  The state is FP32 from the first row to the last and rounded
  * once; state_out must not be NULL, and equals state_in or has no byte in common with it.  `workspace` (16-byte aligned) of
  * glm53f_kda_lin_prefill_workspace_bytes(heads, batch, max_len) bytes lets long sequences of few (sequence, head) chains run in
- * several segments at once; with fewer bytes (0 and NULL among them) every chain is one walk.  Results depend on the number
- * of segments to the order of the FP32 sums, and on nothing else in the batch. */
+ * several segments at once; with fewer bytes (0 and NULL among them) in fewer, or every chain in one walk.  It is the call's own until
+ * the call has run.  What else is in the batch decides how many segments there are and whether up to 32 rows go row by row, which moves results within their
+ * rounding, and nothing more. */
 int64_t glm53f_kda_lin_prefill_workspace_bytes(int32_t heads, int32_t batch, int32_t max_len);
 int glm53f_kda_lin_prefill_varlen(int32_t heads, int32_t qk_heads, int32_t batch, const int32_t* cu_rows, int32_t rows, int32_t max_len,
                                   const glm53f_bf16* q, int64_t q_stride, const glm53f_bf16* k, int64_t k_stride,
@@ -511,7 +513,7 @@ int glm53f_kda_lin_prefill_varlen(int32_t heads, int32_t qk_heads, int32_t batch
  * is drawn from p behind a whole window, else from max(p - q, 0) of the first refused token's row -- without `draft`, from p
  * without that token; from p where this leaves nothing: the lowest index whose running sum, divided by the whole, exceeds
  * u.  Draws are made in 64 bits.  A row that leaves nothing gives next[b] = -1, a request without rows keep 0 and next -1.
- * One launch; nothing is allocated.  vocab >= 1, ld and draft_ld >= vocab. */
+ * One launch; nothing is allocated.  1 <= vocab <= 0x7fffffc0, ld and draft_ld >= vocab. */
 #define GLM53F_KDA_PROBABILITIES 0
 #define GLM53F_KDA_LOGITS_F32 1
 #define GLM53F_KDA_LOGITS_BF16 2

@@ -55,7 +55,7 @@ ACCEPT = "batch cu vocab target kind ld tokens draft draft_ld temperature u keep
 JUDGED = dict(batch=2, cu=AT, vocab=100, target=AT, kind=1, ld=100, tokens=AT, draft=None, draft_ld=0, temperature=None, u=AT, keep=AT, next=AT, stream=None)
 
 
-@pytest.mark.parametrize("bad", [dict(batch=-1), dict(batch=1 << 28), dict(vocab=0), dict(vocab=-3), dict(ld=99), dict(kind=3), dict(kind=-1), dict(kind=0, temperature=AT),
+@pytest.mark.parametrize("bad", [dict(batch=-1), dict(batch=1 << 28), dict(vocab=0), dict(vocab=-3), dict(vocab=0x7fffffc1, ld=1 << 31), dict(ld=99), dict(kind=3), dict(kind=-1), dict(kind=0, temperature=AT),
                                  dict(draft=AT, draft_ld=99), dict(cu=None), dict(target=None), dict(tokens=None), dict(u=None), dict(keep=None), dict(next=None),
                                  dict(target=AT + 2), dict(kind=0, target=AT + 1), dict(kind=2, target=AT + 1), dict(draft=AT + 2, draft_ld=100)], ids=str)
 def test_accept(ffi, bad):
