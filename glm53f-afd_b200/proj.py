@@ -78,6 +78,8 @@ def fused(x: torch.Tensor, ldx: int, x_gstride: int, w: Bf16Mat, rows: int, out:
     if code >= 0:
         return _launched(code, "glm53f_kda_proj_bf16_fused")
     # Not the plain accepted call: the same checks here, with their errors.
+    if min(rows, ldx, x_gstride, ldo, o_gstride, x_offset, out_offset) < 0:
+        raise Invalid("rows, strides and offsets are not negative")
     job = _job(x, ldx, x_gstride, w, rows, out, ldo, o_gstride, out_f32, x_offset, out_offset)
     e = ffi.ProjEpilogue(activation=ACTIVATIONS[activation])
     if bias is not None:

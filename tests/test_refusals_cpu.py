@@ -127,6 +127,11 @@ def test_python_refusals(pkg):
             proj.fused(x, 128, 0, w, 4, out, 64, 0, **kw)
     with pytest.raises(proj.Invalid, match="smaller"):
         proj.fused(x, 128, 0, w, 5, out, 64, 0)
+    for kw in (dict(x_offset=-128), dict(out_offset=-64)):  # before the tensor
+        with pytest.raises(proj.Invalid, match="not negative"):
+            proj.fused(x, 128, 0, w, 2, out, 64, 0, **kw)
+    with pytest.raises(proj.Invalid, match="not negative"):
+        proj.fused(x, 128, -128, w, 2, out, 64, 0)
 
 
 def test_accepting_without_a_round(pkg, monkeypatch):
