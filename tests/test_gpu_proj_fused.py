@@ -148,3 +148,18 @@ def test_a_rows_result_does_not_depend_on_the_others(proj):
         some = torch.empty(rows, n, device="cuda")
         proj.fused(x, k, 0, mat, rows, some, n, 0, True, bias=b, activation="gelu", residual=r)
         assert torch.equal(some, whole[:rows]), rows
+
+
+@pytest.mark.parametrize("act,at_minus_inf,at_inf", [("relu", 0.0, math.inf), ("gelu", 0.0, math.inf), ("silu", None, math.inf), ("gelu_tanh", None, math.inf), ("sigmoid", 0.0, 1.0)])
+def test_infinities_and_nan(proj, act, at_minus_inf, at_inf):
+    """By the bias, at few rows and on SM pairs.  (Where the formula has minus infinity times zero, either that or the limit, 0.)"""
+    for rows in (3, 130):
+        x, w = torch.zeros(rows, 64, dtype=torch.bfloat16, device="cuda"), torch.zeros(64, 64, dtype=torch.bfloat16, device="cuda")
+        y = torch.zeros(64, device="cuda")
+        y[0], y[9], y[17], y[33], y[34] = -math.inf, math.inf, math.nan, 3e38, -3e38
+        out = torch.empty(rows, 64, device="cuda")
+        proj.fused(x, 64, 0, proj.Bf16Mat.dense(w), rows, out, 64, 0, True, bias=y, activation=act)
+        low, high, nan, big, small = (out[:, i] for i in (0, 9, 17, 33, 34))
+        assert nan.isnan().all() and (high == at_inf).all() and (big == (1.0 if act == "sigmoid" else y[33])).all() and (small == 0).all()
+        assert ((low == at_minus_inf) if at_minus_inf is not None else (low.isnan() | (low == 0))).all()
+        assert torch.isfinite(out[:, 40:]).all()
