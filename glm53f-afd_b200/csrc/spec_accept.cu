@@ -10,7 +10,7 @@
 // scratch in global memory, no atomics: the same result every time.
 //
 // Rows are read between their 16-byte boundaries, wherever those lie, through a ring of asynchronous copies for each warp (48 greedy windows of eight rows of
-// 131,072 bf16 logits, 101 MB: 30 us, 3.4 TB/s; with eight loads a lane in registers, which the compiler spills, 47, with two times four 39).  The row that is drawn
+// 131,072 bf16 logits, 101 MB: 28 us, 3.6 TB/s; with eight loads a lane in registers, which the compiler spills, 47, with two times four 39).  The row that is drawn
 // from comes from L2 the second time; a draw of all 48 adds 20 us, another 16 with a drafter's distributions to read and a second pass.
 //
 // A draw decides between neighbours of a sum over the whole vocabulary, so weights and sums are formed in 64 bits there: in 32, the sums'
@@ -326,23 +326,32 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
         if constexpr (LOGITS) {
             auto read = [&](auto is_greedy) {
                 constexpr bool GREEDY = decltype(is_greedy)::value;
-                // The pieces of a row between its 16-byte boundaries, this warp's share of them: address (of the lane's first), number, first entry.
+                // The pieces of the rows between their 16-byte boundaries, in lines of 32, all rows' one after the other; a warp takes consecutive lines, of one row or a few.
+                // (An equal share of every row instead has a warp join its lanes for each: windows of eight rows 4 us longer.)
                 constexpr int kWarpBits = kAccWarps == 16 ? 4 : 3;
                 static_assert(1 << kWarpBits == kAccWarps, "warps");
-                auto share = [&](int i, const unsigned char*& from, int& pieces, int& at) {
+                const int lines = (int)((p.vocab / kEach<KIND> + 31) / 32);
+                const long long mine = (long long)block * kAccWarps + warp, all_lines = (long long)rows_here * lines;
+                const int line0 = (int)(all_lines * mine >> (block_bits + kWarpBits)), line1 = (int)(all_lines * (mine + 1) >> (block_bits + kWarpBits));
+                // The part of row i from line `line` of all on: address (of the lane's first piece), pieces, first entry.  Rows may have fewer pieces than lines make: then none.
+                auto part_of = [&](int i, int line, const unsigned char*& from, int& pieces, int& at) {
                     const unsigned char* row = static_cast<const unsigned char*>(row_at(g0 + i));
                     const int lead = (int)(0 - reinterpret_cast<uintptr_t>(row) & 15);
-                    const long long inside = (p.vocab - lead / kSize) / kEach<KIND>, w = (long long)block * kAccWarps + warp;  // (fewer than none: none)
-                    const int first_piece = (int)(max(inside, 0ll) * w >> (block_bits + kWarpBits));
-                    pieces = (int)(max(inside, 0ll) * (w + 1) >> (block_bits + kWarpBits)) - first_piece;
-                    from = row + lead + (long long)first_piece * 16 + lane * 16;
+                    const int inside = max((int)p.vocab - lead / kSize, 0) / kEach<KIND>, first_piece = (line - i * lines) * 32;
+                    pieces = min(inside, (min(line1, (i + 1) * lines) - i * lines) * 32) - first_piece;
+                    from = row + lead + (long long)(first_piece + lane) * 16;
                     at = lead / kSize + (first_piece + lane) * kEach<KIND>;
                 };
+                if (lane < kAccRows) sh.wmax[lane][warp] = kNoLogit, sh.wsum[lane][warp] = 0.0f, sh.wbest[lane][warp] = -1;  // (rows that this warp has nothing of)
+                __syncwarp();
                 const unsigned char* from = nullptr;
-                int to_row = -1, left = 0, unused, to_slot = 0, slot = 0;
-                auto send = [&] {  // the next chunk's copies; behind the last row's, none
-                    while (left <= 0 && ++to_row < rows_here) share(to_row, from, left, unused);
-                    if (to_row < rows_here) {
+                int row = lines > 0 ? line0 / lines : 0, to_row = row, to_line = line0, left = 0, unused, to_slot = 0, slot = 0;
+                auto send = [&] {  // the next chunk's copies; behind the last line, none
+                    while (left <= 0 && to_line < line1) {
+                        part_of(to_row, to_line, from, left, unused);
+                        to_line = ++to_row * lines;
+                    }
+                    if (left > 0) {
                         unsigned char* to = ring + to_slot * (kPieces * kPiece);
                         if (left >= kChunk) {
 #pragma unroll
@@ -361,11 +370,11 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
 #pragma unroll 1
                 for (int j = 0; j < kDeep; ++j) send();
 #pragma unroll 1
-                for (int i = 0; i < rows_here; ++i) {
+                for (int line = line0; line < line1; line = ++row * lines) {
                     Stats st;
                     const unsigned char* unread;
                     int pieces, at;
-                    share(i, unread, pieces, at);
+                    part_of(row, line, unread, pieces, at);
 #pragma unroll 1
                     for (; pieces > 0; pieces -= kChunk, at += kChunk * kEach<KIND>) {
                         copies_here<kDeep - 1>();
@@ -382,7 +391,7 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
                         send();
                     }
                     join_lanes<GREEDY>(st, scale);
-                    if (lane == 0) sh.wmax[i][warp] = st.m, sh.wsum[i][warp] = st.s, sh.wbest[i][warp] = st.best;
+                    if (lane == 0) sh.wmax[row][warp] = st.m, sh.wsum[row][warp] = st.s, sh.wbest[row][warp] = st.best;
                 }
                 // What lies before the first boundary and behind the last, 14 entries at most: a row to a warp of the first block.
                 if (warp < rows_here) {
@@ -669,7 +678,7 @@ struct AcceptLaunch {
     }
 };
 
-// Few requests: as many threads each as a cluster can have, while all of them run at once.  (Eight windows of eight rows: 14 us in clusters of eight blocks of
+// Few requests: as many threads each as a cluster can have, while all of them run at once.  (Eight windows of eight rows: 11 us in clusters of eight blocks of
 // sixteen warps, which fit, 24 in clusters of sixteen, of which one would have to wait.)  Many: smaller blocks, of which an SM holds three.
 template <int KIND>
 int accept_launch(const AcceptParams& p, int batch, cudaStream_t stream) {
