@@ -10,8 +10,8 @@
 // scratch in global memory, no atomics: the same result every time.
 //
 // Rows are read between their 16-byte boundaries, wherever those lie, through a ring of asynchronous copies for each warp (48 greedy windows of eight rows of
-// 131,072 bf16 logits, 101 MB: 28 us, 3.6 TB/s; with eight loads a lane in registers, which the compiler spills, 47, with two times four 39).  The row that is drawn
-// from comes from L2 the second time; a draw of all 48 adds 20 us, another 16 with a drafter's distributions to read and a second pass.
+// 131,072 bf16 logits, 101 MB: 27 us, 3.7 TB/s; with eight loads a lane in registers, which the compiler spills, 47, with two times four 39).  The row that is drawn
+// from comes from L2 the second time; a draw of all 48 adds 16 us, another 16 with a drafter's distributions to read and a second pass.
 //
 // A draw decides between neighbours of a sum over the whole vocabulary, so weights and sums are formed in 64 bits there: in 32, the sums'
 // rounding moves one draw in a few hundred to the next token.  The maxima and sums that judge a token are 32-bit ones (a relative 1e-7
@@ -265,16 +265,14 @@ __device__ __forceinline__ void join_lanes(Stats& a, float scale) {
     a.m = m;
 }
 
-// Chunks of a warp on their way.
-template <int WARPS>
-constexpr int kRingChunks = WARPS == 8 ? 4 : 2;
+// Chunks of a warp on their way.  (Four: 48 drawn windows 47 us, of which L1, that much smaller then, serves the row's second reading; two: 43.  One: 44.)
+constexpr int kDeep = 2;
 
 // What a draw weighs: the row's distribution p, less the drafter's, or without the refused token.
 enum : int { kWhole = 0, kLessDraft = 1, kWithout = 2 };
 
 template <int KIND, int kAccWarps>
 __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept_kernel(const __grid_constant__ AcceptParams p) {
-    constexpr int kDeep = kRingChunks<kAccWarps>;
     extern __shared__ __align__(16) unsigned char rings[];
     constexpr bool LOGITS = KIND != GLM53F_KDA_PROBABILITIES;
     constexpr int kSize = KIND == GLM53F_KDA_LOGITS_BF16 ? 2 : 4;
@@ -501,7 +499,8 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const double rest = fma((double)fmaxf(y[j], 0.0f), -norm, w[j]);
-                    w[j] = rest > 0.0 ? rest : 0.0;
+                    const int hi = __double2hiint(rest), keep = ~(hi >> 31);  // (by the sign, beside the 64-bit pipe)
+                    w[j] = __hiloint2double(hi & keep, __double2loint(rest) & keep);
                 }
             } else if (mode == kWithout && (unsigned)(token - i) < 8u) {
 #pragma unroll
@@ -641,7 +640,7 @@ struct AcceptLaunch {
     AcceptLaunch(int batch, int blocks, cudaStream_t stream) {
         cfg.gridDim = dim3((unsigned)batch * blocks);
         cfg.blockDim = dim3(WARPS * 32);
-        cfg.dynamicSmemBytes = KIND == GLM53F_KDA_PROBABILITIES ? 0 : WARPS * kRingChunks<WARPS> * kPieces * kPiece;  // (probabilities have no statistics)
+        cfg.dynamicSmemBytes = KIND == GLM53F_KDA_PROBABILITIES ? 0 : WARPS * kDeep * kPieces * kPiece;  // (probabilities have no statistics)
         cfg.stream = stream;
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim.x = (unsigned)blocks;
