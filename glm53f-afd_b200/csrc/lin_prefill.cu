@@ -60,7 +60,7 @@ struct Decays {
 constexpr int oDecays = oY + kTile / 2;
 constexpr int oBars = oDecays + kStages * (int)sizeof(Decays);  // (a chunk's factors come and go with its rows)
 enum : int {
-    bFull = 0, bEmpty = bFull + kStages, bQK = bEmpty + kStages, bP, bReady, bState, bQS, bAdd = bQS + 2, bU = bAdd + 2, bO = bU + 2, bOFree = bO + 2, kBars = bOFree + 2
+    bFull = 0, bEmpty = bFull + kStages, bQK = bEmpty + kStages, bP, bReady, bState, bQS, bAdd = bQS + 2, bU = bAdd + 2, bO = bU + 2, bOFree = bO + 2, bClear = bOFree + 2, kBars
 };
 constexpr int oCtl = oBars + (kBars + 1) / 2 * 16;
 constexpr int kSmem = oCtl + 16 + 1024;
@@ -172,6 +172,7 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
         mbar_init(&bar[bReady], 5);  // q of a chunk (four warps), and the chunk before added to the state
         mbar_init(&bar[bState], 8);
         for (int i = 0; i < 2; ++i) mbar_init(&bar[bQS + i], 1), mbar_init(&bar[bAdd + i], STATE ? 8 : 16), mbar_init(&bar[bU + i], 1), mbar_init(&bar[bO + i], 1), mbar_init(&bar[bOFree + i], 4);
+        mbar_init(&bar[bClear], 8);  // once, by the warps that clear a short last chunk's foreign rows
         ctl[0] = 0u;
         ctl[1] = 0u;
         mbar_init_fence();
@@ -223,6 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
                 for (int at = vt * 16; at < kTile; at += 256 * 16)
                     if (((at >> 7) & (CH - 1)) >= live) *reinterpret_cast<uint4*>(k + at) = *reinterpret_cast<uint4*>(v + at) = make_uint4(0u, 0u, 0u, 0u);
                 fence_proxy_async_smem();
+                arrive(bClear);
             }
             tc::fence_after_sync();
 #pragma unroll 1
@@ -235,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
                     const int r = 32 * sh + 16 * i + 8 * (lane >> 4) + (lane & 7), piece = 4 * w + 2 * half + ((lane >> 3) & 1);
                     tc::ldmatrix_t4(v + (piece >> 3) * kBox + r * 128 + (((piece & 7) ^ (r & 7)) << 4), raw[4 * i], raw[4 * i + 1], raw[4 * i + 2], raw[4 * i + 3]);
                 }
-                if (live < CH) {  // (whether or not the warp that clears these rows has been there)
+                if (live < CH) {  // (whether or not the warp that clears these rows has been there; both products that read them wait: w V K for bAdd, V^T P^T for bClear)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int r = 32 * sh + 8 * i + 2 * (lane & 3);
@@ -330,6 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
         constexpr uint32_t id_qk = tc::idesc_bf16(64, 64, 0, 0, 0), id_pv = tc::idesc_bf16(128, 64, 1, 0, 0);
         const uint32_t leader = tc::elect_one();
         const int n_all = STATE ? 0 : (int)__reduce_max_sync(0xffffffffu, (unsigned)n);
+        const bool cut = __reduce_max_sync(0xffffffffu, (unsigned)(n * CH - rows)) != 0;  // the last chunk is a short one
         const uint32_t tm_all = __reduce_max_sync(0xffffffffu, tm), base = __reduce_max_sync(0xffffffffu, smem_u32(smem));
         uint32_t stage = 0, phase = 0, before = 0;  // of the scores; of the products with V, a chunk behind
         for (int c = 0; c <= n_all && n_all > 0; ++c) {
@@ -347,6 +350,8 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
             }
             if (c > 0) {
                 if (!wait(bQS + ((c - 1) & 1), (c - 1) / 2, kStatusLinS)) goto done;  // which began the accumulator
+                // P is 0 in the columns of foreign rows, but 0 times their NaN is not: they are cleared first.  (Nothing that arrives there waits for this product.)
+                if (c == n_all && cut && !wait(bClear, 0, kStatusLinWV)) goto done;
                 tc::fence_after_sync();
                 const uint32_t v = desc_lo(base + before * kStage + 2 * kTile, kBox), o = tm_all + cO + 64 * ((c - 1) & 1);
                 uint32_t pt = desc_lo(base + oP + ((c - 1) & 1) * 2 * kBox, 16);
