@@ -144,14 +144,14 @@ struct Eight {
 
 // A row's weights in 64 bits: e^x of x = (l - max) / t <= 0.  With z = 32 x / ln 2 = 32 e + j + f, |f| <= 1/2: e^x = 2^e 2^(j/32) e^(f ln 2 / 32), of which
 // Taylor's series to the fourth power leaves 1.3e-12: a draw among 131,072 moves by it once in ten million.  (With the general exponential, and every
-// special case looked at for every entry, a draw's pass took four times as many instructions.)  NaN and what is below e^-690 is 0.  Rows whose
+// special case looked at for every entry, a draw's pass took four times as many instructions.)  NaN and what is below e^-690 is 0, by z itself: where
+// f32 has few steps between max and max - 690 t, a logit at the rounded bound lies far below it, and the exponent's sum wraps there.  Rows whose
 // largest is infinite: see weights() in the kernel.  The pass waits for instructions, of which this is 20 an entry; the table lies in sixteen copies, two banks each.
 constexpr double kTurns = 46.166241308446828384;  // 32 / ln 2
 struct RowScale {
     double max, turns;  // turns: 32 / (t ln 2)
-    float lowest;       // max - 690 t: what counts as 0 lies below
 };
-__device__ __forceinline__ RowScale row_scale_of(float max, float t) { return {(double)max, kTurns / (double)t, fmaf(-690.0f, t, max)}; }
+__device__ __forceinline__ RowScale row_scale_of(float max, float t) { return {(double)max, kTurns / (double)t}; }
 __device__ __forceinline__ double logit_weight(float l, const RowScale& a, const double* power) {  // power: the lane's copy
     constexpr double c = 1.0 / kTurns;
     const double magic = 6755399441055744.0;  // 1.5 2^52: adding it rounds to an integer, which the low word then holds
@@ -164,7 +164,7 @@ __device__ __forceinline__ double logit_weight(float l, const RowScale& a, const
     y = fma(f, y, 1.0);
     const double base = power[(n & 31) * kCopies];
     y *= __hiloint2double(((n & ~31) << 15) + __double2hiint(base), __double2loint(base));
-    return l >= a.lowest ? y : 0.0;
+    return z >= -690.0 * kTurns ? y : 0.0;
 }
 __device__ __forceinline__ float finite_weight(float p) { return p > 0.0f && p < INFINITY ? p : 0.0f; }
 
