@@ -20,6 +20,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "device_counts.h"
 #include "kda_internal.h"
 
 namespace kda {
@@ -632,7 +633,7 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
     }
 }
 
-// The launch of a configuration, and how many of its clusters the device holds at a time (asked for once; 0 where it cannot be told).
+// The launch of a configuration, and how many of its clusters the device holds at a time (asked of each device once; 0 where it cannot be told).
 template <int KIND, int WARPS>
 struct AcceptLaunch {
     cudaLaunchConfig_t cfg{};
@@ -660,13 +661,15 @@ struct AcceptLaunch {
         return e;
     }
     int fit() {
-        static int counted[2] = {-1, -1};
-        int& n = counted[attr[0].val.clusterDim.x == kAccMostBlocks];
-        if (n < 0) {
-            n = 0;
-            if (configure() != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, accept_kernel<KIND, WARPS>, &cfg) != cudaSuccess) cudaGetLastError(), n = 0;
-        }
-        return n;
+        static DeviceCounts<2> counted;
+        int dev = -1;
+        cudaGetDevice(&dev);
+        return counted.get(dev, attr[0].val.clusterDim.x == kAccMostBlocks, [&] {
+            int n = 0;
+            if (configure() == cudaSuccess && cudaOccupancyMaxActiveClusters(&n, accept_kernel<KIND, WARPS>, &cfg) == cudaSuccess) return n;
+            cudaGetLastError();
+            return -1;
+        });
     }
     int run(AcceptParams p) {
         const cudaError_t e = configure();
