@@ -239,7 +239,7 @@ bool lin_args_ok(int32_t heads, int32_t qk_heads, int32_t batch, const void* cu,
         return x != nullptr && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && stride % 8 == 0 && stride >= (int64_t)n * DK;
     };
     if (heads < 1 || heads > 65535 || qk_heads < 1 || heads % qk_heads || batch < 0) return false;
-    if ((int64_t)heads * batch > 0x3fffffff) return false;
+    if ((int64_t)heads * batch > 0x7fffffff / kLinSplit) return false;  // blocks of a launch
     if (batch == 0) return true;
     if (cu == nullptr || state_in == nullptr || state_off == nullptr || g == nullptr) return false;
     if (g_stride != 0 && g_stride < heads) return false;

@@ -456,6 +456,7 @@ int glm53f_kda_debug_wait_test(uint64_t wait_limit_ns, int32_t skip_first_state)
  * Common arguments:
  *   heads, qk_heads   heads of v, g, the states and out (1..65535); heads of q and k, which divide them: heads
  *                     [i * heads / qk_heads, (i + 1) * heads / qk_heads) read head i of q and k
+ *   batch             requests; heads * batch at most 0x1fffffff
  *   cu_rows           device int32 [batch + 1]: request b owns rows [cu_rows[b], cu_rows[b + 1]); requests may have none
  *   q, k, v           bf16, row r at + r * stride (elements): [qk_heads][128] of q and k, [heads][128] of v; 16-byte
  *                     aligned, strides multiples of 8 and at least the row (parts of a fused projection's rows will do)
