@@ -156,7 +156,8 @@ class KdaVerify:
     # ---- accept -----------------------------------------------------------------------------------------------
     def accept(self, tokens, target, u, keep, next, *, probabilities=False, draft=None, temperature=None, stream: Optional[K.Stream] = None) -> None:
         """How many rows of each window of the open round to keep, and the token behind them: `spec.accept_batch` over the round's
-        windows, in its order.  Writes int32 keep[i] and next[i] on the device; `commit(slots, keep[:n].tolist())` follows."""
+        windows, in its order.  Writes int32 keep[i] and next[i] on the device; `commit(slots, keep[:n].tolist())` follows.  On another stream
+        than torch's current one it comes after what is queued there, and what is queued there afterwards comes after it."""
         if self.pending is None:
             raise Invalid("no verify is open")
         rows, n = self.meta.total_rows(), self.meta.batch()
@@ -165,8 +166,27 @@ class KdaVerify:
         stream = stream or self.pool.stream
         self._order(stream)
         cu_rows = self.meta.cu_rows.t[:(n + 1) * 4].view(K._torch().int32)
-        with contextlib.nullcontext() if stream.stream is None else K._torch().cuda.stream(stream.stream):
+        with self._beside_current(stream):
             spec.accept_batch(cu_rows, tokens, target, u, keep, next, probabilities=probabilities, draft=draft, temperature=temperature)
+
+    @contextlib.contextmanager
+    def _beside_current(self, stream: K.Stream):
+        """`stream` as torch's current one: what is launched on it comes after what is queued on the current stream so far, where a call's inputs
+        were made, and before what is queued there next, where its answers are read."""
+        cuda = K._torch().cuda
+        current = None if stream.stream is None else cuda.current_stream()
+        if current is None or stream.stream.cuda_stream == current.cuda_stream:
+            yield
+            return
+        own, ordered = cuda.ExternalStream(stream.stream.cuda_stream), cuda.is_current_stream_capturing()
+        with cuda.stream(own):
+            # (A capture of `stream` alone cannot wait for the current stream; its order is the captured one.)
+            ordered = ordered or not cuda.is_current_stream_capturing()
+            if ordered:
+                own.wait_stream(current)
+            yield
+        if ordered:
+            current.wait_stream(own)
 
     # ---- commit -----------------------------------------------------------------------------------------------
     def commit(self, slots: Sequence[marks.GlmKv], keep: Sequence[int], stream: Optional[K.Stream] = None) -> None:
