@@ -59,7 +59,7 @@ int32_t glm53f_kda_proj_bf16_many(const glm53f_proj_job* jobs, int32_t count, gl
  * sum and rounded once; not in the reference.
  *   bias        [groups][n], bf16 or (bias_f32 != 0) f32, group g at + g * bias_gstride (read only when groups > 1); NULL: none
  *   activation  one of GLM53F_PROJ_*: relu max(y, 0), silu y / (1 + e^-y), gelu y (1 + erf(y / sqrt 2)) / 2, gelu_tanh the
- *               same by tanh(sqrt(2 / pi) (y + 0.044715 y^3)), sigmoid 1 / (1 + e^-y)
+ *               same by tanh(sqrt(2 / pi) (y + 0.044715 y^3)), sigmoid 1 / (1 + e^-y) (0 where that is below 2^-126)
  *   residual    of out's type, row m of group g at + g * r_gstride + m * ldr (ldr >= n); NULL: none.  It may be `out` itself
  *               (same address and strides), and otherwise has no element in common with it
  * The job's fields, checks, row independence and status codes are glm53f_kda_proj_bf16's; bias and residual are aligned to
