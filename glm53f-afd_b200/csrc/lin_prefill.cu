@@ -10,8 +10,10 @@
 //
 // Precision.  Sums and the state are f32 in tensor memory.  What has to become an operand and is not bf16 already keeps more bits than that: w V
 // goes as a sum of three bf16 parts where the state is f32 (24 bits, all that f32 has) and of two where it is stored as bf16, P as a sum of two (16 bits), S and
-// scale e^G Q as f32 operands of which the tensor core takes 11 bits: beside the outputs' rounding to bf16 little is left of their errors (as single bf16
-// operands P and S would add as much again).  Differences of G are of sums in 64 bits, held as two f32: a row that forgets everything (-inf, taken as
+// scale e^G Q as f32 operands of which the tensor core takes 11 bits.  It cuts the rest off, always towards zero; the mean of both cuts is put back by q's factor (q_factor).  Outputs are then
+// 1.67 to 1.69e-3 off 64 bits where their rounding to bf16 alone makes 1.66e-3, and 1e-5 too small on the mean (cut and left so 1.69 to 1.82e-3 and 1.6 to
+// 6.6e-4; every value of q rounded to 11 bits instead the same, 64 heads x 8,192 rows 5 us longer; as single bf16 operands P and S would add as much as
+// the rounding again).  Differences of G are of sums in 64 bits, held as two f32: a row that forgets everything (-inf, taken as
 // -104, which is 0 in f32) must not blur those behind it.
 //
 // Roles of a block, one (sequence, head, segment) each, all meeting at mbarriers:
@@ -145,6 +147,16 @@ __device__ __forceinline__ long long first_slot(const PrefillParams& p, int h, i
 __device__ __forceinline__ float2 sub2(float2 a, float2 b) { return fma2(b, make_float2(-1.0f, -1.0f), a); }
 __device__ __forceinline__ float2 lo_of(uint32_t hi, float2 x) {  // what a pair's hi parts leave
     return sub2(x, make_float2(__uint_as_float(hi << 16), __uint_as_float(hi & 0xffff0000u)));
+}
+
+// What the tensor core cuts off of an f32 operand's entries on the mean, of 11 bits taken: 2^-11 of an entry's power of two, so 2^-11 / (2 ln 2) of the entry where all mantissas are
+// as likely on a logarithmic scale.
+constexpr float kCutOff = 3.52e-4f;
+// The factor of a row of q, scale e^G, with what makes up for the two cuts: of the state, unless it still is what came in as bf16 (`exact`), and of the products of factor and q, unless the
+// factor has no more than the three bits that leave those in 11.
+__device__ __forceinline__ float q_factor(float e, bool exact) {
+    if (exact) return (__float_as_uint(e) & 0x1fffffu) == 0u ? e : e * (1.0f + kCutOff);
+    return e * (1.0f + 2.0f * kCutOff);
 }
 
 // Shared-memory descriptors in the 128-byte swizzle (8-row groups 1,024 bytes apart): the low word from an address and the leading byte offset, which the
@@ -396,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) lin_prefill_kernel(const __grid_c
                 const int r = 2 * lane + j;
                 const float hi = (float)sum[j];
                 x.g[r] = make_float2(hi, (float)(sum[j] - (double)hi));
-                x.e[r] = p.scale * exp2f(hi);
+                x.e[r] = q_factor(p.scale * exp2f(hi), p.state_bf16 && c0 + c == 0);
                 x.w[r] = exp2f((float)(STATE ? total + (all - sum[j]) : all - sum[j]));
             }
             if (lane == 0) x.all = exp2f((float)all);
