@@ -37,7 +37,8 @@ __device__ __forceinline__ float proj_times_sigmoid(float y, float z) {
 // gelu(y) = max(y, 0) - |y| erfc(z) / 2, z = |y| / sqrt 2, in 18 instructions where the library's erfc takes more than twice as many (two groups of 2,048 rows x 8,192
 // results of k = 128: 71 us, 126 with it, 42 without an activation; in two-wide operations the constants take registers that then spill).  erfc(z) / 2 = t 2^(2 e),
 // t = 1 / (1 + z / 2), 2 e = P(t) - z^2 log2 e - 1: P is a polynomial of degree nine that was fitted to log2(erfc(z) e^(z^2) / t) over 0 < t <= 1 so that its largest
-// error is least (a relative 1e-7 of erfc).  Half the exponent twice, so that results down to the smallest subnormal stay; |y| is cut off where there is no
+// error is least (the form of the complementary error function in Press et al., Numerical Recipes, section 6.2; 1.6e-7 of erfc).  In f32 the exponent's rounding adds to that: 5e-7 of erfc
+// down to y = -2, 1.5e-6 to -5, 8e-6 to -13, where the result ends.  Half the exponent twice, so that results down to the smallest subnormal stay; |y| is cut off where there is no
 // result left, so that infinities do not meet zeros.
 __device__ __forceinline__ float proj_gelu(float y) {
     const float a = fminf(fabsf(y), 64.0f), t = rcp_approx(fmaf(a, 0.35355339f, 1.0f));

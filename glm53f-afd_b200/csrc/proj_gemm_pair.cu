@@ -137,7 +137,6 @@ __device__ __forceinline__ PairTile pair_tile(const PairParams& p, long long t) 
     return {q, i - u * q.r_tiles, u % q.n_tiles, u / q.n_tiles};
 }
 
-// SPLIT_ROWS: rows per tile at most where k runs in segments.  
 // A lane's feature of a chunk's rows, one after the other: a whole chunk's as straight stores or loads (with the extents looked at for every row and the address
 // multiplied out, 26 instructions a value were the time: two groups of 333 rows x 8,192 f32 results 33 us, so 16).  Of a residual's rows
 // past the last the last is read again.
@@ -162,6 +161,7 @@ __device__ __forceinline__ void get_rows(const T* from, long long stride, int li
     }
 }
 
+// SPLIT_ROWS: rows per tile at most where k runs in segments.
 template <int SPLIT_ROWS, int EPI>
 __global__ void __launch_bounds__(kPairThreads, 1) proj_gemm_pair_kernel(const __grid_constant__ PairParams p) {
     using L = PairSmem<EPI>;
@@ -294,7 +294,6 @@ __global__ void __launch_bounds__(kPairThreads, 1) proj_gemm_pair_kernel(const _
 #pragma unroll
             for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
         };
-        // The tile's rows c0 .. c0 + 31 (those below row_tile) out, as load() gave them.
         // EPI.  v[j]'s place in the chunk of 32 rows x 32 features, by load()'s layout: feature place 2 ((j / 8) % 2) + (j / 2) % 2 of four, 8 apart, in
         // fragments.
         auto in_fragments = [&](const PairTile& x) { return kFragments && tensor_out(x); };
@@ -364,6 +363,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) proj_gemm_pair_kernel(const _
             else proj_finish(e.act, v, [&](int j) { return b[2 * ((j >> 3) & 1) + ((j >> 1) & 1)]; }, nullptr);
         };
         bool gone = false;  // a residual's copy did not come
+        // The tile's rows c0 .. c0 + 31 (those below row_tile) out, as load() gave them.
         auto emit = [&](const PairTile& x, int c0, float (&v)[kChunk]) {
             const long long row0 = (long long)x.rt * x.q.row_tile + c0;
             const int f0 = x.nt * 2 * kPM + (int)rank * kPM + side * 64;

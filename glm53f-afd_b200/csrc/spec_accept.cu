@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
     const unsigned char* rows = static_cast<const unsigned char*>(p.target) + (long long)first * p.ld * kSize;
     auto row_at = [&](int i) { return static_cast<const void*>(rows + (long long)i * p.ld * kSize); };
     auto draft_at = [&](int i) { return p.draft + (long long)(first + i) * p.draft_ld; };
-    // (Capped: an infinite one would make 0 times infinity of a logit of -inf.)
+    // (Capped, a NaN too: an infinite one would make 0 times infinity of a logit of -inf.)
     const float temperature = LOGITS && p.temperature != nullptr ? (p.temperature[b] < 1e30f ? p.temperature[b] : 1e30f) : 1.0f;
     const bool greedy = LOGITS && !(temperature > 0.0f);
     const float scale = greedy ? 0.0f : kLog2e / temperature;
@@ -407,7 +407,6 @@ __global__ void __launch_bounds__(kAccWarps * 32, kAccWarps == 8 ? 3 : 1) accept
                 }
                 __syncthreads();
                 // A warp to a row: over the block's warps, then over the cluster's blocks.
-                __syncthreads();
                 if (warp < rows_here) {
                     Stats a;
                     if (lane <= kAccWarps) a.m = sh.wmax[warp][lane], a.s = sh.wsum[warp][lane], a.best = sh.wbest[warp][lane];

@@ -508,12 +508,14 @@ int glm53f_kda_lin_prefill_varlen(int32_t heads, int32_t qk_heads, int32_t batch
  *   tokens        int32, one a row (a window's first is not read); one outside [0, vocab) is never kept
  *   draft         f32 [rows][draft_ld]: row i the distribution that tokens[i] was drawn from (a window's first is not read);
  *                 NULL: the drafter had one choice, q(tokens[i]) = 1
- *   temperature   f32 [batch], logits only (NULL: 1 for all); 0 or less: greedy, the largest logit, the lowest index among equals
+ *   temperature   f32 [batch], logits only (NULL: 1 for all); 0 or less: greedy, the largest logit, the lowest index among equals;
+ *                 NaN and above 1e30: 1e30
  *   u             f32 [rows], uniform in [0, 1): u[i] judges tokens[i], a window's first draws the next token
  * A token is kept while u q < p and all before it are (greedy: while it is the largest).  keep[b] = 1 + the tokens kept; next[b]
  * is drawn from p behind a whole window, else from max(p - q, 0) of the first refused token's row -- without `draft`, from p
  * without that token; from p where this leaves nothing: the lowest index whose running sum, divided by the whole, exceeds
- * u.  Draws are made in 64 bits.  A row that leaves nothing gives next[b] = -1, a request without rows keep 0 and next -1.
+ * u.  Draws are made in 64 bits; the sums that judge a token are 32-bit ones, 1e-7 of p.  The same call gives the same answers; the number of requests decides how a row is
+ * divided, so that beside other requests a token within that of its bound may be judged, and a draw that near to a border made, the other way.  A row that leaves nothing gives next[b] = -1, a request without rows keep 0 and next -1.
  * One launch; nothing is allocated.  1 <= vocab <= 0x7fffffc0, ld and draft_ld >= vocab. */
 #define GLM53F_KDA_PROBABILITIES 0
 #define GLM53F_KDA_LOGITS_F32 1
