@@ -8,7 +8,8 @@
 // so a chunk is four products: Q K^T, S Q^T, V^T P^T and (w V)^T K, all on operands as the tensor copies bring them (128-byte
 // swizzle, K- or MN-major).  Bound by HBM where every SM has a chain, a sequence's head (1 KiB a row and head); a chain's own pace is the tensor pipe's.
 //
-// Precision.  Sums and the state are f32 in tensor memory.  What has to become an operand and is not bf16 already keeps more bits than that: w V
+// Precision.  Sums and the state are f32 in tensor memory, where the tensor core cuts each addition off: end states are 2e-7 to 1e-6 off, mostly too small, and 9e-6 after 4,000
+// rows of hardly any decay.  What has to become an operand and is not bf16 already keeps more bits than that: w V
 // goes as a sum of three bf16 parts where the state is f32 (24 bits, all that f32 has) and of two where it is stored as bf16, P as a sum of two (16 bits), S and
 // scale e^G Q as f32 operands of which the tensor core takes 11 bits.  It cuts the rest off, always towards zero; the mean of both cuts is put back by q's factor (q_factor).  Outputs are then
 // 1.67 to 1.69e-3 off 64 bits where their rounding to bf16 alone makes 1.66e-3, and 1e-5 too small on the mean (cut and left so 1.69 to 1.82e-3 and 1.6 to
@@ -26,8 +27,9 @@
 //   warp 29      the products with the state and to it            warp 30  the scores and their products with V
 // A chunk's products take 1,920 cycles of the tensor pipe and, where every SM works, its rows 2,900 of a share of HBM; it takes 3,300 to 4,000.  What bounds it is what
 // the other roles issue (2,200 instructions a scheduler) and the round of the state: its product with Q, its scaling, the sum of w V K, each of which waits
-// for the one before.  So bodies are loops, waits sleep, and operands take the form that costs the fewest instructions.  148 heads x 4,096 rows take 150 us
-// (69 of HBM's time), 64 heads x 8,192 rows in two segments 190 us (84), 8 heads x 65,536 in eighteen 206 us (82).  What was measured and is not here: w V^T through shared
+// for the one before.  So bodies are loops, waits sleep, and operands take the form that costs the fewest instructions.  148 heads x 4,096 rows take 145 us
+// (69 of HBM's time), 64 heads x 8,192 rows in two segments 191 us (84), 8 heads x 65,536 in eighteen 202 us (82), by themselves over an evicted L2; call after call, inputs changing,
+// the last two 210 and 227.  What was measured and is not here: w V^T through shared
 // memory, the state's scaling in registers, registers moved between the roles, polling waits, a second buffer of q, half of q ahead, tiles brought to L2 before.
 //
 // Few chains: a sequence is cut into segments that are walked at the same time, each from the state that the segments before it
