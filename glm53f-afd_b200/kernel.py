@@ -128,6 +128,16 @@ def raw_stream(stream: Stream) -> int:
     return (stream.raw().value or 0) if raw is None else raw
 
 
+def torch_stream(stream: Stream):
+    """The stream as torch has it.  (Of an address of 0, the legacy default stream, `ExternalStream` would make a new one.)"""
+    cuda, s = _torch().cuda, stream.stream
+    if s is None:
+        return cuda.current_stream()
+    if isinstance(s, cuda.Stream):
+        return s
+    return cuda.ExternalStream(s.cuda_stream) if s.cuda_stream else cuda.default_stream()
+
+
 def _launched(code: int, what: str) -> None:
     if code == 0:
         return

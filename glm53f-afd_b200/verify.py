@@ -178,7 +178,7 @@ class KdaVerify:
         if current is None or stream.stream.cuda_stream == current.cuda_stream:
             yield
             return
-        own, ordered = cuda.ExternalStream(stream.stream.cuda_stream), cuda.is_current_stream_capturing()
+        own, ordered = K.torch_stream(stream), cuda.is_current_stream_capturing()
         with cuda.stream(own):
             # (A capture of `stream` alone cannot wait for the current stream; its order is the captured one.)
             ordered = ordered or not cuda.is_current_stream_capturing()
