@@ -219,7 +219,7 @@ class KvPool:
             cuda = kernel._torch().cuda
             current, own = cuda.current_stream(), self.stream.stream.cuda_stream
             if own != current.cuda_stream:
-                cuda.ExternalStream(own).wait_stream(current)
+                kernel.torch_stream(self.stream).wait_stream(current)
 
     # ---- several slots in one launch (an addition: the reference marks slot by slot) -------------------------------
     def _copy_marks(self, kvs, marks_, save: bool) -> None:
