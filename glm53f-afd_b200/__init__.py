@@ -4,7 +4,8 @@
 `kernel`  checked wrappers mirroring the reference crate's host API (crates/glm53f-kda/src/kernel.rs);
 `core`    wrappers of the post-conv ("core") entry points; `marks` state snapshot / restore over pool pages;
 `proj`    the projections' GEMM, with an epilogue if asked; `verify` the verify / accept / commit round over pool slots;
-`linear`  linear attention with one decay a head; `spec` verification of drafted tokens;
+`linear`  linear attention with one decay a head; `gated` gated linear recurrence channel by channel, with its backward pass;
+`spec`    verification of drafted tokens;
 `synth`   seeded synthetic inputs of the benchmark configurations;
 `build()` compiles csrc/ into libglm53f_kda.so (nvcc, sm_100a).
 """

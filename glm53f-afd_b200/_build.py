@@ -25,6 +25,7 @@ SOURCES = {
     "proj_gemm_pair.cu": [], # the same on SM pairs (cta_group::2) for many rows
     "lin_decode.cu": [],     # linear attention with one decay a head: row by row
     "lin_prefill.cu": [],    # ... and chunked
+    "gated_scan.cu": [],     # gated linear recurrence, channel by channel: scan, backward pass, row by row
     "spec_accept.cu": [],    # verification of drafted tokens
     "kda_gather.cu": [],     # host code only: CUDA IPC handles for the full output buffers of a head-sharded prefill
     "fwd_rows.cu": [],       # row gather / scatter and the mark copy: data movement only

@@ -524,6 +524,57 @@ int glm53f_kda_accept_batch(int32_t batch, const int32_t* cu_rows, int32_t vocab
                             const int32_t* tokens, const float* draft, int64_t draft_ld, const float* temperature, const float* u,
                             int32_t* keep, int32_t* next, glm53f_stream_t stream);
 
+/* ===================================================================================================
+ * Part 5: gated linear recurrence, channel by channel
+ *
+ * The vector-state companion of Part 3; not in the reference.  Per row t and channel:
+ *     h_t = a_t h_{t-1} + c_t x_t        out_t = h_t
+ * with a_t = exp(g_t), or with GLM53F_KDA_SCAN_SIGMOID the sigmoid of g_t (a gate as its projection leaves it), and c_t = 1, or with
+ * GLM53F_KDA_SCAN_COMPLEMENT 1 - a_t.
+ *
+ * Common arguments:
+ *   channels, batch   channels of a row (1 or more); requests
+ *   cu_rows           as in Part 3: ascending, row ranges of the requests, some of which may have no rows
+ *   g, x, out         row r at + r * stride (elements), [channels]; g f32, or bf16 with GLM53F_KDA_SCAN_G_BF16; x and out (and their gradients)
+ *                     f32, or bf16 with GLM53F_KDA_SCAN_X_BF16; aligned to their elements, strides at least the channels.  Log decays are at most 0, -inf
+ *                     forgets everything before the row (above 0: while the product of 128 rows' a stays within f32)
+ *   state_in / state_out, state_off   f32; a request's state [channels] begins state_off[b] elements in.  In place, or memory without
+ *                     a byte in common.  Requests that write need regions of their own
+ * What is written has no byte in common with what is read, unless it says so; rows that belong to no request are left as they are.  States and sums are f32;
+ * out and the gradients are rounded once.
+ * =================================================================================================== */
+#define GLM53F_KDA_SCAN_SIGMOID 1
+#define GLM53F_KDA_SCAN_COMPLEMENT 2
+#define GLM53F_KDA_SCAN_G_BF16 4
+#define GLM53F_KDA_SCAN_X_BF16 8
+
+/* Row by row: single tokens and windows of drafted ones, with keep, state_out and out as in glm53f_kda_lin_decode_batch.  A verify and a commit of k rows leave
+ * the bits of k single-row calls. */
+int glm53f_kda_scan_decode_batch(int32_t channels, int32_t batch, const int32_t* cu_rows, const int32_t* keep, const void* g, int64_t g_stride,
+                                 const void* x, int64_t x_stride, int32_t flags, const float* state_in, float* state_out,
+                                 const int64_t* state_off, void* out, int64_t out_stride, glm53f_stream_t stream);
+
+/* Packed sequences, the longest of at most max_len (host) rows; rows (host) >= cu_rows[batch].  A request without rows passes its state through.  out may be NULL (states only).
+ * `saves` (8-byte aligned; NULL: none) takes the states that the backward pass starts from, glm53f_kda_scan_saves_rows(batch, rows) x channels f32 values.
+ * `workspace` (16-byte aligned) of glm53f_kda_scan_workspace_bytes(channels, batch, rows) bytes lets sequences of more than 128 rows run in parts at once; with fewer (0 and
+ * NULL among them) one block walks each 64 channels of a sequence.  It is the call's own until the call has run.  A sequence's results are the same bits with
+ * any workspace and beside any other requests; they agree with the row-by-row form's to the rounding of f32. */
+int64_t glm53f_kda_scan_workspace_bytes(int32_t channels, int32_t batch, int32_t rows);
+int64_t glm53f_kda_scan_saves_rows(int32_t batch, int32_t rows);
+int glm53f_kda_scan_prefill_varlen(int32_t channels, int32_t batch, const int32_t* cu_rows, int32_t rows, int32_t max_len, const void* g,
+                                   int64_t g_stride, const void* x, int64_t x_stride, int32_t flags, const float* state_in, float* state_out,
+                                   const int64_t* state_off, void* out, int64_t out_stride, float* saves, void* workspace,
+                                   int64_t workspace_bytes, glm53f_stream_t stream);
+
+/* The gradients of a prefill call with `saves` over the same cu_rows, rows, g, x and flags: dg (g's type) and dx (x's) from dout (x's) and, where dstate is not
+ * NULL, from the gradient of the end states; dstate_in (NULL: not wanted) takes the start states' gradient.  dstate and dstate_in lie at state_off and may be the same
+ * memory.  The workspace is as above. */
+int glm53f_kda_scan_backward_varlen(int32_t channels, int32_t batch, const int32_t* cu_rows, int32_t rows, int32_t max_len, const void* g,
+                                    int64_t g_stride, const void* x, int64_t x_stride, int32_t flags, const float* saves, const void* dout,
+                                    int64_t dout_stride, const float* dstate, float* dstate_in, const int64_t* state_off, void* dg,
+                                    int64_t dg_stride, void* dx, int64_t dx_stride, void* workspace, int64_t workspace_bytes,
+                                    glm53f_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
