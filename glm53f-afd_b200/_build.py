@@ -27,6 +27,7 @@ SOURCES = {
     "lin_prefill.cu": [],    # ... and chunked
     "gated_scan.cu": [],     # gated linear recurrence, channel by channel: scan, backward pass, row by row
     "spec_accept.cu": [],    # verification of drafted tokens
+    "logprobs.cu": [],       # log probabilities, entropy, alternatives; their gradients
     "kda_gather.cu": [],     # host code only: CUDA IPC handles for the full output buffers of a head-sharded prefill
     "fwd_rows.cu": [],       # row gather / scatter and the mark copy: data movement only
 }

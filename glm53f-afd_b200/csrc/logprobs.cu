@@ -1,0 +1,505 @@
+// Log probabilities of given tokens from rows of logits, with entropy and the best alternatives, and the logits' gradient.
+//
+// With t_j = (x_j - max x) / T and S = sum of e^t_j: log p_j = t_j - log S, entropy = log S - (sum of e^t_j t_j) / S.  Backwards, from the gradients
+// l of the token's log probability and n of the entropy H: dx_j = (l ([j = token] - p_j) - n p_j (log p_j + H)) / T.
+//
+// Bound by HBM: a row is read once (one exponential, 2/3 of what the units give at bf16 logits, and some ten other operations a value).  Every warp keeps
+// its running maximum, its lanes their sums against it, so that the maxima need no pass of their own; blocks of a cluster that share a row meet
+// in distributed shared memory.  No scratch in global memory; the same bits every time.
+//
+// The alternatives need no second pass either.  Each thread knows the largest value it met; 128 groups of threads are 128 disjoint parts of the row, so the
+// k-th largest of the groups' maxima is no larger than the row's k-th largest value.  Of the row's pieces of 32 x 16 bytes, whose
+// maxima lie in shared memory, those that reach this bound (few more than k) are read again from L2, and the few values in them that reach it are
+// ranked by counting.  Equal logits rank by index.  Rows of so many equal values that these do not fit take k rounds over the row instead.
+
+#include <initializer_list>
+#include <type_traits>
+
+#include "common.cuh"
+#include "kda_internal.h"
+
+namespace kda {
+namespace {
+
+constexpr int kWarps = 16, kThreads = 32 * kWarps;
+constexpr int kGroups = 128;
+constexpr int kMostTop = 32;
+constexpr int kPieces = 2048;     // of a block's part of a row
+constexpr int kCandidates = 512;  // of a block's part; kMostBlocks * kMostTop at least
+constexpr int kMostBlocks = 8;    // of a row
+constexpr int kAtOnce = 4;        // pieces of a warp in flight
+constexpr int kMostVocab = 2000000;  // (kMostBlocks * kPieces pieces hold 2,097,152 f32 logits)
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct LogprobParams {
+    const void* logits;
+    long long ld;
+    int vocab, blocks, top;
+    const int32_t* tokens;
+    const float* temperature;
+    float *logprob, *entropy, *lse;
+    int32_t* top_ids;
+    float* top_values;
+    // backward
+    const float *dlogprob, *dentropy;
+    void* dlogits;
+    long long dld;
+};
+
+struct Entry {
+    float v;
+    int id;
+};
+__device__ __forceinline__ bool before(const Entry& a, const Entry& b) { return a.v > b.v || (a.v == b.v && a.id < b.id); }
+
+struct Shared {
+    float piece[kPieces];
+    Entry candidate[kCandidates];
+    float group[kThreads];
+    Entry best[kMostTop];  // this block's, read by the row's first block
+    float max, sum, sum_t;
+    float wmax[kWarps], wsum[kWarps], wsum_t[kWarps];
+    Entry wbest[kWarps];
+    float bound;
+    int candidates;
+};
+
+__device__ __forceinline__ float warp_max(float x) {  // NaN only where all are
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    return x;
+}
+__device__ __forceinline__ uint32_t cluster_place(const void* local, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(local)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float cluster_load(uint32_t at) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// log2(e) / T.  A temperature of 0 or less (a row whose choice is greedy) and NaN: 1.
+__device__ __forceinline__ float heat_of(const float* temperature, long long row) {
+    const float t = temperature == nullptr ? 1.0f : __ldg(temperature + row);
+    return t > 0.0f ? fminf(fmaxf(t, 1e-30f), 1e30f) : 1.0f;
+}
+
+// A row, counted from the 16-byte boundary at or below its start: values [skip, end) are the row's.
+template <bool BF16>
+struct Row {
+    static constexpr int E = BF16 ? 8 : 4;
+    const unsigned char* base;
+    int skip;
+    long long end;
+    __device__ __forceinline__ Row(const void* logits, long long at, int vocab) {
+        const uintptr_t a = reinterpret_cast<uintptr_t>(logits) + at * (BF16 ? 2 : 4);
+        base = reinterpret_cast<const unsigned char*>(a & ~(uintptr_t)15);
+        skip = (int)((a & 15) / (BF16 ? 2 : 4));
+        end = (long long)skip + vocab;
+    }
+    // The 16 bytes of values [E i, E i + E); what is not the row's -inf.
+    __device__ __forceinline__ uint4 load(long long i) const {
+        const long long at = i * E;
+        if (at >= skip && at + E <= end) return *reinterpret_cast<const uint4*>(base + i * 16);
+        uint4 r;
+        uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = BF16 ? 0xff80ff80u : 0xff800000u;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            if (at + j < skip || at + j >= end) continue;
+            if constexpr (BF16) {
+                const uint32_t v = reinterpret_cast<const uint16_t*>(base)[at + j];
+                w[j / 2] = j % 2 ? (w[j / 2] & 0xffffu) | v << 16 : (w[j / 2] & 0xffff0000u) | v;
+            } else {
+                w[j] = reinterpret_cast<const uint32_t*>(base)[at + j];
+            }
+        }
+        return r;
+    }
+};
+template <bool BF16>
+__device__ __forceinline__ float value(const uint4& r, int j) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
+    if constexpr (BF16) return __uint_as_float(j % 2 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+    else return __uint_as_float(w[j]);
+}
+template <bool BF16>
+__device__ __forceinline__ float largest(const uint4& r) {  // (of numbers; NaN where there is none)
+    if constexpr (BF16) {
+        const __nv_bfloat162* w = reinterpret_cast<const __nv_bfloat162*>(&r);
+        const __nv_bfloat162 m = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
+        return fmaxf(__low2float(m), __high2float(m));
+    } else {
+        const float* w = reinterpret_cast<const float*>(&r);
+        return fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
+    }
+}
+
+// Sums of e^t and e^t t against the maximum m, in powers of two.
+struct Sums {
+    float m = -INFINITY, s = 0.0f, w = 0.0f;
+    __device__ __forceinline__ void raise(float to, float c) {  // to > m
+        const float d = (m - to) * c;
+        if (m == -INFINITY) {
+            m = to;
+            return;
+        }
+        const float f = ex2_ftz(d), dd = fmaxf(d, -1000.0f);
+        w = f * fmaf(s, dd, w), s *= f;
+        m = to;
+    }
+    template <bool BF16>
+    __device__ __forceinline__ void add(const uint4& r, float c) {
+        const float from = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int j = 0; j < Row<BF16>::E; ++j) {
+            // (-inf: e^t is 0, and stays 0 times t; a NaN stays one)
+            const float t = max_nan((value<BF16>(r, j) - from) * c, -1000.0f), e = ex2_ftz(t);
+            s += e, w = fmaf(e, t, w);
+        }
+    }
+    __device__ __forceinline__ void join(float om, float os, float ow, float c) {
+        if (om > m) {
+            const float keep_s = s, keep_w = w, keep_m = m;
+            m = om, s = os, w = ow;
+            om = keep_m, os = keep_s, ow = keep_w;
+        }
+        if (om == -INFINITY) {  // (a part of NaN and masked values has a sum without a maximum)
+            s += os, w += ow;
+            return;
+        }
+        const float d = (om - m) * c, f = ex2_ftz(d), dd = fmaxf(d, -1000.0f);
+        s = fmaf(os, f, s), w = fmaf(f, fmaf(os, dd, ow), w);
+    }
+};
+
+// Among n entries, those that fewer than k come before, to their places.
+__device__ __forceinline__ void rank(const Entry* all, int n, int k, Entry* best) {
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const Entry mine = all[i];
+        int ahead = 0;
+        for (int j = 0; j < n; ++j) ahead += before(all[j], mine);
+        if (ahead < k) best[ahead] = mine;
+    }
+}
+
+template <bool BF16>
+__global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobParams p) {
+    constexpr int E = Row<BF16>::E;
+    __shared__ Shared sh;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int part = blockIdx.x % p.blocks;
+    const long long row = blockIdx.x / p.blocks;
+    grid_ready();
+    const Row<BF16> x(p.logits, row * p.ld, p.vocab);
+    const float heat = heat_of(p.temperature, row), c = kLog2e / heat;
+    // The row's pieces (32 lanes of 16 bytes), in as many runs as blocks share it.
+    const int pieces = (int)((x.end + 32 * E - 1) / (32 * E));
+    const int first = (int)((long long)pieces * part / p.blocks), last = (int)((long long)pieces * (part + 1) / p.blocks);
+    if (tid == 0) sh.candidates = 0;
+    if (p.top > 0 && tid < kMostTop) sh.best[tid] = Entry{-INFINITY, -1};
+
+    Sums mine;  // m: the warp's; s, w: the lane's
+    float most = -INFINITY;
+    for (int i = first + warp; i < last; i += kWarps * kAtOnce) {
+        uint4 r[kAtOnce];
+        float top[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+            const long long at = i + u * kWarps < last ? (long long)(i + u * kWarps) * 32 + lane : x.end;  // (past the end: all -inf)
+            r[u] = x.load(at);
+        }
+        float up = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+            const float lane_top = largest<BF16>(r[u]);
+            most = fmaxf(most, lane_top);
+            top[u] = warp_max(lane_top);
+            up = fmaxf(up, top[u]);
+        }
+        if (p.top > 0 && lane == 0)
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u)
+                if (i + u * kWarps < last) sh.piece[i + u * kWarps - first] = top[u];
+        if (up > mine.m) mine.raise(up, c);
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) mine.add<BF16>(r[u], c);
+    }
+    mine.s = warp_sum(mine.s), mine.w = warp_sum(mine.w);
+    if (lane == 0) sh.wmax[warp] = mine.m, sh.wsum[warp] = mine.s, sh.wsum_t[warp] = mine.w;
+    sh.group[tid] = most;
+    __syncthreads();
+    if (tid == 0) {
+        Sums all;
+        for (int w = 0; w < kWarps; ++w) all.join(sh.wmax[w], sh.wsum[w], sh.wsum_t[w], c);
+        sh.max = all.m, sh.sum = all.s, sh.sum_t = all.w;
+    }
+    if (p.top > 0) {
+        const int k = p.top;
+        float g = -INFINITY;
+        if (tid < kGroups) {
+#pragma unroll
+            for (int j = 0; j < kThreads / kGroups; ++j) g = fmaxf(g, sh.group[tid + j * kGroups]);
+        }
+        __syncthreads();
+        if (tid < kGroups) sh.group[tid] = g;
+        __syncthreads();
+        if (tid < kGroups) {
+            int ahead = 0;
+            for (int j = 0; j < kGroups; ++j) ahead += sh.group[j] > g || (sh.group[j] == g && j < tid);
+            if (ahead == k - 1) sh.bound = g;
+        }
+        __syncthreads();
+        const float bound = sh.bound;
+        for (int i = warp * 32; i < last - first; i += kThreads) {
+            const float has = i + lane < last - first ? sh.piece[i + lane] : -INFINITY;
+            uint32_t hits = __ballot_sync(0xffffffffu, has >= bound && has > -INFINITY);
+            while (hits != 0) {
+                const int u = __ffs(hits) - 1;
+                hits &= hits - 1;
+                const long long at = (long long)(first + i + u) * 32 + lane;
+                const uint4 r = x.load(at);
+#pragma unroll
+                for (int j = 0; j < E; ++j) {
+                    const float v = value<BF16>(r, j);
+                    if (!(v >= bound && v > -INFINITY)) continue;
+                    const int to = atomicAdd(&sh.candidates, 1);
+                    if (to < kCandidates) sh.candidate[to] = Entry{v, (int)(at * E + j - x.skip)};
+                }
+            }
+        }
+        __syncthreads();
+        if (sh.candidates <= kCandidates) {
+            rank(sh.candidate, sh.candidates, k, sh.best);
+        } else {
+            // The next entry of the order, k times over the part.
+            Entry bar{INFINITY, -1};
+            for (int n = 0; n < k; ++n) {
+                Entry e{-INFINITY, 0x7fffffff};
+                for (int i = first + warp; i < last; i += kWarps) {
+                    const long long at = (long long)i * 32 + lane;
+                    const uint4 r = x.load(at);
+#pragma unroll
+                    for (int j = 0; j < E; ++j) {
+                        const Entry o{value<BF16>(r, j), (int)(at * E + j - x.skip)};
+                        if (o.v > -INFINITY && before(bar, o) && before(o, e)) e = o;
+                    }
+                }
+#pragma unroll
+                for (int d = 16; d > 0; d >>= 1) {
+                    const Entry o{__shfl_xor_sync(0xffffffffu, e.v, d), __shfl_xor_sync(0xffffffffu, e.id, d)};
+                    if (before(o, e)) e = o;
+                }
+                if (lane == 0) sh.wbest[warp] = e;
+                __syncthreads();
+                e = sh.wbest[0];
+                for (int w = 1; w < kWarps; ++w)
+                    if (before(sh.wbest[w], e)) e = sh.wbest[w];
+                bar = e;
+                if (tid == 0 && e.v > -INFINITY) sh.best[n] = e;
+                __syncthreads();
+            }
+        }
+    }
+    if (p.blocks > 1) cluster_sync();
+    else __syncthreads();
+    if (part == 0) {
+        if (p.blocks > 1 && p.top > 0) {  // the blocks' best together
+            for (int i = tid; i < p.blocks * p.top; i += kThreads) {
+                const uint32_t at = cluster_place(&sh.best[i % p.top], i / p.top);
+                sh.candidate[i] = Entry{cluster_load(at), __float_as_int(cluster_load(at + 4))};
+            }
+            __syncthreads();
+            if (tid < kMostTop) sh.best[tid] = Entry{-INFINITY, -1};
+            __syncthreads();
+            rank(sh.candidate, p.blocks * p.top, p.top, sh.best);  // (empty places come behind; equal ones among them keep theirs)
+            __syncthreads();
+        }
+        if (warp == 0) {
+            Sums all;
+            all.m = sh.max, all.s = sh.sum, all.w = sh.sum_t;
+            for (int b = 1; b < p.blocks; ++b)
+                all.join(cluster_load(cluster_place(&sh.max, b)), cluster_load(cluster_place(&sh.sum, b)), cluster_load(cluster_place(&sh.sum_t, b)), c);
+            const bool none = all.m == -INFINITY && all.s == 0.0f;  // a row whose mask leaves nothing
+            const float l2 = log2f(all.s);
+            if (lane == 0) {
+                const int token = p.tokens == nullptr ? -1 : __ldg(p.tokens + row);
+                if (p.logprob != nullptr) {
+                    float lp = 0.0f;
+                    if (token >= 0 && token < p.vocab) {
+                        float v;
+                        if constexpr (BF16) v = bf16_bits_to_f32(__ldg(static_cast<const uint16_t*>(p.logits) + row * p.ld + token));
+                        else v = __ldg(static_cast<const float*>(p.logits) + row * p.ld + token);
+                        lp = none ? -INFINITY : kLn2 * ((v - all.m) * c - l2);
+                    }
+                    p.logprob[row] = lp;
+                }
+                if (p.entropy != nullptr) p.entropy[row] = none ? 0.0f : kLn2 * (l2 - all.w / all.s);
+                if (p.lse != nullptr) p.lse[row] = none ? -INFINITY : fmaf(kLn2, l2, all.m / heat);
+            }
+            if (lane < p.top) {
+                const Entry e = sh.best[lane];
+                p.top_ids[row * p.top + lane] = e.id;
+                p.top_values[row * p.top + lane] = e.id < 0 ? -INFINITY : kLn2 * ((e.v - all.m) * c - l2);
+            }
+        }
+    }
+    if (p.blocks > 1) cluster_sync();  // nobody leaves while its results may be read
+}
+
+// A block takes kBackThreads x kBackAtOnce pieces of 16 bytes of the gradient's row.  (Plain loads: the gradient may take the logits' place, each thread's pieces its own.)
+constexpr int kBackThreads = 256, kBackAtOnce = 4;
+template <bool BF16>
+__global__ void __launch_bounds__(kBackThreads) logprob_backward_kernel(const LogprobParams p) {
+    constexpr int E = Row<BF16>::E;
+    grid_ready();
+    const long long row = blockIdx.x / p.blocks;
+    const long long first = (long long)(blockIdx.x % p.blocks) * kBackThreads * kBackAtOnce + threadIdx.x;
+    const Row<BF16> d(p.dlogits, row * p.dld, p.vocab);  // pieces by the gradient's boundaries
+    const Row<BF16> x(p.logits, row * p.ld, p.vocab);
+    const bool same = d.skip == x.skip;
+    const float heat = heat_of(p.temperature, row), inv = 1.0f / heat, lse = __ldg(p.lse + row);
+    const int token = __ldg(p.tokens + row);
+    const bool named = token >= 0 && token < p.vocab;
+    const float l = named && p.dlogprob != nullptr ? __ldg(p.dlogprob + row) * inv : 0.0f;
+    const float n = p.dentropy != nullptr ? __ldg(p.dentropy + row) * inv : 0.0f, entropy = n != 0.0f ? __ldg(p.entropy + row) : 0.0f;
+    const bool none = lse == -INFINITY;
+    uint4 r[kBackAtOnce];
+#pragma unroll
+    for (int u = 0; u < kBackAtOnce; ++u) {
+        const long long i = first + u * kBackThreads;
+        if (i * E >= d.end) continue;
+        if (same) {
+            r[u] = x.load(i);
+        } else {  // (rows that lie differently on their 16 bytes)
+            uint32_t* w = reinterpret_cast<uint32_t*>(&r[u]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = 0u;
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                const long long at = i * E + j - d.skip;
+                if (at < 0 || at >= p.vocab) continue;
+                if constexpr (BF16) w[j / 2] |= (uint32_t) static_cast<const uint16_t*>(p.logits)[row * p.ld + at] << (j % 2 * 16);
+                else w[j] = static_cast<const uint32_t*>(p.logits)[row * p.ld + at];
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kBackAtOnce; ++u) {
+        const long long i = first + u * kBackThreads;
+        if (i * E >= d.end) continue;
+        float y[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            const float lp = max_nan(fmaf(value<BF16>(r[u], j), inv, -lse), -1000.0f), q = ex2_ftz(lp * kLog2e);
+            y[j] = none ? 0.0f : -q * fmaf(n, lp + entropy, l);
+            if (named && i * E + j - d.skip == token && !none) y[j] += l;
+        }
+        unsigned char* to = const_cast<unsigned char*>(d.base) + i * 16;
+        if (i * E >= d.skip && i * E + E <= d.end) {
+            uint4 o;
+            uint32_t* w = reinterpret_cast<uint32_t*>(&o);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (BF16) {
+                    const __nv_bfloat162 two = __floats2bfloat162_rn(y[2 * j], y[2 * j + 1]);
+                    w[j] = *reinterpret_cast<const uint32_t*>(&two);
+                } else {
+                    w[j] = __float_as_uint(y[j]);
+                }
+            }
+            *reinterpret_cast<uint4*>(to) = o;
+        } else {
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                if (i * E + j < d.skip || i * E + j >= d.end) continue;
+                if constexpr (BF16) reinterpret_cast<uint16_t*>(to)[j] = f32_to_bf16_bits(y[j]);
+                else reinterpret_cast<float*>(to)[j] = y[j];
+            }
+        }
+    }
+}
+
+// Blocks that share a row: enough that a small call fills the GPU, while each still has a piece a warp.
+int row_blocks(long long rows, int vocab, bool bf16) {
+    const int pieces = vocab / (bf16 ? 256 : 128) + 2;
+    int n = 1;
+    while (n < kMostBlocks && (pieces > n * kPieces || (rows * n < 2 * sm_count() && pieces >= 2 * n * kWarps))) n *= 2;
+    return n;
+}
+
+bool logits_ok(const void* p, int32_t kind, int64_t ld, int32_t vocab) {
+    if (kind != GLM53F_KDA_LOGITS_F32 && kind != GLM53F_KDA_LOGITS_BF16) return false;
+    return p != nullptr && (reinterpret_cast<uintptr_t>(p) & (kind == GLM53F_KDA_LOGITS_BF16 ? 1 : 3)) == 0 && ld >= vocab;
+}
+bool words(std::initializer_list<const void*> all) {
+    for (const void* p : all)
+        if (reinterpret_cast<uintptr_t>(p) & 3) return false;
+    return true;
+}
+
+}  // namespace
+}  // namespace kda
+
+extern "C" int glm53f_kda_logprobs(int32_t rows, int32_t vocab, const void* logits, int32_t kind, int64_t ld, const int32_t* tokens, const float* temperature,
+                                   float* logprob, float* entropy, float* lse, int32_t top, int32_t* top_ids, float* top_values, glm53f_stream_t stream) {
+    using namespace kda;
+    if (rows < 0 || vocab < 1 || vocab > kMostVocab || top < 0 || top > kMostTop) return kInvalid;
+    if (rows == 0) return 0;
+    if (!logits_ok(logits, kind, ld, vocab) || !words({tokens, temperature, logprob, entropy, lse, top_ids, top_values})) return kInvalid;
+    if ((logprob != nullptr) != (tokens != nullptr) || (top > 0) != (top_ids != nullptr) || (top > 0) != (top_values != nullptr)) return kInvalid;
+    if (logprob == nullptr && entropy == nullptr && lse == nullptr && top == 0) return kInvalid;
+    const bool bf16 = kind == GLM53F_KDA_LOGITS_BF16;
+    LogprobParams p{};
+    p.logits = logits, p.ld = ld, p.vocab = vocab, p.blocks = row_blocks(rows, vocab, bf16), p.top = top;
+    p.tokens = tokens, p.temperature = temperature, p.logprob = logprob, p.entropy = entropy, p.lse = lse, p.top_ids = top_ids, p.top_values = top_values;
+    if ((long long)rows * p.blocks > 0x7fffffff) return kInvalid;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(rows * p.blocks));
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr[2];
+    unsigned na = early_attribute(attr[0]);
+    if (p.blocks > 1) {
+        attr[na].id = cudaLaunchAttributeClusterDimension;
+        attr[na].val.clusterDim.x = (unsigned)p.blocks;
+        attr[na].val.clusterDim.y = 1;
+        attr[na].val.clusterDim.z = 1;
+        ++na;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = na;
+    return (int)(bf16 ? cudaLaunchKernelEx(&cfg, logprob_kernel<true>, p) : cudaLaunchKernelEx(&cfg, logprob_kernel<false>, p));
+}
+
+extern "C" int glm53f_kda_logprobs_backward(int32_t rows, int32_t vocab, const void* logits, int32_t kind, int64_t ld, const int32_t* tokens,
+                                            const float* temperature, const float* lse, const float* entropy, const float* dlogprob, const float* dentropy,
+                                            void* dlogits, int64_t dld, glm53f_stream_t stream) {
+    using namespace kda;
+    if (rows < 0 || vocab < 1 || vocab > kMostVocab) return kInvalid;
+    if (rows == 0) return 0;
+    if (!logits_ok(logits, kind, ld, vocab) || !logits_ok(dlogits, kind, dld, vocab) || !words({tokens, temperature, lse, entropy, dlogprob, dentropy})) return kInvalid;
+    if (lse == nullptr || tokens == nullptr || (dlogprob == nullptr && dentropy == nullptr) || (dentropy != nullptr && entropy == nullptr)) return kInvalid;
+    const bool bf16 = kind == GLM53F_KDA_LOGITS_BF16;
+    const int per = kBackThreads * kBackAtOnce * (bf16 ? 8 : 4);
+    LogprobParams p{};
+    p.logits = logits, p.ld = ld, p.vocab = vocab;
+    // (values before a row's start on its 16 bytes: at most these)
+    const int size = bf16 ? 2 : 4, most = 16 / size - 1, skip = dld % (16 / size) == 0 ? (int)((reinterpret_cast<uintptr_t>(dlogits) & 15) / size) : most;
+    p.blocks = (int)(((long long)vocab + skip + per - 1) / per);
+    p.tokens = tokens, p.temperature = temperature, p.lse = const_cast<float*>(lse), p.entropy = const_cast<float*>(entropy);
+    p.dlogprob = dlogprob, p.dentropy = dentropy, p.dlogits = dlogits, p.dld = dld;
+    if ((long long)rows * p.blocks > 0x7fffffff) return kInvalid;
+    const dim3 grid((unsigned)(rows * p.blocks));
+    if (bf16) return launch_early(logprob_backward_kernel<true>, grid, kBackThreads, 0, reinterpret_cast<cudaStream_t>(stream), p);
+    return launch_early(logprob_backward_kernel<false>, grid, kBackThreads, 0, reinterpret_cast<cudaStream_t>(stream), p);
+}

@@ -86,10 +86,13 @@ SIGNATURES = {
     "glm53f_kda_scan_prefill_varlen": (C.c_int, [I32, I32, P, I32, I32, P, I64, P, I64, I32, P, P, P, P, I64, P, P, I64, P]),
     "glm53f_kda_scan_backward_varlen": (C.c_int, [I32, I32, P, I32, I32, P, I64, P, I64, I32, P, P, I64, P, P, P, P, I64, P, I64, P, I64, P]),
     "glm53f_kda_accept_batch": (C.c_int, [I32, P, I32, P, I32, I64, P, P, I64, P, P, P, P, P]),
+    # Part 6: log probabilities
+    "glm53f_kda_logprobs": (C.c_int, [I32, I32, P, I32, I64, P, P, P, P, P, I32, P, P, P]),
+    "glm53f_kda_logprobs_backward": (C.c_int, [I32, I32, P, I32, I64, P, P, P, P, P, P, P, I64, P]),
 }
 
 # The reference's thirteen (crates/glm53f-kda/tests/provenance.rs:41-69 asserts exactly these).
-REFERENCE_SYMBOLS = [n for n in SIGNATURES if n.startswith("glm53f_kda_") and "_core_" not in n and "_gather_" not in n and "_lin_" not in n and "_scan_" not in n and n not in ("glm53f_kda_device_status", "glm53f_kda_debug_wait_test", "glm53f_kda_prefill_mode", "glm53f_kda_verify_mode", "glm53f_kda_commit_mode", "glm53f_kda_mark_copy", "glm53f_kda_mark_copy_slots", "glm53f_kda_mark_copy_list", "glm53f_kda_store_words", "glm53f_kda_proj_bf16", "glm53f_kda_proj_bf16_many", "glm53f_kda_proj_bf16_fused", "glm53f_kda_accept_batch", "glm53f_kda_chain_commit_batch")]
+REFERENCE_SYMBOLS = [n for n in SIGNATURES if n.startswith("glm53f_kda_") and "_core_" not in n and "_gather_" not in n and "_lin_" not in n and "_scan_" not in n and n not in ("glm53f_kda_device_status", "glm53f_kda_debug_wait_test", "glm53f_kda_prefill_mode", "glm53f_kda_verify_mode", "glm53f_kda_commit_mode", "glm53f_kda_mark_copy", "glm53f_kda_mark_copy_slots", "glm53f_kda_mark_copy_list", "glm53f_kda_store_words", "glm53f_kda_proj_bf16", "glm53f_kda_proj_bf16_many", "glm53f_kda_proj_bf16_fused", "glm53f_kda_accept_batch", "glm53f_kda_chain_commit_batch", "glm53f_kda_logprobs", "glm53f_kda_logprobs_backward")]
 
 
 def library_path() -> str:

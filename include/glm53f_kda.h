@@ -575,6 +575,30 @@ int glm53f_kda_scan_backward_varlen(int32_t channels, int32_t batch, const int32
                                     int64_t dg_stride, void* dx, int64_t dx_stride, void* workspace, int64_t workspace_bytes,
                                     glm53f_stream_t stream);
 
+/* ===================================================================================================
+ * Part 6: log probabilities
+ * =================================================================================================== */
+
+/* Of each row of `logits` (f32 or bf16: `kind` GLM53F_KDA_LOGITS_F32 or _BF16; row r at + r * ld elements, `vocab` long, aligned to its elements), with
+ * p = softmax(logits / temperature[r]):
+ *   logprob   f32 [rows]: log p of tokens[r] (int32; outside [0, vocab): no token, 0)
+ *   entropy   f32 [rows]: -sum of p log p
+ *   lse       f32 [rows]: log of the sum of e^(logits / temperature), for the backward pass
+ *   top_ids, top_values   int32 and f32 [rows][top], top <= 32: the largest logits' indices, ties to the lowest, and their log p.  Places that
+ *             fewer logits above -inf leave are -1 and -inf; NaN entries are in none
+ * Any of them may be NULL (tokens with logprob; top 0 with top_ids and top_values).  temperature f32 [rows], NULL: 1; a row's 0 or less and NaN: 1, otherwise held within
+ * 1e-30 and 1e30.  -inf logits have p = 0 and add nothing to the entropy; a row of nothing else gives log p -inf, entropy 0 and lse -inf.  A row with a NaN or
+ * +inf gives NaN.  Sums are f32: log p and the entropy are within a few 1e-7 of the logits' span.  1 <= vocab <= 2,000,000.  One launch. */
+int glm53f_kda_logprobs(int32_t rows, int32_t vocab, const void* logits, int32_t kind, int64_t ld, const int32_t* tokens, const float* temperature,
+                        float* logprob, float* entropy, float* lse, int32_t top, int32_t* top_ids, float* top_values, glm53f_stream_t stream);
+
+/* The logits' gradient, of their type, row r at + r * dld: dlogits_j = (dlogprob [j = token] - dlogprob p_j - dentropy p_j (log p_j + entropy)) / temperature from the
+ * gradients dlogprob and dentropy (f32 [rows]; one of them may be NULL) of a call that gave lse and, where dentropy is not NULL, entropy.  A row without a
+ * token takes nothing from dlogprob; a row that masks everything gets 0.  dlogits may be `logits` itself (with dld = ld), and otherwise has no byte in common with it. */
+int glm53f_kda_logprobs_backward(int32_t rows, int32_t vocab, const void* logits, int32_t kind, int64_t ld, const int32_t* tokens,
+                                 const float* temperature, const float* lse, const float* entropy, const float* dlogprob, const float* dentropy,
+                                 void* dlogits, int64_t dld, glm53f_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
