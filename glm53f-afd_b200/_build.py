@@ -23,6 +23,7 @@ SOURCES = {
     "kda_prefill_sp.cu": [],  # tensor-core prefill: agrees with the chain to rounding, so default FP flags
     "proj_gemm.cu": [],      # the projections: tcgen05 GEMM
     "proj_gemm_pair.cu": [], # the same on SM pairs (cta_group::2) for many rows
+    "proj_int4.cu": [],      # the projections with 4-bit weights
     "lin_decode.cu": [],     # linear attention with one decay a head: row by row
     "lin_prefill.cu": [],    # ... and chunked
     "gated_scan.cu": [],     # gated linear recurrence, channel by channel: scan, backward pass, row by row

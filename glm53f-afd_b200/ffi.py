@@ -75,6 +75,9 @@ SIGNATURES = {
     "glm53f_kda_proj_bf16": (I32, [P, I64, I64, P, I64, I64, I32, I32, I32, I32, P, I32, I64, I64, P]),
     "glm53f_kda_proj_bf16_many": (I32, [P, I32, P]),
     "glm53f_kda_proj_bf16_fused": (I32, [C.POINTER(ProjJob), C.POINTER(ProjEpilogue), P]),
+    "glm53f_kda_int4_bytes": (I64, [I32, I32, I32, I32]),
+    "glm53f_kda_int4_pack": (I32, [P, P, P, I32, I32, I32, P, P]),
+    "glm53f_kda_proj_int4": (I32, [P, I64, P, I32, I32, I32, I32, I32, P, I32, I64, P]),
     # Parts 3 and 4 of include/glm53f_kda.h: linear attention with one decay a head, the verification of drafted tokens
     "glm53f_kda_lin_decode_batch": (C.c_int, [I32, I32, I32, P, P, P, I64, P, I64, P, I64, P, I64, P, P, P, I32, F32, P, I64, P]),
     "glm53f_kda_lin_prefill_workspace_bytes": (I64, [I32, I32, I32]),
@@ -92,7 +95,7 @@ SIGNATURES = {
 }
 
 # The reference's thirteen (crates/glm53f-kda/tests/provenance.rs:41-69 asserts exactly these).
-REFERENCE_SYMBOLS = [n for n in SIGNATURES if n.startswith("glm53f_kda_") and "_core_" not in n and "_gather_" not in n and "_lin_" not in n and "_scan_" not in n and n not in ("glm53f_kda_device_status", "glm53f_kda_debug_wait_test", "glm53f_kda_prefill_mode", "glm53f_kda_verify_mode", "glm53f_kda_commit_mode", "glm53f_kda_mark_copy", "glm53f_kda_mark_copy_slots", "glm53f_kda_mark_copy_list", "glm53f_kda_store_words", "glm53f_kda_proj_bf16", "glm53f_kda_proj_bf16_many", "glm53f_kda_proj_bf16_fused", "glm53f_kda_accept_batch", "glm53f_kda_chain_commit_batch", "glm53f_kda_logprobs", "glm53f_kda_logprobs_backward")]
+REFERENCE_SYMBOLS = [n for n in SIGNATURES if n.startswith("glm53f_kda_") and "_core_" not in n and "_gather_" not in n and "_lin_" not in n and "_scan_" not in n and n not in ("glm53f_kda_device_status", "glm53f_kda_debug_wait_test", "glm53f_kda_prefill_mode", "glm53f_kda_verify_mode", "glm53f_kda_commit_mode", "glm53f_kda_mark_copy", "glm53f_kda_mark_copy_slots", "glm53f_kda_mark_copy_list", "glm53f_kda_store_words", "glm53f_kda_proj_bf16", "glm53f_kda_proj_bf16_many", "glm53f_kda_proj_bf16_fused", "glm53f_kda_accept_batch", "glm53f_kda_chain_commit_batch", "glm53f_kda_logprobs", "glm53f_kda_logprobs_backward", "glm53f_kda_int4_bytes", "glm53f_kda_int4_pack", "glm53f_kda_proj_int4")]
 
 
 def library_path() -> str:

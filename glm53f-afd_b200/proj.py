@@ -101,6 +101,88 @@ def fused(x: torch.Tensor, ldx: int, x_gstride: int, w: Bf16Mat, rows: int, out:
     _launched(code, "glm53f_kda_proj_bf16_fused")
 
 
+INT4_GROUPS = (32, 64, 128)
+INT4_MOST_K = 65536
+
+
+@dataclass
+class Int4Mat:
+    """A weight [n][k] of 4-bit codes, laid out for `int4`: w = scale * (code - zero), a scale and a zero point (`zeros`; else 8) for each `group` k."""
+
+    t: torch.Tensor
+    n: int
+    k: int
+    group: int
+    zeros: bool
+
+    @classmethod
+    def pack(cls, codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, *, group: int = 128) -> "Int4Mat":
+        """From codes uint8 [n][k / 2] (the even k in the low halves), scales bf16 [n][k / group] and zeros uint8 [n][k / group] of 0 .. 15, on the
+        device: one launch, on the current stream."""
+        if codes.dim() != 2 or codes.dtype != torch.uint8:
+            raise Invalid("codes must be uint8 [n][k / 2]")
+        n, k = codes.shape[0], 2 * codes.shape[1]
+        if group not in INT4_GROUPS or n < 1 or k < 64 or k % 64 or k % group or k > INT4_MOST_K:
+            raise Invalid(f"a weight of {n} x {k} in groups of {group}: k a multiple of 64 and of the group (32, 64 or 128), at most {INT4_MOST_K}")
+        for t, name, dtype in ((scales, "scales", torch.bfloat16), (zeros, "zeros", torch.uint8)):
+            if t is not None and (t.dtype != dtype or tuple(t.shape) != (n, k // group)):
+                raise Invalid(f"{name} must be {dtype} [{n}][{k // group}], got {t.dtype} {tuple(t.shape)}")
+        here = torch.cuda.current_device()
+        for t in (codes, scales, zeros):
+            if t is not None and (not t.is_cuda or t.device.index != here or not t.is_contiguous()):
+                raise Invalid(f"codes, scales and zeros are contiguous CUDA tensors on the current device, cuda:{here}")
+        packed = torch.empty(ffi.glm53f_kda_int4_bytes(n, k, group, int(zeros is not None)), dtype=torch.uint8, device=codes.device)
+        _launched(ffi.glm53f_kda_int4_pack(codes.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), n, k, group, packed.data_ptr(),
+                                           torch.cuda.current_stream().cuda_stream), "glm53f_kda_int4_pack")
+        return cls(packed, n, k, group, zeros is not None)
+
+    @classmethod
+    def quantise(cls, w: torch.Tensor, *, group: int = 128, zeros: bool = False) -> "Int4Mat":
+        """The nearest codes of a weight [n][k]: a group's scale is its largest magnitude / 7, or with `zeros` its span (0 within) / 15, as bf16."""
+        if w.dim() != 2 or group not in INT4_GROUPS or w.shape[1] % group or w.shape[1] % 64:
+            raise Invalid(f"a weight [n][k], k a multiple of 64 and of the group (32, 64 or 128), got {tuple(w.shape)}")
+        n, k = w.shape
+        g = w.float().view(n, k // group, group)
+        if zeros:
+            low, high = g.amin(-1).clamp(max=0), g.amax(-1).clamp(min=0)
+            scales = ((high - low) / 15).bfloat16()
+        else:
+            scales = (g.abs().amax(-1) / 7).bfloat16()
+        step = torch.where(scales == 0, 1.0, scales.float())
+        zero = torch.round(-low / step).clamp(0, 15) if zeros else torch.full_like(step, 8.0)
+        codes = (torch.round(g / step[..., None]) + zero[..., None]).clamp(0, 15).to(torch.uint8).view(n, k)
+        return cls.pack(codes[:, 0::2] | (codes[:, 1::2] << 4), scales, zero.to(torch.uint8) if zeros else None, group=group)
+
+    def bytes(self) -> int:
+        return self.n * self.k // 2 + self.n * (self.k // self.group) * (3 if self.zeros else 2)
+
+
+def int4(x: torch.Tensor, ldx: int, w: Int4Mat, rows: int, out: torch.Tensor, ldo: int, out_f32: bool = False, x_offset: int = 0, out_offset: int = 0) -> None:
+    """out[m][o] = sum_k x[m][k] w[o][k] with 4-bit weights (glm53f_kda_proj_int4); strides and offsets in elements, as in `bf16`.  No weight is rounded: group sums
+    are multiplied by their scales in f32."""
+    if rows == 0:
+        return
+    if min(rows, ldx, ldo, x_offset, out_offset) < 0 or max(rows, ldx, ldo) > 0x7fffffff:
+        raise Invalid("rows, strides and offsets are not negative, and rows and strides below 2^31")
+    if x.dtype not in _BF:
+        raise Invalid("x is bf16")
+    if (out.dtype != torch.float32) if out_f32 else (out.dtype not in _BF):
+        raise Invalid("out is f32 when out_f32, else bf16")
+    if ldx < w.k or ldo < w.n:
+        raise Invalid(f"rows of {ldx} and {ldo} for {w.k} inputs and {w.n} outputs")
+    if x.numel() < x_offset + (rows - 1) * ldx + w.k or out.numel() < out_offset + (rows - 1) * ldo + w.n or not x.is_contiguous() or not out.is_contiguous():
+        raise Invalid("a buffer is not contiguous or smaller than the shapes named")
+    here = torch.cuda.current_device()
+    for t in (x, w.t, out):
+        if not t.is_cuda or t.device.index != here:
+            raise Invalid(f"a tensor on {t.device}, the current device is cuda:{here}")
+    if w.t.numel() < ffi.glm53f_kda_int4_bytes(w.n, w.k, w.group, int(w.zeros)):
+        raise Invalid("the weight is smaller than the shapes named")
+    code = ffi.load().glm53f_kda_proj_int4(x.data_ptr() + 2 * x_offset, ldx, w.t.data_ptr(), w.n, w.k, w.group, int(w.zeros), rows,
+                                           out.data_ptr() + out_offset * out.element_size(), int(out_f32), ldo, torch.cuda.current_stream().cuda_stream)
+    _launched(code, "glm53f_kda_proj_int4")
+
+
 def _job(x, ldx, x_gstride, w: Bf16Mat, rows, out, ldo, o_gstride, out_f32=False, x_offset=0, out_offset=0) -> tuple:
     """The checked arguments of one GEMM: those of glm53f_kda_proj_bf16 before the stream, the fields of ffi.ProjJob."""
     if x.dtype not in _BF or w.t.dtype not in _BF:

@@ -79,6 +79,24 @@ typedef struct glm53f_proj_epilogue {
 } glm53f_proj_epilogue;
 int32_t glm53f_kda_proj_bf16_fused(const glm53f_proj_job* job, const glm53f_proj_epilogue* epilogue, glm53f_stream_t stream);
 
+/* Projections with 4-bit weights; not in the reference.  A weight [n][k] is codes q of 0 .. 15 with a scale s for each group of 32, 64 or 128 k of a row, and maybe a zero
+ * point z of 0 .. 15 (without: 8):  w[o][i] = s[o][i / group] * (q[o][i] - z[o][i / group]).
+ *
+ * glm53f_kda_int4_pack lays it out once, into glm53f_kda_int4_bytes(n, k, group, zeros != NULL) bytes (16-byte aligned), from
+ *   codes    [n][k / 2] bytes: value 2 i in the low half of byte i, 2 i + 1 in the high
+ *   scales   bf16 [n][k / group]
+ *   zeros    bytes [n][k / group], or NULL
+ * n >= 1, k % 64 == 0, k % group == 0, k <= 65,536.  The packed bytes are read by glm53f_kda_proj_int4 with the same n, k, group and `zeros` != 0 where they were given. */
+int64_t glm53f_kda_int4_bytes(int32_t n, int32_t k, int32_t group, int32_t zeros);
+int32_t glm53f_kda_int4_pack(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int32_t n, int32_t k, int32_t group, void* packed,
+                             glm53f_stream_t stream);
+
+/* out[m][o] = sum_i x[m][i] * w[o][i] for rows m < rows: x bf16 at x + m * ldx (16-byte aligned, ldx >= k a multiple of 8), out at out + m * ldo (ldo >= n), bf16 or, with
+ * out_f32 != 0, f32, memory of its own.  x times code is exact, a group's sum f32, multiplied by its scale in f32: no weight is rounded; the result is rounded once.  rows == 0
+ * launches nothing.  Status codes as glm53f_kda_proj_bf16. */
+int32_t glm53f_kda_proj_int4(const uint16_t* x, int64_t ldx, const void* packed, int32_t n, int32_t k, int32_t group, int32_t zeros, int32_t rows,
+                             void* out, int32_t out_f32, int64_t ldo, glm53f_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
