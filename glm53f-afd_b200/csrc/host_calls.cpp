@@ -456,6 +456,223 @@ int proj_fused(PyObject* const* a) {
     return unlocked([&] { return glm53f_kda_proj_bf16_fused(&job, &e, st); });
 }
 
+// ---- gated.py, spec.logprobs and proj.int4 ----------------------------------------------------------------------------------------
+struct Plain {  // `rows` rows of `width` f32 or bf16 values, any stride apart
+    void* ptr;
+    int64_t stride;
+    bool bf16;
+};
+inline Plain plain_rows(PyObject* o, int64_t rows, int64_t width, int dev) {
+    const at::Tensor& t = on_device(o, dev);
+    const bool bf16 = t.scalar_type() == at::kBFloat16;
+    if ((!bf16 && t.scalar_type() != at::kFloat) || t.dim() != 2 || t.size(0) < rows || t.size(1) != width || (width > 1 && t.stride(1) != 1)) throw Miss{};
+    const int64_t stride = t.size(0) > 1 ? t.stride(0) : width;
+    if (stride < width) throw Miss{};
+    return {t.data_ptr(), stride, bf16};
+}
+inline void typed_as(const Plain& a, const Plain& b) {
+    if (a.bf16 != b.bf16) throw Miss{};
+}
+// A contiguous f32 state, a request's region of `width` values beginning `most` in at the furthest (None: not said).
+inline float* vector_state(PyObject* o, int64_t width, PyObject* most, int dev) {
+    auto* p = need_here<float>(o, kF32, 0, dev);
+    if (most != Py_None) {
+        const int64_t at = to_i64(most);
+        if (at < 0 || tensor(o).numel() < mul_add(at, 1, width)) throw Miss{};
+    }
+    return p;
+}
+inline void apart_or_same(PyObject* a, PyObject* b) {
+    const at::Tensor &x = tensor(a), &y = tensor(b);
+    const auto p = reinterpret_cast<uintptr_t>(x.data_ptr()), q = reinterpret_cast<uintptr_t>(y.data_ptr());
+    if (p != q && q < p + x.nbytes() && p < q + y.nbytes()) throw Miss{};
+}
+struct Scan {
+    int64_t channels, rows, max_len, batch, flags;
+    int dev;
+    const int32_t* cu;
+    const int64_t* off;
+    Plain g, x;
+    void* ws = nullptr;
+    int64_t ws_bytes = 0;
+};
+// (channels, rows, max_len, cu_rows, g, x, state_off, kinds, workspace)
+Scan scan_args(PyObject* channels, PyObject* rows, PyObject* max_len, PyObject* cu, PyObject* g, PyObject* x, PyObject* off, PyObject* kinds, PyObject* workspace) {
+    Scan s;
+    s.channels = to_i64(channels), s.rows = to_i64(rows), s.max_len = to_i64(max_len), s.flags = to_i64(kinds);
+    if (s.channels < 1 || s.channels > 0x7fffffff || s.rows < 1 || s.rows > 0x7fffffff || s.max_len < 0 || s.max_len > s.rows || s.flags < 0) throw Miss{};
+    s.dev = here();
+    s.cu = need_here<const int32_t>(cu, kI32, 2, s.dev);
+    s.batch = tensor(cu).numel() - 1;
+    if (s.batch > 0x7fffffff) throw Miss{};
+    s.off = need_here<const int64_t>(off, kI64, s.batch, s.dev);
+    s.g = plain_rows(g, s.rows, s.channels, s.dev), s.x = plain_rows(x, s.rows, s.channels, s.dev);
+    s.flags |= (s.g.bf16 ? GLM53F_KDA_SCAN_G_BF16 : 0) | (s.x.bf16 ? GLM53F_KDA_SCAN_X_BF16 : 0);
+    if (workspace != Py_None) {
+        const at::Tensor& w = on_device(workspace, s.dev);
+        if (!w.is_contiguous()) throw Miss{};
+        s.ws_bytes = (int64_t)w.nbytes();
+        s.ws = s.ws_bytes != 0 ? w.data_ptr() : nullptr;
+        if (reinterpret_cast<uintptr_t>(s.ws) & 15) throw Miss{};
+    }
+    return s;
+}
+float* scan_saves(PyObject* o, const Scan& s) {
+    auto* p = need_here<float>(o, kF32, mul_add(glm53f_kda_scan_saves_rows((int32_t)s.batch, (int32_t)s.rows), s.channels, 0), s.dev);
+    if (reinterpret_cast<uintptr_t>(p) & 7) throw Miss{};
+    return p;
+}
+inline glm53f_stream_t current_stream() { return reinterpret_cast<glm53f_stream_t>(c10::cuda::getCurrentCUDAStream().stream()); }
+
+// scan(prefill, channels, rows, max_len, cu_rows, g, x, state, state_off, kinds, keep, state_out, out, saves, workspace, max_state_off)
+int scan(PyObject* const* a) {
+    const bool prefill = a[0] == Py_True;
+    const Scan s = scan_args(a[1], a[2], a[3], a[4], a[5], a[6], a[8], a[9], a[14]);
+    float *si = vector_state(a[7], s.channels, a[15], s.dev), *so = nullptr;
+    if (PyUnicode_Check(a[11])) {
+        so = si;
+    } else if (a[11] != Py_None) {
+        so = vector_state(a[11], s.channels, a[15], s.dev);
+        if (tensor(a[11]).numel() < tensor(a[7]).numel()) throw Miss{};
+        apart_or_same(a[7], a[11]);
+    }
+    Plain out{nullptr, 0, false};
+    if (a[12] != Py_None) {
+        out = plain_rows(a[12], s.rows, s.channels, s.dev);
+        typed_as(out, s.x);
+    }
+    const auto st = current_stream();
+    if (!prefill) {
+        const auto* keep = a[10] == Py_None ? nullptr : need_here<const int32_t>(a[10], kI32, s.batch, s.dev);
+        if (so == nullptr && out.ptr == nullptr) throw Miss{};
+        return unlocked([&] {
+            return glm53f_kda_scan_decode_batch((int32_t)s.channels, (int32_t)s.batch, s.cu, keep, s.g.ptr, s.g.stride, s.x.ptr, s.x.stride, (int32_t)s.flags, si, so,
+                                                s.off, out.ptr, out.stride, st);
+        });
+    }
+    if (so == nullptr) throw Miss{};
+    float* saves = a[13] == Py_None ? nullptr : scan_saves(a[13], s);
+    return unlocked([&] {
+        return glm53f_kda_scan_prefill_varlen((int32_t)s.channels, (int32_t)s.batch, s.cu, (int32_t)s.rows, (int32_t)s.max_len, s.g.ptr, s.g.stride, s.x.ptr, s.x.stride,
+                                              (int32_t)s.flags, si, so, s.off, out.ptr, out.stride, saves, s.ws, s.ws_bytes, st);
+    });
+}
+
+// scan_backward(channels, rows, max_len, cu_rows, g, x, saves, state_off, kinds, dout, dg, dx, dstate, dstate_in, workspace, max_state_off)
+int scan_backward(PyObject* const* a) {
+    const Scan s = scan_args(a[0], a[1], a[2], a[3], a[4], a[5], a[7], a[8], a[14]);
+    const float* saves = scan_saves(a[6], s);
+    const Plain dout = plain_rows(a[9], s.rows, s.channels, s.dev), dg = plain_rows(a[10], s.rows, s.channels, s.dev), dx = plain_rows(a[11], s.rows, s.channels, s.dev);
+    typed_as(dout, s.x), typed_as(dg, s.g), typed_as(dx, s.x);
+    float *end = nullptr, *start = nullptr;
+    if (a[12] != Py_None) end = vector_state(a[12], s.channels, a[15], s.dev);
+    if (a[13] != Py_None) start = vector_state(a[13], s.channels, a[15], s.dev);
+    if (end != nullptr && start != nullptr) apart_or_same(a[12], a[13]);
+    const auto st = current_stream();
+    return unlocked([&] {
+        return glm53f_kda_scan_backward_varlen((int32_t)s.channels, (int32_t)s.batch, s.cu, (int32_t)s.rows, (int32_t)s.max_len, s.g.ptr, s.g.stride, s.x.ptr, s.x.stride,
+                                               (int32_t)s.flags, saves, dout.ptr, dout.stride, end, start, s.off, dg.ptr, dg.stride, dx.ptr, dx.stride, s.ws,
+                                               s.ws_bytes, st);
+    });
+}
+
+struct Logits {
+    void* ptr;
+    int64_t rows, vocab, ld;
+    bool bf16;
+};
+Logits logits_of(PyObject* o, int dev) {
+    const at::Tensor& t = on_device(o, dev);
+    const bool bf16 = t.scalar_type() == at::kBFloat16;
+    if ((!bf16 && t.scalar_type() != at::kFloat) || t.dim() != 2 || t.size(0) < 1 || t.size(0) > 0x7fffffff || t.size(1) < 1 || t.size(1) > 2000000 ||
+        (t.size(1) > 1 && t.stride(1) != 1))
+        throw Miss{};
+    const int64_t ld = t.size(0) > 1 ? t.stride(0) : t.size(1);
+    if (ld < t.size(1)) throw Miss{};
+    return {t.data_ptr(), t.size(0), t.size(1), ld, bf16};
+}
+template <typename T>
+T* per_row(PyObject* o, Kind kind, int64_t rows, int dev) {
+    if (o == Py_None) return nullptr;
+    T* p = need_here<T>(o, kind, rows, dev);
+    if (tensor(o).numel() != rows) throw Miss{};
+    return p;
+}
+
+// logprobs(logits, tokens, logprob, temperature, entropy, lse, top)
+int logprobs(PyObject* const* a) {
+    const int dev = here();
+    const Logits x = logits_of(a[0], dev);
+    const auto* tokens = per_row<const int32_t>(a[1], kI32, x.rows, dev);
+    auto *lp = per_row<float>(a[2], kF32, x.rows, dev), *entropy = per_row<float>(a[4], kF32, x.rows, dev), *lse = per_row<float>(a[5], kF32, x.rows, dev);
+    const auto* temperature = per_row<const float>(a[3], kF32, x.rows, dev);
+    if ((tokens == nullptr) != (lp == nullptr)) throw Miss{};
+    int64_t top = 0;
+    int32_t* ids = nullptr;
+    float* values = nullptr;
+    if (a[6] != Py_None) {
+        if (!PyTuple_CheckExact(a[6]) || PyTuple_GET_SIZE(a[6]) != 2) throw Miss{};
+        const at::Tensor &i = on_device(PyTuple_GET_ITEM(a[6], 0), dev), &v = on_device(PyTuple_GET_ITEM(a[6], 1), dev);
+        if (i.dim() != 2 || v.dim() != 2 || i.size(0) != x.rows || v.size(0) != x.rows || i.size(1) != v.size(1) || i.size(1) < 1 || i.size(1) > 32) throw Miss{};
+        top = i.size(1);
+        ids = need<int32_t>(PyTuple_GET_ITEM(a[6], 0), kI32, x.rows * top), values = need<float>(PyTuple_GET_ITEM(a[6], 1), kF32, x.rows * top);
+    }
+    if (lp == nullptr && entropy == nullptr && lse == nullptr && ids == nullptr) throw Miss{};
+    const auto st = current_stream();
+    return unlocked([&] {
+        return glm53f_kda_logprobs((int32_t)x.rows, (int32_t)x.vocab, x.ptr, x.bf16 ? GLM53F_KDA_LOGITS_BF16 : GLM53F_KDA_LOGITS_F32, x.ld, tokens, temperature, lp, entropy,
+                                   lse, (int32_t)top, ids, values, st);
+    });
+}
+
+// logprobs_backward(logits, tokens, lse, dlogprob, dlogits, temperature, entropy, dentropy)
+int logprobs_backward(PyObject* const* a) {
+    const int dev = here();
+    const Logits x = logits_of(a[0], dev), d = logits_of(a[4], dev);
+    if (x.bf16 != d.bf16 || x.rows != d.rows || x.vocab != d.vocab) throw Miss{};
+    const auto* tokens = per_row<const int32_t>(a[1], kI32, x.rows, dev);
+    const auto *lse = per_row<const float>(a[2], kF32, x.rows, dev), *dlp = per_row<const float>(a[3], kF32, x.rows, dev);
+    const auto *temperature = per_row<const float>(a[5], kF32, x.rows, dev), *entropy = per_row<const float>(a[6], kF32, x.rows, dev),
+               *dh = per_row<const float>(a[7], kF32, x.rows, dev);
+    if (tokens == nullptr || lse == nullptr || (dlp == nullptr && dh == nullptr) || (dh != nullptr && entropy == nullptr)) throw Miss{};
+    if (x.ptr != d.ptr || x.ld != d.ld) {
+        const int64_t size = x.bf16 ? 2 : 4;
+        const auto p = reinterpret_cast<uintptr_t>(x.ptr), q = reinterpret_cast<uintptr_t>(d.ptr);
+        if (q < p + (mul_add(x.rows - 1, x.ld, x.vocab)) * size && p < q + mul_add(d.rows - 1, d.ld, d.vocab) * size) throw Miss{};
+    }
+    const auto st = current_stream();
+    return unlocked([&] {
+        return glm53f_kda_logprobs_backward((int32_t)x.rows, (int32_t)x.vocab, x.ptr, x.bf16 ? GLM53F_KDA_LOGITS_BF16 : GLM53F_KDA_LOGITS_F32, x.ld, tokens, temperature,
+                                            lse, entropy, dlp, dh, d.ptr, d.ld, st);
+    });
+}
+
+// proj_int4(x, ldx, w, n, k, group, zeros, rows, out, ldo, out_f32, x_offset, out_offset)
+int proj_int4(PyObject* const* a) {
+    const int dev = here();
+    const at::Tensor &x = on_device(a[0], dev), &w = on_device(a[2], dev), &out = on_device(a[8], dev);
+    const int64_t ldx = to_i64(a[1]), n = to_i64(a[3]), k = to_i64(a[4]), group = to_i64(a[5]), rows = to_i64(a[7]), ldo = to_i64(a[9]), x_offset = to_i64(a[11]),
+                  o_offset = to_i64(a[12]);
+    const bool f32 = a[10] == Py_True, zeros = a[6] == Py_True;
+    if ((!f32 && a[10] != Py_False) || (!zeros && a[6] != Py_False)) throw Miss{};
+    for (int64_t v : {ldx, n, k, rows, ldo})
+        if (v < 1 || v > 0x7fffffff) throw Miss{};
+    if (group < 1 || group > 128 || x_offset < 0 || o_offset < 0 || ldx < k || ldo < n) throw Miss{};
+    if (!is_bf16(x) || (f32 ? out.scalar_type() != at::kFloat : !is_bf16(out)) || !x.is_contiguous() || !out.is_contiguous() || w.scalar_type() != at::kByte ||
+        !w.is_contiguous())
+        throw Miss{};
+    if (x.numel() < mul_add(rows - 1, ldx, mul_add(x_offset, 1, k)) || out.numel() < mul_add(rows - 1, ldo, mul_add(o_offset, 1, n))) throw Miss{};
+    const int64_t bytes = glm53f_kda_int4_bytes((int32_t)n, (int32_t)k, (int32_t)group, zeros);
+    if (bytes == 0 || w.numel() < bytes) throw Miss{};
+    const auto st = current_stream();
+    const auto* xp = static_cast<const uint16_t*>(x.data_ptr()) + x_offset;
+    auto* op = static_cast<unsigned char*>(out.data_ptr()) + o_offset * out.element_size();
+    const void* wp = w.data_ptr();
+    return unlocked([&] {
+        return glm53f_kda_proj_int4(xp, ldx, wp, (int32_t)n, (int32_t)k, (int32_t)group, zeros, (int32_t)rows, op, f32, ldo, st);
+    });
+}
+
 template <typename F>
 PyObject* answer(F&& f) {
     long code = -1;
@@ -485,6 +702,10 @@ PyObject* py_accept(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 PyObject* py_proj_fused(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return answer([&] { return n == 22 ? proj_fused(args) : -1; });
+}
+template <int (*F)(PyObject* const*), int N>
+PyObject* py_call(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return answer([&] { return n == N ? F(args) : -1; });
 }
 // raw_stream(Stream) -> the CUDA stream's address, or None for a stream it does not know.
 PyObject* py_raw_stream(PyObject*, PyObject* s) {
@@ -519,6 +740,11 @@ PyMethodDef methods[] = {
     {"lin", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_lin)), METH_FASTCALL, nullptr},
     {"accept", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_accept)), METH_FASTCALL, nullptr},
     {"proj_fused", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_proj_fused)), METH_FASTCALL, nullptr},
+    {"scan", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_call<scan, 16>)), METH_FASTCALL, nullptr},
+    {"scan_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_call<scan_backward, 16>)), METH_FASTCALL, nullptr},
+    {"logprobs", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_call<logprobs, 7>)), METH_FASTCALL, nullptr},
+    {"logprobs_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_call<logprobs_backward, 8>)), METH_FASTCALL, nullptr},
+    {"proj_int4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_call<proj_int4, 13>)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Native host path of the per-layer launches.", -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -128,7 +128,7 @@ _native = None
 class _PythonPath:
     """Stands in for the native host path: it takes no call, so every launch goes through the Python checks and ctypes."""
 
-    core_decode = chain_batch = lin = accept = proj_fused = staticmethod(lambda *_: -1)
+    core_decode = chain_batch = lin = accept = proj_fused = scan = scan_backward = logprobs = logprobs_backward = proj_int4 = staticmethod(lambda *_: -1)
     raw_stream = staticmethod(lambda _: None)
 
 

@@ -63,6 +63,11 @@ def _common(channels, rows, cu_rows, state_off, gate, input, max_len=0):
     return batch
 
 
+def _kinds(gate, input):
+    """The flags that name a call's kinds, or what the native path takes for none."""
+    return GATES.get(gate, -1) | INPUTS.get(input, -1)
+
+
 def _flags(gate, input, g, x):
     return GATES[gate] | INPUTS[input] | (G_BF16 if g.dtype == torch.bfloat16 else 0) | (X_BF16 if x.dtype == torch.bfloat16 else 0)
 
@@ -88,6 +93,10 @@ def decode_batch(channels, rows, cu_rows, g, x, state, state_off, *, gate="decay
     int32 [batch + 1], `state_off` int64 [batch] and `keep` int32 [batch] (the rows of each request that count; None: all) on the device.
     state_out: "in_place", None (a verify: not written) or a tensor; out=None writes no outputs (a commit of kept rows).  A verify and a commit
     of k rows leave the bits of k single-row calls."""
+    code = ffi.host().scan(False, channels, rows, 0, cu_rows, g, x, state, state_off, _kinds(gate, input), keep, state_out, out, None, None, max_state_off)
+    if code >= 0:
+        return _launched(code, "glm53f_kda_scan_decode_batch")
+    # Not the plain accepted call: the same checks here, with their errors.
     batch = _common(channels, rows, cu_rows, state_off, gate, input)
     gp, gs = _matrix(g, "g", rows, channels)
     xp, xs = _matrix(x, "x", rows, channels)
@@ -133,6 +142,9 @@ def prefill_varlen(channels, rows, cu_rows, max_len, g, x, state, state_off, *, 
     """glm53f_kda_scan_prefill_varlen: packed sequences, the longest of at most max_len rows.  out=None writes the end states only.  `saves`: f32
     [saves_rows(batch, rows)][channels], for a backward pass.  `workspace`: a CUDA uint8 tensor of `workspace_bytes` bytes, or None: results are the same
     bits, long sequences of few channels take longer."""
+    code = ffi.host().scan(True, channels, rows, max_len, cu_rows, g, x, state, state_off, _kinds(gate, input), None, state_out, out, saves, workspace, max_state_off)
+    if code >= 0:
+        return _launched(code, "glm53f_kda_scan_prefill_varlen")
     batch = _common(channels, rows, cu_rows, state_off, gate, input, max_len)
     gp, gs = _matrix(g, "g", rows, channels)
     xp, xs = _matrix(x, "x", rows, channels)
@@ -152,6 +164,10 @@ def backward_varlen(channels, rows, cu_rows, max_len, g, x, saves, state_off, do
                     workspace=None, max_state_off=None):
     """glm53f_kda_scan_backward_varlen: from dout (x's type) and `dstate` (f32, the gradient of the end states at state_off; None: zero), writes dg (g's type), dx (x's) and
     `dstate_in` (the start states' gradient; None: not wanted; may be `dstate`).  g, x, saves, gate, input and the row ranges are those of the `prefill_varlen` call."""
+    code = ffi.host().scan_backward(channels, rows, max_len, cu_rows, g, x, saves, state_off, _kinds(gate, input), dout, dg, dx, dstate, dstate_in, workspace,
+                                    max_state_off)
+    if code >= 0:
+        return _launched(code, "glm53f_kda_scan_backward_varlen")
     batch = _common(channels, rows, cu_rows, state_off, gate, input, max_len)
     gp, gs = _matrix(g, "g", rows, channels)
     xp, xs = _matrix(x, "x", rows, channels)

@@ -162,6 +162,10 @@ def int4(x: torch.Tensor, ldx: int, w: Int4Mat, rows: int, out: torch.Tensor, ld
     are multiplied by their scales in f32."""
     if rows == 0:
         return
+    code = ffi.host().proj_int4(x, ldx, w.t, w.n, w.k, w.group, w.zeros, rows, out, ldo, out_f32, x_offset, out_offset)
+    if code >= 0:
+        return _launched(code, "glm53f_kda_proj_int4")
+    # Not the plain accepted call: the same checks here, with their errors.
     if min(rows, ldx, ldo, x_offset, out_offset) < 0 or max(rows, ldx, ldo) > 0x7fffffff:
         raise Invalid("rows, strides and offsets are not negative, and rows and strides below 2^31")
     if x.dtype not in _BF:

@@ -90,6 +90,10 @@ def logprobs(logits, tokens, logprob, *, temperature=None, entropy=None, lse=Non
     tokens[row] (int32; outside the vocabulary: none, 0), `entropy` and `lse` (for `logprobs_backward`), and in `top` = (int32 ids, f32 values), both
     [rows][up to 32], the largest logits' indices, ties to the lowest, with their log p (-1 and -inf where fewer logits are above -inf).  tokens
     and logprob may be None together, as may the others.  temperature f32 [rows]; 0 or less, and None: 1."""
+    code = ffi.host().logprobs(logits, tokens, logprob, temperature, entropy, lse, top)
+    if code >= 0:
+        return _launched(code, "glm53f_kda_logprobs")
+    # Not the plain accepted call: the same checks here, with their errors.
     rows, vocab, ld, kind = _logits(logits, "logits")
     if (tokens is None) != (logprob is None):
         raise Invalid("tokens and logprob come together")
@@ -116,6 +120,9 @@ def logprobs(logits, tokens, logprob, *, temperature=None, entropy=None, lse=Non
 def logprobs_backward(logits, tokens, lse, dlogprob, dlogits, *, temperature=None, entropy=None, dentropy=None):
     """glm53f_kda_logprobs_backward: writes `dlogits` (the logits' type; may be the logits themselves) from the gradients of `logprobs`' logprob and entropy (f32
     [rows]; one of them may be None).  lse and, with dentropy, entropy are what `logprobs` gave for the same logits, tokens and temperature."""
+    code = ffi.host().logprobs_backward(logits, tokens, lse, dlogprob, dlogits, temperature, entropy, dentropy)
+    if code >= 0:
+        return _launched(code, "glm53f_kda_logprobs_backward")
     rows, vocab, ld, kind = _logits(logits, "logits")
     if dlogits is None or dlogits.dtype != logits.dtype or dlogits.shape != logits.shape:
         raise Invalid("dlogits has the logits' type and shape")
