@@ -5,11 +5,17 @@
 // dg_t = D_t a'_t (h_{t-1} - [c = 1 - a] x_t), a' the gate's slope.
 //
 // Bound by HBM: a few operations a value, each value read once and written once.  Rows compose: over rows i..j the recurrence is
-// h_j = A h_{i-1} + B with A the product of the a.  A tile is kRows rows of 64 channels; its values stay in registers (eight rows of two
-// channels a thread, all loads in flight at once) while the warps' (A, B) meet in shared memory and the tile's in global memory, so a sequence is divided
-// over the GPU and still read once: a tile says its (A, B), then looks at those of the tiles before it up to the nearest
-// whose end state is known, and says its own.  Tiles are taken from a counter in their order, so whatever a tile waits for is with a block that
-// runs already; the wait is bounded all the same (status 160, 161).
+// h_j = A h_{i-1} + B with A the product of the a.  A tile is 64 rows of 64 channels.  A sequence is divided over the GPU and still read once: a tile says its
+// (A, B) in global memory, looks at those of the tiles before it up to the nearest whose end state is known, and says its own.  Tiles are taken from
+// a counter in their order, so whatever a tile waits for is with a block that runs already; the wait is bounded all the same (status 160).
+//
+// What passes between tiles takes 1 to 2 us, longer than a tile's share of the memory time (0.75 us), so several tiles of a block are under way at once, one block an SM:
+//   a producer warp    finds the tiles and copies their rows into a ring of shared memory by tensor copies (64 x 64 boxes), two to three ahead;
+//   two groups of eight warps, a tile each in turn: the (A, B) of the eight rows of every warp; then, when the state that reaches the tile before
+//                      is there, the rows of that one, whose gates are formed again from shared memory: registers would hold only half as many;
+//   pairs of chain warps, a channel a lane, a tile in turn: the tile's (A, B) from the warps', what passes between tiles, every warp's start.
+// (With all of a tile done by one set of threads, two blocks an SM, 65,536 rows x 1,024 channels took 198 us, of 12,600 cycles a tile 4,300 in the wait for
+// the state and 2,100 in asking for rows.)
 //
 // The states between tiles come from one chain of h <- A h + B whatever a tile found ready: the same bits every time, with any workspace and beside any other request.
 
@@ -18,18 +24,21 @@
 
 #include "common.cuh"
 #include "kda_internal.h"
+#include "tensor_map.cuh"
 
 namespace kda {
 namespace {
 
-constexpr int kChannels = 64;              // of a tile: two a lane
-constexpr int kPer = 8;                    // rows of a thread
-constexpr int kSave = 64;                  // rows between saved states
-constexpr int kForwardWarps = 16, kBackwardWarps = 8;
-constexpr int kForwardRows = kPer * kForwardWarps, kBackwardRows = kPer * kBackwardWarps;
-static_assert(kForwardRows % kSave == 0 && kBackwardRows == kSave, "");
+constexpr int kChannels = 64;  // of a tile: two a lane
+constexpr int kRows = 64;      // of a tile
+constexpr int kPer = 8;        // rows of a warp
+constexpr int kWarps = kRows / kPer;  // of a group
+constexpr int kGroups = 2;
+constexpr int kAcross = 8;     // tiles that a look takes in at once
+constexpr int kMostShared = 226 * 1024;
 
-enum : int { kStatusScanBefore = 160, kStatusScanBehind = 161 };
+// Every wait is bounded; the codes say which one gave up.
+enum : int { kStatusScanChain = 160, kStatusScanEmpty = 161, kStatusScanFull = 162, kStatusScanSums = 163, kStatusScanStart = 164 };
 enum : unsigned { kNothing = 0, kPart = 1, kWhole = 2 };  // what a tile has said
 
 struct Record;
@@ -50,18 +59,21 @@ struct ScanParams {
     long long tiles;
     int slots;
     int* status;
+    // Rows that lie on 16 bytes come by tensor copies: (channel, row) maps of the inputs, boxes of a tile.
+    int boxes;
+    CUtensorMap tm_g, tm_x, tm_dout;
 };
 
-// Tile slots: sequence b's tiles of T rows lie at cu[b] / T + b and behind.  Every sequence has a slot at least, slots ascend with b, and rows / T + batch are enough.
-__device__ __forceinline__ int slot_of(int first, int b, int tile_rows) { return first / tile_rows + b; }
+// Tile slots: sequence b's tiles lie at cu[b] / 64 + b and behind.  Every sequence has a slot at least, slots ascend with b, and rows / 64 + batch are enough.
+__device__ __forceinline__ int slot_of(int first, int b) { return first / kRows + b; }
 
 // The sequence that slot lies in, by a converged warp: the last b with slot_of(cu[b], b) <= slot.
-__device__ int sequence_of(const int32_t* cu, int batch, int slot, int tile_rows) {
+__device__ int sequence_of(const int32_t* cu, int batch, int slot) {
     const int lane = threadIdx.x & 31;
     int lo = 0, n = batch;
     while (n > 1) {
         const int step = (n + 31) / 32, at = lane * step;
-        const bool below = at < n && slot_of(__ldg(cu + lo + at), lo + at, tile_rows) <= slot;
+        const bool below = at < n && slot_of(__ldg(cu + lo + at), lo + at) <= slot;
         const int count = max(__popc(__ballot_sync(0xffffffffu, below)), 1);
         lo += (count - 1) * step;
         n = min(step, n - (count - 1) * step);
@@ -81,12 +93,12 @@ __device__ __forceinline__ void store_release(unsigned* p, unsigned v) { asm vol
 template <bool BF16>
 struct Pair {
     float2 v;
-    __device__ __forceinline__ float get(int i) const { return i ? v.y : v.x; }
+    __device__ __forceinline__ float2 get() const { return v; }
 };
 template <>
 struct Pair<true> {
     uint32_t v;
-    __device__ __forceinline__ float get(int i) const { return __uint_as_float(i ? v & 0xffff0000u : v << 16); }
+    __device__ __forceinline__ float2 get() const { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
 };
 // `valid` of two channels of a row, each an access of its own; the others 0.
 template <bool BF16>
@@ -146,55 +158,68 @@ __device__ __forceinline__ void copy_async(void* to, const void* from) {
 }
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// The rows of a tile that are on their way to a thread: places of shared memory that only it reads, so no barrier is needed between the copies and it.
-template <bool BF16, int THREADS>
-struct Inbox {
-    Pair<BF16> v[kPer][THREADS];
-    // Asks for m rows.
-    __device__ __forceinline__ void ask(const Walk& w, int m, int valid, bool vec) {
+// A tile's rows of one matrix.  Where they come by boxes all of them do; else each thread asks for its own channels of its warp's rows, which only it reads.
+template <bool BF16>
+struct __align__(128) Inbox {
+    static constexpr uint32_t kBoxBytes = kRows * kChannels * kBytes<BF16>;
+    Pair<BF16> v[kWarps][kPer][32];
+    __device__ __forceinline__ float2 get(int warp, int r) const { return v[warp][r][threadIdx.x & 31].get(); }
+    __device__ __forceinline__ void box(const CUtensorMap& tm, int channel, int row, uint64_t* bar) {
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(v)),
+                     "l"(reinterpret_cast<uint64_t>(&tm)), "r"(smem_u32(bar)), "r"(channel), "r"(row)
+                     : "memory");
+    }
+    __device__ __forceinline__ void ask(int warp, const Walk& w, int m, int valid, bool vec) {
         if (valid <= 0) return;
         const unsigned char* p = w.at;
-#pragma unroll
-        for (int r = 0; r < kPer; ++r, p += w.step) {
-            if (r >= m) break;
-            Pair<BF16>* to = &v[r][threadIdx.x];
+#pragma unroll 2
+        for (int r = 0; r < m; ++r, p += w.step) {
+            Pair<BF16>* to = &v[warp][r][threadIdx.x & 31];
             if (vec) copy_async<2 * kBytes<BF16>>(to, p);
             else if (!BF16 && valid > 1) copy_async<4>(to, p), copy_async<4>(reinterpret_cast<float*>(to) + 1, p + 4);
             else *to = load_apart<BF16>(p, valid);
         }
     }
-    __device__ __forceinline__ Pair<BF16> get(int r) const { return v[r][threadIdx.x]; }
 };
 
-// e^x for x <= 0 or little above, to two units in the last place or so: the power of two of x log2(e) and what its rounding left.  Below 2^-126: 0.
-__device__ __forceinline__ float exp_of(float x) {
-    x = max_nan(x, -200.0f);  // (-inf: no infinities among the parts)
-    const float t = x * kLog2e, rest = fmaf(x, kLog2e, -t), e = ex2_ftz(t);
-    return fmaf(e, rest * 0.69314718f, e);
+__device__ __forceinline__ float2 two(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 ex2_two(float2 t) { return make_float2(ex2_ftz(t.x), ex2_ftz(t.y)); }
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
-// a, and 1 - a without the cancellation where a is near one.  Of the sigmoid both from e^-|g|: no overflow, and the smaller one keeps its digits.
-// Of e^g by the series of the exponential where a > 1/2.
+// a, and with REST 1 - a without the cancellation where a is near one.  Below 2^-126: 0.
+//   e^g: the exponent's rounding costs |g| 2^-24 of a, nothing where a is near one; 1 - a by the exponential's series where a > 1/2.
+//   sigmoid: both from e^-|g|, whose exponent's rounding is made good, so that the smaller one keeps its digits: no overflow either.
 template <bool SIGMOID, bool REST>
-__device__ __forceinline__ void gate(float g, float& a, float& rest) {
+__device__ __forceinline__ void gate(float2 g, float2& a, float2& rest) {
     if constexpr (SIGMOID) {
-        const float e = exp_of(-fabsf(g)), d = 1.0f + e;
-        float r = rcp_approx(d);
-        r = fmaf(r, fmaf(-d, r, 1.0f), r);  // (to half a step and a little)
-        const float small = e * r;
-        a = g < 0.0f ? small : r, rest = g < 0.0f ? r : small;
+        const float2 m = make_float2(min_nan(fabsf(g.x), 200.0f), min_nan(fabsf(g.y), 200.0f));
+        const float2 t = mul2(m, two(-kLog2e)), left = fma2(m, two(-kLog2e), make_float2(-t.x, -t.y));
+        float2 e = ex2_two(t);
+        e = fma2(e, mul2(left, two(0.69314718f)), e);
+        // 1 / (1 + e) by Newton's steps from the best straight line on [1, 2] (1/17 off, so 1/289, 1.2e-5, 1.4e-10): with the units for special functions
+        // busy with the exponentials of both passes, theirs would be the bound.
+        const float2 d = make_float2(1.0f + e.x, 1.0f + e.y), minus = make_float2(-d.x, -d.y);
+        float2 r = fma2(d, two(-8.0f / 17.0f), two(24.0f / 17.0f));
+#pragma unroll
+        for (int i = 0; i < 3; ++i) r = fma2(r, fma2(minus, r, two(1.0f)), r);
+        const float2 small = mul2(e, r);
+        a = make_float2(g.x < 0.0f ? small.x : r.x, g.y < 0.0f ? small.y : r.y);
+        rest = make_float2(g.x < 0.0f ? r.x : small.x, g.y < 0.0f ? r.y : small.y);
     } else {
-        a = exp_of(g);
+        a = ex2_two(mul2(g, two(kLog2e)));
         if constexpr (REST) {
-            float s = fmaf(g, 2.7557319e-6f, 2.4801587e-5f);  // 1 / 9!, 1 / 8!, ...
-            s = fmaf(g, s, 1.9841270e-4f);
-            s = fmaf(g, s, 1.3888889e-3f);
-            s = fmaf(g, s, 8.3333333e-3f);
-            s = fmaf(g, s, 4.1666667e-2f);
-            s = fmaf(g, s, 1.6666667e-1f);
-            s = fmaf(g, s, 0.5f);
-            rest = fabsf(g) < 0.6931472f ? -fmaf(g * g, s, g) : 1.0f - a;
-        } else {
-            rest = 1.0f;
+            float2 s = fma2(g, two(2.7557319e-6f), two(2.4801587e-5f));  // 1 / 9!, 1 / 8!, ...
+            s = fma2(g, s, two(1.9841270e-4f));
+            s = fma2(g, s, two(1.3888889e-3f));
+            s = fma2(g, s, two(8.3333333e-3f));
+            s = fma2(g, s, two(4.1666667e-2f));
+            s = fma2(g, s, two(1.6666667e-1f));
+            s = fma2(g, s, two(0.5f));
+            s = fma2(mul2(g, g), s, g);
+            rest = make_float2(fabsf(g.x) < 0.6931472f ? -s.x : 1.0f - a.x, fabsf(g.y) < 0.6931472f ? -s.y : 1.0f - a.y);
         }
     }
 }
@@ -223,95 +248,138 @@ __device__ __forceinline__ Record heard(const Record* from) {
     return r;
 }
 
-// The state that reaches this tile, for the threads below kChannels (a channel each), called by the whole block.  `count` tiles of its sequence lie before it (STEP -1) or behind
-// it (STEP 1), `more`: one waits for its end state.  Each warp asks one of the nearest tiles, all channels; the chain runs from the nearest whole one.
-template <int STEP, int WARPS>
-__device__ __forceinline__ float join(const ScanParams& p, Record (*near)[kChannels], long long slot, int stripe, int count, float A, float B, float start, bool more) {
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const long long pitch = (long long)p.stripes * kChannels;
-    Record* mine = p.records + slot * pitch + stripe * kChannels;
-    if (tid < kChannels && more) say(mine + tid, count == 0 ? Record{A, B, fmaf(A, start, B), kWhole} : Record{A, B, 0.0f, kPart});
-    if (count == 0) return start;
-    const int window = min(count, WARPS);
-    const Record* theirs = mine + STEP * (1 + warp) * pitch;
+// The state that reaches the tile in `slot` from the `count` > 0 tiles of its sequence before it (STEP -1) or behind it (STEP 1), a channel a lane: the chain from the nearest
+// whole tile on, over (A, B) of those in between.
+template <int STEP>
+__device__ float look(const ScanParams& p, const Record* mine, int count) {
+    const long long pitch = STEP * (long long)p.stripes * kChannels;
     uint64_t t0 = 0;
     float h = 0.0f;
-    for (int polls = 0;; ++polls) {
-        if (warp < window) {
-            const Record r0 = heard(theirs + lane), r1 = heard(theirs + 32 + lane);
-            near[warp][lane] = r0, near[warp][32 + lane] = r1;
+    bool found = false;
+    for (int polls = 0; !found; ++polls) {
+        // Outwards in steps of kAcross, twice at most: a lane's chain lies in registers.
+        Record near[kAcross], far[kAcross];
+        int whole = -1;
+#pragma unroll
+        for (int d = 0; d < kAcross; ++d) near[d] = d < count ? heard(mine + (d + 1) * pitch) : Record{0.0f, 0.0f, 0.0f, kNothing};
+        bool parts = true;
+#pragma unroll
+        for (int d = 0; d < kAcross; ++d) {
+            if (parts && near[d].said == kWhole) whole = d;
+            parts = parts && near[d].said == kPart;
         }
-        __syncthreads();
-        bool found = true;
-        if (tid < kChannels) {
-            int d = 0;
-            while (d < window && near[d][tid].said == kPart) ++d;
-            found = d < window && near[d][tid].said == kWhole;
-            if (found) {
-                h = near[d][tid].whole;
-                while (--d >= 0) h = fmaf(near[d][tid].a, h, near[d][tid].b);
+        if (parts) {
+#pragma unroll
+            for (int d = 0; d < kAcross; ++d) far[d] = d + kAcross < count ? heard(mine + (d + kAcross + 1) * pitch) : Record{0.0f, 0.0f, 0.0f, kNothing};
+#pragma unroll
+            for (int d = 0; d < kAcross; ++d) {
+                if (parts && far[d].said == kWhole) whole = d + kAcross;
+                parts = parts && far[d].said == kPart;
+            }
+            if (whole >= 0) {
+#pragma unroll
+                for (int d = kAcross - 1; d >= 0; --d) {
+                    if (d + kAcross == whole) h = far[d].whole;
+                    else if (d + kAcross < whole) h = fmaf(far[d].a, h, far[d].b);
+                }
             }
         }
-        bool over = false;
-        if (polls % 64 == 63) {
+        if (whole >= 0) {
+#pragma unroll
+            for (int d = kAcross - 1; d >= 0; --d) {
+                if (d == whole) h = near[d].whole;
+                else if (d < whole) h = fmaf(near[d].a, h, near[d].b);
+            }
+            found = true;
+        }
+        if (!found && polls % 64 == 63) {
             const uint64_t now = global_timer_ns();
             if (t0 == 0) t0 = now;
-            over = now - t0 > kWaitLimitNs || load_acquire(p.control + 1) != 0;
-        }
-        const int missing = __syncthreads_or(found ? 0 : 1);
-        if (!missing) break;
-        if (polls % 64 == 63 && __syncthreads_or(over)) {  // give up, and let the others know
-            if (tid == 0) {
-                atomicCAS(p.status, 0, STEP < 0 ? kStatusScanBefore : kStatusScanBehind);
+            if (now - t0 > kWaitLimitNs || load_acquire(p.control + 1) != 0) {  // give up, and let the others know
+                atomicCAS(p.status, 0, kStatusScanChain);
                 store_release(p.control + 1, 1u);
+                return __int_as_float(0x7fc00000);
             }
-            h = __int_as_float(0x7fc00000);
-            break;
         }
     }
-    if (tid < kChannels && more) say(mine + tid, Record{A, B, fmaf(A, h, B), kWhole});
+    return h;
+}
+// The same, and what is said of this tile: its (A, B) at once, its end state when it is known, where `more`: another tile waits for it.
+template <int STEP>
+__device__ __forceinline__ float join(const ScanParams& p, long long slot, int stripe, int channel, int count, float A, float B, float start, bool more) {
+    Record* mine = p.records + (slot * p.stripes + stripe) * kChannels + channel;
+    if (count == 0) {
+        if (more) say(mine, Record{A, B, fmaf(A, start, B), kWhole});
+        return start;
+    }
+    if (more) say(mine, Record{A, B, 0.0f, kPart});
+    const float h = look<STEP>(p, mine, count);
+    if (more) say(mine, Record{A, B, fmaf(A, h, B), kWhole});
     return h;
 }
 
-__global__ void scan_clear_kernel(const ScanParams p) {
+__global__ void scan_clear_kernel(const __grid_constant__ ScanParams p) {
     grid_ready();
     const long long n = p.tiles * kChannels;
     if (blockIdx.x == 0 && threadIdx.x < 2) p.control[threadIdx.x] = 0u;
     for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) p.records[i].said = kNothing;
 }
 
-// Which tile a block is at.  LOOK: tiles come from the counter; otherwise the block walks its sequence's tiles, from the end that the pass starts at.
+// A tile's place.
 struct Place {
-    int stripe, slot, b, first, n, tile, tiles;  // b < 0: no more
-    __device__ __forceinline__ bool live() const { return b >= 0 && tile < tiles; }  // (a slot may lie between two sequences' tiles)
+    int stripe, slot, b, first, n, tile, tiles;  // b < 0: no more tiles
 };
-template <int T>
 __device__ __forceinline__ void place_sequence(const ScanParams& p, Place& at) {
     at.first = min(max(__ldg(p.cu + at.b), 0), p.rows);
     at.n = max(min(__ldg(p.cu + at.b + 1), p.rows) - at.first, 0);
-    at.tiles = max((at.n + T - 1) / T, 1);  // a sequence without rows has a tile all the same: its state passes through
+    at.tiles = max((at.n + kRows - 1) / kRows, 1);  // a sequence without rows has a tile all the same: its state passes through
 }
-// The counter's tile `ticket`, by a converged warp.  Sequences' tiles run forwards, or with REVERSE backwards, the stripes of channels fastest.
-template <int T, bool REVERSE>
-__device__ __forceinline__ void place_ticket(const ScanParams& p, unsigned ticket, Place& at) {
-    at.b = -1;
-    if (ticket >= p.tiles) return;
-    at.stripe = (int)(ticket % p.stripes);
-    const int i = (int)(ticket / p.stripes);
-    at.slot = REVERSE ? p.slots - 1 - i : i;
-    at.b = sequence_of(p.cu, p.batch, at.slot, T);
-    place_sequence<T>(p, at);
-    at.tile = at.slot - slot_of(at.first, at.b, T);
-}
-template <int T, bool REVERSE>
-__device__ __forceinline__ void place_walk(const ScanParams& p, int walked, Place& at) {
-    at.stripe = blockIdx.x % p.stripes;
-    at.b = blockIdx.x / p.stripes;
-    at.slot = 0;
-    place_sequence<T>(p, at);
-    at.tile = REVERSE ? at.tiles - 1 - walked : walked;
-    if (walked >= at.tiles) at.b = -1;
-}
+
+// A block's tiles one after another, by a converged warp.  LOOK: from the counter, sequences' tiles forwards (backwards with REVERSE), the stripes of channels fastest;
+// otherwise all of a sequence's 64 channels, then another one's.
+template <bool LOOK, bool REVERSE>
+struct Tiles {
+    unsigned ticket = 0;
+    long long item = blockIdx.x;
+    int walked = 0;
+    Place seen;
+    __device__ __forceinline__ Tiles(const ScanParams& p) {
+        if (LOOK && (threadIdx.x & 31) == 0) ticket = atomicAdd(p.control, 1u);
+        seen.b = -1;
+    }
+    __device__ __forceinline__ Place next(const ScanParams& p) {
+        Place at;
+        if constexpr (LOOK) {
+            for (;;) {
+                const unsigned now = __shfl_sync(0xffffffffu, ticket, 0);
+                if ((threadIdx.x & 31) == 0) ticket = atomicAdd(p.control, 1u);  // the next one, on its way
+                at.b = -1;
+                if (now >= p.tiles) return at;
+                at.stripe = (int)(now % p.stripes);
+                const int i = (int)(now / p.stripes);
+                at.slot = REVERSE ? p.slots - 1 - i : i;
+                at.b = sequence_of(p.cu, p.batch, at.slot);
+                place_sequence(p, at);
+                at.tile = at.slot - slot_of(at.first, at.b);
+                if (at.tile < at.tiles) return at;  // (else a slot between two sequences)
+            }
+        } else {
+            if (seen.b >= 0 && walked == seen.tiles) item += gridDim.x, seen.b = -1;
+            if (seen.b < 0) {
+                at.b = -1;
+                if (item >= (long long)p.stripes * p.batch) return at;
+                seen.stripe = (int)(item % p.stripes), seen.b = (int)(item / p.stripes);
+                place_sequence(p, seen);
+                walked = 0;
+            }
+            at = seen;
+            at.tile = REVERSE ? at.tiles - 1 - walked : walked;
+            at.slot = slot_of(at.first, at.b) + at.tile;
+            ++walked;
+            return at;
+        }
+    }
+};
 
 // Calls f(sigmoid, complement) with the flags as compile-time constants.
 template <typename F>
@@ -326,301 +394,366 @@ __device__ __forceinline__ void with_flags(int flags, F&& f) {
     }
 }
 
-// A block's tiles, two known ahead: the copies of the next one's rows are asked for while this one is worked on.
-template <int T, int WARPS, bool LOOK, bool REVERSE>
-struct Tiles {
-    Place (&ring)[3];
-    unsigned ticket = 0;
-    const bool guide = threadIdx.x / 32 == WARPS - 1;
-    __device__ __forceinline__ Place next(const ScanParams& p, int i) {  // the guide's: tile i's place
-        Place at;
-        if constexpr (LOOK) {
-            const unsigned now = __shfl_sync(0xffffffffu, ticket, 0);
-            if ((threadIdx.x & 31) == 0) ticket = atomicAdd(p.control, 1u);
-            place_ticket<T, REVERSE>(p, now, at);
-        } else {
-            place_walk<T, REVERSE>(p, i, at);
-        }
-        return at;
-    }
-    __device__ __forceinline__ void put(const ScanParams& p, int i) {
-        if (!guide) return;
-        const Place at = next(p, i);
-        if ((threadIdx.x & 31) == 0) ring[i % 3] = at;
-    }
-    __device__ __forceinline__ Tiles(const ScanParams& p, Place (&r)[3]) : ring(r) {
-        if (LOOK && guide && (threadIdx.x & 31) == 0) ticket = atomicAdd(p.control, 1u);
-        put(p, 0);
-        put(p, 1);
-        __syncthreads();
+template <bool GB, bool XB>
+struct ForwardTile {
+    Inbox<GB> g;
+    Inbox<XB> x;
+    float2 sums[kWarps][kChannels];  // (A, B) of a warp's rows; then in A's place the state before them
+    static constexpr uint32_t kBoxBytes = Inbox<GB>::kBoxBytes + Inbox<XB>::kBoxBytes;
+};
+template <bool GB, bool XB>
+struct BackwardTile {
+    Inbox<GB> g;
+    Inbox<XB> x, dy;
+    float2 sums[kWarps][kChannels];  // as above
+    float back[kWarps][kChannels];   // what a warp's rows add to e; then the e behind them
+    static constexpr uint32_t kBoxBytes = Inbox<GB>::kBoxBytes + 2 * Inbox<XB>::kBoxBytes;
+};
+template <typename TILE>
+struct Shared {
+    static constexpr int kRing0 = kMostShared / (int)(sizeof(TILE) + sizeof(Place) + 32), kRing = kRing0 < 8 ? kRing0 : 8;
+    static_assert(kRing >= 2 * kGroups, "a group holds two tiles");
+    TILE tile[kRing];
+    uint64_t full[kRing], summed[kRing], started[kRing], empty[kRing];
+    Place place[kRing];
+    uint32_t control[2];
+};
+// Chain warps: pairs, a tile each in turn.  A walking block has one, which carries the state.
+template <bool LOOK>
+constexpr int kPairs = LOOK ? 3 : 1;
+template <bool LOOK>
+constexpr int kThreads = 32 * (kGroups * kWarps + 2 * kPairs<LOOK> + 1);
+
+// The ring's position of the i-th tile of a block, and the parity of its barriers' phases.
+template <int RING>
+struct Turn {
+    int s;
+    uint32_t parity;
+    __device__ __forceinline__ explicit Turn(int i) : s(i % RING), parity(i / RING & 1) {}
+    __device__ __forceinline__ void step(int n) {
+        s += n;
+        if (s >= RING) s -= RING, parity ^= 1;
     }
 };
 
-// This thread's rows of a tile, and how many there are.
-template <int T>
-__device__ __forceinline__ int rows_of(const Place& at, int& row0, long long& row) {
-    row0 = at.tile * T + (threadIdx.x >> 5) * kPer;
+// The warps' common frame: barriers, roles, the end.  PASS: load(at, tile, bar) asks for a tile's boxes, ask(at, tile, warp) for a thread's rows without boxes,
+// sum(at, tile, warp) forms the warp's sums, chain(at, tile, channel) what reaches the tile, finish(at, tile, warp) the rows.
+template <typename TILE, bool LOOK, bool REVERSE, typename PASS>
+__device__ __forceinline__ void run(const ScanParams& p, PASS& pass) {
+    using S = Shared<TILE>;
+    constexpr int R = S::kRing;
+    extern __shared__ __align__(128) unsigned char smem[];
+    S& sh = *reinterpret_cast<S*>(smem);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int s = 0; s < R; ++s) {
+            mbar_init(&sh.full[s], 1);
+            mbar_init(&sh.summed[s], kWarps);
+            mbar_init(&sh.started[s], 2);
+            mbar_init(&sh.empty[s], kWarps);
+        }
+        sh.control[0] = sh.control[1] = 0u;
+        mbar_init_fence();
+    }
+    __syncthreads();
+    const WaitCtx ctx{&sh.control[0], &sh.control[1], p.status};
+    auto wait = [&](uint64_t* bar, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, ctx, code)); };
+    grid_ready();
+    if (warp < kGroups * kWarps) {
+        const int group = warp / kWarps, w = warp % kWarps;
+        Turn<R> now(group), last(group);
+        bool pending = false;
+        auto finish = [&] {
+            if (!wait(&sh.started[last.s], last.parity, kStatusScanStart)) return false;
+            pass.finish(sh.place[last.s], sh.tile[last.s], w);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.empty[last.s]);
+            return true;
+        };
+        // Without boxes: the copies of this group's next tile, while it has work left.
+        auto next = [&](const Turn<R>& t) {
+            if (p.boxes) return true;
+            if (!wait(&sh.full[t.s], t.parity, kStatusScanFull)) return false;
+            if (sh.place[t.s].b >= 0) pass.ask(sh.place[t.s], sh.tile[t.s], w);
+            return true;
+        };
+        bool ok = next(now);
+        while (ok) {
+            if (p.boxes) {
+                ok = wait(&sh.full[now.s], now.parity, kStatusScanFull);
+                if (!ok) break;
+            } else {
+                copies_done();
+            }
+            const bool more = sh.place[now.s].b >= 0;
+            Turn<R> after = now;
+            after.step(kGroups);
+            if (more) {
+                pass.sum(sh.place[now.s], sh.tile[now.s], w);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.summed[now.s]);
+                // (a ring of three tiles a group has room for the next one before the last is done)
+                if (R >= 3 * kGroups) ok = next(after);
+            }
+            if (ok && pending) ok = finish();
+            if (!more) break;
+            if (R < 3 * kGroups) ok = ok && next(after);
+            last = now, pending = true, now = after;
+        }
+    } else if (warp < kGroups * kWarps + 2 * kPairs<LOOK>) {
+        const int i = warp - kGroups * kWarps, channel = (i & 1) * 32 + lane;
+        Turn<R> now(i / 2);
+        for (;;) {
+            if (!wait(&sh.full[now.s], now.parity, kStatusScanFull) || sh.place[now.s].b < 0) break;
+            if (!wait(&sh.summed[now.s], now.parity, kStatusScanSums)) break;
+            pass.chain(sh.place[now.s], sh.tile[now.s], channel);
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&sh.started[now.s]);
+                sh.control[0] = sh.control[0] + 1u;
+            }
+            now.step(kPairs<LOOK>);
+        }
+    } else {
+        Tiles<LOOK, REVERSE> tiles(p);
+        Turn<R> now(0);
+        constexpr int kEnds = kGroups > kPairs<LOOK> ? kGroups : kPairs<LOOK>;  // every group and every pair meets an end
+        int ends = 0;
+        Place at;
+        at.b = 0;
+        for (int i = 0; ends < kEnds; ++i) {
+            if (i >= R && !wait(&sh.empty[now.s], now.parity ^ 1u, kStatusScanEmpty)) break;
+            if (at.b >= 0) at = tiles.next(p);
+            if (lane == 0) {
+                sh.place[now.s] = at;
+                if (at.b >= 0 && at.n > 0 && p.boxes) {
+                    mbar_arrive_expect_tx(&sh.full[now.s], TILE::kBoxBytes);
+                    pass.load(at, sh.tile[now.s], &sh.full[now.s]);
+                } else {
+                    mbar_arrive(&sh.full[now.s]);
+                }
+            }
+            ends += at.b < 0;
+            now.step(1);
+        }
+    }
+    if (sh.control[1]) {  // after a wait that gave up, copies into this block's shared memory may still be in flight: a bounded time for them
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 2000000ull) {
+        }
+    }
+}
+
+// A warp's rows of a tile: how many there are, and the first one's place.
+__device__ __forceinline__ int rows_of(const Place& at, int warp, long long& row) {
+    const int row0 = at.tile * kRows + warp * kPer;
     row = (long long)at.first + row0;
     return min(max(at.n - row0, 0), kPer);
 }
 
-template <bool GB, bool XB>
-struct ForwardShared {
-    Inbox<GB, kForwardWarps * 32> g;
-    Inbox<XB, kForwardWarps * 32> x;
-    Record near[kForwardWarps][kChannels];
-    float4 agg[2][kForwardWarps][32];  // (A, B) of a warp's rows, two channels; two tiles' worth, so that one barrier a tile is enough
-    float carry[kChannels];
-    Place ring[3];
-};
-
 template <bool LOOK, bool GB, bool XB>
-__global__ void __launch_bounds__(kForwardWarps * 32, 2) scan_forward_kernel(const ScanParams p) {
-    constexpr int T = kForwardRows;
-    extern __shared__ __align__(16) unsigned char smem[];
-    auto& sh = *reinterpret_cast<ForwardShared<GB, XB>*>(smem);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const bool vec = p.vec;
-    float walk = 0.0f;  // a walking block's state between its tiles, a channel a thread of the first two warps
-    grid_ready();
-    Tiles<T, kForwardWarps, LOOK, false> tiles(p, sh.ring);
-    auto ask = [&](const Place& at) {
-        if (!at.live()) return;
-        int row0;
+struct Forward {
+    using TILE = ForwardTile<GB, XB>;
+    const ScanParams& p;
+    float walk = 0.0f;  // a walking block's state between its tiles
+    __device__ __forceinline__ explicit Forward(const ScanParams& q) : p(q) {}
+    __device__ __forceinline__ void load(const Place& at, TILE& t, uint64_t* bar) const {
+        const int c = at.stripe * kChannels, row = at.first + at.tile * kRows;
+        t.g.box(p.tm_g, c, row, bar);
+        t.x.box(p.tm_x, c, row, bar);
+    }
+    __device__ __forceinline__ void ask(const Place& at, TILE& t, int w) const {
         long long row;
-        const int m = rows_of<T>(at, row0, row), c0 = at.stripe * kChannels + 2 * lane, valid = p.channels - c0;
-        sh.g.ask(Walk(p.g, row, p.g_stride, c0, kBytes<GB>), m, valid, vec);
-        sh.x.ask(Walk(p.x, row, p.x_stride, c0, kBytes<XB>), m, valid, vec);
-    };
-    ask(sh.ring[0]);
-    for (int i = 0;; ++i) {
-        const Place at = sh.ring[i % 3];
-        if (at.b < 0) return;
-        auto& agg = sh.agg[i & 1];
-        int row0;
+        const int m = rows_of(at, w, row), c = at.stripe * kChannels + 2 * (threadIdx.x & 31);
+        t.g.ask(w, Walk(p.g, row, p.g_stride, c, kBytes<GB>), m, p.channels - c, p.vec);
+        t.x.ask(w, Walk(p.x, row, p.x_stride, c, kBytes<XB>), m, p.channels - c, p.vec);
+    }
+    __device__ __forceinline__ void sum(const Place& at, TILE& t, int w) const {
         long long row;
-        const int m = rows_of<T>(at, row0, row), c0 = at.stripe * kChannels + 2 * lane, valid = p.channels - c0;
-        float a[kPer][2], b[kPer][2];
-        copies_done();
-        if (at.live()) {
-            with_flags(p.flags, [&](auto sigmoid, auto complement) {
+        const int m = rows_of(at, w, row), lane = threadIdx.x & 31;
+        float2 A = two(1.0f), B = two(0.0f);
+        with_flags(p.flags, [&](auto sigmoid, auto complement) {
+            constexpr bool S = decltype(sigmoid)::value, C = decltype(complement)::value;
 #pragma unroll
-                for (int r = 0; r < kPer; ++r) {
-                    const Pair<GB> g = sh.g.get(r);
-                    const Pair<XB> x = sh.x.get(r);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        float rest;
-                        gate<decltype(sigmoid)::value, decltype(complement)::value>(g.get(j), a[r][j], rest);
-                        b[r][j] = decltype(complement)::value ? rest * x.get(j) : x.get(j);
-                    }
-                }
-            });
-            if (m < kPer)  // rows past the end leave the state as it is
-#pragma unroll
-                for (int r = 0; r < kPer; ++r)
-                    if (r >= m) a[r][0] = a[r][1] = 1.0f, b[r][0] = b[r][1] = 0.0f;
-            float A[2] = {1.0f, 1.0f}, B[2] = {0.0f, 0.0f};
-#pragma unroll
-            for (int r = 0; r < kPer; ++r)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) A[j] *= a[r][j], B[j] = fmaf(a[r][j], B[j], b[r][j]);
-            agg[warp][lane] = make_float4(A[0], B[0], A[1], B[1]);
-        }
-        __syncthreads();
-        ask(sh.ring[(i + 1) % 3]);
-        tiles.put(p, i + 2);
-        if (!at.live()) continue;
-        float TA = 1.0f, TB = 0.0f, start = walk;
-        const int c = at.stripe * kChannels + tid;
-        if (tid < kChannels) {  // a channel a thread
-#pragma unroll
-            for (int w = 0; w < kForwardWarps; ++w) {
-                const float2 ab = reinterpret_cast<const float2*>(agg[w])[tid];
-                TA *= ab.x, TB = fmaf(ab.x, TB, ab.y);
+            for (int r = 0; r < kPer; ++r) {
+                float2 a, rest, b = t.x.get(w, r);
+                gate<S, C>(t.g.get(w, r), a, rest);
+                if constexpr (C) b = mul2(rest, b);
+                if (r < m) A = mul2(A, a), B = fma2(a, B, b);  // rows past the end leave the state as it is
             }
-            if (at.tile == 0 && c < p.channels) start = p.state_in[p.state_off[at.b] + c];
-        }
-        float h0 = start;
-        if constexpr (LOOK) h0 = join<-1, kForwardWarps>(p, sh.near, at.slot, at.stripe, at.tile, TA, TB, start, at.tile + 1 < at.tiles);
-        else walk = fmaf(TA, h0, TB);
-        if (tid < kChannels) {
-            sh.carry[tid] = h0;
-            if (at.n == 0 && c < p.channels) p.state_out[p.state_off[at.b] + c] = h0;
-        }
-        __syncthreads();
-        float h[2] = {sh.carry[2 * lane], sh.carry[2 * lane + 1]};
-        for (int w = 0; w < warp; ++w) {
-            const float4 ab = agg[w][lane];
-            h[0] = fmaf(ab.x, h[0], ab.y), h[1] = fmaf(ab.z, h[1], ab.w);
-        }
-        if (p.saves != nullptr && (warp * kPer) % kSave == 0 && (m > 0 || row0 == 0))
-            store_pair<false>(reinterpret_cast<unsigned char*>(p.saves + ((long long)slot_of(at.first, at.b, kSave) + row0 / kSave) * p.channels + c0), valid,
-                              p.channels % 2 == 0, h[0], h[1]);
-        Walk out(p.out, row, p.out_stride, c0, kBytes<XB>);
+        });
+        reinterpret_cast<float4*>(t.sums[w])[lane] = make_float4(A.x, B.x, A.y, B.y);
+    }
+    __device__ __forceinline__ void chain(const Place& at, TILE& t, int channel) {
+        const int c = at.stripe * kChannels + channel;
+        const bool ok = c < p.channels;
+        const long long off = p.state_off[at.b] + c;
+        float TA = 1.0f, TB = 0.0f, h = at.tile == 0 ? (ok ? p.state_in[off] : 0.0f) : walk;
 #pragma unroll
-        for (int r = 0; r < kPer; ++r, out.at += out.step) {
-            h[0] = fmaf(a[r][0], h[0], b[r][0]), h[1] = fmaf(a[r][1], h[1], b[r][1]);
-            if (r < m && p.out != nullptr) store_pair<XB>(out.at, valid, vec, h[0], h[1]);
+        for (int w = 0; w < kWarps; ++w) {
+            const float2 ab = t.sums[w][channel];
+            TA *= ab.x, TB = fmaf(ab.x, TB, ab.y);
         }
-        if (m > 0 && row0 + m == at.n) {
-            float* s = p.state_out + p.state_off[at.b] + c0;
-            if (valid > 0) s[0] = h[0];
-            if (valid > 1) s[1] = h[1];
+        if constexpr (LOOK) h = join<-1>(p, at.slot, at.stripe, channel, at.tile, TA, TB, h, at.tile + 1 < at.tiles);
+        else walk = fmaf(TA, h, TB);
+        if (p.saves != nullptr && ok) p.saves[(long long)at.slot * p.channels + c] = h;
+        if (at.n == 0 && ok) p.state_out[off] = h;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float2 ab = t.sums[w][channel];
+            t.sums[w][channel].x = h;
+            h = fmaf(ab.x, h, ab.y);
         }
     }
-}
-
-template <bool GB, bool XB>
-struct BackwardShared {
-    struct Rows {
-        Inbox<GB, kBackwardWarps * 32> g;
-        Inbox<XB, kBackwardWarps * 32> x, dy;
-    } rows[2];  // (a tile's are read again at its end, when the next one's are on their way)
-    Record near[kBackwardWarps][kChannels];
-    float4 agg[2][kBackwardWarps][32];
-    float2 back[2][kBackwardWarps][32];  // what a warp's rows add to e
-    float carry[kChannels];
-    Place ring[3];
+    __device__ __forceinline__ void finish(const Place& at, const TILE& t, int w) const {
+        long long row;
+        const int m = rows_of(at, w, row), lane = threadIdx.x & 31, c = at.stripe * kChannels + 2 * lane, valid = p.channels - c;
+        if (m == 0) return;
+        const float4 s = reinterpret_cast<const float4*>(t.sums[w])[lane];
+        float2 h = make_float2(s.x, s.z);
+        Walk out(p.out, row, p.out_stride, c, kBytes<XB>);
+        const bool vec = p.vec, write = p.out != nullptr;
+        with_flags(p.flags, [&](auto sigmoid, auto complement) {
+            constexpr bool S = decltype(sigmoid)::value, C = decltype(complement)::value;
+#pragma unroll
+            for (int r = 0; r < kPer; ++r, out.at += out.step) {
+                float2 a, rest, b = t.x.get(w, r);
+                gate<S, C>(t.g.get(w, r), a, rest);
+                if constexpr (C) b = mul2(rest, b);
+                if (r < m) {
+                    h = fma2(a, h, b);
+                    if (write) store_pair<XB>(out.at, valid, vec, h.x, h.y);
+                }
+            }
+        });
+        if (at.tile * kRows + w * kPer + m == at.n) {
+            float* to = p.state_out + p.state_off[at.b] + c;
+            if (valid > 0) to[0] = h.x;
+            if (valid > 1) to[1] = h.y;
+        }
+    }
 };
 
 // As the forward pass from the other end, e in h's place: D_t = dy_t + e_t, e_{t-1} = a_t D_t.  The h of the tile's rows are formed again from the saved state at its start.
 template <bool LOOK, bool GB, bool XB>
-__global__ void __launch_bounds__(kBackwardWarps * 32, XB ? 3 : 2) scan_backward_kernel(const ScanParams p) {
-    constexpr int T = kBackwardRows;
-    extern __shared__ __align__(16) unsigned char smem[];
-    auto& sh = *reinterpret_cast<BackwardShared<GB, XB>*>(smem);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const bool vec = p.vec;
+struct Backward {
+    using TILE = BackwardTile<GB, XB>;
+    const ScanParams& p;
     float walk = 0.0f;
-    grid_ready();
-    Tiles<T, kBackwardWarps, LOOK, true> tiles(p, sh.ring);
-    auto ask = [&](const Place& at, auto& to) {
-        if (!at.live()) return;
-        int row0;
+    __device__ __forceinline__ explicit Backward(const ScanParams& q) : p(q) {}
+    __device__ __forceinline__ void load(const Place& at, TILE& t, uint64_t* bar) const {
+        const int c = at.stripe * kChannels, row = at.first + at.tile * kRows;
+        t.g.box(p.tm_g, c, row, bar);
+        t.x.box(p.tm_x, c, row, bar);
+        t.dy.box(p.tm_dout, c, row, bar);
+    }
+    __device__ __forceinline__ void ask(const Place& at, TILE& t, int w) const {
         long long row;
-        const int m = rows_of<T>(at, row0, row), c0 = at.stripe * kChannels + 2 * lane, valid = p.channels - c0;
-        to.g.ask(Walk(p.g, row, p.g_stride, c0, kBytes<GB>), m, valid, vec);
-        to.x.ask(Walk(p.x, row, p.x_stride, c0, kBytes<XB>), m, valid, vec);
-        to.dy.ask(Walk(p.dout, row, p.dout_stride, c0, kBytes<XB>), m, valid, vec);
-    };
-    ask(sh.ring[0], sh.rows[0]);
-    for (int i = 0;; ++i) {
-        const Place at = sh.ring[i % 3];
-        if (at.b < 0) return;
-        auto& agg = sh.agg[i & 1];
-        auto& back = sh.back[i & 1];
-        const auto& in = sh.rows[i & 1];
-        int row0;
+        const int m = rows_of(at, w, row), c = at.stripe * kChannels + 2 * (threadIdx.x & 31);
+        t.g.ask(w, Walk(p.g, row, p.g_stride, c, kBytes<GB>), m, p.channels - c, p.vec);
+        t.x.ask(w, Walk(p.x, row, p.x_stride, c, kBytes<XB>), m, p.channels - c, p.vec);
+        t.dy.ask(w, Walk(p.dout, row, p.dout_stride, c, kBytes<XB>), m, p.channels - c, p.vec);
+    }
+    __device__ __forceinline__ void sum(const Place& at, TILE& t, int w) const {
         long long row;
-        const int m = rows_of<T>(at, row0, row), c0 = at.stripe * kChannels + 2 * lane, valid = p.channels - c0;
-        const float* save = p.saves + ((long long)slot_of(at.first, at.b, kSave) + at.tile) * p.channels + c0;
-        float before[2] = {at.live() && valid > 0 ? __ldg(save) : 0.0f, at.live() && valid > 1 ? __ldg(save + 1) : 0.0f};
-        copies_done();
+        const int m = rows_of(at, w, row), lane = threadIdx.x & 31;
+        float2 A = two(1.0f), B = two(0.0f), F = two(0.0f);
         with_flags(p.flags, [&](auto sigmoid, auto complement) {
             constexpr bool S = decltype(sigmoid)::value, C = decltype(complement)::value;
-            float a[kPer][2], b[kPer][2];
-            if (at.live()) {
 #pragma unroll
-                for (int r = 0; r < kPer; ++r) {
-                    const Pair<GB> g = in.g.get(r);
-                    const Pair<XB> x = in.x.get(r);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        float rest;
-                        gate<S, C>(g.get(j), a[r][j], rest);
-                        b[r][j] = C ? rest * x.get(j) : x.get(j);
-                        if (r >= m) a[r][j] = 1.0f, b[r][j] = 0.0f;
-                    }
+            for (int r = 0; r < kPer; ++r) {
+                float2 a, rest, b = t.x.get(w, r);
+                gate<S, C>(t.g.get(w, r), a, rest);
+                if constexpr (C) b = mul2(rest, b);
+                if (r < m) {
+                    A = mul2(A, a), B = fma2(a, B, b);
+                    F = fma2(A, t.dy.get(w, r), F);  // sum of a_0 .. a_r dy_r: what reaches the rows before these
                 }
-                float A[2] = {1.0f, 1.0f}, B[2] = {0.0f, 0.0f}, F[2] = {0.0f, 0.0f};
-#pragma unroll
-                for (int r = 0; r < kPer; ++r)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) A[j] *= a[r][j], B[j] = fmaf(a[r][j], B[j], b[r][j]);
-#pragma unroll
-                for (int r = kPer - 1; r >= 0; --r) {
-                    const Pair<XB> dy = in.dy.get(r);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) F[j] = a[r][j] * ((r < m ? dy.get(j) : 0.0f) + F[j]);
-                }
-                agg[warp][lane] = make_float4(A[0], B[0], A[1], B[1]);
-                back[warp][lane] = make_float2(F[0], F[1]);
             }
-            __syncthreads();
-            ask(sh.ring[(i + 1) % 3], sh.rows[(i + 1) & 1]);
-            tiles.put(p, i + 2);
-            if (!at.live()) return;
-            // The states before this warp's rows, and before each of them.
-            for (int w = 0; w < warp; ++w) {
-                const float4 ab = agg[w][lane];
-                before[0] = fmaf(ab.x, before[0], ab.y), before[1] = fmaf(ab.z, before[1], ab.w);
-            }
+        });
+        reinterpret_cast<float4*>(t.sums[w])[lane] = make_float4(A.x, B.x, A.y, B.y);
+        reinterpret_cast<float2*>(t.back[w])[lane] = F;
+    }
+    __device__ __forceinline__ void chain(const Place& at, TILE& t, int channel) {
+        const int c = at.stripe * kChannels + channel;
+        const bool ok = c < p.channels;
+        float h = ok ? __ldg(p.saves + (long long)at.slot * p.channels + c) : 0.0f;
+        const long long off = p.state_off[at.b] + c;
+        float TA = 1.0f, TF = 0.0f, e = at.tile + 1 == at.tiles ? (ok && p.state_in != nullptr ? p.state_in[off] : 0.0f) : walk;
 #pragma unroll
-            for (int r = 0; r < kPer; ++r)
+        for (int w = kWarps - 1; w >= 0; --w) {
+            const float a = t.sums[w][channel].x;
+            TA *= a, TF = fmaf(a, TF, t.back[w][channel]);
+        }
+        if constexpr (LOOK) e = join<1>(p, at.slot, at.stripe, channel, at.tiles - 1 - at.tile, TA, TF, e, at.tile > 0);
+        else walk = fmaf(TA, e, TF);
+        if (at.n == 0 && ok && p.state_out != nullptr) p.state_out[off] = e;
+        float A[kWarps];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const float h = before[j];
-                    before[j] = fmaf(a[r][j], h, b[r][j]);
-                    b[r][j] = h;
-                }
-            float TA = 1.0f, TF = 0.0f, start = walk;
-            const int c = at.stripe * kChannels + tid;
-            if (tid < kChannels) {
+        for (int w = 0; w < kWarps; ++w) {
+            const float2 ab = t.sums[w][channel];
+            t.sums[w][channel].x = h;
+            h = fmaf(ab.x, h, ab.y);
+            A[w] = ab.x;
+        }
 #pragma unroll
-                for (int w = kBackwardWarps - 1; w >= 0; --w) {
-                    const float wa = reinterpret_cast<const float2*>(agg[w])[tid].x;
-                    TA *= wa, TF = fmaf(wa, TF, reinterpret_cast<const float*>(back[w])[tid]);
-                }
-                if (at.tile + 1 == at.tiles) start = c < p.channels && p.state_in != nullptr ? p.state_in[p.state_off[at.b] + c] : 0.0f;
+        for (int w = kWarps - 1; w >= 0; --w) {
+            const float f = t.back[w][channel];
+            t.back[w][channel] = e;
+            e = fmaf(A[w], e, f);
+        }
+    }
+    __device__ __forceinline__ void finish(const Place& at, const TILE& t, int w) const {
+        long long row;
+        const int m = rows_of(at, w, row), lane = threadIdx.x & 31, c = at.stripe * kChannels + 2 * lane, valid = p.channels - c;
+        if (m == 0) return;
+        const float4 s = reinterpret_cast<const float4*>(t.sums[w])[lane];
+        float2 h = make_float2(s.x, s.z), e = reinterpret_cast<const float2*>(t.back[w])[lane];
+        Walk dxs(p.dx, row + kPer - 1, p.dx_stride, c, kBytes<XB>), dgs(p.dg, row + kPer - 1, p.dg_stride, c, kBytes<GB>);
+        const bool vec = p.vec;
+        with_flags(p.flags, [&](auto sigmoid, auto complement) {
+            constexpr bool S = decltype(sigmoid)::value, C = decltype(complement)::value;
+            float2 a[kPer], from[kPer], rest[kPer];  // from: h before the row, less x where the gate decides over both
+#pragma unroll
+            for (int r = 0; r < kPer; ++r) {
+                const float2 x = t.x.get(w, r);
+                gate<S, C>(t.g.get(w, r), a[r], rest[r]);
+                from[r] = C ? make_float2(h.x - x.x, h.y - x.y) : h;
+                h = fma2(a[r], h, C ? mul2(rest[r], x) : x);
             }
-            float e0 = start;
-            if constexpr (LOOK) e0 = join<1, kBackwardWarps>(p, sh.near, at.slot, at.stripe, at.tiles - 1 - at.tile, TA, TF, start, at.tile > 0);
-            else walk = fmaf(TA, e0, TF);
-            if (tid < kChannels) {
-                sh.carry[tid] = e0;
-                if (at.n == 0 && c < p.channels && p.state_out != nullptr) p.state_out[p.state_off[at.b] + c] = e0;
-            }
-            __syncthreads();
-            float e[2] = {sh.carry[2 * lane], sh.carry[2 * lane + 1]};
-            for (int w = kBackwardWarps - 1; w > warp; --w) {
-                const float4 ab = agg[w][lane];
-                const float2 f = back[w][lane];
-                e[0] = fmaf(ab.x, e[0], f.x), e[1] = fmaf(ab.z, e[1], f.y);
-            }
-            Walk dxs(p.dx, row + kPer - 1, p.dx_stride, c0, kBytes<XB>), dgs(p.dg, row + kPer - 1, p.dg_stride, c0, kBytes<GB>);
 #pragma unroll
             for (int r = kPer - 1; r >= 0; --r, dxs.at -= dxs.step, dgs.at -= dgs.step) {
                 if (r >= m) continue;
-                const Pair<GB> g = in.g.get(r);
-                const Pair<XB> x = in.x.get(r), dy = in.dy.get(r);
-                float dg[2], dx[2];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const float d = dy.get(j) + e[j];
-                    float again = a[r][j], rest = 1.0f;
-                    if constexpr (C || S) gate<S, C>(g.get(j), again, rest);  // (its other half again, from shared memory rather than kept)
-                    const float slope = S ? again * rest : again;
-                    dx[j] = C ? rest * d : d;
-                    dg[j] = d * slope * (C ? b[r][j] - x.get(j) : b[r][j]);
-                    e[j] = again * d;
-                }
-                store_pair<XB>(dxs.at, valid, vec, dx[0], dx[1]);
-                store_pair<GB>(dgs.at, valid, vec, dg[0], dg[1]);
-            }
-            if (row0 == 0 && m > 0 && p.state_out != nullptr) {
-                float* s = p.state_out + p.state_off[at.b] + c0;
-                if (valid > 0) s[0] = e[0];
-                if (valid > 1) s[1] = e[1];
+                const float2 dy = t.dy.get(w, r), d = make_float2(dy.x + e.x, dy.y + e.y), slope = S ? mul2(a[r], rest[r]) : a[r];
+                const float2 dx = C ? mul2(rest[r], d) : d, dg = mul2(mul2(d, slope), from[r]);
+                e = mul2(a[r], d);
+                store_pair<XB>(dxs.at, valid, vec, dx.x, dx.y);
+                store_pair<GB>(dgs.at, valid, vec, dg.x, dg.y);
             }
         });
+        if (at.tile == 0 && w == 0 && p.state_out != nullptr) {
+            float* to = p.state_out + p.state_off[at.b] + c;
+            if (valid > 0) to[0] = e.x;
+            if (valid > 1) to[1] = e.y;
+        }
     }
+};
+
+template <bool LOOK, bool GB, bool XB>
+__global__ void __launch_bounds__(kThreads<LOOK>, 1) scan_forward_kernel(const __grid_constant__ ScanParams p) {
+    Forward<LOOK, GB, XB> pass(p);
+    run<ForwardTile<GB, XB>, LOOK, false>(p, pass);
+}
+template <bool LOOK, bool GB, bool XB>
+__global__ void __launch_bounds__(kThreads<LOOK>, 1) scan_backward_kernel(const __grid_constant__ ScanParams p) {
+    Backward<LOOK, GB, XB> pass(p);
+    run<BackwardTile<GB, XB>, LOOK, true>(p, pass);
 }
 
 // Row by row, two channels a thread, eight rows' loads in flight.
 constexpr int kStepThreads = 128;
 template <bool GB, bool XB>
-__global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const ScanParams p) {
+__global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const __grid_constant__ ScanParams p) {
     grid_ready();
     const int parts = (p.channels + 2 * kStepThreads - 1) / (2 * kStepThreads);
     const int b = blockIdx.x / parts, c0 = (int)(blockIdx.x % parts) * 2 * kStepThreads + 2 * (int)threadIdx.x, valid = min(p.channels - c0, 2);
@@ -629,7 +762,7 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const ScanParam
     int n = max(__ldg(p.cu + b + 1) - first, 0);
     if (p.keep != nullptr) n = min(n, max(__ldg(p.keep + b), 0));
     const long long off = p.state_off[b] + c0;
-    float h[2] = {p.state_in[off], valid > 1 ? p.state_in[off + 1] : 0.0f};
+    float2 h = make_float2(p.state_in[off], valid > 1 ? p.state_in[off + 1] : 0.0f);
     for (int t = 0; t < n; t += kPer) {
         Pair<GB> g[kPer];
         Pair<XB> x[kPer];
@@ -646,19 +779,17 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const ScanParam
 #pragma unroll
             for (int r = 0; r < kPer; ++r, out.at += out.step) {
                 if (r >= m) break;
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    float a, rest;
-                    gate<decltype(sigmoid)::value, decltype(complement)::value>(g[r].get(j), a, rest);
-                    h[j] = fmaf(a, h[j], decltype(complement)::value ? rest * x[r].get(j) : x[r].get(j));
-                }
-                if (p.out != nullptr) store_pair<XB>(out.at, valid, p.vec, h[0], h[1]);
+                float2 a, rest, b = x[r].get();
+                gate<decltype(sigmoid)::value, decltype(complement)::value>(g[r].get(), a, rest);
+                if constexpr (decltype(complement)::value) b = mul2(rest, b);
+                h = fma2(a, h, b);
+                if (p.out != nullptr) store_pair<XB>(out.at, valid, p.vec, h.x, h.y);
             }
         });
     }
     if (p.state_out != nullptr) {
-        p.state_out[off] = h[0];
-        if (valid > 1) p.state_out[off + 1] = h[1];
+        p.state_out[off] = h.x;
+        if (valid > 1) p.state_out[off + 1] = h.y;
     }
 }
 
@@ -667,8 +798,8 @@ constexpr int kAllFlags = GLM53F_KDA_SCAN_SIGMOID | GLM53F_KDA_SCAN_COMPLEMENT |
 
 struct Layout {  // of the workspace: bytes from its start
     long long slots, stripes, records, bytes;
-    Layout(int64_t channels, int64_t batch, int64_t rows, int tile_rows) {
-        slots = rows / tile_rows + batch;
+    Layout(int64_t channels, int64_t batch, int64_t rows) {
+        slots = rows / kRows + batch;
         stripes = (channels + kChannels - 1) / kChannels;
         records = 256;
         bytes = records + slots * stripes * kChannels * (long long)sizeof(Record);
@@ -693,6 +824,17 @@ bool matrices_ok(const ScanParams& p, std::initializer_list<Matrix> all, int& ve
     return true;
 }
 
+// A map of rows that lie on 16 bytes, for boxes of a tile.
+bool row_boxes(CUtensorMap* tm, const Matrix& m, int channels, int rows) {
+    const long long size = m.bf16 ? 2 : 4;
+    EncodeTiled enc = encode_tiled();
+    if (enc == nullptr || rows < 1 || (reinterpret_cast<uintptr_t>(m.p) & 15) || m.stride * size % 16) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)channels, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)(m.stride * size)};
+    const cuuint32_t box[2] = {kChannels, kRows}, estr[2] = {1u, 1u};
+    return enc(tm, m.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(m.p), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Starts LAUNCH(look, gb, xb) with the flags as constants.
 template <typename F>
 int with_types(int flags, bool look, F&& f) {
@@ -704,18 +846,21 @@ int with_types(int flags, bool look, F&& f) {
     return look ? types(true_type{}) : types(false_type{});
 }
 
-// The launch over tiles: with sequences of more than one tile and a workspace that holds what tiles say, taken from the counter; else a block walks each (sequence, stripe).
+// The launch over tiles: with sequences of more than one tile and a workspace that holds what tiles say, taken from the counter; else a block walks (sequence, stripe) after
+// (sequence, stripe).
 template <bool BACKWARD>
 int tiles_launch(ScanParams& p, int max_len, void* workspace, int64_t workspace_bytes, cudaStream_t stream) {
-    constexpr int T = BACKWARD ? kBackwardRows : kForwardRows, threads = 32 * (BACKWARD ? kBackwardWarps : kForwardWarps);
-    const Layout at(p.channels, p.batch, p.rows, T);
-    p.stripes = (int)at.stripes;
-    const bool look = max_len > T && workspace != nullptr && workspace_bytes >= at.bytes;
+    const Layout at(p.channels, p.batch, p.rows);
     if (at.stripes * p.batch > 0x7fffffff || at.slots * at.stripes > 0x7fffffff) return kInvalid;
-    long long blocks = at.stripes * p.batch;
+    p.stripes = (int)at.stripes;
+    p.status = status_word();
+    if (p.status == nullptr) return (int)cudaErrorUnknown;
+    const bool look = max_len > kRows && workspace != nullptr && workspace_bytes >= at.bytes;
+    const bool gb = p.flags & GLM53F_KDA_SCAN_G_BF16, xb = p.flags & GLM53F_KDA_SCAN_X_BF16;
+    p.boxes = row_boxes(&p.tm_g, {p.g, p.g_stride, gb}, p.channels, p.rows) && row_boxes(&p.tm_x, {p.x, p.x_stride, xb}, p.channels, p.rows) &&
+              (!BACKWARD || row_boxes(&p.tm_dout, {p.dout, p.dout_stride, xb}, p.channels, p.rows));
+    p.tiles = at.stripes * p.batch;
     if (look) {
-        p.status = status_word();
-        if (p.status == nullptr) return (int)cudaErrorUnknown;
         auto* w = static_cast<unsigned char*>(workspace);
         p.control = reinterpret_cast<unsigned*>(w);
         p.records = reinterpret_cast<Record*>(w + at.records);
@@ -725,17 +870,16 @@ int tiles_launch(ScanParams& p, int max_len, void* workspace, int64_t workspace_
         const int rc = launch_early(scan_clear_kernel, dim3((unsigned)(clear < some ? clear : some)), 256, 0, stream, p);
         if (rc != 0) return rc;
     }
-    return with_types(p.flags, look, [&](auto l, auto gb, auto xb) {
-        constexpr bool L = decltype(l)::value, G = decltype(gb)::value, X = decltype(xb)::value;
-        auto launch = [&](auto kernel, size_t shared, int per_sm) {
+    const long long blocks = p.tiles < sm_count() ? p.tiles : sm_count();
+    return with_types(p.flags, look, [&](auto l, auto g_bf16, auto x_bf16) {
+        constexpr bool L = decltype(l)::value, G = decltype(g_bf16)::value, X = decltype(x_bf16)::value;
+        auto launch = [&](auto kernel, size_t shared) {
             const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
             if (e != cudaSuccess) return (int)e;
-            const long long most = (long long)per_sm * sm_count();
-            if (L) blocks = p.tiles < most ? p.tiles : most;
-            return launch_early(kernel, dim3((unsigned)blocks), threads, shared, stream, p);
+            return launch_early(kernel, dim3((unsigned)blocks), kThreads<L>, shared, stream, p);
         };
-        if constexpr (BACKWARD) return launch(scan_backward_kernel<L, G, X>, sizeof(BackwardShared<G, X>), X ? 3 : 2);
-        else return launch(scan_forward_kernel<L, G, X>, sizeof(ForwardShared<G, X>), 2);
+        if constexpr (BACKWARD) return launch(scan_backward_kernel<L, G, X>, sizeof(Shared<BackwardTile<G, X>>));
+        else return launch(scan_forward_kernel<L, G, X>, sizeof(Shared<ForwardTile<G, X>>));
     });
 }
 
@@ -750,11 +894,10 @@ bool state_ok(const void* state) { return state != nullptr && (reinterpret_cast<
 extern "C" int64_t glm53f_kda_scan_workspace_bytes(int32_t channels, int32_t batch, int32_t rows) {
     using namespace kda;
     if (channels < 1 || batch < 1 || rows < 0) return 0;
-    const Layout f(channels, batch, rows, kForwardRows), b(channels, batch, rows, kBackwardRows);
-    return f.bytes > b.bytes ? f.bytes : b.bytes;
+    return Layout(channels, batch, rows).bytes;
 }
 
-extern "C" int64_t glm53f_kda_scan_saves_rows(int32_t batch, int32_t rows) { return batch < 1 || rows < 0 ? 0 : (int64_t)rows / kda::kSave + batch; }
+extern "C" int64_t glm53f_kda_scan_saves_rows(int32_t batch, int32_t rows) { return batch < 1 || rows < 0 ? 0 : (int64_t)rows / kda::kRows + batch; }
 
 extern "C" int glm53f_kda_scan_decode_batch(int32_t channels, int32_t batch, const int32_t* cu_rows, const int32_t* keep, const void* g, int64_t g_stride,
                                             const void* x, int64_t x_stride, int32_t flags, const float* state_in, float* state_out, const int64_t* state_off,

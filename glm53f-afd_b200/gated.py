@@ -123,7 +123,7 @@ def _state_out(state, state_out, channels, max_state_off):
 
 
 def workspace_bytes(channels, batch, rows):
-    """The workspace with which `prefill_varlen` and `backward_varlen` divide sequences of more than 128 rows over the GPU."""
+    """The workspace with which `prefill_varlen` and `backward_varlen` divide sequences of more than 64 rows over the GPU."""
     return int(ffi.glm53f_kda_scan_workspace_bytes(channels, batch, rows))
 
 
