@@ -587,8 +587,7 @@ struct Forward {
     __device__ __forceinline__ void chain(const Place& at, TILE& t, int channel) {
         const int c = at.stripe * kChannels + channel;
         const bool ok = c < p.channels;
-        const long long off = p.state_off[at.b] + c;
-        float TA = 1.0f, TB = 0.0f, h = at.tile == 0 ? (ok ? p.state_in[off] : 0.0f) : walk;
+        float TA = 1.0f, TB = 0.0f, h = at.tile == 0 ? (ok ? p.state_in[p.state_off[at.b] + c] : 0.0f) : walk;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             const float2 ab = t.sums[w][channel];
@@ -597,7 +596,7 @@ struct Forward {
         if constexpr (LOOK) h = join<-1>(p, at.slot, at.stripe, channel, at.tile, TA, TB, h, at.tile + 1 < at.tiles);
         else walk = fmaf(TA, h, TB);
         if (p.saves != nullptr && ok) p.saves[(long long)at.slot * p.channels + c] = h;
-        if (at.n == 0 && ok) p.state_out[off] = h;
+        if (at.n == 0 && ok) p.state_out[p.state_off[at.b] + c] = h;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             const float2 ab = t.sums[w][channel];
@@ -613,19 +612,32 @@ struct Forward {
         float2 h = make_float2(s.x, s.z);
         Walk out(p.out, row, p.out_stride, c, kBytes<XB>);
         const bool vec = p.vec, write = p.out != nullptr;
+        // (The gates of all rows before the first store: the compiler moves no load from shared memory over a store, and a row would wait for the one before it.)
+        float2 a[kPer], b[kPer];
         with_flags(p.flags, [&](auto sigmoid, auto complement) {
             constexpr bool S = decltype(sigmoid)::value, C = decltype(complement)::value;
 #pragma unroll
-            for (int r = 0; r < kPer; ++r, out.at += out.step) {
-                float2 a, rest, b = t.x.get(w, r);
-                gate<S, C>(t.g.get(w, r), a, rest);
-                if constexpr (C) b = mul2(rest, b);
-                if (r < m) {
-                    h = fma2(a, h, b);
-                    if (write) store_pair<XB>(out.at, valid, vec, h.x, h.y);
-                }
+            for (int r = 0; r < kPer; ++r) {
+                float2 rest;
+                b[r] = t.x.get(w, r);
+                gate<S, C>(t.g.get(w, r), a[r], rest);
+                if constexpr (C) b[r] = mul2(rest, b[r]);
             }
         });
+        if (m == kPer && vec && valid > 0 && write) {
+#pragma unroll
+            for (int r = 0; r < kPer; ++r, out.at += out.step) {
+                h = fma2(a[r], h, b[r]);
+                store_pair<XB>(out.at, 2, true, h.x, h.y);
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < kPer; ++r, out.at += out.step) {
+                if (r >= m) break;
+                h = fma2(a[r], h, b[r]);
+                if (write) store_pair<XB>(out.at, valid, vec, h.x, h.y);
+            }
+        }
         if (at.tile * kRows + w * kPer + m == at.n) {
             float* to = p.state_out + p.state_off[at.b] + c;
             if (valid > 0) to[0] = h.x;
@@ -678,8 +690,7 @@ struct Backward {
         const int c = at.stripe * kChannels + channel;
         const bool ok = c < p.channels;
         float h = ok ? __ldg(p.saves + (long long)at.slot * p.channels + c) : 0.0f;
-        const long long off = p.state_off[at.b] + c;
-        float TA = 1.0f, TF = 0.0f, e = at.tile + 1 == at.tiles ? (ok && p.state_in != nullptr ? p.state_in[off] : 0.0f) : walk;
+        float TA = 1.0f, TF = 0.0f, e = at.tile + 1 == at.tiles ? (ok && p.state_in != nullptr ? p.state_in[p.state_off[at.b] + c] : 0.0f) : walk;
 #pragma unroll
         for (int w = kWarps - 1; w >= 0; --w) {
             const float a = t.sums[w][channel].x;
@@ -687,7 +698,7 @@ struct Backward {
         }
         if constexpr (LOOK) e = join<1>(p, at.slot, at.stripe, channel, at.tiles - 1 - at.tile, TA, TF, e, at.tile > 0);
         else walk = fmaf(TA, e, TF);
-        if (at.n == 0 && ok && p.state_out != nullptr) p.state_out[off] = e;
+        if (at.n == 0 && ok && p.state_out != nullptr) p.state_out[p.state_off[at.b] + c] = e;
         float A[kWarps];
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {

@@ -15,6 +15,8 @@
 #include "common.cuh"
 #include "glm53f_proj.h"
 #include "kda_internal.h"
+#include "tc.cuh"
+#include "tensor_map.cuh"
 
 namespace kda {
 namespace {
@@ -178,6 +180,285 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
     }
 }
 
+// ---- many rows ----------------------------------------------------------------------------------------------------------------
+// From nine rows on, a tcgen05 product: a tile is 128 weight rows (the M operand) x N rows of x.  Warps that widen turn the packed words into bf16 fragments and store
+// them into tensor memory, where a matrix instruction takes its first operand from: the packed layout is that of the fragments, so nothing is
+// shuffled and shared memory holds x only.  A group's products go into one of two accumulators of their own; warps that sum fetch each, multiply it
+// by the group's scales (a lane is a weight row) and add it to the f32 sums in their registers.  Roles of a block:
+//   warp 0        tensor copies of x (64 k x N rows, 128-byte swizzle) into a ring
+//   warp 1        the matrix instructions
+//   warps 4-7     widen, 128 k at a time, two such stages in tensor memory; their words are on the way one stage ahead
+//   warps 8-      sum: a warpgroup for each kSumCols columns (MT == 2: for each half of 256 weight rows)
+// Few tiles: the blocks of a cluster share a tile's k and add their sums, each for some rows, in rank order through distributed shared memory.
+
+enum : int { kStatusInt4Empty = 170, kStatusInt4Full = 171, kStatusInt4AEmpty = 172, kStatusInt4AFull = 173, kStatusInt4AccEmpty = 174, kStatusInt4AccFull = 175 };
+
+struct ManyParams {
+    CUtensorMap tm_x;
+    const uint4* codes;
+    const uint16_t* scales;
+    const uint16_t* zeros;  // or none
+    void* out;
+    long long ldo;
+    int rows, n, k, out_f32, group;
+    int tiles, pieces, groups;  // of 16 weight rows, of 64 k, of a row's scales
+    int m_tiles, split;         // tiles of weight rows; blocks that share a tile's k
+    int* status;
+};
+
+template <int N, int MT>
+struct Many {
+    static constexpr int kSumCols = MT == 2 ? N : N < 32 ? N : 32 * ((N + 63) / 64);  // (N = 128: 64)
+    static constexpr int kSumGroups = MT == 2 ? 2 : N / kSumCols;
+    static constexpr int kThreads = 256 + 128 * kSumGroups;
+    static constexpr int kBoxBytes = N * 128;
+    static constexpr int kRing = MT == 2 ? 6 : N <= 64 ? 6 : 8;
+    static constexpr int kStages = 2;                     // of 128 k in tensor memory
+    static constexpr int kStageCols = 64 * MT;
+    static constexpr int kAccCols = 2 * N;
+    static constexpr int kUsed = kAccCols + kStages * kStageCols;
+    static constexpr int kCols = kUsed <= 256 ? 256 : 512;
+    static constexpr int kBlocks = kCols == 256 ? 2 : 1;  // an SM
+    static constexpr int oBars = kRing * kBoxBytes;
+    static constexpr int oCtl = oBars + (2 * kRing + 2 * kStages + 4) * 8;
+    static constexpr int kBytes = oCtl + 32 + 1024;
+};
+
+__device__ __forceinline__ void tensor_load_2d(void* to, const void* tm, int x, int y, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(to)),
+                 "l"(reinterpret_cast<uint64_t>(tm)), "r"(smem_u32(bar)), "r"(x), "r"(y)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_meet() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float peer_load(const void* local, uint32_t rank) {
+    uint32_t at;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(local)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+
+template <int N, int MT>
+__global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) int4_many_kernel(const __grid_constant__ ManyParams p) {
+    using C = Many<N, MT>;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::oBars);
+    uint64_t *empty = full + C::kRing, *a_full = empty + C::kRing, *a_empty = a_full + C::kStages, *acc_full = a_empty + C::kStages, *acc_empty = acc_full + 2;
+    volatile uint32_t* ctl = reinterpret_cast<volatile uint32_t*>(smem + C::oCtl);
+    uint32_t* tmem_slot = const_cast<uint32_t*>(ctl) + 2;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int i = 0; i < C::kRing; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+        for (int i = 0; i < C::kStages; ++i) mbar_init(&a_full[i], 4), mbar_init(&a_empty[i], 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], MT == 2 ? 4 : 4 * C::kSumGroups);
+        ctl[0] = ctl[1] = 0u;
+        mbar_init_fence();
+    }
+    if (warp == 1) tc::tmem_alloc(tmem_slot, C::kCols);
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tm = *tmem_slot, stages0 = tm + C::kAccCols;
+    const WaitCtx ctx{ctl, ctl + 1, p.status};
+    const int split = p.split, part = split > 1 ? (int)cluster_rank() : 0, tile = (int)blockIdx.x / split;
+    const int mt = tile % p.m_tiles, row0 = tile / p.m_tiles * N;       // this block's weight rows (in units of 128 MT) and rows of x
+    const int per = p.pieces / split, piece0 = part * per, stages = (per + 1) / 2;
+    const int job_steps = p.group / 16;                                  // k steps of 16 of a group: 2, 4 or 8
+    grid_ready();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0;
+            uint32_t ph = 0;
+            for (int i = 0; i < per; ++i) {
+                if (!mbar_wait(&empty[s], ph ^ 1u, ctx, kStatusInt4Empty)) break;
+                mbar_arrive_expect_tx(&full[s], C::kBoxBytes);
+                tensor_load_2d(smem + s * C::kBoxBytes, &p.tm_x, (piece0 + i) * kPiece, row0, &full[s]);
+                if (++s == C::kRing) s = 0, ph ^= 1u;
+            }
+        }
+    } else if (warp == 1) {
+        constexpr uint32_t idesc = tc::idesc_bf16(128, N, 0, 0, 0);
+        const uint32_t leader = tc::elect_one();
+        int s = 0, job = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int st = 0; st < stages && ok; ++st) {
+            const int a = st % C::kStages, steps = min(per - 2 * st, 2) * 4;
+            if (!(ok = tc::warp_all(mbar_wait(&a_full[a], st / C::kStages & 1, ctx, kStatusInt4AFull)))) break;
+            // The x of the stage's pieces: ring places s and the next.
+            int at[2], have = 0;
+            for (int step0 = 0; step0 < steps && ok; step0 += job_steps) {
+                while (have * 4 < step0 + job_steps && have * 4 < steps) {
+                    if (!(ok = tc::warp_all(mbar_wait(&full[s], ph, ctx, kStatusInt4Full)))) break;
+                    at[have & 1] = s;
+                    ++have;
+                    if (++s == C::kRing) s = 0, ph ^= 1u;
+                }
+                for (int m = 0; m < MT && ok; ++m, ++job) {
+                    const int buf = job & 1;
+                    if (!(ok = tc::warp_all(mbar_wait(&acc_empty[buf], (job >> 1 & 1) ^ 1u, ctx, kStatusInt4AccEmpty)))) break;
+                    tc::fence_after_sync();
+                    for (int i = 0; i < job_steps; ++i) {
+                        const int step = step0 + i;
+                        const unsigned char* x = smem + (step < 4 ? at[0] : at[1]) * C::kBoxBytes;
+                        tc::mma_bf16_ts_if(leader, tm + buf * N, stages0 + a * C::kStageCols + m * 64 + step * 8, tc::desc_sw128_kmajor(x, N, 16 * (step & 3)), idesc, i > 0);
+                    }
+                    tc::mma_commit_if(leader, &acc_full[buf]);
+                }
+            }
+            if (!ok) break;
+            tc::mma_commit_if(leader, &a_empty[a]);
+            for (int i = 0; i < have; ++i) tc::mma_commit_if(leader, &empty[at[i]]);
+            if (leader) ctl[0] = ctl[0] + 1u;
+        }
+    } else if (warp >= 4 && warp < 8) {
+        // Weight rows 32 q .. of each 128: two tiles of 16, the lanes' words of both pieces of a stage.
+        const int q = warp & 3, g = lane >> 2;
+        uint4 next[2][MT][2];
+        auto load = [&](int st) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const int w = (mt * MT + m) * 8 + q * 2 + t, piece = 2 * st + i;
+                        next[i][m][t] = w < p.tiles && piece < per ? __ldcs(p.codes + ((long long)w * p.pieces + piece0 + piece) * 32 + lane) : make_uint4(0u, 0u, 0u, 0u);
+                    }
+        };
+        load(0);
+        for (int st = 0; st < stages; ++st) {
+            const int a = st % C::kStages, pieces = min(per - 2 * st, 2);
+            uint4 now[2][MT][2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) now[i][m][t] = next[i][m][t];
+            if (st + 1 < stages) load(st + 1);
+            if (!tc::warp_all(mbar_wait(&a_empty[a], (st / C::kStages & 1) ^ 1u, ctx, kStatusInt4AEmpty))) break;
+            tc::fence_after_sync();
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (i >= pieces) break;
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const int w = (mt * MT + m) * 8 + q * 2 + t;
+                        const uint32_t words[4] = {now[i][m][t].x, now[i][m][t].y, now[i][m][t].z, now[i][m][t].w};
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {  // 32 k: their group's zero points
+                            uint32_t lo = 0x43084308u, hi = 0x43084308u;
+                            if (p.zeros != nullptr && w < p.tiles) {
+                                const uint32_t z = __ldg(p.zeros + ((long long)w * p.groups + ((piece0 + 2 * st + i) * kPiece + 32 * h) / p.group) * 8 + g);
+                                lo = 0x43004300u | (z & 0xffu) * 0x00010001u, hi = 0x43004300u | (z >> 8) * 0x00010001u;
+                            }
+                            uint32_t f[4], e[4];
+                            widen(words[2 * h], lo, hi, f);
+                            widen(words[2 * h + 1], lo, hi, e);
+                            const uint32_t r[8] = {f[0], f[1], f[2], f[3], e[0], e[1], e[2], e[3]};
+                            tc::tmem_st_pairs(stages0 + a * C::kStageCols + m * 64 + i * 32 + h * 16 + ((uint32_t)(q * 32 + t * 16) << 16), r);
+                        }
+                    }
+            }
+            tc::tmem_st_wait();
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&a_full[a]);
+        }
+    } else if (warp >= 8) {
+        const int sg = (warp - 8) >> 2, q = warp & 3, m = MT == 2 ? sg : 0, col0 = MT == 2 ? 0 : sg * C::kSumCols;
+        const int w = (mt * MT + m) * 8 + q * 2 + (lane >> 4);  // this lane's tile of 16 weight rows
+        const int o = ((mt * MT + m) * 128) + q * 32 + lane;
+        const bool there = w < p.tiles;
+        const uint16_t* scale = p.scales + ((long long)(there ? w : 0) * p.groups * 8 + (lane & 7)) * 2 + (lane >> 3 & 1);
+        const int group0 = piece0 * kPiece / p.group, jobs = per * kPiece / p.group;
+        float sum[C::kSumCols];
+#pragma unroll
+        for (int c = 0; c < C::kSumCols; ++c) sum[c] = 0.0f;
+        // Scales four groups ahead: a group of 32 k takes less time than a load.
+        uint16_t ahead[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) ahead[u] = there && u < jobs ? __ldg(scale + (long long)(group0 + u) * 16) : 0;
+        bool ok = true;
+        for (int j = 0; j < jobs && ok; j += 4) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (j + u >= jobs || !ok) continue;
+                const int i = j + u, buf = MT == 2 ? m : i & 1;
+                const float s = bf16_bits_to_f32(ahead[u]);
+                ahead[u] = there && i + 4 < jobs ? __ldg(scale + (long long)(group0 + i + 4) * 16) : 0;
+                if (!(ok = tc::warp_all(mbar_wait(&acc_full[buf], MT == 2 ? i & 1 : i >> 1 & 1, ctx, kStatusInt4AccFull)))) continue;
+                tc::fence_after_sync();
+                const float2 s2 = make_float2(s, s);
+#pragma unroll
+                for (int c0 = 0; c0 < C::kSumCols; c0 += 16) {
+                    uint32_t r[16];
+                    tc::tmem_ld16(tc::tmem_addr(tm, q, buf * N + col0 + c0), r);
+                    tc::tmem_ld_wait();
+#pragma unroll
+                    for (int c = 0; c < 16; c += 2) {
+                        const float2 v = fma2(s2, make_float2(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), make_float2(sum[c0 + c], sum[c0 + c + 1]));
+                        sum[c0 + c] = v.x, sum[c0 + c + 1] = v.y;
+                    }
+                }
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&acc_empty[buf]);
+            }
+        }
+        auto store = [&](int c, float v) {
+            const long long r = row0 + c;
+            if (o < p.n && r < p.rows) {
+                if (p.out_f32) static_cast<float*>(p.out)[r * p.ldo + o] = v;
+                else static_cast<uint16_t*>(p.out)[r * p.ldo + o] = f32_to_bf16_bits(v);
+            }
+        };
+        if (split == 1) {
+            if (ok)
+#pragma unroll
+                for (int c = 0; c < C::kSumCols; ++c) store(col0 + c, sum[c]);
+        } else {
+            // x has been read; its ring takes the sums, [N][128].
+            float* red = reinterpret_cast<float*>(smem);
+#pragma unroll
+            for (int c = 0; c < C::kSumCols; ++c) red[(col0 + c) * 128 + q * 32 + lane] = sum[c];
+        }
+    }
+    if (ctl[1]) {  // after a wait that gave up, copies into this block's shared memory may still be in flight: a bounded time for them
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 2000000ull) {
+        }
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    if (warp == 1) tc::tmem_dealloc(tm, C::kCols);
+    if (split > 1) {
+        cluster_meet();
+        const float* red = reinterpret_cast<const float*>(smem);
+        const int mine = N / split;
+        for (int e = tid; e < mine * 128; e += C::kThreads) {
+            const int c = part * mine + e / 128, f = e % 128, o = mt * 128 + f;
+            const long long r = row0 + c;
+            if (o >= p.n || r >= p.rows) continue;
+            float v = 0.0f;
+            for (int b = 0; b < split; ++b) v += peer_load(red + c * 128 + f, b);
+            if (p.out_f32) static_cast<float*>(p.out)[r * p.ldo + o] = v;
+            else static_cast<uint16_t*>(p.out)[r * p.ldo + o] = f32_to_bf16_bits(v);
+        }
+        cluster_meet();
+    }
+}
+
 // A thread a word of the packed weight, or a group's pair of scales and zero points.
 __global__ void int4_pack_kernel(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int n, int k, int group, uint32_t* to, uint32_t* to_scales,
                                  uint16_t* to_zeros) {
@@ -224,6 +505,44 @@ int few_launch(const Int4Params& p, unsigned blocks, int shared, cudaStream_t st
     return launch_early(int4_few_kernel<G, ZEROS>, dim3(blocks), kFewThreads, shared, stream, p);
 }
 
+template <int N, int MT>
+int many_launch(ManyParams& p, const uint16_t* x, long long ldx, cudaStream_t stream) {
+    using C = Many<N, MT>;
+    EncodeTiled enc = encode_tiled();
+    if (enc == nullptr) return (int)cudaErrorNotSupported;
+    const cuuint64_t dims[2] = {(cuuint64_t)p.k, (cuuint64_t)p.rows}, strides[1] = {(cuuint64_t)ldx * 2};
+    const cuuint32_t box[2] = {kPiece, N}, estr[2] = {1u, 1u};
+    if (enc(&p.tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<uint16_t*>(x), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return (int)cudaErrorNotSupported;
+    p.m_tiles = (p.n + 128 * MT - 1) / (128 * MT);
+    const long long tiles = (long long)p.m_tiles * ((p.rows + N - 1) / N), room = (long long)sm_count() * C::kBlocks;
+    p.split = 1;
+    if (MT == 1)  // parts of k for the blocks of a cluster, of whole stages and groups, while all blocks run at once
+        for (int s = 8; s > 1 && p.split == 1; s /= 2)
+            if (p.pieces % (2 * s) == 0 && p.pieces / s >= 4 && tiles * s <= room) p.split = s;
+    if (tiles * p.split > 0x7fffffff) return kInvalid;
+    cudaError_t e = cudaFuncSetAttribute(int4_many_kernel<N, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes);
+    if (e != cudaSuccess) return (int)e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(tiles * p.split));
+    cfg.blockDim = dim3(C::kThreads);
+    cfg.dynamicSmemBytes = C::kBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    unsigned na = early_attribute(attr[0]);
+    if (p.split > 1) {
+        attr[na].id = cudaLaunchAttributeClusterDimension;
+        attr[na].val.clusterDim.x = (unsigned)p.split;
+        attr[na].val.clusterDim.y = 1;
+        attr[na].val.clusterDim.z = 1;
+        ++na;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = na;
+    return (int)cudaLaunchKernelEx(&cfg, int4_many_kernel<N, MT>, p);
+}
+
 }  // namespace
 }  // namespace kda
 
@@ -253,6 +572,20 @@ extern "C" int32_t glm53f_kda_proj_int4(const uint16_t* x, int64_t ldx, const vo
     const Int4Layout at(n, k, group, zeros != 0);
     if (at.tiles > 0x3fffffff) return kInvalid;
     const auto* w = static_cast<const unsigned char*>(packed);
+    if (rows > kFewRows) {
+        ManyParams m{};
+        m.codes = reinterpret_cast<const uint4*>(w), m.scales = reinterpret_cast<const uint16_t*>(w + at.scales);
+        m.zeros = zeros ? reinterpret_cast<const uint16_t*>(w + at.zeros) : nullptr;
+        m.out = out, m.ldo = ldo, m.rows = rows, m.n = n, m.k = k, m.out_f32 = out_f32 != 0, m.group = group;
+        m.tiles = (int)at.tiles, m.pieces = (int)at.pieces, m.groups = (int)at.groups;
+        m.status = status_word();
+        if (m.status == nullptr) return (int)cudaErrorUnknown;
+        const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+        if (rows <= 16) return many_launch<16, 1>(m, x, ldx, s);
+        if (rows <= 32) return many_launch<32, 1>(m, x, ldx, s);
+        if (rows <= 64) return many_launch<64, 1>(m, x, ldx, s);
+        return many_launch<128, 1>(m, x, ldx, s);
+    }
     Int4Params p{};
     p.ldx = ldx, p.ldo = ldo, p.n = n, p.k = k, p.out_f32 = out_f32 != 0;
     p.codes = reinterpret_cast<const uint4*>(w), p.scales = reinterpret_cast<const uint32_t*>(w + at.scales), p.zeros = reinterpret_cast<const uint16_t*>(w + at.zeros);
