@@ -269,7 +269,6 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
     const int split = p.split, part = split > 1 ? (int)cluster_rank() : 0, tile = (int)blockIdx.x / split;
     const int mt = tile % p.m_tiles, row0 = tile / p.m_tiles * N;       // this block's weight rows (in units of 128 MT) and rows of x
     const int per = p.pieces / split, piece0 = part * per, stages = (per + 1) / 2;
-    const int job_steps = p.group / 16;                                  // k steps of 16 of a group: 2, 4 or 8
     grid_ready();
 
     if (warp == 0) {
@@ -286,42 +285,52 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
     } else if (warp == 1) {
         constexpr uint32_t idesc = tc::idesc_bf16(128, N, 0, 0, 0);
         const uint32_t leader = tc::elect_one();
-        int s = 0, job = 0;
-        uint32_t ph = 0;
-        bool ok = true;
-        for (int st = 0; st < stages && ok; ++st) {
-            const int a = st % C::kStages, steps = min(per - 2 * st, 2) * 4;
-            if (!(ok = tc::warp_all(mbar_wait(&a_full[a], st / C::kStages & 1, ctx, kStatusInt4AFull)))) break;
-            // The x of the stage's pieces: ring places s and the next.
-            int at[2], have = 0;
-            for (int step0 = 0; step0 < steps && ok; step0 += job_steps) {
-                while (have * 4 < step0 + job_steps && have * 4 < steps) {
-                    if (!(ok = tc::warp_all(mbar_wait(&full[s], ph, ctx, kStatusInt4Full)))) break;
-                    at[have & 1] = s;
-                    ++have;
+        // The warp converged, one lane issuing, a stage's eight k steps unrolled for the group's size: little stands between two instructions (a loop that asks at each step
+        // whether a group begins or ends took 190 cycles a step, three times the product's).  Of a descriptor only the low half changes.
+        auto products = [&](auto group_steps) {
+            constexpr int js = decltype(group_steps)::value;  // k steps of 16 of a group
+            constexpr uint64_t high = (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61 | (uint64_t)(16 >> 4) << 16;
+            const uint32_t ring0 = (smem_u32(smem) & 0x3FFFFu) >> 4;
+            int s = 0, job = 0;
+            uint32_t ph = 0;
+            for (int st = 0; st < stages; ++st) {
+                const int a = st % C::kStages;
+                const uint32_t w = stages0 + (uint32_t)(a * C::kStageCols);
+                if (!tc::warp_all(mbar_wait(&a_full[a], st / C::kStages & 1, ctx, kStatusInt4AFull))) return;
+#pragma unroll
+                for (int piece = 0; piece < 2; ++piece) {
+                    if (piece == 1 && 2 * st + 1 == per) break;
+                    if (!tc::warp_all(mbar_wait(&full[s], ph, ctx, kStatusInt4Full))) return;
+                    const uint64_t x = high | (ring0 + (uint32_t)(s * (C::kBoxBytes >> 4)));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int step = piece * 4 + i;
+                        const uint32_t buf = job & 1;
+                        if (step % js == 0) {
+                            if (!tc::warp_all(mbar_wait(&acc_empty[buf], (job >> 1 & 1) ^ 1u, ctx, kStatusInt4AccEmpty))) return;
+                            tc::fence_after_sync();
+                        }
+                        tc::mma_bf16_ts_if(leader, tm + buf * N, w + step * 8, x + 2 * i, idesc, step % js != 0);
+                        if (step % js == js - 1) {
+                            tc::mma_commit_if(leader, &acc_full[buf]);
+                            ++job;
+                        }
+                    }
+                    tc::mma_commit_if(leader, &empty[s]);
                     if (++s == C::kRing) s = 0, ph ^= 1u;
                 }
-                for (int m = 0; m < MT && ok; ++m, ++job) {
-                    const int buf = job & 1;
-                    if (!(ok = tc::warp_all(mbar_wait(&acc_empty[buf], (job >> 1 & 1) ^ 1u, ctx, kStatusInt4AccEmpty)))) break;
-                    tc::fence_after_sync();
-                    for (int i = 0; i < job_steps; ++i) {
-                        const int step = step0 + i;
-                        const unsigned char* x = smem + (step < 4 ? at[0] : at[1]) * C::kBoxBytes;
-                        tc::mma_bf16_ts_if(leader, tm + buf * N, stages0 + a * C::kStageCols + m * 64 + step * 8, tc::desc_sw128_kmajor(x, N, 16 * (step & 3)), idesc, i > 0);
-                    }
-                    tc::mma_commit_if(leader, &acc_full[buf]);
-                }
+                tc::mma_commit_if(leader, &a_empty[a]);
+                if (leader) ctl[0] = ctl[0] + 1u;
             }
-            if (!ok) break;
-            tc::mma_commit_if(leader, &a_empty[a]);
-            for (int i = 0; i < have; ++i) tc::mma_commit_if(leader, &empty[at[i]]);
-            if (leader) ctl[0] = ctl[0] + 1u;
-        }
+        };
+        if (p.group == 128) products(std::integral_constant<int, 8>{});
+        else if (p.group == 64) products(std::integral_constant<int, 4>{});
+        else products(std::integral_constant<int, 2>{});
     } else if (warp >= 4 && warp < 8) {
         // Weight rows 32 q .. of each 128: two tiles of 16, the lanes' words of both pieces of a stage.
         const int q = warp & 3, g = lane >> 2;
         uint4 next[2][MT][2];
+        uint32_t zero[2][MT][2];  // of a piece's two halves of 32 k, 16 bits each
         auto load = [&](int st) {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -330,19 +339,28 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
                         const int w = (mt * MT + m) * 8 + q * 2 + t, piece = 2 * st + i;
-                        next[i][m][t] = w < p.tiles && piece < per ? __ldcs(p.codes + ((long long)w * p.pieces + piece0 + piece) * 32 + lane) : make_uint4(0u, 0u, 0u, 0u);
+                        const bool ok = w < p.tiles && piece < per;
+                        next[i][m][t] = ok ? __ldcs(p.codes + ((long long)w * p.pieces + piece0 + piece) * 32 + lane) : make_uint4(0u, 0u, 0u, 0u);
+                        zero[i][m][t] = 0x08080808u;
+                        if (p.zeros != nullptr && ok) {
+                            const int k0 = (piece0 + piece) * kPiece;
+                            const uint16_t* z = p.zeros + (long long)w * p.groups * 8 + g;
+                            const uint32_t z0 = __ldg(z + k0 / p.group * 8);
+                            zero[i][m][t] = z0 | (p.group == 32 ? (uint32_t)__ldg(z + (k0 / 32 + 1) * 8) : z0) << 16;
+                        }
                     }
         };
         load(0);
         for (int st = 0; st < stages; ++st) {
             const int a = st % C::kStages, pieces = min(per - 2 * st, 2);
             uint4 now[2][MT][2];
+            uint32_t now_zero[2][MT][2];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) now[i][m][t] = next[i][m][t];
+                    for (int t = 0; t < 2; ++t) now[i][m][t] = next[i][m][t], now_zero[i][m][t] = zero[i][m][t];
             if (st + 1 < stages) load(st + 1);
             if (!tc::warp_all(mbar_wait(&a_empty[a], (st / C::kStages & 1) ^ 1u, ctx, kStatusInt4AEmpty))) break;
             tc::fence_after_sync();
@@ -353,15 +371,10 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
-                        const int w = (mt * MT + m) * 8 + q * 2 + t;
                         const uint32_t words[4] = {now[i][m][t].x, now[i][m][t].y, now[i][m][t].z, now[i][m][t].w};
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {  // 32 k: their group's zero points
-                            uint32_t lo = 0x43084308u, hi = 0x43084308u;
-                            if (p.zeros != nullptr && w < p.tiles) {
-                                const uint32_t z = __ldg(p.zeros + ((long long)w * p.groups + ((piece0 + 2 * st + i) * kPiece + 32 * h) / p.group) * 8 + g);
-                                lo = 0x43004300u | (z & 0xffu) * 0x00010001u, hi = 0x43004300u | (z >> 8) * 0x00010001u;
-                            }
+                            const uint32_t z = now_zero[i][m][t] >> (16 * h), lo = 0x43004300u | (z & 0xffu) * 0x00010001u, hi = 0x43004300u | (z >> 8 & 0xffu) * 0x00010001u;
                             uint32_t f[4], e[4];
                             widen(words[2 * h], lo, hi, f);
                             widen(words[2 * h + 1], lo, hi, e);
