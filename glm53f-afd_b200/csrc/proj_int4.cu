@@ -187,8 +187,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
 // by the group's scales (a lane is a weight row) and add it to the f32 sums in their registers.  Roles of a block:
 //   warp 0        tensor copies of x (64 k x N rows, 128-byte swizzle) into a ring
 //   warp 1        the matrix instructions
-//   warps 4-7     widen, 128 k at a time, two such stages in tensor memory; their words are on the way one stage ahead
-//   warps 8-      sum: a warpgroup for each kSumCols columns (MT == 2: for each half of 256 weight rows)
+//   warps 4-      widen, 128 k at a time, two such stages in tensor memory; their words are on the way one stage ahead
+//   the others    sum: a warpgroup for each kSumCols columns (MT == 2: for each half of 256 weight rows)
 // Few tiles: the blocks of a cluster share a tile's k and add their sums, each for some rows, in rank order through distributed shared memory.
 
 enum : int { kStatusInt4Empty = 170, kStatusInt4Full = 171, kStatusInt4AEmpty = 172, kStatusInt4AFull = 173, kStatusInt4AccEmpty = 174, kStatusInt4AccFull = 175 };
@@ -210,7 +210,9 @@ template <int N, int MT>
 struct Many {
     static constexpr int kSumCols = MT == 2 ? N : N < 32 ? N : 32 * ((N + 63) / 64);  // (N = 128: 64)
     static constexpr int kSumGroups = MT == 2 ? 2 : N / kSumCols;
-    static constexpr int kThreads = 256 + 128 * kSumGroups;
+    static constexpr int kWideners = N <= 64 ? 1 : 2;     // warpgroups that widen, a stage each in turn (of small tiles two blocks share an SM)
+    static constexpr int kSumWarp = 4 + 4 * kWideners;    // the first warp that sums
+    static constexpr int kThreads = 32 * kSumWarp + 128 * kSumGroups;
     static constexpr int kBoxBytes = N * 128;
     static constexpr int kRing = MT == 2 ? 6 : N <= 64 ? 6 : 8;
     static constexpr int kStages = 2;                     // of 128 k in tensor memory
@@ -326,9 +328,9 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
         if (p.group == 128) products(std::integral_constant<int, 8>{});
         else if (p.group == 64) products(std::integral_constant<int, 4>{});
         else products(std::integral_constant<int, 2>{});
-    } else if (warp >= 4 && warp < 8) {
+    } else if (warp >= 4 && warp < C::kSumWarp) {
         // Weight rows 32 q .. of each 128: two tiles of 16, the lanes' words of both pieces of a stage.
-        const int q = warp & 3, g = lane >> 2;
+        const int q = warp & 3, g = lane >> 2, turn = (warp - 4) >> 2;
         uint4 next[2][MT][2];
         uint32_t zero[2][MT][2];  // of a piece's two halves of 32 k, 16 bits each
         auto load = [&](int st) {
@@ -350,8 +352,8 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
                         }
                     }
         };
-        load(0);
-        for (int st = 0; st < stages; ++st) {
+        load(turn);
+        for (int st = turn; st < stages; st += C::kWideners) {
             const int a = st % C::kStages, pieces = min(per - 2 * st, 2);
             uint4 now[2][MT][2];
             uint32_t now_zero[2][MT][2];
@@ -361,7 +363,7 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
                     for (int t = 0; t < 2; ++t) now[i][m][t] = next[i][m][t], now_zero[i][m][t] = zero[i][m][t];
-            if (st + 1 < stages) load(st + 1);
+            if (st + C::kWideners < stages) load(st + C::kWideners);
             if (!tc::warp_all(mbar_wait(&a_empty[a], (st / C::kStages & 1) ^ 1u, ctx, kStatusInt4AEmpty))) break;
             tc::fence_after_sync();
 #pragma unroll
@@ -388,8 +390,8 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
             __syncwarp();
             if (lane == 0) mbar_arrive(&a_full[a]);
         }
-    } else if (warp >= 8) {
-        const int sg = (warp - 8) >> 2, q = warp & 3, m = MT == 2 ? sg : 0, col0 = MT == 2 ? 0 : sg * C::kSumCols;
+    } else if (warp >= C::kSumWarp) {
+        const int sg = (warp - C::kSumWarp) >> 2, q = warp & 3, m = MT == 2 ? sg : 0, col0 = MT == 2 ? 0 : sg * C::kSumCols;
         const int w = (mt * MT + m) * 8 + q * 2 + (lane >> 4);  // this lane's tile of 16 weight rows
         const int o = ((mt * MT + m) * 128) + q * 32 + lane;
         const bool there = w < p.tiles;
