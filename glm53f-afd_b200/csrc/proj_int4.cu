@@ -187,11 +187,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
 // by the group's scales (a lane is a weight row) and add it to the f32 sums in their registers.  Roles of a block:
 //   warp 0        tensor copies of x (64 k x N rows, 128-byte swizzle) into a ring
 //   warp 1        the matrix instructions
-//   warps 4-      widen, 128 k at a time, two such stages in tensor memory; their words are on the way one stage ahead
+//   warp 2        bulk copies of the packed words, 128 k at a time, into another
+//   warps 4-      widen, 128 k at a time, two such stages in tensor memory
 //   the others    sum: a warpgroup for each kSumCols columns (MT == 2: for each half of 256 weight rows)
 // Few tiles: the blocks of a cluster share a tile's k and add their sums, each for some rows, in rank order through distributed shared memory.
 
-enum : int { kStatusInt4Empty = 170, kStatusInt4Full = 171, kStatusInt4AEmpty = 172, kStatusInt4AFull = 173, kStatusInt4AccEmpty = 174, kStatusInt4AccFull = 175 };
+enum : int { kStatusInt4Empty = 170, kStatusInt4Full = 171, kStatusInt4AEmpty = 172, kStatusInt4AFull = 173, kStatusInt4AccEmpty = 174, kStatusInt4AccFull = 175, kStatusInt4Words = 176, kStatusInt4WordsFull = 177 };
 
 struct ManyParams {
     CUtensorMap tm_x;
@@ -213,16 +214,19 @@ struct Many {
     static constexpr int kWideners = N <= 64 ? 1 : 2;     // warpgroups that widen, a stage each in turn (of small tiles two blocks share an SM)
     static constexpr int kSumWarp = 4 + 4 * kWideners;    // the first warp that sums
     static constexpr int kThreads = 32 * kSumWarp + 128 * kSumGroups;
-    static constexpr int kBoxBytes = N * 128;
-    static constexpr int kRing = MT == 2 ? 6 : N <= 64 ? 6 : 8;
-    static constexpr int kStages = 2;                     // of 128 k in tensor memory
+    static constexpr int kBoxBytes = N * 128;             // 64 k of x
+    static constexpr int kRing = N <= 32 ? 6 : 4;         // stages of 128 k: of x
+    static constexpr int kStages = 2;                     // ... in tensor memory
     static constexpr int kStageCols = 64 * MT;
     static constexpr int kAccCols = 2 * N;
     static constexpr int kUsed = kAccCols + kStages * kStageCols;
     static constexpr int kCols = kUsed <= 256 ? 256 : 512;
     static constexpr int kBlocks = kCols == 256 ? 2 : 1;  // an SM
-    static constexpr int oBars = kRing * kBoxBytes;
-    static constexpr int oCtl = oBars + (2 * kRing + 2 * kStages + 4) * 8;
+    static constexpr int kWords = N <= 32 ? 6 : 4;        // stages of packed words in shared memory
+    static constexpr int kWordBytes = 8 * MT * 1024;      // of a stage: two pieces of 8 MT tiles
+    static constexpr int oWords = kRing * 2 * kBoxBytes;
+    static constexpr int oBars = oWords + kWords * kWordBytes;
+    static constexpr int oCtl = oBars + (2 * kRing + 2 * kWords + 2 * kStages + 4) * 8;
     static constexpr int kBytes = oCtl + 32 + 1024;
 };
 
@@ -251,12 +255,13 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::oBars);
-    uint64_t *empty = full + C::kRing, *a_full = empty + C::kRing, *a_empty = a_full + C::kStages, *acc_full = a_empty + C::kStages, *acc_empty = acc_full + 2;
+    uint64_t *empty = full + C::kRing, *w_full = empty + C::kRing, *w_empty = w_full + C::kWords, *a_full = w_empty + C::kWords, *a_empty = a_full + C::kStages, *acc_full = a_empty + C::kStages, *acc_empty = acc_full + 2;
     volatile uint32_t* ctl = reinterpret_cast<volatile uint32_t*>(smem + C::oCtl);
     uint32_t* tmem_slot = const_cast<uint32_t*>(ctl) + 2;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < C::kRing; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+        for (int i = 0; i < C::kWords; ++i) mbar_init(&w_full[i], 1), mbar_init(&w_empty[i], 4);
         for (int i = 0; i < C::kStages; ++i) mbar_init(&a_full[i], 4), mbar_init(&a_empty[i], 1);
         for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], MT == 2 ? 4 : 4 * C::kSumGroups);
         ctl[0] = ctl[1] = 0u;
@@ -277,62 +282,83 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
         if (lane == 0) {
             int s = 0;
             uint32_t ph = 0;
-            for (int i = 0; i < per; ++i) {
+            for (int st = 0; st < stages; ++st) {
+                const int pieces = min(per - 2 * st, 2);
                 if (!mbar_wait(&empty[s], ph ^ 1u, ctx, kStatusInt4Empty)) break;
-                mbar_arrive_expect_tx(&full[s], C::kBoxBytes);
-                tensor_load_2d(smem + s * C::kBoxBytes, &p.tm_x, (piece0 + i) * kPiece, row0, &full[s]);
+                mbar_arrive_expect_tx(&full[s], pieces * C::kBoxBytes);
+                for (int i = 0; i < pieces; ++i)
+                    tensor_load_2d(smem + (2 * s + i) * C::kBoxBytes, &p.tm_x, (piece0 + 2 * st + i) * kPiece, row0, &full[s]);
                 if (++s == C::kRing) s = 0, ph ^= 1u;
             }
+        }
+    } else if (warp == 2) {
+        // A lane a tile of 16 weight rows: the words of its two pieces lie together.
+        const int w = mt * MT * 8 + lane;
+        const bool mine = lane < 8 * MT && w < p.tiles;
+        const uint32_t tiles = __popc(__ballot_sync(0xffffffffu, mine));
+        const unsigned char* from = reinterpret_cast<const unsigned char*>(p.codes) + ((long long)w * p.pieces + piece0) * 512;
+        int c = 0;
+        uint32_t ph = 0;
+        for (int st = 0; st < stages; ++st) {
+            const int pieces = min(per - 2 * st, 2);
+            if (!tc::warp_all(mbar_wait(&w_empty[c], ph ^ 1u, ctx, kStatusInt4Words))) break;
+            if (lane == 0) mbar_arrive_expect_tx(&w_full[c], tiles * pieces * 512);
+            __syncwarp();
+            if (mine) bulk_load(smem + C::oWords + c * C::kWordBytes + lane * 1024, from + st * 1024, pieces * 512, &w_full[c]);
+            if (++c == C::kWords) c = 0, ph ^= 1u;
         }
     } else if (warp == 1) {
         constexpr uint32_t idesc = tc::idesc_bf16(128, N, 0, 0, 0);
         const uint32_t leader = tc::elect_one();
         // The warp converged, one lane issuing, a stage's eight k steps unrolled for the group's size: little stands between two instructions (a loop that asks at each step
-        // whether a group begins or ends took 190 cycles a step, three times the product's).  Of a descriptor only the low half changes.
-        auto products = [&](auto group_steps) {
+        // whether a group begins or ends took 190 cycles a step, three times the product's).  Of a descriptor only the low half changes, and where the tensor
+        // memory begins is a constant, so that every operand is computed in uniform registers.
+        auto products = [&](auto group_steps, auto begin) {
             constexpr int js = decltype(group_steps)::value;  // k steps of 16 of a group
+            constexpr uint32_t tm0 = decltype(begin)::value, stage0 = tm0 + C::kAccCols;
             constexpr uint64_t high = (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61 | (uint64_t)(16 >> 4) << 16;
             const uint32_t ring0 = (smem_u32(smem) & 0x3FFFFu) >> 4;
             int s = 0, job = 0;
             uint32_t ph = 0;
             for (int st = 0; st < stages; ++st) {
                 const int a = st % C::kStages;
-                const uint32_t w = stages0 + (uint32_t)(a * C::kStageCols);
+                const uint32_t w = stage0 + (uint32_t)(a * C::kStageCols);
+                const bool whole = 2 * st + 1 < per;
+                if (!tc::warp_all(mbar_wait(&full[s], ph, ctx, kStatusInt4Full))) return;
                 if (!tc::warp_all(mbar_wait(&a_full[a], st / C::kStages & 1, ctx, kStatusInt4AFull))) return;
+                const uint64_t x = high | (ring0 + (uint32_t)(s * 2 * (C::kBoxBytes >> 4)));
 #pragma unroll
-                for (int piece = 0; piece < 2; ++piece) {
-                    if (piece == 1 && 2 * st + 1 == per) break;
-                    if (!tc::warp_all(mbar_wait(&full[s], ph, ctx, kStatusInt4Full))) return;
-                    const uint64_t x = high | (ring0 + (uint32_t)(s * (C::kBoxBytes >> 4)));
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int step = piece * 4 + i;
-                        const uint32_t buf = job & 1;
-                        if (step % js == 0) {
-                            if (!tc::warp_all(mbar_wait(&acc_empty[buf], (job >> 1 & 1) ^ 1u, ctx, kStatusInt4AccEmpty))) return;
-                            tc::fence_after_sync();
-                        }
-                        tc::mma_bf16_ts_if(leader, tm + buf * N, w + step * 8, x + 2 * i, idesc, step % js != 0);
-                        if (step % js == js - 1) {
-                            tc::mma_commit_if(leader, &acc_full[buf]);
-                            ++job;
-                        }
+                for (int step = 0; step < 8; ++step) {
+                    if (step == 4 && !whole) break;
+                    const uint32_t buf = job & 1;
+                    if (step % js == 0) {
+                        if (!tc::warp_all(mbar_wait(&acc_empty[buf], (job >> 1 & 1) ^ 1u, ctx, kStatusInt4AccEmpty))) return;
+                        tc::fence_after_sync();
                     }
-                    tc::mma_commit_if(leader, &empty[s]);
-                    if (++s == C::kRing) s = 0, ph ^= 1u;
+                    tc::mma_bf16_ts_if(leader, tm0 + buf * N, w + step * 8, x + (step / 4) * (C::kBoxBytes >> 4) + 2 * (step % 4), idesc, step % js != 0);
+                    if (step % js == js - 1) {
+                        tc::mma_commit_if(leader, &acc_full[buf]);
+                        ++job;
+                    }
                 }
                 tc::mma_commit_if(leader, &a_empty[a]);
+                tc::mma_commit_if(leader, &empty[s]);
+                if (++s == C::kRing) s = 0, ph ^= 1u;
                 if (leader) ctl[0] = ctl[0] + 1u;
             }
         };
-        if (p.group == 128) products(std::integral_constant<int, 8>{});
-        else if (p.group == 64) products(std::integral_constant<int, 4>{});
-        else products(std::integral_constant<int, 2>{});
+        auto from = [&](auto begin) {
+            if (p.group == 128) products(std::integral_constant<int, 8>{}, begin);
+            else if (p.group == 64) products(std::integral_constant<int, 4>{}, begin);
+            else products(std::integral_constant<int, 2>{}, begin);
+        };
+        // (All 512 columns begin at 0; 256 at 0 or 256.)
+        if (C::kCols == 512 || tm == 0) from(std::integral_constant<uint32_t, 0>{});
+        else from(std::integral_constant<uint32_t, 256>{});
     } else if (warp >= 4 && warp < C::kSumWarp) {
         // Weight rows 32 q .. of each 128: two tiles of 16, the lanes' words of both pieces of a stage.
         const int q = warp & 3, g = lane >> 2, turn = (warp - 4) >> 2;
-        uint4 next[2][MT][2];
-        uint32_t zero[2][MT][2];  // of a piece's two halves of 32 k, 16 bits each
+        uint32_t zero[2][MT][2];  // zero points of a piece's two halves of 32 k, 16 bits each: one stage ahead
         auto load = [&](int st) {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -341,10 +367,8 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
                         const int w = (mt * MT + m) * 8 + q * 2 + t, piece = 2 * st + i;
-                        const bool ok = w < p.tiles && piece < per;
-                        next[i][m][t] = ok ? __ldcs(p.codes + ((long long)w * p.pieces + piece0 + piece) * 32 + lane) : make_uint4(0u, 0u, 0u, 0u);
                         zero[i][m][t] = 0x08080808u;
-                        if (p.zeros != nullptr && ok) {
+                        if (p.zeros != nullptr && w < p.tiles && piece < per) {
                             const int k0 = (piece0 + piece) * kPiece;
                             const uint16_t* z = p.zeros + (long long)w * p.groups * 8 + g;
                             const uint32_t z0 = __ldg(z + k0 / p.group * 8);
@@ -354,16 +378,24 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
         };
         load(turn);
         for (int st = turn; st < stages; st += C::kWideners) {
-            const int a = st % C::kStages, pieces = min(per - 2 * st, 2);
-            uint4 now[2][MT][2];
+            const int a = st % C::kStages, c = st % C::kWords, pieces = min(per - 2 * st, 2);
             uint32_t now_zero[2][MT][2];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) now[i][m][t] = next[i][m][t], now_zero[i][m][t] = zero[i][m][t];
+                    for (int t = 0; t < 2; ++t) now_zero[i][m][t] = zero[i][m][t];
             if (st + C::kWideners < stages) load(st + C::kWideners);
+            if (!tc::warp_all(mbar_wait(&w_full[c], st / C::kWords & 1, ctx, kStatusInt4WordsFull))) break;
+            uint4 now[2][MT][2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+                        now[i][m][t] = *reinterpret_cast<const uint4*>(smem + C::oWords + c * C::kWordBytes + (m * 8 + q * 2 + t) * 1024 + i * 512 + lane * 16);
             if (!tc::warp_all(mbar_wait(&a_empty[a], (st / C::kStages & 1) ^ 1u, ctx, kStatusInt4AEmpty))) break;
             tc::fence_after_sync();
 #pragma unroll
@@ -388,7 +420,7 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
             tc::tmem_st_wait();
             tc::fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&a_full[a]);
+            if (lane == 0) mbar_arrive(&a_full[a]), mbar_arrive(&w_empty[c]);
         }
     } else if (warp >= C::kSumWarp) {
         const int sg = (warp - C::kSumWarp) >> 2, q = warp & 3, m = MT == 2 ? sg : 0, col0 = MT == 2 ? 0 : sg * C::kSumCols;
