@@ -64,11 +64,23 @@ __device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
     asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
-// The fragments of one k step: rows i (even registers) and i + 8, less lo and hi (128 + z in both halves).
-__device__ __forceinline__ void widen(uint32_t w, uint32_t lo, uint32_t hi, uint32_t (&a)[4]) {
+// The fragments of one k step: rows i (even registers) and i + 8, less lo and hi (128 + z in both halves).  The mask and the exponent come in registers: an
+// instruction takes one constant, and with two the compiler makes two of it.
+struct Widen {
+    uint32_t mask, exponent;
+    __device__ __forceinline__ Widen() {
+        asm volatile("mov.b32 %0, 0x000f000f;" : "=r"(mask));
+        asm volatile("mov.b32 %0, 0x43004300;" : "=r"(exponent));
+    }
+    __device__ __forceinline__ void operator()(uint32_t w, uint32_t lo, uint32_t hi, uint32_t (&a)[4]) const {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) a[j] = sub_bf16x2(((w >> (4 * j)) & 0x000f000fu) | 0x43004300u, j % 2 ? hi : lo);
-}
+        for (int j = 0; j < 4; ++j) {
+            uint32_t r;
+            asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w >> (4 * j)), "r"(mask), "r"(exponent));  // (w & mask) | exponent
+            a[j] = sub_bf16x2(r, j % 2 ? hi : lo);
+        }
+    }
+};
 
 // A piece on its way: its codes, the scales of its groups and their zero points.
 template <int G, bool ZEROS>
@@ -92,6 +104,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
     const int groups = p.k / G, g = lane >> 2;
     grid_ready();
 
+    const Widen widen;
     // The next piece to load: its tile and place there.
     int ltile = tile0, li = 0;
     auto load = [&](P& x) {
@@ -216,9 +229,10 @@ struct Many {
     static constexpr int kThreads = 32 * kSumWarp + 128 * kSumGroups;
     static constexpr int kBoxBytes = N * 128;             // 64 k of x
     static constexpr int kRing = N <= 32 ? 6 : 4;         // stages of 128 k: of x
-    static constexpr int kStages = 2;                     // ... in tensor memory
+    static constexpr int kStages = N == 128 ? 4 : N == 64 ? 2 : 3;  // ... in tensor memory
     static constexpr int kStageCols = 64 * MT;
-    static constexpr int kAccCols = 2 * N;
+    static constexpr int kAccs = 2;                       // accumulators, a group's products each
+    static constexpr int kAccCols = kAccs * N;
     static constexpr int kUsed = kAccCols + kStages * kStageCols;
     static constexpr int kCols = kUsed <= 256 ? 256 : 512;
     static constexpr int kBlocks = kCols == 256 ? 2 : 1;  // an SM
@@ -226,7 +240,7 @@ struct Many {
     static constexpr int kWordBytes = 8 * MT * 1024;      // of a stage: two pieces of 8 MT tiles
     static constexpr int oWords = kRing * 2 * kBoxBytes;
     static constexpr int oBars = oWords + kWords * kWordBytes;
-    static constexpr int oCtl = oBars + (2 * kRing + 2 * kWords + 2 * kStages + 4) * 8;
+    static constexpr int oCtl = oBars + (2 * kRing + 2 * kWords + 2 * kStages + 2 * kAccs) * 8;
     static constexpr int kBytes = oCtl + 32 + 1024;
 };
 
@@ -256,7 +270,7 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::oBars);
-    uint64_t *empty = full + C::kRing, *w_full = empty + C::kRing, *w_empty = w_full + C::kWords, *a_full = w_empty + C::kWords, *a_empty = a_full + C::kStages, *acc_full = a_empty + C::kStages, *acc_empty = acc_full + 2;
+    uint64_t *empty = full + C::kRing, *w_full = empty + C::kRing, *w_empty = w_full + C::kWords, *a_full = w_empty + C::kWords, *a_empty = a_full + C::kStages, *acc_full = a_empty + C::kStages, *acc_empty = acc_full + C::kAccs;
     volatile uint32_t* ctl = reinterpret_cast<volatile uint32_t*>(smem + C::oCtl);
     uint32_t* tmem_slot = const_cast<uint32_t*>(ctl) + 2;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -264,7 +278,7 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
         for (int i = 0; i < C::kRing; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
         for (int i = 0; i < C::kWords; ++i) mbar_init(&w_full[i], 1), mbar_init(&w_empty[i], 4);
         for (int i = 0; i < C::kStages; ++i) mbar_init(&a_full[i], 4), mbar_init(&a_empty[i], 1);
-        for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], MT == 2 ? 4 : 4 * C::kSumGroups);
+        for (int i = 0; i < C::kAccs; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], 4 * C::kSumGroups);
         ctl[0] = ctl[1] = 0u;
         mbar_init_fence();
     }
@@ -319,8 +333,8 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
             constexpr uint32_t tm0 = decltype(begin)::value, stage0 = tm0 + C::kAccCols;
             constexpr uint64_t high = (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61 | (uint64_t)(16 >> 4) << 16;
             const uint32_t ring0 = (smem_u32(smem) & 0x3FFFFu) >> 4;
-            int s = 0, job = 0;
-            uint32_t ph = 0;
+            int s = 0, buf = 0;
+            uint32_t ph = 0, acc_ph = 1;
             for (int st = 0; st < stages; ++st) {
                 const int a = st % C::kStages;
                 const uint32_t w = stage0 + (uint32_t)(a * C::kStageCols);
@@ -331,15 +345,14 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
 #pragma unroll
                 for (int step = 0; step < 8; ++step) {
                     if (step == 4 && !whole) break;
-                    const uint32_t buf = job & 1;
                     if (step % js == 0) {
-                        if (!tc::warp_all(mbar_wait(&acc_empty[buf], (job >> 1 & 1) ^ 1u, ctx, kStatusInt4AccEmpty))) return;
+                        if (!tc::warp_all(mbar_wait(&acc_empty[buf], acc_ph, ctx, kStatusInt4AccEmpty))) return;
                         tc::fence_after_sync();
                     }
-                    tc::mma_bf16_ts_if(leader, tm0 + buf * N, w + step * 8, x + (step / 4) * (C::kBoxBytes >> 4) + 2 * (step % 4), idesc, step % js != 0);
+                    tc::mma_bf16_ts_if(leader, tm0 + (uint32_t)(buf * N), w + step * 8, x + (step / 4) * (C::kBoxBytes >> 4) + 2 * (step % 4), idesc, step % js != 0);
                     if (step % js == js - 1) {
                         tc::mma_commit_if(leader, &acc_full[buf]);
-                        ++job;
+                        if (++buf == C::kAccs) buf = 0, acc_ph ^= 1u;
                     }
                 }
                 tc::mma_commit_if(leader, &a_empty[a]);
@@ -358,6 +371,7 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
         else from(std::integral_constant<uint32_t, 256>{});
     } else if (warp >= 4 && warp < C::kSumWarp) {
         // Weight rows 32 q .. of each 128: two tiles of 16, the lanes' words of both pieces of a stage.
+        const Widen widen;
         const int q = warp & 3, g = lane >> 2, turn = (warp - 4) >> 2;
         uint32_t zero[2][MT][2];  // zero points of a piece's two halves of 32 k, 16 bits each: one stage ahead
         auto load = [&](int st) {
@@ -442,30 +456,36 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
 #pragma unroll
         for (int u = 0; u < 4; ++u) ahead[u] = there && u < jobs ? __ldg(scale + (long long)(group0 + u) * 16) : 0;
         bool ok = true;
+        int buf = 0;
+        uint32_t ph = 0;
         for (int j = 0; j < jobs && ok; j += 4) {
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 if (j + u >= jobs || !ok) continue;
-                const int i = j + u, buf = MT == 2 ? m : i & 1;
+                const int i = j + u;
                 const float s = bf16_bits_to_f32(ahead[u]);
                 ahead[u] = there && i + 4 < jobs ? __ldg(scale + (long long)(group0 + i + 4) * 16) : 0;
-                if (!(ok = tc::warp_all(mbar_wait(&acc_full[buf], MT == 2 ? i & 1 : i >> 1 & 1, ctx, kStatusInt4AccFull)))) continue;
+                if (!(ok = tc::warp_all(mbar_wait(&acc_full[buf], ph, ctx, kStatusInt4AccFull)))) continue;
                 tc::fence_after_sync();
                 const float2 s2 = make_float2(s, s);
+                constexpr int W = 16;
 #pragma unroll
-                for (int c0 = 0; c0 < C::kSumCols; c0 += 16) {
-                    uint32_t r[16];
+                for (int c0 = 0; c0 < C::kSumCols; c0 += W) {
+                    uint32_t r[W];
                     tc::tmem_ld16(tc::tmem_addr(tm, q, buf * N + col0 + c0), r);
                     tc::tmem_ld_wait();
+                    if (c0 + W == C::kSumCols) {  // the accumulator is free as soon as its last columns are in registers
+                        tc::fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&acc_empty[buf]);
+                    }
 #pragma unroll
-                    for (int c = 0; c < 16; c += 2) {
+                    for (int c = 0; c < W; c += 2) {
                         const float2 v = fma2(s2, make_float2(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), make_float2(sum[c0 + c], sum[c0 + c + 1]));
                         sum[c0 + c] = v.x, sum[c0 + c + 1] = v.y;
                     }
                 }
-                tc::fence_before_sync();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&acc_empty[buf]);
+                if (++buf == C::kAccs) buf = 0, ph ^= 1u;
             }
         }
         auto store = [&](int c, float v) {
