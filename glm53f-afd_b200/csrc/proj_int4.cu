@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
 // shuffled and shared memory holds x only.  A group's products go into one of two accumulators of their own; warps that sum fetch each, multiply it
 // by the group's scales (a lane is a weight row) and add it to the f32 sums in their registers.  Roles of a block:
 //   warp 0        tensor copies of x (64 k x N rows, 128-byte swizzle) into a ring
-//   warp 1        the matrix instructions
+//   warps 1, 3    the matrix instructions (a stage each in turn, with groups of 128: the waits of a stage take one warp longer than its products the tensor cores)
 //   warp 2        bulk copies of the packed words, 128 k at a time, into another
 //   warps 4-      widen, 128 k at a time, two such stages in tensor memory
 //   the others    sum: a warpgroup for each kSumCols columns (MT == 2: for each half of 256 weight rows)
@@ -229,7 +229,7 @@ struct Many {
     static constexpr int kThreads = 32 * kSumWarp + 128 * kSumGroups;
     static constexpr int kBoxBytes = N * 128;             // 64 k of x
     static constexpr int kRing = N <= 32 ? 6 : 4;         // stages of 128 k: of x
-    static constexpr int kStages = N == 128 ? 4 : N == 64 ? 2 : 3;  // ... in tensor memory
+    static constexpr int kStages = N == 128 ? 4 : 2;      // ... in tensor memory (even, as the rings are: each of two warps that take turns then meets every phase of a place)
     static constexpr int kStageCols = 64 * MT;
     static constexpr int kAccs = 2;                       // accumulators, a group's products each
     static constexpr int kAccCols = kAccs * N;
@@ -299,7 +299,8 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
             uint32_t ph = 0;
             for (int st = 0; st < stages; ++st) {
                 const int pieces = min(per - 2 * st, 2);
-                if (!mbar_wait(&empty[s], ph ^ 1u, ctx, kStatusInt4Empty)) break;
+                if (!mbar_wait(C::kRing != C::kStages ? &empty[s] : &a_empty[s], ph ^ 1u, ctx, kStatusInt4Empty)) break;
+                ctl[0] = ctl[0] + 1u;
                 mbar_arrive_expect_tx(&full[s], pieces * C::kBoxBytes);
                 for (int i = 0; i < pieces; ++i)
                     tensor_load_2d(smem + (2 * s + i) * C::kBoxBytes, &p.tm_x, (piece0 + 2 * st + i) * kPiece, row0, &full[s]);
@@ -322,7 +323,7 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
             if (mine) bulk_load(smem + C::oWords + c * C::kWordBytes + lane * 1024, from + st * 1024, pieces * 512, &w_full[c]);
             if (++c == C::kWords) c = 0, ph ^= 1u;
         }
-    } else if (warp == 1) {
+    } else if (warp == 1 || warp == 3) {
         constexpr uint32_t idesc = tc::idesc_bf16(128, N, 0, 0, 0);
         const uint32_t leader = tc::elect_one();
         // The warp converged, one lane issuing, a stage's eight k steps unrolled for the group's size: little stands between two instructions (a loop that asks at each step
@@ -333,32 +334,29 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
             constexpr uint32_t tm0 = decltype(begin)::value, stage0 = tm0 + C::kAccCols;
             constexpr uint64_t high = (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61 | (uint64_t)(16 >> 4) << 16;
             const uint32_t ring0 = (smem_u32(smem) & 0x3FFFFu) >> 4;
-            int s = 0, buf = 0;
-            uint32_t ph = 0, acc_ph = 1;
-            for (int st = 0; st < stages; ++st) {
-                const int a = st % C::kStages;
+            // With groups of 128 two warps take turns, each with an accumulator of its own; smaller groups use both within a stage, and a wait tells two of an accumulator's phases
+            // apart, not three: one warp.
+            constexpr int turns = js == 8 ? 2 : 1;
+            for (int st = warp >> 1; st < stages && warp >> 1 < turns; st += turns) {
+                const int a = st % C::kStages, s = st % C::kRing;
                 const uint32_t w = stage0 + (uint32_t)(a * C::kStageCols);
                 const bool whole = 2 * st + 1 < per;
-                if (!tc::warp_all(mbar_wait(&full[s], ph, ctx, kStatusInt4Full))) return;
+                if (!tc::warp_all(mbar_wait(&full[s], st / C::kRing & 1, ctx, kStatusInt4Full))) return;
                 if (!tc::warp_all(mbar_wait(&a_full[a], st / C::kStages & 1, ctx, kStatusInt4AFull))) return;
                 const uint64_t x = high | (ring0 + (uint32_t)(s * 2 * (C::kBoxBytes >> 4)));
 #pragma unroll
                 for (int step = 0; step < 8; ++step) {
                     if (step == 4 && !whole) break;
+                    const int job = st * (8 / js) + step / js, buf = job & 1;
                     if (step % js == 0) {
-                        if (!tc::warp_all(mbar_wait(&acc_empty[buf], acc_ph, ctx, kStatusInt4AccEmpty))) return;
+                        if (!tc::warp_all(mbar_wait(&acc_empty[buf], (job >> 1 & 1) ^ 1u, ctx, kStatusInt4AccEmpty))) return;
                         tc::fence_after_sync();
                     }
                     tc::mma_bf16_ts_if(leader, tm0 + (uint32_t)(buf * N), w + step * 8, x + (step / 4) * (C::kBoxBytes >> 4) + 2 * (step % 4), idesc, step % js != 0);
-                    if (step % js == js - 1) {
-                        tc::mma_commit_if(leader, &acc_full[buf]);
-                        if (++buf == C::kAccs) buf = 0, acc_ph ^= 1u;
-                    }
+                    if (step % js == js - 1) tc::mma_commit_if(leader, &acc_full[buf]);
                 }
                 tc::mma_commit_if(leader, &a_empty[a]);
-                tc::mma_commit_if(leader, &empty[s]);
-                if (++s == C::kRing) s = 0, ph ^= 1u;
-                if (leader) ctl[0] = ctl[0] + 1u;
+                if (C::kRing != C::kStages) tc::mma_commit_if(leader, &empty[s]);
             }
         };
         auto from = [&](auto begin) {
@@ -456,16 +454,14 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
 #pragma unroll
         for (int u = 0; u < 4; ++u) ahead[u] = there && u < jobs ? __ldg(scale + (long long)(group0 + u) * 16) : 0;
         bool ok = true;
-        int buf = 0;
-        uint32_t ph = 0;
         for (int j = 0; j < jobs && ok; j += 4) {
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 if (j + u >= jobs || !ok) continue;
-                const int i = j + u;
+                const int i = j + u, buf = i & 1;
                 const float s = bf16_bits_to_f32(ahead[u]);
                 ahead[u] = there && i + 4 < jobs ? __ldg(scale + (long long)(group0 + i + 4) * 16) : 0;
-                if (!(ok = tc::warp_all(mbar_wait(&acc_full[buf], ph, ctx, kStatusInt4AccFull)))) continue;
+                if (!(ok = tc::warp_all(mbar_wait(&acc_full[buf], i >> 1 & 1, ctx, kStatusInt4AccFull)))) continue;
                 tc::fence_after_sync();
                 const float2 s2 = make_float2(s, s);
                 constexpr int W = 16;
@@ -485,7 +481,6 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
                         sum[c0 + c] = v.x, sum[c0 + c + 1] = v.y;
                     }
                 }
-                if (++buf == C::kAccs) buf = 0, ph ^= 1u;
             }
         }
         auto store = [&](int c, float v) {
