@@ -3,7 +3,7 @@
 // With t_j = (x_j - max x) / T and S = sum of e^t_j: log p_j = t_j - log S, entropy = log S - (sum of e^t_j t_j) / S.  Backwards, from the gradients
 // l of the token's log probability and n of the entropy H: dx_j = (l ([j = token] - p_j) - n p_j (log p_j + H)) / T.
 //
-// Bound by HBM: a row is read once (one exponential, 2/3 of what the units give at bf16 logits, and some ten other operations a value).  Every warp keeps
+// Bound by HBM and the operations next to it: a row is read once (one exponential, 2/3 of what the units give at bf16 logits, and five or six instructions a value, in pairs).  Every warp keeps
 // its running maximum, its lanes their sums against it, so that the maxima need no pass of their own; blocks of a cluster that share a row meet
 // in distributed shared memory.  No scratch in global memory; the same bits every time.
 //
@@ -21,13 +21,11 @@
 namespace kda {
 namespace {
 
-constexpr int kWarps = 16, kThreads = 32 * kWarps;
 constexpr int kGroups = 128;
 constexpr int kMostTop = 32;
 constexpr int kPieces = 2048;     // of a block's part of a row
 constexpr int kCandidates = 512;  // of a block's part; kMostBlocks * kMostTop at least
 constexpr int kMostBlocks = 8;    // of a row
-constexpr int kAtOnce = 4;        // pieces of a warp in flight
 constexpr int kMostVocab = 2000000;  // (kMostBlocks * kPieces pieces hold 2,097,152 f32 logits)
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -52,14 +50,16 @@ struct Entry {
 };
 __device__ __forceinline__ bool before(const Entry& a, const Entry& b) { return a.v > b.v || (a.v == b.v && a.id < b.id); }
 
+template <int WARPS>
 struct Shared {
     float piece[kPieces];
     Entry candidate[kCandidates];
-    float group[kThreads];
+    int ahead[kCandidates];
+    alignas(16) float group[32 * WARPS];
     Entry best[kMostTop];  // this block's, read by the row's first block
     float max, sum, sum_t;
-    float wmax[kWarps], wsum[kWarps], wsum_t[kWarps];
-    Entry wbest[kWarps];
+    float wmax[WARPS], wsum[WARPS], wsum_t[WARPS];
+    Entry wbest[WARPS];
     float bound;
     int candidates;
 };
@@ -144,29 +144,14 @@ __device__ __forceinline__ float largest(const uint4& r) {  // (of numbers; NaN 
     }
 }
 
+// t = (x - m) log2(e) / T: the difference first, so that the largest logit's t is 0 itself, and no size of x or T does harm.
+// Stands for -inf where maximum and temperature are ordinary (`plain`): finite times finite, so that no 0 meets an infinity.  (A bf16 value.)
+constexpr float kFloor = -9.969209968386869e29f;
+__device__ __forceinline__ bool plain(float m, float c) { return c >= 1e-6f && c <= 1e6f && (m == -INFINITY || fabsf(m) <= 1e29f); }
+
 // Sums of e^t and e^t t against the maximum m, in powers of two.
 struct Sums {
     float m = -INFINITY, s = 0.0f, w = 0.0f;
-    __device__ __forceinline__ void raise(float to, float c) {  // to > m
-        const float d = (m - to) * c;
-        if (m == -INFINITY) {
-            m = to;
-            return;
-        }
-        const float f = ex2_ftz(d), dd = fmaxf(d, -1000.0f);
-        w = f * fmaf(s, dd, w), s *= f;
-        m = to;
-    }
-    template <bool BF16>
-    __device__ __forceinline__ void add(const uint4& r, float c) {
-        const float from = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-        for (int j = 0; j < Row<BF16>::E; ++j) {
-            // (-inf: e^t is 0, and stays 0 times t; a NaN stays one)
-            const float t = max_nan((value<BF16>(r, j) - from) * c, -1000.0f), e = ex2_ftz(t);
-            s += e, w = fmaf(e, t, w);
-        }
-    }
     __device__ __forceinline__ void join(float om, float os, float ow, float c) {
         if (om > m) {
             const float keep_s = s, keep_w = w, keep_m = m;
@@ -181,21 +166,83 @@ struct Sums {
         s = fmaf(os, f, s), w = fmaf(f, fmaf(os, dd, ow), w);
     }
 };
-
-// Among n entries, those that fewer than k come before, to their places.
-__device__ __forceinline__ void rank(const Entry* all, int n, int k, Entry* best) {
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-        const Entry mine = all[i];
-        int ahead = 0;
-        for (int j = 0; j < n; ++j) ahead += before(all[j], mine);
-        if (ahead < k) best[ahead] = mine;
+// A lane's, of values in pairs.
+struct LaneSums {
+    float m = -INFINITY;
+    float2 s = {0.0f, 0.0f}, w = {0.0f, 0.0f};
+    __device__ __forceinline__ void raise(float to, float c) {  // to > m
+        if (m != -INFINITY) {
+            const float d = (m - to) * c, f = ex2_ftz(d), dd = fmaxf(d, -1000.0f);
+            w = mul2(make_float2(f, f), fma2(s, make_float2(dd, dd), w)), s = mul2(make_float2(f, f), s);
+        }
+        m = to;
     }
+    template <bool BF16>
+    __device__ __forceinline__ void add_plain(uint4 r, float c) {
+        uint32_t* u = reinterpret_cast<uint32_t*>(&r);
+        const float from = m == -INFINITY ? 0.0f : -m;
+        const float2 c2 = make_float2(c, c), minus = make_float2(from, from);
+#pragma unroll
+        for (int j = 0; j < Row<BF16>::E / 2; ++j) {
+            float2 x;
+            if constexpr (BF16) {
+                asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(u[j]) : "r"(0xf149f149u));
+                x = make_float2(__uint_as_float(u[j] << 16), __uint_as_float(u[j] & 0xffff0000u));
+            } else {
+                x = make_float2(max_nan(__uint_as_float(u[2 * j]), kFloor), max_nan(__uint_as_float(u[2 * j + 1]), kFloor));
+            }
+            const float2 t = mul2(add2(x, minus), c2), e = make_float2(ex2_ftz(t.x), ex2_ftz(t.y));
+            s = add2(s, e), w = fma2(e, t, w);
+        }
+    }
+    template <bool BF16>
+    __device__ __forceinline__ void add(const uint4& r, float c) {
+        const float from = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int j = 0; j < Row<BF16>::E; ++j) {
+            // (-inf: e^t is 0, and stays 0 times t; a NaN stays one)
+            const float t = max_nan((value<BF16>(r, j) - from) * c, -1000.0f), e = ex2_ftz(t);
+            s.x += e, w.x = fmaf(e, t, w.x);
+        }
+    }
+};
+
+// The sums of the first `lanes` (a power of two) lanes together, in pairs (a fixed order), in every lane.
+__device__ __forceinline__ void join_lanes(Sums& x, int lanes, float c) {
+    for (int d = 1; d < lanes; d *= 2) {
+        const float m = __shfl_xor_sync(0xffffffffu, x.m, d), s = __shfl_xor_sync(0xffffffffu, x.s, d), w = __shfl_xor_sync(0xffffffffu, x.w, d);
+        x.join(m, s, w, c);
+    }
+    x.m = __shfl_sync(0xffffffffu, x.m, 0), x.s = __shfl_sync(0xffffffffu, x.s, 0), x.w = __shfl_sync(0xffffffffu, x.w, 0);
 }
 
-template <bool BF16>
-__global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobParams p) {
-    constexpr int E = Row<BF16>::E;
-    __shared__ Shared sh;
+// Among n entries, those that fewer than k come before, to their places.  By the whole block, several threads an entry, a part of the others each.
+template <int WARPS>
+__device__ __forceinline__ void rank(Shared<WARPS>& sh, int n, int k) {
+    constexpr int kThreads = 32 * WARPS;
+    int parts = 1;
+    while (parts < 32 && 2 * parts * n <= kThreads) parts *= 2;
+    for (int i = threadIdx.x; i < n; i += kThreads) sh.ahead[i] = 0;
+    __syncthreads();
+    for (int e = threadIdx.x; e < n * parts; e += kThreads) {
+        const int i = e / parts, part = e % parts;
+        const Entry mine = sh.candidate[i];
+        int ahead = 0;
+#pragma unroll 4
+        for (int j = part; j < n; j += parts) ahead += before(sh.candidate[j], mine);
+        if (parts == 1) sh.ahead[i] = ahead;
+        else if (ahead != 0) atomicAdd(&sh.ahead[i], ahead);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads)
+        if (sh.ahead[i] < k) sh.best[sh.ahead[i]] = sh.candidate[i];
+}
+
+// Few rows: blocks of sixteen warps, a round of loads each.  Many: of eight, of which an SM holds four, so that no row waits for another's last step.
+template <bool BF16, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 2) logprob_kernel(const LogprobParams p) {
+    constexpr int E = Row<BF16>::E, kThreads = 32 * WARPS, kWarps = WARPS, kAtOnce = WARPS == 8 ? 8 : 4;  // pieces of a warp in flight
+    __shared__ Shared<WARPS> sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int part = blockIdx.x % p.blocks;
     const long long row = blockIdx.x / p.blocks;
@@ -208,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobParam
     if (tid == 0) sh.candidates = 0;
     if (p.top > 0 && tid < kMostTop) sh.best[tid] = Entry{-INFINITY, -1};
 
-    Sums mine;  // m: the warp's; s, w: the lane's
+    LaneSums mine;  // m: the warp's
     float most = -INFINITY;
     for (int i = first + warp; i < last; i += kWarps * kAtOnce) {
         uint4 r[kAtOnce];
@@ -231,17 +278,23 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobParam
             for (int u = 0; u < kAtOnce; ++u)
                 if (i + u * kWarps < last) sh.piece[i + u * kWarps - first] = top[u];
         if (up > mine.m) mine.raise(up, c);
+        if (plain(mine.m, c)) {
 #pragma unroll
-        for (int u = 0; u < kAtOnce; ++u) mine.add<BF16>(r[u], c);
+            for (int u = 0; u < kAtOnce; ++u) mine.add_plain<BF16>(r[u], c);
+        } else {
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) mine.add<BF16>(r[u], c);
+        }
     }
-    mine.s = warp_sum(mine.s), mine.w = warp_sum(mine.w);
-    if (lane == 0) sh.wmax[warp] = mine.m, sh.wsum[warp] = mine.s, sh.wsum_t[warp] = mine.w;
+    const float sum = warp_sum(mine.s.x + mine.s.y), sum_t = warp_sum(mine.w.x + mine.w.y);
+    if (lane == 0) sh.wmax[warp] = mine.m, sh.wsum[warp] = sum, sh.wsum_t[warp] = sum_t;
     sh.group[tid] = most;
     __syncthreads();
-    if (tid == 0) {
+    if (warp == kWarps - 1) {
         Sums all;
-        for (int w = 0; w < kWarps; ++w) all.join(sh.wmax[w], sh.wsum[w], sh.wsum_t[w], c);
-        sh.max = all.m, sh.sum = all.s, sh.sum_t = all.w;
+        if (lane < kWarps) all.m = sh.wmax[lane], all.s = sh.wsum[lane], all.w = sh.wsum_t[lane];
+        join_lanes(all, kWarps, c);
+        if (lane == 0) sh.max = all.m, sh.sum = all.s, sh.sum_t = all.w;
     }
     if (p.top > 0) {
         const int k = p.top;
@@ -254,32 +307,48 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobParam
         if (tid < kGroups) sh.group[tid] = g;
         __syncthreads();
         if (tid < kGroups) {
-            int ahead = 0;
-            for (int j = 0; j < kGroups; ++j) ahead += sh.group[j] > g || (sh.group[j] == g && j < tid);
-            if (ahead == k - 1) sh.bound = g;
+            // (g is the k-th largest where fewer than k are larger and at least k no smaller)
+            int larger = 0, no_smaller = 0;
+#pragma unroll 8
+            for (int j = 0; j < kGroups; j += 4) {
+                const float4 o = *reinterpret_cast<const float4*>(sh.group + j);
+                larger += (o.x > g) + (o.y > g) + (o.z > g) + (o.w > g);
+                no_smaller += (o.x >= g) + (o.y >= g) + (o.z >= g) + (o.w >= g);
+            }
+            if (larger < k && no_smaller >= k) sh.bound = g;
         }
         __syncthreads();
         const float bound = sh.bound;
-        for (int i = warp * 32; i < last - first; i += kThreads) {
-            const float has = i + lane < last - first ? sh.piece[i + lane] : -INFINITY;
+        // A warp looks at pieces warp, warp + kWarps, ..., as it read them: a lane a piece, then the lanes a piece together, two of them at a time.
+        for (int i = warp; i < last - first; i += 32 * kWarps) {
+            const int at = i + lane * kWarps;
+            const float has = at < last - first ? sh.piece[at] : -INFINITY;
             uint32_t hits = __ballot_sync(0xffffffffu, has >= bound && has > -INFINITY);
             while (hits != 0) {
-                const int u = __ffs(hits) - 1;
-                hits &= hits - 1;
-                const long long at = (long long)(first + i + u) * 32 + lane;
-                const uint4 r = x.load(at);
+                long long piece[2];
+                uint4 r[2];
 #pragma unroll
-                for (int j = 0; j < E; ++j) {
-                    const float v = value<BF16>(r, j);
-                    if (!(v >= bound && v > -INFINITY)) continue;
-                    const int to = atomicAdd(&sh.candidates, 1);
-                    if (to < kCandidates) sh.candidate[to] = Entry{v, (int)(at * E + j - x.skip)};
+                for (int u = 0; u < 2; ++u) {
+                    piece[u] = hits != 0 ? (long long)(first + i + (__ffs(hits) - 1) * kWarps) * 32 + lane : x.end;
+                    hits &= hits - 1;
+                    r[u] = x.load(piece[u]);
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    if (!(largest<BF16>(r[u]) >= bound)) continue;
+#pragma unroll
+                    for (int j = 0; j < E; ++j) {
+                        const float v = value<BF16>(r[u], j);
+                        if (!(v >= bound && v > -INFINITY)) continue;
+                        const int to = atomicAdd(&sh.candidates, 1);
+                        if (to < kCandidates) sh.candidate[to] = Entry{v, (int)(piece[u] * E + j - x.skip)};
+                    }
                 }
             }
         }
         __syncthreads();
         if (sh.candidates <= kCandidates) {
-            rank(sh.candidate, sh.candidates, k, sh.best);
+            rank(sh, sh.candidates, k);
         } else {
             // The next entry of the order, k times over the part.
             Entry bar{INFINITY, -1};
@@ -321,14 +390,18 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobParam
             __syncthreads();
             if (tid < kMostTop) sh.best[tid] = Entry{-INFINITY, -1};
             __syncthreads();
-            rank(sh.candidate, p.blocks * p.top, p.top, sh.best);  // (empty places come behind; equal ones among them keep theirs)
+            rank(sh, p.blocks * p.top, p.top);  // (empty places come behind; equal ones among them keep theirs)
             __syncthreads();
         }
         if (warp == 0) {
             Sums all;
-            all.m = sh.max, all.s = sh.sum, all.w = sh.sum_t;
-            for (int b = 1; b < p.blocks; ++b)
-                all.join(cluster_load(cluster_place(&sh.max, b)), cluster_load(cluster_place(&sh.sum, b)), cluster_load(cluster_place(&sh.sum_t, b)), c);
+            if (p.blocks == 1) {
+                all.m = sh.max, all.s = sh.sum, all.w = sh.sum_t;
+            } else {
+                if (lane < p.blocks)
+                    all.m = cluster_load(cluster_place(&sh.max, lane)), all.s = cluster_load(cluster_place(&sh.sum, lane)), all.w = cluster_load(cluster_place(&sh.sum_t, lane));
+                join_lanes(all, p.blocks, c);
+            }
             const bool none = all.m == -INFINITY && all.s == 0.0f;  // a row whose mask leaves nothing
             const float l2 = log2f(all.s);
             if (lane == 0) {
@@ -430,10 +503,10 @@ __global__ void __launch_bounds__(kBackThreads) logprob_backward_kernel(const Lo
 }
 
 // Blocks that share a row: enough that a small call fills the GPU, while each still has a piece a warp.
-int row_blocks(long long rows, int vocab, bool bf16) {
+int row_blocks(long long rows, int vocab, bool bf16, int warps) {
     const int pieces = vocab / (bf16 ? 256 : 128) + 2;
     int n = 1;
-    while (n < kMostBlocks && (pieces > n * kPieces || (rows * n < 2 * sm_count() && pieces >= 2 * n * kWarps))) n *= 2;
+    while (n < kMostBlocks && (pieces > n * kPieces || (rows * n < 2 * sm_count() && pieces >= 2 * n * warps))) n *= 2;
     return n;
 }
 
@@ -460,12 +533,14 @@ extern "C" int glm53f_kda_logprobs(int32_t rows, int32_t vocab, const void* logi
     if (logprob == nullptr && entropy == nullptr && lse == nullptr && top == 0) return kInvalid;
     const bool bf16 = kind == GLM53F_KDA_LOGITS_BF16;
     LogprobParams p{};
-    p.logits = logits, p.ld = ld, p.vocab = vocab, p.blocks = row_blocks(rows, vocab, bf16), p.top = top;
+    p.logits = logits, p.ld = ld, p.vocab = vocab, p.top = top;
+    const int warps = (long long)rows * kMostBlocks <= 2 * sm_count() ? 16 : 8;
+    p.blocks = row_blocks(rows, vocab, bf16, warps);
     p.tokens = tokens, p.temperature = temperature, p.logprob = logprob, p.entropy = entropy, p.lse = lse, p.top_ids = top_ids, p.top_values = top_values;
     if ((long long)rows * p.blocks > 0x7fffffff) return kInvalid;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(rows * p.blocks));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(32 * warps);
     cfg.stream = reinterpret_cast<cudaStream_t>(stream);
     cudaLaunchAttribute attr[2];
     unsigned na = early_attribute(attr[0]);
@@ -478,7 +553,8 @@ extern "C" int glm53f_kda_logprobs(int32_t rows, int32_t vocab, const void* logi
     }
     cfg.attrs = attr;
     cfg.numAttrs = na;
-    return (int)(bf16 ? cudaLaunchKernelEx(&cfg, logprob_kernel<true>, p) : cudaLaunchKernelEx(&cfg, logprob_kernel<false>, p));
+    if (warps == 16) return (int)(bf16 ? cudaLaunchKernelEx(&cfg, logprob_kernel<true, 16>, p) : cudaLaunchKernelEx(&cfg, logprob_kernel<false, 16>, p));
+    return (int)(bf16 ? cudaLaunchKernelEx(&cfg, logprob_kernel<true, 8>, p) : cudaLaunchKernelEx(&cfg, logprob_kernel<false, 8>, p));
 }
 
 extern "C" int glm53f_kda_logprobs_backward(int32_t rows, int32_t vocab, const void* logits, int32_t kind, int64_t ld, const int32_t* tokens,
