@@ -105,20 +105,24 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
     grid_ready();
 
     const Widen widen;
-    // The next piece to load: its tile and place there.
+    // The next piece to load: its tile and place there.  Where its codes and scales lie moves on by the same steps: every split but one is even, and with one there are no groups of
+    // two pieces.
     int ltile = tile0, li = 0;
+    const uint4* lcodes = p.codes + ((long long)tile0 * p.pieces + kw) * 32 + lane;
+    long long lgroup = ((long long)tile0 * groups + kw * kPiece / G) * 8 + g;
+    const long long code_turn = ((long long)step * p.pieces - (long long)(per - 1) * p.split) * 32;
+    const int code_step = p.split * 32, group_step = p.split * kPiece / G * 8;
+    const long long group_turn = (long long)step * groups * 8 - (long long)(per - 1) * group_step;
     auto load = [&](P& x) {
-        const int piece = kw + li * p.split;
-        const bool ok = ltile < p.tiles && piece < p.pieces;
-        if (ok) x.codes = __ldcs(p.codes + ((long long)ltile * p.pieces + piece) * 32 + lane);
-        else x.codes = make_uint4(0u, 0u, 0u, 0u);
+        const bool ok = ltile < p.tiles && kw + li * p.split < p.pieces;
+        x.codes = ok ? __ldcs(lcodes) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
         for (int j = 0; j < P::N; ++j) {
-            const long long at = ((long long)ltile * groups + (piece * kPiece + j * G) / G) * 8 + g;
-            x.scale[j] = ok ? __ldg(p.scales + at) : 0u;
-            if constexpr (ZEROS) x.zero[j] = ok ? (uint32_t)__ldg(p.zeros + at) : 0u;
+            x.scale[j] = ok ? __ldg(p.scales + lgroup + j * 8) : 0u;
+            if constexpr (ZEROS) x.zero[j] = ok ? (uint32_t)__ldg(p.zeros + lgroup + j * 8) : 0u;
         }
-        if (++li == per) li = 0, ltile += step;
+        if (++li == per) li = 0, ltile += step, lcodes += code_turn, lgroup += group_turn;
+        else lcodes += code_step, lgroup += group_step;
     };
     P ahead[kAhead];
 #pragma unroll
@@ -156,8 +160,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
                     const int j = s / kSteps;
                     uint32_t lo = 0x43084308u, hi = 0x43084308u;
                     if constexpr (ZEROS) {
-                        lo = 0x43004300u | (x.zero[j] & 0xffu) * 0x00010001u;
-                        hi = 0x43004300u | (x.zero[j] >> 8) * 0x00010001u;
+                        lo = __byte_perm(x.zero[j], 0x43434343u, 0x4040);
+                        hi = __byte_perm(x.zero[j], 0x43434343u, 0x4141);
                     }
                     uint32_t a[4];
                     widen(w[s], lo, hi, a);
@@ -423,8 +427,7 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
                         for (int h = 0; h < 2; ++h) {  // 32 k: their group's zero points
                             uint32_t lo = 0x43084308u, hi = 0x43084308u;
                             if constexpr (ZEROS) {
-                                const uint32_t z = now_zero[i][m][t] >> (16 * h);
-                                lo = 0x43004300u | (z & 0xffu) * 0x00010001u, hi = 0x43004300u | (z >> 8 & 0xffu) * 0x00010001u;
+                                lo = __byte_perm(now_zero[i][m][t], 0x43434343u, h ? 0x4242 : 0x4040), hi = __byte_perm(now_zero[i][m][t], 0x43434343u, h ? 0x4343 : 0x4141);
                             }
                             uint32_t f[4], e[4];
                             widen(words[2 * h], lo, hi, f);
@@ -662,6 +665,7 @@ extern "C" int32_t glm53f_kda_proj_int4(const uint16_t* x, int64_t ldx, const vo
     p.codes = reinterpret_cast<const uint4*>(w), p.scales = reinterpret_cast<const uint32_t*>(w + at.scales), p.zeros = reinterpret_cast<const uint16_t*>(w + at.zeros);
     p.tiles = (int)at.tiles, p.pieces = (int)at.pieces;
     p.split = 1;
+
     while (p.split < kFewWarps && p.split * 2 <= p.pieces) p.split *= 2;
     const int pitch = (k + kRowPad) * 2, fit = kMostShared / pitch, most = fit < kFewRows ? fit : kFewRows;  // rows of x that shared memory holds
     const int abreast = kFewWarps / p.split, sms = sm_count();
