@@ -23,10 +23,10 @@ namespace {
 
 constexpr int kTile = 16;        // weight rows of a tile
 constexpr int kPiece = 64;       // k of a piece
-constexpr int kFewWarps = 16, kFewThreads = 32 * kFewWarps;
-constexpr int kFewRows = 8;      // of x at a time
-constexpr int kAhead = 8;        // pieces of a warp in flight
-constexpr int kMostShared = 200 * 1024;  // for the rows of x
+constexpr int kFewWarps = 16, kFewThreads = 32 * (kFewWarps + 1);  // the last warp loads
+constexpr int kFewRows = 8;
+constexpr int kFewStages = 16;   // of the ring, at most
+constexpr int kFewX = 150 * 1024, kFewShared = 208 * 1024;  // bytes for the rows of x, and with the ring
 constexpr int kRowPad = 8;       // bf16 between them: the eight rows that one load of fragments reads lie in different banks
 
 struct Int4Layout {  // bytes from the packed weight's start
@@ -49,6 +49,8 @@ struct Int4Params {
     void* out;
     int rows, n, k, out_f32;
     int tiles, pieces, split;  // warps that share a tile
+    int x_bytes, stages;       // of shared memory for the rows of x; of the ring behind them
+    int* status;
 };
 
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -82,117 +84,141 @@ struct Widen {
     }
 };
 
-// A piece on its way: its codes, the scales of its groups and their zero points.
+enum : int { kStatusInt4FewEmpty = 178, kStatusInt4FewFull = 179 };
+
+// A stage of the ring: a piece for each warp, the scales and zero points of their groups.
 template <int G, bool ZEROS>
-struct Piece {
-    static constexpr int N = G < kPiece ? kPiece / G : 1;
-    uint4 codes;
-    uint32_t scale[N];
-    uint32_t zero[ZEROS ? N : 1];
+struct Few {
+    static constexpr int N = G < kPiece ? kPiece / G : 1;         // groups that a piece lies in
+    static constexpr int kScaleBytes = kPiece * 32 / G;           // of a piece (a group of 128: half of them, its pieces come in pairs)
+    static constexpr int kZeroBytes = ZEROS ? kPiece * 16 / G : 0;
+    static constexpr int oScales = kFewWarps * 512, oZeros = oScales + kFewWarps * kScaleBytes, kStage = oZeros + kFewWarps * kZeroBytes;
 };
 
 template <int G, bool ZEROS>
 __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Params p) {
-    using P = Piece<G, ZEROS>;
-    extern __shared__ __align__(16) unsigned char smem[];
+    using F = Few<G, ZEROS>;
+    extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float sums[2][kFewWarps][kTile * kFewRows];
     __shared__ __align__(16) uint4 nothing;  // what rows that are not there hold
+    __shared__ __align__(8) uint64_t full[kFewStages], empty[kFewStages];
+    __shared__ volatile uint32_t ctl[2];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int kw = warp % p.split, tw = warp / p.split, abreast = kFewWarps / p.split;  // this warp's part of k, its tile among those at a time
-    const int per = (p.pieces + p.split - 1) / p.split;
-    const int step = gridDim.x * abreast, tile0 = blockIdx.x * abreast + tw;
-    const int groups = p.k / G, g = lane >> 2;
-    grid_ready();
-
-    const Widen widen;
-    // The next piece to load: its tile and place there.  Where its codes and scales lie moves on by the same steps: every split but one is even, and with one there are no groups of
-    // two pieces.
-    int ltile = tile0, li = 0;
-    const uint4* lcodes = p.codes + ((long long)tile0 * p.pieces + kw) * 32 + lane;
-    long long lgroup = ((long long)tile0 * groups + kw * kPiece / G) * 8 + g;
-    const long long code_turn = ((long long)step * p.pieces - (long long)(per - 1) * p.split) * 32;
-    const int code_step = p.split * 32, group_step = p.split * kPiece / G * 8;
-    const long long group_turn = (long long)step * groups * 8 - (long long)(per - 1) * group_step;
-    auto load = [&](P& x) {
-        const bool ok = ltile < p.tiles && kw + li * p.split < p.pieces;
-        x.codes = ok ? __ldcs(lcodes) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-        for (int j = 0; j < P::N; ++j) {
-            x.scale[j] = ok ? __ldg(p.scales + lgroup + j * 8) : 0u;
-            if constexpr (ZEROS) x.zero[j] = ok ? (uint32_t)__ldg(p.zeros + lgroup + j * 8) : 0u;
-        }
-        if (++li == per) li = 0, ltile += step, lcodes += code_turn, lgroup += group_turn;
-        else lcodes += code_step, lgroup += group_step;
-    };
-    P ahead[kAhead];
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) load(ahead[u]);
-
-    // The rows of x.
+    const int abreast = kFewWarps / p.split;                          // tiles at a time
+    const int per = (p.pieces + p.split - 1) / p.split;               // stages of a tile
+    const int groups = p.k / G, step = gridDim.x * abreast;
     const int pitch = (p.k + kRowPad) * 2;
-    if (tid == 0) nothing = make_uint4(0u, 0u, 0u, 0u);
-    for (int r = 0; r < p.rows; ++r)
-        for (int i = tid; i < p.k / 8; i += kFewThreads)
-            *reinterpret_cast<uint4*>(smem + r * pitch + i * 16) = __ldg(reinterpret_cast<const uint4*>(p.x + r * p.ldx) + i);
+    unsigned char* ring = smem + p.x_bytes;
+    if (tid == 0) {
+        for (int i = 0; i < p.stages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], kFewWarps);
+        ctl[0] = ctl[1] = 0u;
+        nothing = make_uint4(0u, 0u, 0u, 0u);
+        mbar_init_fence();
+    }
     __syncthreads();
-    const int xr = lane & 7;
-    const bool there = xr < p.rows;
-    const uint32_t xrow = there ? smem_u32(smem + xr * pitch + (lane >> 3) * 16) : smem_u32(&nothing);
+    const WaitCtx ctx{ctl, ctl + 1, p.status};
+    grid_ready();
+    int s = 0;
+    uint32_t ph = 0;
 
-    float acc[4] = {};
-    int i = 0, tile = tile0, buf = 0, round = 0;
-    // Rounds: every warp of the block takes part in each, with or without a tile, as the barrier needs them.
-    const int rounds = (p.tiles - (int)blockIdx.x * abreast + step - 1) / step;
-    while (round < rounds) {
+    if (warp == kFewWarps) {
+        // A lane a tile: its pieces of a stage lie together, their scales and zero points too.
+        for (int tile = blockIdx.x * abreast; tile < p.tiles; tile += step) {
+            const int tiles = min(abreast, p.tiles - tile);
+            const long long t = tile + lane;
+            for (int c = 0; c < per; ++c) {
+                const int piece = c * p.split, pieces = min(p.split, p.pieces - piece);
+                if (!tc::warp_all(mbar_wait(&empty[s], ph ^ 1u, ctx, kStatusInt4FewEmpty))) break;
+                if (lane == 0) {
+                    ctl[0] = ctl[0] + 1u;
+                    mbar_arrive_expect_tx(&full[s], tiles * pieces * (512 + F::kScaleBytes + F::kZeroBytes));
+                }
+                __syncwarp();
+                if (lane < tiles) {
+                    unsigned char* to = ring + s * F::kStage;
+                    const long long group = t * groups + piece * kPiece / G;
+                    bulk_load(to + lane * p.split * 512, p.codes + (t * p.pieces + piece) * 32, pieces * 512, &full[s]);
+                    bulk_load(to + F::oScales + lane * p.split * F::kScaleBytes, p.scales + group * 8, pieces * F::kScaleBytes, &full[s]);
+                    if constexpr (ZEROS) bulk_load(to + F::oZeros + lane * p.split * F::kZeroBytes, p.zeros + group * 8, pieces * F::kZeroBytes, &full[s]);
+                }
+                if (++s == p.stages) s = 0, ph ^= 1u;
+            }
+        }
+    } else {
+        for (int r = 0; r < p.rows; ++r)
+            for (int i = tid; i < p.k / 8; i += 32 * kFewWarps)
+                *reinterpret_cast<uint4*>(smem + r * pitch + i * 16) = __ldg(reinterpret_cast<const uint4*>(p.x + r * p.ldx) + i);
+        named_bar_sync(1, 32 * kFewWarps);
+        const Widen widen;
+        const int kw = warp % p.split, tw = warp / p.split, g = lane >> 2;  // this warp's part of k, its tile of those at a time
+        const int xr = lane & 7;
+        const bool there = xr < p.rows;
+        const uint32_t xrow = there ? smem_u32(smem + xr * pitch + (lane >> 3) * 16) + kw * kPiece * 2 : smem_u32(&nothing), half = there ? 64u : 0u, xstep = there ? p.split * kPiece * 2 : 0u;
+        int buf = 0;
+        // Every warp takes part in each round, with or without a tile, as the barrier needs them.
+        for (int tile = blockIdx.x * abreast; tile < p.tiles; tile += step, buf ^= 1) {
+            float acc[4] = {};
+            for (int c = 0; c < per; ++c) {
+                tc::warp_all(mbar_wait(&full[s], ph, ctx, kStatusInt4FewFull));  // (after a wait that gave up all others do: the sums are lost, the status says so)
+                const bool mine = tile + tw < p.tiles && kw + c * p.split < p.pieces;
+                const unsigned char* from = ring + s * F::kStage;
+                uint4 codes;
+                uint32_t scale[F::N], zero[F::N];
+                if (mine) {
+                    codes = *reinterpret_cast<const uint4*>(from + warp * 512 + lane * 16);
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            if (round < rounds) {
-                const P x = ahead[u];
-                load(ahead[u]);
-                const int piece = kw + i * p.split;
-                const uint32_t xat = there && piece < p.pieces ? xrow + piece * kPiece * 2 : smem_u32(&nothing), half = there && piece < p.pieces ? 64u : 0u;
-                const uint32_t* w = reinterpret_cast<const uint32_t*>(&x.codes);
-                constexpr int kSteps = 4 / P::N;  // of a group in the piece
-                uint32_t b[4];
-                float c[4] = {};
-#pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    const int j = s / kSteps;
-                    uint32_t lo = 0x43084308u, hi = 0x43084308u;
-                    if constexpr (ZEROS) {
-                        lo = __byte_perm(x.zero[j], 0x43434343u, 0x4040);
-                        hi = __byte_perm(x.zero[j], 0x43434343u, 0x4141);
-                    }
-                    uint32_t a[4];
-                    widen(w[s], lo, hi, a);
-                    if (s % 2 == 0) ldmatrix_4(xat + (s / 2) * half, b[0], b[1], b[2], b[3]);
-                    mma(c, a, s % 2 ? b[2] : b[0], s % 2 ? b[3] : b[1]);
-                    if (s % kSteps == kSteps - 1) {
-                        const float s0 = __uint_as_float(x.scale[j] << 16), s1 = __uint_as_float(x.scale[j] & 0xffff0000u);
-                        acc[0] = fmaf(s0, c[0], acc[0]), acc[1] = fmaf(s0, c[1], acc[1]);
-                        acc[2] = fmaf(s1, c[2], acc[2]), acc[3] = fmaf(s1, c[3], acc[3]);
-                        c[0] = c[1] = c[2] = c[3] = 0.0f;
+                    for (int j = 0; j < F::N; ++j) {
+                        const int at = (warp * kPiece / G + j) * 8 + g;
+                        scale[j] = *(reinterpret_cast<const uint32_t*>(from + F::oScales) + at);
+                        if constexpr (ZEROS) zero[j] = *(reinterpret_cast<const uint16_t*>(from + F::oZeros) + at);
                     }
                 }
-                if (++i == per) {
-                    float* to = sums[buf][warp];
-                    *reinterpret_cast<float2*>(to + g * kFewRows + 2 * (lane & 3)) = make_float2(acc[0], acc[1]);
-                    *reinterpret_cast<float2*>(to + (g + 8) * kFewRows + 2 * (lane & 3)) = make_float2(acc[2], acc[3]);
-                    acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
-                    __syncthreads();
-                    // (the next tile's sums go to the other buffer; this one is written again behind the next barrier)
-                    for (int e = tid; e < abreast * kTile * kFewRows; e += kFewThreads) {
-                        const int t = e / (kTile * kFewRows), in = e % (kTile * kFewRows), f = in % kTile, r = in / kTile;
-                        const int o = (tile - tw + t) * kTile + f;
-                        if (r >= p.rows || o >= p.n) continue;
-                        float sum = 0.0f;
-                        for (int q = 0; q < p.split; ++q) sum += sums[buf][t * p.split + q][f * kFewRows + r];
-                        if (p.out_f32) static_cast<float*>(p.out)[r * p.ldo + o] = sum;
-                        else static_cast<uint16_t*>(p.out)[r * p.ldo + o] = f32_to_bf16_bits(sum);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty[s]);
+                if (++s == p.stages) s = 0, ph ^= 1u;
+                if (!mine) continue;
+                const uint32_t xat = xrow + c * xstep;
+                const uint32_t* w = reinterpret_cast<const uint32_t*>(&codes);
+                constexpr int kSteps = 4 / F::N;  // of a group in the piece
+                uint32_t b[8];
+                ldmatrix_4(xat, b[0], b[1], b[2], b[3]);
+                ldmatrix_4(xat + half, b[4], b[5], b[6], b[7]);
+                float d[4] = {};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int j = q / kSteps;
+                    uint32_t lo = 0x43084308u, hi = 0x43084308u;
+                    if constexpr (ZEROS) lo = __byte_perm(zero[j], 0x43434343u, 0x4040), hi = __byte_perm(zero[j], 0x43434343u, 0x4141);
+                    uint32_t a[4];
+                    widen(w[q], lo, hi, a);
+                    mma(d, a, b[2 * q], b[2 * q + 1]);
+                    if (q % kSteps == kSteps - 1) {
+                        const float s0 = __uint_as_float(scale[j] << 16), s1 = __uint_as_float(scale[j] & 0xffff0000u);
+                        acc[0] = fmaf(s0, d[0], acc[0]), acc[1] = fmaf(s0, d[1], acc[1]);
+                        acc[2] = fmaf(s1, d[2], acc[2]), acc[3] = fmaf(s1, d[3], acc[3]);
+                        d[0] = d[1] = d[2] = d[3] = 0.0f;
                     }
-                    i = 0, tile += step, buf ^= 1, ++round;
                 }
             }
+            float* to = sums[buf][warp];
+            *reinterpret_cast<float2*>(to + g * kFewRows + 2 * (lane & 3)) = make_float2(acc[0], acc[1]);
+            *reinterpret_cast<float2*>(to + (g + 8) * kFewRows + 2 * (lane & 3)) = make_float2(acc[2], acc[3]);
+            named_bar_sync(1, 32 * kFewWarps);
+            // (the next tile's sums go to the other buffer; this one is written again behind the next barrier)
+            for (int e = tid; e < abreast * kTile * kFewRows; e += 32 * kFewWarps) {
+                const int t = e / (kTile * kFewRows), in = e % (kTile * kFewRows), f = in % kTile, r = in / kTile;
+                const int o = (tile + t) * kTile + f;
+                if (r >= p.rows || o >= p.n) continue;
+                float sum = 0.0f;
+                for (int q = 0; q < p.split; ++q) sum += sums[buf][t * p.split + q][f * kFewRows + r];
+                if (p.out_f32) static_cast<float*>(p.out)[r * p.ldo + o] = sum;
+                else static_cast<uint16_t*>(p.out)[r * p.ldo + o] = f32_to_bf16_bits(sum);
+            }
+        }
+    }
+    if (ctl[1]) {  // after a wait that gave up, copies into this block's shared memory may still be in flight: a bounded time for them
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 2000000ull) {
         }
     }
 }
@@ -569,10 +595,13 @@ bool shape_ok(int32_t n, int32_t k, int32_t group) {
 bool on16(const void* p) { return p != nullptr && (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 template <int G, bool ZEROS>
-int few_launch(const Int4Params& p, unsigned blocks, int shared, cudaStream_t stream) {
-    const cudaError_t e = cudaFuncSetAttribute(int4_few_kernel<G, ZEROS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared);
+int few_launch(Int4Params& p, unsigned blocks, cudaStream_t stream) {
+    using F = Few<G, ZEROS>;
+    const int stages = (kFewShared - p.x_bytes) / F::kStage;
+    p.stages = stages < kFewStages ? stages : kFewStages;
+    const cudaError_t e = cudaFuncSetAttribute(int4_few_kernel<G, ZEROS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewShared);
     if (e != cudaSuccess) return (int)e;
-    return launch_early(int4_few_kernel<G, ZEROS>, dim3(blocks), kFewThreads, shared, stream, p);
+    return launch_early(int4_few_kernel<G, ZEROS>, dim3(blocks), kFewThreads, p.x_bytes + p.stages * F::kStage, stream, p);
 }
 
 template <int N, int MT, bool ZEROS>
@@ -642,48 +671,40 @@ extern "C" int32_t glm53f_kda_proj_int4(const uint16_t* x, int64_t ldx, const vo
     const Int4Layout at(n, k, group, zeros != 0);
     if (at.tiles > 0x3fffffff) return kInvalid;
     const auto* w = static_cast<const unsigned char*>(packed);
-    if (rows > kFewRows) {
+    int* status = status_word();
+    if (status == nullptr) return (int)cudaErrorUnknown;
+    const cudaStream_t on = reinterpret_cast<cudaStream_t>(stream);
+    const int x_bytes = (int)(((long long)(rows < kFewRows ? rows : kFewRows) * (k + kRowPad) * 2 + 127) / 128 * 128);
+    if (rows > kFewRows || x_bytes > kFewX) {
         ManyParams m{};
         m.codes = reinterpret_cast<const uint4*>(w), m.scales = reinterpret_cast<const uint16_t*>(w + at.scales);
         m.zeros = zeros ? reinterpret_cast<const uint16_t*>(w + at.zeros) : nullptr;
         m.out = out, m.ldo = ldo, m.rows = rows, m.n = n, m.k = k, m.out_f32 = out_f32 != 0, m.group = group;
         m.tiles = (int)at.tiles, m.pieces = (int)at.pieces, m.groups = (int)at.groups;
-        m.status = status_word();
-        if (m.status == nullptr) return (int)cudaErrorUnknown;
-        const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+        m.status = status;
         auto launch = [&](auto z) {
             constexpr bool Z = decltype(z)::value;
-            if (rows <= 16) return many_launch<16, 1, Z>(m, x, ldx, s);
-            if (rows <= 32) return many_launch<32, 1, Z>(m, x, ldx, s);
-            if (rows <= 64) return many_launch<64, 1, Z>(m, x, ldx, s);
-            return many_launch<128, 1, Z>(m, x, ldx, s);
+            if (rows <= 16) return many_launch<16, 1, Z>(m, x, ldx, on);
+            if (rows <= 32) return many_launch<32, 1, Z>(m, x, ldx, on);
+            if (rows <= 64) return many_launch<64, 1, Z>(m, x, ldx, on);
+            return many_launch<128, 1, Z>(m, x, ldx, on);
         };
         return zeros ? launch(std::true_type{}) : launch(std::false_type{});
     }
     Int4Params p{};
-    p.ldx = ldx, p.ldo = ldo, p.n = n, p.k = k, p.out_f32 = out_f32 != 0;
+    p.x = x, p.ldx = ldx, p.out = out, p.ldo = ldo, p.rows = rows, p.n = n, p.k = k, p.out_f32 = out_f32 != 0;
     p.codes = reinterpret_cast<const uint4*>(w), p.scales = reinterpret_cast<const uint32_t*>(w + at.scales), p.zeros = reinterpret_cast<const uint16_t*>(w + at.zeros);
-    p.tiles = (int)at.tiles, p.pieces = (int)at.pieces;
+    p.tiles = (int)at.tiles, p.pieces = (int)at.pieces, p.x_bytes = x_bytes, p.status = status;
     p.split = 1;
-
     while (p.split < kFewWarps && p.split * 2 <= p.pieces) p.split *= 2;
-    const int pitch = (k + kRowPad) * 2, fit = kMostShared / pitch, most = fit < kFewRows ? fit : kFewRows;  // rows of x that shared memory holds
     const int abreast = kFewWarps / p.split, sms = sm_count();
     const long long want = (at.tiles + abreast - 1) / abreast;
     const unsigned blocks = (unsigned)(want < sms ? want : sms);
-    for (int r = 0; r < rows; r += most) {
-        p.rows = rows - r < most ? rows - r : most;
-        p.x = x + (long long)r * ldx;
-        p.out = static_cast<unsigned char*>(out) + (long long)r * ldo * (out_f32 ? 4 : 2);
-        auto launch = [&](auto g) {
-            constexpr int G = decltype(g)::value;
-            const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-            return zeros ? few_launch<G, true>(p, blocks, pitch * p.rows, s) : few_launch<G, false>(p, blocks, pitch * p.rows, s);
-        };
-        const int rc = group == 32   ? launch(std::integral_constant<int, 32>{})
-                       : group == 64 ? launch(std::integral_constant<int, 64>{})
-                                     : launch(std::integral_constant<int, 128>{});
-        if (rc != 0) return rc;
-    }
-    return 0;
+    auto launch = [&](auto g) {
+        constexpr int G = decltype(g)::value;
+        return zeros ? few_launch<G, true>(p, blocks, on) : few_launch<G, false>(p, blocks, on);
+    };
+    return group == 32   ? launch(std::integral_constant<int, 32>{})
+           : group == 64 ? launch(std::integral_constant<int, 64>{})
+                         : launch(std::integral_constant<int, 128>{});
 }
