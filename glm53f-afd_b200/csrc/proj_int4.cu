@@ -86,13 +86,13 @@ struct Widen {
 
 enum : int { kStatusInt4FewEmpty = 178, kStatusInt4FewFull = 179 };
 
-// A stage of the ring: a piece for each warp, the scales and zero points of their groups.
+// A stage of the ring: two pieces (128 k) for each warp, the scales and zero points of their groups.
 template <int G, bool ZEROS>
 struct Few {
-    static constexpr int N = G < kPiece ? kPiece / G : 1;         // groups that a piece lies in
-    static constexpr int kScaleBytes = kPiece * 32 / G;           // of a piece (a group of 128: half of them, its pieces come in pairs)
+    static constexpr int N = 2 * kPiece / G;                      // groups of a warp's pieces
+    static constexpr int kScaleBytes = kPiece * 32 / G;           // of a piece (of 128: half of them, its pieces come in pairs)
     static constexpr int kZeroBytes = ZEROS ? kPiece * 16 / G : 0;
-    static constexpr int oScales = kFewWarps * 512, oZeros = oScales + kFewWarps * kScaleBytes, kStage = oZeros + kFewWarps * kZeroBytes;
+    static constexpr int oScales = kFewWarps * 1024, oZeros = oScales + 2 * kFewWarps * kScaleBytes, kStage = oZeros + 2 * kFewWarps * kZeroBytes;
 };
 
 template <int G, bool ZEROS>
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
     __shared__ volatile uint32_t ctl[2];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int abreast = kFewWarps / p.split;                          // tiles at a time
-    const int per = (p.pieces + p.split - 1) / p.split;               // stages of a tile
+    const int at_once = 2 * p.split, per = (p.pieces + at_once - 1) / at_once;  // pieces of a tile in a stage; stages of a tile
     const int groups = p.k / G, step = gridDim.x * abreast;
     const int pitch = (p.k + kRowPad) * 2;
     unsigned char* ring = smem + p.x_bytes;
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
             const int tiles = min(abreast, p.tiles - tile);
             const long long t = tile + lane;
             for (int c = 0; c < per; ++c) {
-                const int piece = c * p.split, pieces = min(p.split, p.pieces - piece);
+                const int piece = c * at_once, pieces = min(at_once, p.pieces - piece);
                 if (!tc::warp_all(mbar_wait(&empty[s], ph ^ 1u, ctx, kStatusInt4FewEmpty))) break;
                 if (lane == 0) {
                     ctl[0] = ctl[0] + 1u;
@@ -137,9 +137,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
                 if (lane < tiles) {
                     unsigned char* to = ring + s * F::kStage;
                     const long long group = t * groups + piece * kPiece / G;
-                    bulk_load(to + lane * p.split * 512, p.codes + (t * p.pieces + piece) * 32, pieces * 512, &full[s]);
-                    bulk_load(to + F::oScales + lane * p.split * F::kScaleBytes, p.scales + group * 8, pieces * F::kScaleBytes, &full[s]);
-                    if constexpr (ZEROS) bulk_load(to + F::oZeros + lane * p.split * F::kZeroBytes, p.zeros + group * 8, pieces * F::kZeroBytes, &full[s]);
+                    bulk_load(to + lane * at_once * 512, p.codes + (t * p.pieces + piece) * 32, pieces * 512, &full[s]);
+                    bulk_load(to + F::oScales + lane * at_once * F::kScaleBytes, p.scales + group * 8, pieces * F::kScaleBytes, &full[s]);
+                    if constexpr (ZEROS) bulk_load(to + F::oZeros + lane * at_once * F::kZeroBytes, p.zeros + group * 8, pieces * F::kZeroBytes, &full[s]);
                 }
                 if (++s == p.stages) s = 0, ph ^= 1u;
             }
@@ -153,22 +153,23 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
         const int kw = warp % p.split, tw = warp / p.split, g = lane >> 2;  // this warp's part of k, its tile of those at a time
         const int xr = lane & 7;
         const bool there = xr < p.rows;
-        const uint32_t xrow = there ? smem_u32(smem + xr * pitch + (lane >> 3) * 16) + kw * kPiece * 2 : smem_u32(&nothing), half = there ? 64u : 0u, xstep = there ? p.split * kPiece * 2 : 0u;
+        const uint32_t xrow = there ? smem_u32(smem + xr * pitch + (lane >> 3) * 16) + kw * kPiece * 4 : smem_u32(&nothing), half = there ? 64u : 0u, xstep = there ? at_once * kPiece * 2 : 0u;
         int buf = 0;
         // Every warp takes part in each round, with or without a tile, as the barrier needs them.
         for (int tile = blockIdx.x * abreast; tile < p.tiles; tile += step, buf ^= 1) {
             float acc[4] = {};
             for (int c = 0; c < per; ++c) {
-                tc::warp_all(mbar_wait(&full[s], ph, ctx, kStatusInt4FewFull));  // (after a wait that gave up all others do: the sums are lost, the status says so)
-                const bool mine = tile + tw < p.tiles && kw + c * p.split < p.pieces;
+                mbar_wait(&full[s], ph, ctx, kStatusInt4FewFull);  // (after a wait that gave up all others do: the sums are lost, the status says so)
+                const int mine = tile + tw < p.tiles ? p.pieces - c * at_once - 2 * kw : 0;  // pieces, of two
                 const unsigned char* from = ring + s * F::kStage;
-                uint4 codes;
+                uint4 codes[2];
                 uint32_t scale[F::N], zero[F::N];
-                if (mine) {
-                    codes = *reinterpret_cast<const uint4*>(from + warp * 512 + lane * 16);
+                if (mine > 0) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) codes[u] = *reinterpret_cast<const uint4*>(from + warp * 1024 + u * 512 + lane * 16);
 #pragma unroll
                     for (int j = 0; j < F::N; ++j) {
-                        const int at = (warp * kPiece / G + j) * 8 + g;
+                        const int at = (warp * F::N + j) * 8 + g;
                         scale[j] = *(reinterpret_cast<const uint32_t*>(from + F::oScales) + at);
                         if constexpr (ZEROS) zero[j] = *(reinterpret_cast<const uint16_t*>(from + F::oZeros) + at);
                     }
@@ -176,27 +177,30 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&empty[s]);
                 if (++s == p.stages) s = 0, ph ^= 1u;
-                if (!mine) continue;
                 const uint32_t xat = xrow + c * xstep;
-                const uint32_t* w = reinterpret_cast<const uint32_t*>(&codes);
-                constexpr int kSteps = 4 / F::N;  // of a group in the piece
-                uint32_t b[8];
-                ldmatrix_4(xat, b[0], b[1], b[2], b[3]);
-                ldmatrix_4(xat + half, b[4], b[5], b[6], b[7]);
+                constexpr int kSteps = G / 16;  // of a group
                 float d[4] = {};
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int j = q / kSteps;
-                    uint32_t lo = 0x43084308u, hi = 0x43084308u;
-                    if constexpr (ZEROS) lo = __byte_perm(zero[j], 0x43434343u, 0x4040), hi = __byte_perm(zero[j], 0x43434343u, 0x4141);
-                    uint32_t a[4];
-                    widen(w[q], lo, hi, a);
-                    mma(d, a, b[2 * q], b[2 * q + 1]);
-                    if (q % kSteps == kSteps - 1) {
-                        const float s0 = __uint_as_float(scale[j] << 16), s1 = __uint_as_float(scale[j] & 0xffff0000u);
-                        acc[0] = fmaf(s0, d[0], acc[0]), acc[1] = fmaf(s0, d[1], acc[1]);
-                        acc[2] = fmaf(s1, d[2], acc[2]), acc[3] = fmaf(s1, d[3], acc[3]);
-                        d[0] = d[1] = d[2] = d[3] = 0.0f;
+                for (int u = 0; u < 2; ++u) {
+                    if (u >= mine) break;
+                    const uint32_t w[4] = {codes[u].x, codes[u].y, codes[u].z, codes[u].w};
+                    uint32_t b[8];
+                    ldmatrix_4(xat + u * 2 * half, b[0], b[1], b[2], b[3]);
+                    ldmatrix_4(xat + u * 2 * half + half, b[4], b[5], b[6], b[7]);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int step = 4 * u + q, j = step / kSteps;
+                        uint32_t lo = 0x43084308u, hi = 0x43084308u;
+                        if constexpr (ZEROS) lo = __byte_perm(zero[j], 0x43434343u, 0x4040), hi = __byte_perm(zero[j], 0x43434343u, 0x4141);
+                        uint32_t a[4];
+                        widen(w[q], lo, hi, a);
+                        mma(d, a, b[2 * q], b[2 * q + 1]);
+                        if (step % kSteps == kSteps - 1) {
+                            const float s0 = __uint_as_float(scale[j] << 16), s1 = __uint_as_float(scale[j] & 0xffff0000u);
+                            acc[0] = fmaf(s0, d[0], acc[0]), acc[1] = fmaf(s0, d[1], acc[1]);
+                            acc[2] = fmaf(s1, d[2], acc[2]), acc[3] = fmaf(s1, d[3], acc[3]);
+                            d[0] = d[1] = d[2] = d[3] = 0.0f;
+                        }
                     }
                 }
             }
@@ -696,7 +700,7 @@ extern "C" int32_t glm53f_kda_proj_int4(const uint16_t* x, int64_t ldx, const vo
     p.codes = reinterpret_cast<const uint4*>(w), p.scales = reinterpret_cast<const uint32_t*>(w + at.scales), p.zeros = reinterpret_cast<const uint16_t*>(w + at.zeros);
     p.tiles = (int)at.tiles, p.pieces = (int)at.pieces, p.x_bytes = x_bytes, p.status = status;
     p.split = 1;
-    while (p.split < kFewWarps && p.split * 2 <= p.pieces) p.split *= 2;
+    while (p.split < kFewWarps && p.split * 4 <= p.pieces) p.split *= 2;
     const int abreast = kFewWarps / p.split, sms = sm_count();
     const long long want = (at.tiles + abreast - 1) / abreast;
     const unsigned blocks = (unsigned)(want < sms ? want : sms);
