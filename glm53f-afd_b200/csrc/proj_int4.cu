@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float sums[2][kFewWarps][kTile * kFewRows];
     __shared__ __align__(16) uint4 nothing;  // what rows that are not there hold
-    __shared__ __align__(8) uint64_t full[kFewStages], empty[kFewStages];
+    __shared__ __align__(8) uint64_t full[kFewStages], empty[kFewStages], x_full;
     __shared__ volatile uint32_t ctl[2];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int abreast = kFewWarps / p.split;                          // tiles at a time
@@ -111,6 +111,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
     unsigned char* ring = smem + p.x_bytes;
     if (tid == 0) {
         for (int i = 0; i < p.stages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], kFewWarps);
+        mbar_init(&x_full, 1);
         ctl[0] = ctl[1] = 0u;
         nothing = make_uint4(0u, 0u, 0u, 0u);
         mbar_init_fence();
@@ -145,15 +146,17 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
             }
         }
     } else {
-        for (int r = 0; r < p.rows; ++r)
-            for (int i = tid; i < p.k / 8; i += 32 * kFewWarps)
-                *reinterpret_cast<uint4*>(smem + r * pitch + i * 16) = __ldg(reinterpret_cast<const uint4*>(p.x + r * p.ldx) + i);
-        named_bar_sync(1, 32 * kFewWarps);
+        if (warp == 0) {
+            if (lane == 0) mbar_arrive_expect_tx(&x_full, p.rows * p.k * 2);
+            __syncwarp();
+            if (lane < p.rows) bulk_load(smem + lane * pitch, p.x + lane * p.ldx, p.k * 2, &x_full);
+        }
         const Widen widen;
         const int kw = warp % p.split, tw = warp / p.split, g = lane >> 2;  // this warp's part of k, its tile of those at a time
         const int xr = lane & 7;
         const bool there = xr < p.rows;
         const uint32_t xrow = there ? smem_u32(smem + xr * pitch + (lane >> 3) * 16) + kw * kPiece * 4 : smem_u32(&nothing), half = there ? 64u : 0u, xstep = there ? at_once * kPiece * 2 : 0u;
+        mbar_wait(&x_full, 0u, ctx, kStatusInt4FewFull);
         int buf = 0;
         // Every warp takes part in each round, with or without a tile, as the barrier needs them.
         for (int tile = blockIdx.x * abreast; tile < p.tiles; tile += step, buf ^= 1) {
