@@ -239,16 +239,14 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
 //   warps 1, 3    the matrix instructions (a stage each in turn, with groups of 128: the waits of a stage take one warp longer than its products the tensor cores)
 //   warp 2        bulk copies of the packed words, 128 k at a time, into another
 //   warps 4-      widen, 128 k at a time, two such stages in tensor memory
-//   the others    sum: a warpgroup for each kSumCols columns (MT == 2: for each half of 256 weight rows)
+//   the others    sum: a warpgroup for each kSumCols columns
 // Few tiles: the blocks of a cluster share a tile's k and add their sums, each for some rows, in rank order through distributed shared memory.
 
 enum : int { kStatusInt4Empty = 170, kStatusInt4Full = 171, kStatusInt4AEmpty = 172, kStatusInt4AFull = 173, kStatusInt4AccEmpty = 174, kStatusInt4AccFull = 175, kStatusInt4Words = 176, kStatusInt4WordsFull = 177 };
 
 struct ManyParams {
-    CUtensorMap tm_x;
-    const uint4* codes;
+    CUtensorMap tm_x, tm_words, tm_scales, tm_zeros;  // (the last one with zero points only)
     const uint16_t* scales;
-    const uint16_t* zeros;  // or none
     void* out;
     long long ldo;
     int rows, n, k, out_f32, group;
@@ -257,24 +255,24 @@ struct ManyParams {
     int* status;
 };
 
-template <int N, int MT>
+template <int N>
 struct Many {
-    static constexpr int kSumCols = MT == 2 ? N : N < 32 ? N : 32 * ((N + 63) / 64);  // (N = 128: 64)
-    static constexpr int kSumGroups = MT == 2 ? 2 : N / kSumCols;
+    static constexpr int kSumCols = N < 32 ? N : 32 * ((N + 63) / 64);  // (N = 128: 64)
+    static constexpr int kSumGroups = N / kSumCols;
     static constexpr int kWideners = N <= 64 ? 1 : 2;     // warpgroups that widen, a stage each in turn (of small tiles two blocks share an SM)
     static constexpr int kSumWarp = 4 + 4 * kWideners;    // the first warp that sums
     static constexpr int kThreads = 32 * kSumWarp + 128 * kSumGroups;
     static constexpr int kBoxBytes = N * 128;             // 64 k of x
     static constexpr int kRing = N <= 32 ? 6 : 4;         // stages of 128 k: of x
     static constexpr int kStages = N == 128 ? 4 : 2;      // ... in tensor memory (even, as the rings are: each of two warps that take turns then meets every phase of a place)
-    static constexpr int kStageCols = 64 * MT;
+    static constexpr int kStageCols = 64;
     static constexpr int kAccs = 2;                       // accumulators, a group's products each
     static constexpr int kAccCols = kAccs * N;
     static constexpr int kUsed = kAccCols + kStages * kStageCols;
     static constexpr int kCols = kUsed <= 256 ? 256 : 512;
     static constexpr int kBlocks = kCols == 256 ? 2 : 1;  // an SM
     static constexpr int kWords = N <= 32 ? 6 : 4;        // stages of packed words in shared memory
-    static constexpr int kWordBytes = 8 * MT * 1024;      // of a stage: two pieces of 8 MT tiles
+    static constexpr int oZeros = 8 * 1024, kWordBytes = oZeros + 512;  // of a stage: two pieces of 8 tiles, and their zero points
     static constexpr int oWords = kRing * 2 * kBoxBytes;
     static constexpr int oBars = oWords + kWords * kWordBytes;
     static constexpr int oCtl = oBars + (2 * kRing + 2 * kWords + 2 * kStages + 2 * kAccs) * 8;
@@ -285,6 +283,9 @@ __device__ __forceinline__ void tensor_load_2d(void* to, const void* tm, int x, 
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(to)),
                  "l"(reinterpret_cast<uint64_t>(tm)), "r"(smem_u32(bar)), "r"(x), "r"(y)
                  : "memory");
+}
+__device__ __forceinline__ void tensor_prefetch_2d(const void* tm, int x, int y) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y) : "memory");
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -301,9 +302,9 @@ __device__ __forceinline__ float peer_load(const void* local, uint32_t rank) {
 }
 
 // ZEROS: zero points are read; without them they are a constant (their forming takes a fifth of what widening does).
-template <int N, int MT, bool ZEROS>
-__global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) int4_many_kernel(const __grid_constant__ ManyParams p) {
-    using C = Many<N, MT>;
+template <int N, bool ZEROS>
+__global__ void __launch_bounds__(Many<N>::kThreads, Many<N>::kBlocks) int4_many_kernel(const __grid_constant__ ManyParams p) {
+    using C = Many<N>;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::oBars);
@@ -326,7 +327,7 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
     const uint32_t tm = *tmem_slot, stages0 = tm + C::kAccCols;
     const WaitCtx ctx{ctl, ctl + 1, p.status};
     const int split = p.split, part = split > 1 ? (int)cluster_rank() : 0, tile = (int)blockIdx.x / split;
-    const int mt = tile % p.m_tiles, row0 = tile / p.m_tiles * N;       // this block's weight rows (in units of 128 MT) and rows of x
+    const int mt = tile % p.m_tiles, row0 = tile / p.m_tiles * N;       // this block's weight rows (in units of 128) and rows of x
     const int per = p.pieces / split, piece0 = part * per, stages = (per + 1) / 2;
     grid_ready();
 
@@ -345,20 +346,20 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
             }
         }
     } else if (warp == 2) {
-        // A lane a tile of 16 weight rows: the words of its two pieces lie together.
-        const int w = mt * MT * 8 + lane;
-        const bool mine = lane < 8 * MT && w < p.tiles;
-        const uint32_t tiles = __popc(__ballot_sync(0xffffffffu, mine));
-        const unsigned char* from = reinterpret_cast<const unsigned char*>(p.codes) + ((long long)w * p.pieces + piece0) * 512;
-        int c = 0;
-        uint32_t ph = 0;
-        for (int st = 0; st < stages; ++st) {
-            const int pieces = min(per - 2 * st, 2);
-            if (!tc::warp_all(mbar_wait(&w_empty[c], ph ^ 1u, ctx, kStatusInt4Words))) break;
-            if (lane == 0) mbar_arrive_expect_tx(&w_full[c], tiles * pieces * 512);
-            __syncwarp();
-            if (mine) bulk_load(smem + C::oWords + c * C::kWordBytes + lane * 1024, from + st * 1024, pieces * 512, &w_full[c]);
-            if (++c == C::kWords) c = 0, ph ^= 1u;
+        // Eight tiles' words of two pieces, and their zero points, a box each; their scales, which the warps that sum fetch four groups ahead, into L2.
+        if (lane == 0) {
+            const int per_stage = 2 * kPiece / p.group, group0 = piece0 * kPiece / p.group;
+            int c = 0;
+            uint32_t ph = 0;
+            for (int st = 0; st < stages; ++st) {
+                if (!mbar_wait(&w_empty[c], ph ^ 1u, ctx, kStatusInt4Words)) break;
+                unsigned char* words = smem + C::oWords + c * C::kWordBytes;
+                mbar_arrive_expect_tx(&w_full[c], C::oZeros + (ZEROS ? 8 * per_stage * 16 : 0));
+                tensor_load_2d(words, &p.tm_words, (piece0 + 2 * st) * 128, mt * 8, &w_full[c]);
+                if constexpr (ZEROS) tensor_load_2d(words + C::oZeros, &p.tm_zeros, (group0 + st * per_stage) * 8, mt * 8, &w_full[c]);
+                tensor_prefetch_2d(&p.tm_scales, (group0 + st * per_stage) * 8, mt * 8);
+                if (++c == C::kWords) c = 0, ph ^= 1u;
+            }
         }
     } else if (warp == 1 || warp == 3) {
         constexpr uint32_t idesc = tc::idesc_bf16(128, N, 0, 0, 0);
@@ -408,67 +409,41 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
         // Weight rows 32 q .. of each 128: two tiles of 16, the lanes' words of both pieces of a stage.
         const Widen widen;
         const int q = warp & 3, g = lane >> 2, turn = (warp - 4) >> 2;
-        uint32_t zero[2][MT][2];  // zero points of a piece's two halves of 32 k, 16 bits each: one stage ahead
-        auto load = [&](int st) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        const int w = (mt * MT + m) * 8 + q * 2 + t, piece = 2 * st + i;
-                        zero[i][m][t] = 0u;
-                        if (ZEROS && w < p.tiles && piece < per) {
-                            const int k0 = (piece0 + piece) * kPiece;
-                            const uint16_t* z = p.zeros + (long long)w * p.groups * 8 + g;
-                            const uint32_t z0 = __ldg(z + k0 / p.group * 8);
-                            zero[i][m][t] = z0 | (p.group == 32 ? (uint32_t)__ldg(z + (k0 / 32 + 1) * 8) : z0) << 16;
-                        }
-                    }
-        };
-        load(turn);
+        const int halves = 2 * kPiece / p.group, half_shift = p.group == 32 ? 0 : p.group == 64 ? 1 : 2;  // groups of a stage; which of them its halves of a piece (32 k) lie in
         for (int st = turn; st < stages; st += C::kWideners) {
             const int a = st % C::kStages, c = st % C::kWords, pieces = min(per - 2 * st, 2);
-            uint32_t now_zero[2][MT][2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) now_zero[i][m][t] = zero[i][m][t];
-            if (st + C::kWideners < stages) load(st + C::kWideners);
             if (!tc::warp_all(mbar_wait(&w_full[c], st / C::kWords & 1, ctx, kStatusInt4WordsFull))) break;
-            uint4 now[2][MT][2];
+            const unsigned char* from = smem + C::oWords + c * C::kWordBytes;
+            uint4 now[2][2];
+            uint32_t zero[2][2][2];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
+                for (int t = 0; t < 2; ++t) {
+                    now[i][t] = *reinterpret_cast<const uint4*>(from + (q * 2 + t) * 1024 + i * 512 + lane * 16);
 #pragma unroll
-                    for (int t = 0; t < 2; ++t)
-                        now[i][m][t] = *reinterpret_cast<const uint4*>(smem + C::oWords + c * C::kWordBytes + (m * 8 + q * 2 + t) * 1024 + i * 512 + lane * 16);
+                    for (int h = 0; h < 2; ++h)
+                        if constexpr (ZEROS) zero[i][t][h] = reinterpret_cast<const uint16_t*>(from + C::oZeros)[((q * 2 + t) * halves + ((2 * i + h) >> half_shift)) * 8 + g];
+                }
             if (!tc::warp_all(mbar_wait(&a_empty[a], (st / C::kStages & 1) ^ 1u, ctx, kStatusInt4AEmpty))) break;
             tc::fence_after_sync();
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 if (i >= pieces) break;
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
+                for (int t = 0; t < 2; ++t) {
+                    const uint32_t words[4] = {now[i][t].x, now[i][t].y, now[i][t].z, now[i][t].w};
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        const uint32_t words[4] = {now[i][m][t].x, now[i][m][t].y, now[i][m][t].z, now[i][m][t].w};
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {  // 32 k: their group's zero points
-                            uint32_t lo = 0x43084308u, hi = 0x43084308u;
-                            if constexpr (ZEROS) {
-                                lo = __byte_perm(now_zero[i][m][t], 0x43434343u, h ? 0x4242 : 0x4040), hi = __byte_perm(now_zero[i][m][t], 0x43434343u, h ? 0x4343 : 0x4141);
-                            }
-                            uint32_t f[4], e[4];
-                            widen(words[2 * h], lo, hi, f);
-                            widen(words[2 * h + 1], lo, hi, e);
-                            const uint32_t r[8] = {f[0], f[1], f[2], f[3], e[0], e[1], e[2], e[3]};
-                            tc::tmem_st_pairs(stages0 + a * C::kStageCols + m * 64 + i * 32 + h * 16 + ((uint32_t)(q * 32 + t * 16) << 16), r);
-                        }
+                    for (int h = 0; h < 2; ++h) {  // 32 k: their group's zero points
+                        uint32_t lo = 0x43084308u, hi = 0x43084308u;
+                        if constexpr (ZEROS) lo = __byte_perm(zero[i][t][h], 0x43434343u, 0x4040), hi = __byte_perm(zero[i][t][h], 0x43434343u, 0x4141);
+                        uint32_t f[4], e[4];
+                        widen(words[2 * h], lo, hi, f);
+                        widen(words[2 * h + 1], lo, hi, e);
+                        const uint32_t r[8] = {f[0], f[1], f[2], f[3], e[0], e[1], e[2], e[3]};
+                        tc::tmem_st_pairs(stages0 + a * C::kStageCols + i * 32 + h * 16 + ((uint32_t)(q * 32 + t * 16) << 16), r);
                     }
+                }
             }
             tc::tmem_st_wait();
             tc::fence_before_sync();
@@ -476,9 +451,9 @@ __global__ void __launch_bounds__(Many<N, MT>::kThreads, Many<N, MT>::kBlocks) i
             if (lane == 0) mbar_arrive(&a_full[a]), mbar_arrive(&w_empty[c]);
         }
     } else if (warp >= C::kSumWarp) {
-        const int sg = (warp - C::kSumWarp) >> 2, q = warp & 3, m = MT == 2 ? sg : 0, col0 = MT == 2 ? 0 : sg * C::kSumCols;
-        const int w = (mt * MT + m) * 8 + q * 2 + (lane >> 4);  // this lane's tile of 16 weight rows
-        const int o = ((mt * MT + m) * 128) + q * 32 + lane;
+        const int sg = (warp - C::kSumWarp) >> 2, q = warp & 3, col0 = sg * C::kSumCols;
+        const int w = mt * 8 + q * 2 + (lane >> 4);  // this lane's tile of 16 weight rows
+        const int o = mt * 128 + q * 32 + lane;
         const bool there = w < p.tiles;
         const uint16_t* scale = p.scales + ((long long)(there ? w : 0) * p.groups * 8 + (lane & 7)) * 2 + (lane >> 3 & 1);
         const int group0 = piece0 * kPiece / p.group, jobs = per * kPiece / p.group;
@@ -611,24 +586,32 @@ int few_launch(Int4Params& p, unsigned blocks, cudaStream_t stream) {
     return launch_early(int4_few_kernel<G, ZEROS>, dim3(blocks), kFewThreads, p.x_bytes + p.stages * F::kStage, stream, p);
 }
 
-template <int N, int MT, bool ZEROS>
-int many_launch(ManyParams& p, const uint16_t* x, long long ldx, cudaStream_t stream) {
-    using C = Many<N, MT>;
+template <int N, bool ZEROS>
+int many_launch(ManyParams& p, const uint16_t* x, long long ldx, const unsigned char* w, const Int4Layout& at, cudaStream_t stream) {
+    using C = Many<N>;
     EncodeTiled enc = encode_tiled();
     if (enc == nullptr) return (int)cudaErrorNotSupported;
-    const cuuint64_t dims[2] = {(cuuint64_t)p.k, (cuuint64_t)p.rows}, strides[1] = {(cuuint64_t)ldx * 2};
-    const cuuint32_t box[2] = {kPiece, N}, estr[2] = {1u, 1u};
-    if (enc(&p.tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<uint16_t*>(x), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    auto map = [&](CUtensorMap* to, CUtensorMapDataType type, const void* from, long long inner, long long outer, long long pitch, int box_inner, int box_outer, CUtensorMapSwizzle swizzle) {
+        const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer}, strides[1] = {(cuuint64_t)pitch};
+        const cuuint32_t box[2] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer}, estr[2] = {1u, 1u};
+        return enc(to, type, 2, const_cast<void*>(from), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    };
+    const int per_stage = 2 * kPiece / p.group;
+    const long long groups = at.groups;
+    if (!map(&p.tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, p.k, p.rows, ldx * 2, kPiece, N, CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !map(&p.tm_words, CU_TENSOR_MAP_DATA_TYPE_UINT32, w, at.pieces * 128, at.tiles, at.pieces * 512, 256, 8, CU_TENSOR_MAP_SWIZZLE_NONE) ||
+        !map(&p.tm_scales, CU_TENSOR_MAP_DATA_TYPE_UINT32, w + at.scales, groups * 8, at.tiles, groups * 32, per_stage * 8, 8, CU_TENSOR_MAP_SWIZZLE_NONE) ||
+        (ZEROS && !map(&p.tm_zeros, CU_TENSOR_MAP_DATA_TYPE_UINT16, w + at.zeros, groups * 8, at.tiles, groups * 16, per_stage * 8, 8, CU_TENSOR_MAP_SWIZZLE_NONE)))
         return (int)cudaErrorNotSupported;
-    p.m_tiles = (p.n + 128 * MT - 1) / (128 * MT);
+    p.m_tiles = (p.n + 127) / 128;
     const long long tiles = (long long)p.m_tiles * ((p.rows + N - 1) / N), room = (long long)sm_count() * C::kBlocks;
     p.split = 1;
-    if (MT == 1)  // parts of k for the blocks of a cluster, of whole stages and groups, while all blocks run at once
-        for (int s = 8; s > 1 && p.split == 1; s /= 2)
-            if (p.pieces % (2 * s) == 0 && p.pieces / s >= 4 && tiles * s <= room) p.split = s;
+    // Parts of k for the blocks of a cluster, of whole stages and groups, while all blocks run at once.
+    for (int s = 8; s > 1 && p.split == 1; s /= 2)
+        if (p.pieces % (2 * s) == 0 && p.pieces / s >= 4 && tiles * s <= room) p.split = s;
     if (tiles * p.split > 0x7fffffff) return kInvalid;
-    cudaError_t e = cudaFuncSetAttribute(int4_many_kernel<N, MT, ZEROS>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes);
+    cudaError_t e = cudaFuncSetAttribute(int4_many_kernel<N, ZEROS>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes);
     if (e != cudaSuccess) return (int)e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(tiles * p.split));
@@ -646,7 +629,7 @@ int many_launch(ManyParams& p, const uint16_t* x, long long ldx, cudaStream_t st
     }
     cfg.attrs = attr;
     cfg.numAttrs = na;
-    return (int)cudaLaunchKernelEx(&cfg, int4_many_kernel<N, MT, ZEROS>, p);
+    return (int)cudaLaunchKernelEx(&cfg, int4_many_kernel<N, ZEROS>, p);
 }
 
 }  // namespace
@@ -684,17 +667,16 @@ extern "C" int32_t glm53f_kda_proj_int4(const uint16_t* x, int64_t ldx, const vo
     const int x_bytes = (int)(((long long)(rows < kFewRows ? rows : kFewRows) * (k + kRowPad) * 2 + 127) / 128 * 128);
     if (rows > kFewRows || x_bytes > kFewX) {
         ManyParams m{};
-        m.codes = reinterpret_cast<const uint4*>(w), m.scales = reinterpret_cast<const uint16_t*>(w + at.scales);
-        m.zeros = zeros ? reinterpret_cast<const uint16_t*>(w + at.zeros) : nullptr;
         m.out = out, m.ldo = ldo, m.rows = rows, m.n = n, m.k = k, m.out_f32 = out_f32 != 0, m.group = group;
+        m.scales = reinterpret_cast<const uint16_t*>(w + at.scales);
         m.tiles = (int)at.tiles, m.pieces = (int)at.pieces, m.groups = (int)at.groups;
         m.status = status;
         auto launch = [&](auto z) {
             constexpr bool Z = decltype(z)::value;
-            if (rows <= 16) return many_launch<16, 1, Z>(m, x, ldx, on);
-            if (rows <= 32) return many_launch<32, 1, Z>(m, x, ldx, on);
-            if (rows <= 64) return many_launch<64, 1, Z>(m, x, ldx, on);
-            return many_launch<128, 1, Z>(m, x, ldx, on);
+            if (rows <= 16) return many_launch<16, Z>(m, x, ldx, w, at, on);
+            if (rows <= 32) return many_launch<32, Z>(m, x, ldx, w, at, on);
+            if (rows <= 64) return many_launch<64, Z>(m, x, ldx, w, at, on);
+            return many_launch<128, Z>(m, x, ldx, w, at, on);
         };
         return zeros ? launch(std::true_type{}) : launch(std::false_type{});
     }
