@@ -36,6 +36,7 @@ constexpr int kWarps = kRows / kPer;  // of a group
 constexpr int kGroups = 2;
 constexpr int kAcross = 8;     // tiles that a look takes in at once
 constexpr int kMostShared = 226 * 1024;
+constexpr int kMost = 1 << 30;  // channels, rows: their tiles' ends are ints
 
 // Every wait is bounded; the codes say which one gave up.
 enum : int { kStatusScanChain = 160, kStatusScanEmpty = 161, kStatusScanFull = 162, kStatusScanSums = 163, kStatusScanStart = 164 };
@@ -895,7 +896,7 @@ int tiles_launch(ScanParams& p, int max_len, void* workspace, int64_t workspace_
 }
 
 bool common_ok(int32_t channels, int32_t batch, const int32_t* cu, int32_t flags) {
-    return channels >= 1 && batch >= 0 && (flags & ~kAllFlags) == 0 && (batch == 0 || cu != nullptr);
+    return channels >= 1 && channels <= kMost && batch >= 0 && (flags & ~kAllFlags) == 0 && (batch == 0 || cu != nullptr);
 }
 bool state_ok(const void* state) { return state != nullptr && (reinterpret_cast<uintptr_t>(state) & 3) == 0; }
 
@@ -904,7 +905,7 @@ bool state_ok(const void* state) { return state != nullptr && (reinterpret_cast<
 
 extern "C" int64_t glm53f_kda_scan_workspace_bytes(int32_t channels, int32_t batch, int32_t rows) {
     using namespace kda;
-    if (channels < 1 || batch < 1 || rows < 0) return 0;
+    if (channels < 1 || channels > kMost || batch < 1 || rows < 0 || rows > kMost) return 0;
     return Layout(channels, batch, rows).bytes;
 }
 
@@ -937,7 +938,7 @@ extern "C" int glm53f_kda_scan_prefill_varlen(int32_t channels, int32_t batch, c
                                               const int64_t* state_off, void* out, int64_t out_stride, float* saves, void* workspace, int64_t workspace_bytes,
                                               glm53f_stream_t stream) {
     using namespace kda;
-    if (!common_ok(channels, batch, cu_rows, flags) || rows < 0 || max_len < 0 || max_len > rows || workspace_bytes < 0) return kInvalid;
+    if (!common_ok(channels, batch, cu_rows, flags) || rows < 0 || rows > kMost || max_len < 0 || max_len > rows || workspace_bytes < 0) return kInvalid;
     if (batch == 0) return 0;
     ScanParams p{};
     p.channels = channels, p.batch = batch, p.rows = rows, p.flags = flags, p.cu = cu_rows;
@@ -956,7 +957,7 @@ extern "C" int glm53f_kda_scan_backward_varlen(int32_t channels, int32_t batch, 
                                                int64_t dg_stride, void* dx, int64_t dx_stride, void* workspace, int64_t workspace_bytes,
                                                glm53f_stream_t stream) {
     using namespace kda;
-    if (!common_ok(channels, batch, cu_rows, flags) || rows < 0 || max_len < 0 || max_len > rows || workspace_bytes < 0) return kInvalid;
+    if (!common_ok(channels, batch, cu_rows, flags) || rows < 0 || rows > kMost || max_len < 0 || max_len > rows || workspace_bytes < 0) return kInvalid;
     if (batch == 0) return 0;
     ScanParams p{};
     p.channels = channels, p.batch = batch, p.rows = rows, p.flags = flags, p.cu = cu_rows;

@@ -572,7 +572,7 @@ __global__ void int4_pack_kernel(const uint8_t* codes, const uint16_t* scales, c
 }
 
 bool shape_ok(int32_t n, int32_t k, int32_t group) {
-    return n >= 1 && k >= kPiece && k % kPiece == 0 && k <= 65536 && (group == 32 || group == 64 || group == 128) && k % group == 0;
+    return n >= 1 && n <= 1 << 30 && k >= kPiece && k % kPiece == 0 && k <= 65536 && (group == 32 || group == 64 || group == 128) && k % group == 0;
 }
 bool on16(const void* p) { return p != nullptr && (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -605,7 +605,7 @@ int many_launch(ManyParams& p, const uint16_t* x, long long ldx, const unsigned 
         (ZEROS && !map(&p.tm_zeros, CU_TENSOR_MAP_DATA_TYPE_UINT16, w + at.zeros, groups * 8, at.tiles, groups * 16, per_stage * 8, 8, CU_TENSOR_MAP_SWIZZLE_NONE)))
         return (int)cudaErrorNotSupported;
     p.m_tiles = (p.n + 127) / 128;
-    const long long tiles = (long long)p.m_tiles * ((p.rows + N - 1) / N), room = (long long)sm_count() * C::kBlocks;
+    const long long tiles = (long long)p.m_tiles * ((p.rows - 1) / N + 1), room = (long long)sm_count() * C::kBlocks;
     p.split = 1;
     // Parts of k for the blocks of a cluster, of whole stages and groups, while all blocks run at once.
     for (int s = 8; s > 1 && p.split == 1; s /= 2)
@@ -659,7 +659,6 @@ extern "C" int32_t glm53f_kda_proj_int4(const uint16_t* x, int64_t ldx, const vo
     if (rows == 0) return 0;
     if (!on16(x) || !on16(packed) || out == nullptr || (reinterpret_cast<uintptr_t>(out) & (out_f32 ? 3 : 1))) return kInvalid;
     const Int4Layout at(n, k, group, zeros != 0);
-    if (at.tiles > 0x3fffffff) return kInvalid;
     const auto* w = static_cast<const unsigned char*>(packed);
     int* status = status_word();
     if (status == nullptr) return (int)cudaErrorUnknown;

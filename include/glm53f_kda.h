@@ -533,7 +533,7 @@ int glm53f_kda_accept_batch(int32_t batch, const int32_t* cu_rows, int32_t vocab
  * GLM53F_KDA_SCAN_COMPLEMENT 1 - a_t.
  *
  * Common arguments:
- *   channels, batch   channels of a row (1 or more); requests
+ *   channels, batch   channels of a row (1 to 2^30); requests
  *   cu_rows           as in Part 3: ascending, row ranges of the requests, some of which may have no rows
  *   g, x, out         row r at + r * stride (elements), [channels]; g f32, or bf16 with GLM53F_KDA_SCAN_G_BF16; x and out (and their gradients)
  *                     f32, or bf16 with GLM53F_KDA_SCAN_X_BF16; aligned to their elements, strides at least the channels.  Log decays are at most 0, -inf
@@ -554,7 +554,7 @@ int glm53f_kda_scan_decode_batch(int32_t channels, int32_t batch, const int32_t*
                                  const void* x, int64_t x_stride, int32_t flags, const float* state_in, float* state_out,
                                  const int64_t* state_off, void* out, int64_t out_stride, glm53f_stream_t stream);
 
-/* Packed sequences, the longest of at most max_len (host) rows; rows (host) >= cu_rows[batch].  A request without rows passes its state through.  out may be NULL (states only).
+/* Packed sequences, the longest of at most max_len (host) rows; rows (host) >= cu_rows[batch], at most 2^30.  A request without rows passes its state through.  out may be NULL (states only).
  * `saves` (8-byte aligned; NULL: none) takes the states that the backward pass starts from, glm53f_kda_scan_saves_rows(batch, rows) x channels f32 values.
  * `workspace` (16-byte aligned) of glm53f_kda_scan_workspace_bytes(channels, batch, rows) bytes lets sequences of more than 64 rows run in parts at once; with fewer (0 and
  * NULL among them) one block walks each 64 channels of a sequence.  It is the call's own until the call has run.  A sequence's results are the same bits with

@@ -86,7 +86,7 @@ int32_t glm53f_kda_proj_bf16_fused(const glm53f_proj_job* job, const glm53f_proj
  *   codes    [n][k / 2] bytes: value 2 i in the low half of byte i, 2 i + 1 in the high
  *   scales   bf16 [n][k / group]
  *   zeros    bytes [n][k / group], or NULL
- * n >= 1, k % 64 == 0, k % group == 0, k <= 65,536.  The packed bytes are read by glm53f_kda_proj_int4 with the same n, k, group and `zeros` != 0 where they were given. */
+ * 1 <= n <= 2^30, k % 64 == 0, k % group == 0, k <= 65,536.  The packed bytes are read by glm53f_kda_proj_int4 with the same n, k, group and `zeros` != 0 where they were given. */
 int64_t glm53f_kda_int4_bytes(int32_t n, int32_t k, int32_t group, int32_t zeros);
 int32_t glm53f_kda_int4_pack(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int32_t n, int32_t k, int32_t group, void* packed,
                              glm53f_stream_t stream);
