@@ -818,6 +818,19 @@ struct Layout {  // of the workspace: bytes from its start
     }
 };
 
+// Whether a call's sequences are divided, or one block walks each 64 channels of a sequence.  A walked tile has nothing to wait for: 0.6 us by itself and 0.87 with all SMs at it, against
+// 1.3 us a tile of an SM's share and 5 us more where tiles look back; without tensor copies 1.3 to 3.1 us against 1.9 to 3.5.  A walk takes as long as its
+// busiest block.  Measured, us walked and divided (f32 g, bf16 x): 4,096 channels 100 rows 4.0 and 6.4, 2,000 rows 22.6 and 23.6, 4,000 rows 39.9 and 38.1, 8,192 rows 76 and 69;
+// 1,024 channels 1,000 rows 11.6 and 9.2, 16 x 1,000 rows 27 and 43; 64 channels 300 rows 5.4 and 5.8, 3,000 rows 29 and 7.6; there and back 2,048 channels, 16,289 rows in four sequences 163 and 200;
+// 1,001 channels (no tensor copies) 1,000 rows 41 and 13.
+bool divide(const Layout& at, int batch, int max_len, bool boxes) {
+    if (max_len <= kRows) return false;
+    const long long items = at.stripes * batch, sms = sm_count(), longest = (max_len + kRows - 1) / kRows, tiles = at.slots * at.stripes;
+    const long long share = (tiles + sms - 1) / sms;
+    const long long walked = items <= sms || share + longest / 2 < longest ? longest : share + longest / 2;  // by the busiest block
+    return walked > (boxes ? 2 * share + 7 : share + 2);
+}
+
 bool even(const void* p, bool bf16) { return (reinterpret_cast<uintptr_t>(p) & (bf16 ? 3 : 7)) == 0; }
 bool aligned(const void* p, bool bf16) { return (reinterpret_cast<uintptr_t>(p) & (bf16 ? 1 : 3)) == 0; }
 
@@ -867,11 +880,11 @@ int tiles_launch(ScanParams& p, int max_len, void* workspace, int64_t workspace_
     p.stripes = (int)at.stripes;
     p.status = status_word();
     if (p.status == nullptr) return (int)cudaErrorUnknown;
-    const bool look = max_len > kRows && workspace != nullptr && workspace_bytes >= at.bytes;
     const bool gb = p.flags & GLM53F_KDA_SCAN_G_BF16, xb = p.flags & GLM53F_KDA_SCAN_X_BF16;
     p.boxes = row_boxes(&p.tm_g, {p.g, p.g_stride, gb}, p.channels, p.rows) && row_boxes(&p.tm_x, {p.x, p.x_stride, xb}, p.channels, p.rows) &&
               (!BACKWARD || row_boxes(&p.tm_dout, {p.dout, p.dout_stride, xb}, p.channels, p.rows));
     p.tiles = at.stripes * p.batch;
+    const bool look = workspace != nullptr && workspace_bytes >= at.bytes && divide(at, p.batch, max_len, p.boxes);
     if (look) {
         auto* w = static_cast<unsigned char*>(workspace);
         p.control = reinterpret_cast<unsigned*>(w);

@@ -556,8 +556,8 @@ int glm53f_kda_scan_decode_batch(int32_t channels, int32_t batch, const int32_t*
 
 /* Packed sequences, the longest of at most max_len (host) rows; rows (host) >= cu_rows[batch], at most 2^30.  A request without rows passes its state through.  out may be NULL (states only).
  * `saves` (8-byte aligned; NULL: none) takes the states that the backward pass starts from, glm53f_kda_scan_saves_rows(batch, rows) x channels f32 values.
- * `workspace` (16-byte aligned) of glm53f_kda_scan_workspace_bytes(channels, batch, rows) bytes lets sequences of more than 64 rows run in parts at once; with fewer (0 and
- * NULL among them) one block walks each 64 channels of a sequence.  It is the call's own until the call has run.  A sequence's results are the same bits with
+ * `workspace` (16-byte aligned) of glm53f_kda_scan_workspace_bytes(channels, batch, rows) bytes lets long sequences of few channels run in parts at once; with fewer (0 and
+ * NULL among them) one block walks each 64 channels of a sequence, as it does where there are enough of them.  It is the call's own until the call has run.  A sequence's results are the same bits with
  * any workspace and beside any other requests; they agree with the row-by-row form's to the rounding of f32. */
 int64_t glm53f_kda_scan_workspace_bytes(int32_t channels, int32_t batch, int32_t rows);
 int64_t glm53f_kda_scan_saves_rows(int32_t batch, int32_t rows);
