@@ -7,8 +7,12 @@
 // lane of a warp, the four k steps' fragments a word each; in a word the pairs of neighbouring k lie 16 bits apart, so that a shift, a mask and one
 // or put two of them into bf16s of 128 + q, from which 128 + z is taken.
 //
-// Few rows (this kernel): bound by HBM, the weights' bytes, and next to it by the seven operations that two words of weights cost.  A block an SM; the rows lie in its shared memory, its warps
-// divide the k of a tile between them, pieces on their way in registers eight deep, across tiles; the warps' sums meet in shared memory once a tile.
+// Few rows (this kernel): bound by HBM, the weights' bytes, and next to it by the eleven operations that a word of eight weights costs.  A block an SM; a warp copies tiles in bulk into a ring
+// of shared memory, 120 to 190 KB ahead; the rows lie beside it; sixteen warps divide the k of a tile between them, two pieces at a time, and their sums meet in
+// shared memory once a tile.  24,640 x 4,096 in groups of 128: 17.4 us a row (3.0 TB/s; 14.2 without widening and products), 18.7 for eight; 4,096 x 8,192: 7 and 8.6 us.
+// (Loads into registers eight pieces ahead shared their scoreboards, so that each waited for all: 21.5 us.  One piece a stage, whose waiting and addresses cost as
+// much as its products: 21.6 us.)  Eight rows are one instruction's columns and cost what one does; from nine on, or where they do not fit, the other kernel takes them: eight
+// rows take it 23.0, 11.4 and, of 500 x 512, 4.5 us, and this one 18.7, 8.5 and 2.6.
 
 #include <type_traits>
 
@@ -241,6 +245,11 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
 //   warps 4-      widen, 128 k at a time, two such stages in tensor memory
 //   the others    sum: a warpgroup for each kSumCols columns
 // Few tiles: the blocks of a cluster share a tile's k and add their sums, each for some rows, in rank order through distributed shared memory.
+//
+// N is the smallest that holds the rows, 128 at most (64 for more than 64 rows: 100 rows x 4,096 x 8,192 26.9 us against 20.8, 700 rows 133 against 113, 2,048 rows 195 against 145; only
+// 500 x 512 is faster, 7.3 against 8.9).  Bound by the issue of widening and summing and by the chain from words to sums: 2,048 rows x 4,096 x 8,192 in groups of 128 take
+// 145 to 159 us, 0.5 of the measured bf16 rate (their products alone 83); groups of 64 217, of 32 384, a fetch of the accumulator for each.  40 rows in groups of 64 with zero points 16.7 us.
+// (Scales and zero points fetched a few groups ahead, without L2 asked before: 154 and 21.3 us.)
 
 enum : int { kStatusInt4Empty = 170, kStatusInt4Full = 171, kStatusInt4AEmpty = 172, kStatusInt4AFull = 173, kStatusInt4AccEmpty = 174, kStatusInt4AccFull = 175, kStatusInt4Words = 176, kStatusInt4WordsFull = 177 };
 
