@@ -8,7 +8,7 @@
 // or put two of them into bf16s of 128 + q, from which 128 + z is taken.
 //
 // Few rows (this kernel): bound by HBM, the weights' bytes, and next to it by the eleven operations that a word of eight weights costs.  A block an SM; a warp copies tiles in bulk into a ring
-// of shared memory, 120 to 190 KB ahead; the rows lie beside it; sixteen warps divide the k of a tile between them, two pieces at a time, and their sums meet in
+// of shared memory, 58 KB (many long rows) to 200 KB ahead; the rows lie beside it; sixteen warps divide the k of a tile between them, two pieces at a time, and their sums meet in
 // shared memory once a tile.  24,640 x 4,096 in groups of 128: 17.4 us a row (3.0 TB/s; 14.2 without widening and products), 18.7 for eight; 4,096 x 8,192: 7 and 8.6 us.
 // (Loads into registers eight pieces ahead shared their scoreboards, so that each waited for all: 21.5 us.  One piece a stage, whose waiting and addresses cost as
 // much as its products: 21.6 us.)  Eight rows are one instruction's columns and cost what one does; from nine on, or where they do not fit, the other kernel takes them: eight
