@@ -242,13 +242,13 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
 //   warp 0        tensor copies of x (64 k x N rows, 128-byte swizzle) into a ring
 //   warps 1, 3    the matrix instructions (a stage each in turn, with groups of 128: the waits of a stage take one warp longer than its products the tensor cores)
 //   warp 2        bulk copies of the packed words, 128 k at a time, into another
-//   warps 4-      widen, 128 k at a time, two such stages in tensor memory
+//   warps 4-      widen, 128 k at a time, two or four such stages in tensor memory
 //   the others    sum: a warpgroup for each kSumCols columns
 // Few tiles: the blocks of a cluster share a tile's k and add their sums, each for some rows, in rank order through distributed shared memory.
 //
 // N is the smallest that holds the rows, 128 at most (64 for more than 64 rows: 100 rows x 4,096 x 8,192 26.9 us against 20.8, 700 rows 133 against 113, 2,048 rows 195 against 145; only
 // 500 x 512 is faster, 7.3 against 8.9).  Bound by the issue of widening and summing and by the chain from words to sums: 2,048 rows x 4,096 x 8,192 in groups of 128 take
-// 145 to 159 us, 0.5 of the measured bf16 rate (their products alone 83); groups of 64 217, of 32 384, a fetch of the accumulator for each.  40 rows in groups of 64 with zero points 16.7 us.
+// 145 to 159 us, 0.5 of the measured bf16 rate (their products alone 83); groups of 64 217, of 32 384, a fetch of the accumulator for each.  40 rows in groups of 64 with zero points 14.9 us.
 // (Scales and zero points fetched a few groups ahead, without L2 asked before: 154 and 21.3 us.)
 
 enum : int { kStatusInt4Empty = 170, kStatusInt4Full = 171, kStatusInt4AEmpty = 172, kStatusInt4AFull = 173, kStatusInt4AccEmpty = 174, kStatusInt4AccFull = 175, kStatusInt4Words = 176, kStatusInt4WordsFull = 177 };
@@ -268,12 +268,14 @@ template <int N>
 struct Many {
     static constexpr int kSumCols = N < 32 ? N : 32 * ((N + 63) / 64);  // (N = 128: 64)
     static constexpr int kSumGroups = N / kSumCols;
-    static constexpr int kWideners = N <= 64 ? 1 : 2;     // warpgroups that widen, a stage each in turn (of small tiles two blocks share an SM)
+    // Warpgroups that widen, a stage each in turn.  Up to 32 rows one, two blocks an SM; more: two, one block.  (4,096 x 8,192, groups of 64, us, one and two: 16 rows 12.1 and 12.8, 40 rows 16.8 and
+    // 14.9; 24,640 x 4,096 16 rows 23.3 and 28.0, 40 rows 32.4 and 33.8.)
+    static constexpr int kWideners = N <= 32 ? 1 : 2;
     static constexpr int kSumWarp = 4 + 4 * kWideners;    // the first warp that sums
     static constexpr int kThreads = 32 * kSumWarp + 128 * kSumGroups;
     static constexpr int kBoxBytes = N * 128;             // 64 k of x
     static constexpr int kRing = N <= 32 ? 6 : 4;         // stages of 128 k: of x
-    static constexpr int kStages = N == 128 ? 4 : 2;      // ... in tensor memory (even, as the rings are: each of two warps that take turns then meets every phase of a place)
+    static constexpr int kStages = N <= 32 ? 2 : 4;      // ... in tensor memory (even, as the rings are: each of two warps that take turns then meets every phase of a place)
     static constexpr int kStageCols = 64;
     static constexpr int kAccs = 2;                       // accumulators, a group's products each
     static constexpr int kAccCols = kAccs * N;
