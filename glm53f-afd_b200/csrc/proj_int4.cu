@@ -246,8 +246,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
 //   the others    sum: a warpgroup for each kSumCols columns
 // Few tiles: the blocks of a cluster share a tile's k and add their sums, each for some rows, in rank order through distributed shared memory.
 //
-// N is the smallest that holds the rows, 128 at most (64 for more than 64 rows: 100 rows x 4,096 x 8,192 26.9 us against 20.8, 700 rows 133 against 113, 2,048 rows 195 against 145; only
-// 500 x 512 is faster, 7.3 against 8.9).  Bound by the issue of widening and summing and by the chain from words to sums: 2,048 rows x 4,096 x 8,192 in groups of 128 take
+// N is the smallest that holds the rows, 128 at most (64 for more than 64 rows: 100 rows x 4,096 x 8,192 23.5 us against 20.8, 400 rows 76 against 58, 2,048 rows 202 against 145; only
+// 500 x 512 is faster, 6.6 against 8.9).  Bound by the issue of widening and summing and by the chain from words to sums: 2,048 rows x 4,096 x 8,192 in groups of 128 take
 // 145 to 159 us, 0.5 of the measured bf16 rate (their products alone 83); groups of 64 217, of 32 384, a fetch of the accumulator for each.  40 rows in groups of 64 with zero points 14.9 us.
 // (Scales and zero points fetched a few groups ahead, without L2 asked before: 154 and 21.3 us.)
 
