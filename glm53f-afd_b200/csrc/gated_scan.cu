@@ -362,7 +362,7 @@ struct Tiles {
                 at.b = sequence_of(p.cu, p.batch, at.slot);
                 place_sequence(p, at);
                 at.tile = at.slot - slot_of(at.first, at.b);
-                if (at.tile < at.tiles) return at;  // (else a slot between two sequences)
+                if (at.tile >= 0 && at.tile < at.tiles) return at;  // (else a slot between two sequences, or before the first one's rows)
             }
         } else {
             if (seen.b >= 0 && walked == seen.tiles) item += gridDim.x, seen.b = -1;
