@@ -312,6 +312,12 @@ __device__ __forceinline__ float peer_load(const void* local, uint32_t rank) {
     return v;
 }
 
+// Where a block's tensor memory begins, known when it is compiled.
+template <uint32_t AT>
+struct Column {
+    __device__ __forceinline__ constexpr operator uint32_t() const { return AT; }
+};
+
 // ZEROS: zero points are read; without them they are a constant (their forming takes a fifth of what widening does).
 template <int N, bool ZEROS>
 __global__ void __launch_bounds__(Many<N>::kThreads, Many<N>::kBlocks) int4_many_kernel(const __grid_constant__ ManyParams p) {
@@ -377,10 +383,10 @@ __global__ void __launch_bounds__(Many<N>::kThreads, Many<N>::kBlocks) int4_many
         const uint32_t leader = tc::elect_one();
         // The warp converged, one lane issuing, a stage's eight k steps unrolled for the group's size: little stands between two instructions (a loop that asks at each step
         // whether a group begins or ends took 190 cycles a step, three times the product's).  Of a descriptor only the low half changes, and where the tensor
-        // memory begins is a constant, so that every operand is computed in uniform registers.
+        // memory begins is a constant wherever this kernel is alone on the SM, so that every operand is computed in uniform registers.
         auto products = [&](auto group_steps, auto begin) {
             constexpr int js = decltype(group_steps)::value;  // k steps of 16 of a group
-            constexpr uint32_t tm0 = decltype(begin)::value, stage0 = tm0 + C::kAccCols;
+            const uint32_t tm0 = begin, stage0 = tm0 + C::kAccCols;
             constexpr uint64_t high = (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61 | (uint64_t)(16 >> 4) << 16;
             const uint32_t ring0 = (smem_u32(smem) & 0x3FFFFu) >> 4;
             // With groups of 128 two warps take turns, each with an accumulator of its own; smaller groups use both within a stage, and a wait tells two of an accumulator's phases
@@ -413,9 +419,10 @@ __global__ void __launch_bounds__(Many<N>::kThreads, Many<N>::kBlocks) int4_many
             else if (p.group == 64) products(std::integral_constant<int, 4>{}, begin);
             else products(std::integral_constant<int, 2>{}, begin);
         };
-        // (All 512 columns begin at 0; 256 at 0 or 256.)
-        if (C::kCols == 512 || tm == 0) from(std::integral_constant<uint32_t, 0>{});
-        else from(std::integral_constant<uint32_t, 256>{});
+        // All 512 columns begin at 0; 256 at 0 or 256 beside another block of this kernel, and anywhere beside another kernel's smaller part.
+        if (C::kCols == 512 || tm == 0) from(Column<0>{});
+        else if (tm == 256) from(Column<256>{});
+        else from(tm);
     } else if (warp >= 4 && warp < C::kSumWarp) {
         // Weight rows 32 q .. of each 128: two tiles of 16, the lanes' words of both pieces of a stage.
         const Widen widen;
