@@ -11,8 +11,10 @@
 // of shared memory, 58 KB (many long rows) to 200 KB ahead; the rows lie beside it; sixteen warps divide the k of a tile between them, two pieces at a time, and their sums meet in
 // shared memory once a tile.  24,640 x 4,096 in groups of 128: 17.4 us a row (3.0 TB/s; 14.2 without widening and products), 18.7 for eight; 4,096 x 8,192: 7 and 8.6 us.
 // (Loads into registers eight pieces ahead shared their scoreboards, so that each waited for all: 21.5 us.  One piece a stage, whose waiting and addresses cost as
-// much as its products: 21.6 us.)  Eight rows are one instruction's columns and cost what one does; from nine on, or where they do not fit, the other kernel takes them: eight
-// rows take it 23.0, 11.4 and, of 500 x 512, 4.5 us, and this one 18.7, 8.5 and 2.6.
+// much as its products: 21.6 us.)  Eight rows are one instruction's columns and cost what one does; from nine on the other kernel takes them: eight
+// rows take it 23.0, 11.4 and, of 500 x 512, 4.5 us, and this one 18.7, 8.5 and 2.6.  Rows of more than 150 KB together come with the weights, so that a row's bits depend on nothing but the row: 4,096
+// outputs, eight rows of k = 9,600 10.5 us (38 by the other kernel), 12,288 12.3 (12.5), 16,384 in groups of 64 16.2 (19.1); 8,192 outputs, k = 28,672 46.9 (38.4) and 65,536 104 (81), of which
+// the bits are the price.
 
 #include <type_traits>
 
@@ -54,6 +56,7 @@ struct Int4Params {
     int rows, n, k, out_f32;
     int tiles, pieces, split;  // warps that share a tile
     int x_bytes, stages;       // of shared memory for the rows of x; of the ring behind them
+    int stage;                 // bytes of one
     int* status;
 };
 
@@ -90,16 +93,19 @@ struct Widen {
 
 enum : int { kStatusInt4FewEmpty = 178, kStatusInt4FewFull = 179 };
 
-// A stage of the ring: two pieces (128 k) for each warp, the scales and zero points of their groups.
+// A stage of the ring: two pieces (128 k) for each warp, the scales and zero points of their groups; LONG: and the rows of x over the same k.
 template <int G, bool ZEROS>
 struct Few {
     static constexpr int N = 2 * kPiece / G;                      // groups of a warp's pieces
     static constexpr int kScaleBytes = kPiece * 32 / G;           // of a piece (of 128: half of them, its pieces come in pairs)
     static constexpr int kZeroBytes = ZEROS ? kPiece * 16 / G : 0;
     static constexpr int oScales = kFewWarps * 1024, oZeros = oScales + 2 * kFewWarps * kScaleBytes, kStage = oZeros + 2 * kFewWarps * kZeroBytes;
+    static constexpr int kLongPitch = 2 * kFewWarps * kPiece * 2 + 2 * kRowPad;  // between rows of x
 };
 
-template <int G, bool ZEROS>
+// LONG: rows that do not all fit beside the ring.  They come with the weights, for every tile again (all warps share a tile then), and everything is summed in the same order: what up to eight
+// rows hold, and how many there are, changes no bit of another.
+template <int G, bool ZEROS, bool LONG>
 __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Params p) {
     using F = Few<G, ZEROS>;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -111,8 +117,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
     const int abreast = kFewWarps / p.split;                          // tiles at a time
     const int at_once = 2 * p.split, per = (p.pieces + at_once - 1) / at_once;  // pieces of a tile in a stage; stages of a tile
     const int groups = p.k / G, step = gridDim.x * abreast;
-    const int pitch = (p.k + kRowPad) * 2;
-    unsigned char* ring = smem + p.x_bytes;
+    const int pitch = LONG ? F::kLongPitch : (p.k + kRowPad) * 2, stage = LONG ? p.stage : F::kStage;
+    unsigned char *ring = smem + p.x_bytes, *rows = LONG ? ring + F::kStage : smem;
     if (tid == 0) {
         for (int i = 0; i < p.stages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], kFewWarps);
         mbar_init(&x_full, 1);
@@ -136,11 +142,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
                 if (!tc::warp_all(mbar_wait(&empty[s], ph ^ 1u, ctx, kStatusInt4FewEmpty))) break;
                 if (lane == 0) {
                     ctl[0] = ctl[0] + 1u;
-                    mbar_arrive_expect_tx(&full[s], tiles * pieces * (512 + F::kScaleBytes + F::kZeroBytes));
+                    mbar_arrive_expect_tx(&full[s], tiles * pieces * (512 + F::kScaleBytes + F::kZeroBytes) + (LONG ? p.rows * pieces * kPiece * 2 : 0));
                 }
                 __syncwarp();
+                if (LONG && lane < p.rows) bulk_load(rows + s * stage + lane * pitch, p.x + lane * p.ldx + piece * kPiece, pieces * kPiece * 2, &full[s]);
                 if (lane < tiles) {
-                    unsigned char* to = ring + s * F::kStage;
+                    unsigned char* to = ring + s * stage;
                     const long long group = t * groups + piece * kPiece / G;
                     bulk_load(to + lane * at_once * 512, p.codes + (t * p.pieces + piece) * 32, pieces * 512, &full[s]);
                     bulk_load(to + F::oScales + lane * at_once * F::kScaleBytes, p.scales + group * 8, pieces * F::kScaleBytes, &full[s]);
@@ -150,7 +157,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
             }
         }
     } else {
-        if (warp == 0) {
+        if (!LONG && warp == 0) {
             if (lane == 0) mbar_arrive_expect_tx(&x_full, p.rows * p.k * 2);
             __syncwarp();
             if (lane < p.rows) bulk_load(smem + lane * pitch, p.x + lane * p.ldx, p.k * 2, &x_full);
@@ -159,8 +166,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
         const int kw = warp % p.split, tw = warp / p.split, g = lane >> 2;  // this warp's part of k, its tile of those at a time
         const int xr = lane & 7;
         const bool there = xr < p.rows;
-        const uint32_t xrow = there ? smem_u32(smem + xr * pitch + (lane >> 3) * 16) + kw * kPiece * 4 : smem_u32(&nothing), half = there ? 64u : 0u, xstep = there ? at_once * kPiece * 2 : 0u;
-        mbar_wait(&x_full, 0u, ctx, kStatusInt4FewFull);
+        const uint32_t xrow = there ? smem_u32(rows + xr * pitch + (lane >> 3) * 16) + kw * kPiece * 4 : smem_u32(&nothing), half = there ? 64u : 0u;
+        const uint32_t xstep = !there ? 0u : LONG ? stage : at_once * kPiece * 2;  // from a stage to the next
+        if (!LONG) mbar_wait(&x_full, 0u, ctx, kStatusInt4FewFull);
         int buf = 0;
         // Every warp takes part in each round, with or without a tile, as the barrier needs them.
         for (int tile = blockIdx.x * abreast; tile < p.tiles; tile += step, buf ^= 1) {
@@ -168,7 +176,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
             for (int c = 0; c < per; ++c) {
                 mbar_wait(&full[s], ph, ctx, kStatusInt4FewFull);  // (after a wait that gave up all others do: the sums are lost, the status says so)
                 const int mine = tile + tw < p.tiles ? p.pieces - c * at_once - 2 * kw : 0;  // pieces, of two
-                const unsigned char* from = ring + s * F::kStage;
+                const unsigned char* from = ring + s * stage;
+                const uint32_t xat = xrow + (LONG ? s : c) * xstep;
                 uint4 codes[2];
                 uint32_t scale[F::N], zero[F::N];
                 if (mine > 0) {
@@ -181,10 +190,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
                         if constexpr (ZEROS) zero[j] = *(reinterpret_cast<const uint16_t*>(from + F::oZeros) + at);
                     }
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&empty[s]);
-                if (++s == p.stages) s = 0, ph ^= 1u;
-                const uint32_t xat = xrow + c * xstep;
+                auto taken = [&] {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&empty[s]);
+                    if (++s == p.stages) s = 0, ph ^= 1u;
+                };
+                if (!LONG) taken();
                 constexpr int kSteps = G / 16;  // of a group
                 float d[4] = {};
 #pragma unroll
@@ -210,6 +221,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
                         }
                     }
                 }
+                if (LONG) taken();
             }
             float* to = sums[buf][warp];
             *reinterpret_cast<float2*>(to + g * kFewRows + 2 * (lane & 3)) = make_float2(acc[0], acc[1]);
@@ -594,14 +606,15 @@ bool shape_ok(int32_t n, int32_t k, int32_t group) {
 }
 bool on16(const void* p) { return p != nullptr && (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-template <int G, bool ZEROS>
+template <int G, bool ZEROS, bool LONG>
 int few_launch(Int4Params& p, unsigned blocks, cudaStream_t stream) {
     using F = Few<G, ZEROS>;
-    const int stages = (kFewShared - p.x_bytes) / F::kStage;
+    p.stage = LONG ? (F::kStage + p.rows * F::kLongPitch + 127) / 128 * 128 : F::kStage;
+    const int stages = (kFewShared - p.x_bytes) / p.stage;
     p.stages = stages < kFewStages ? stages : kFewStages;
-    const cudaError_t e = cudaFuncSetAttribute(int4_few_kernel<G, ZEROS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewShared);
+    const cudaError_t e = cudaFuncSetAttribute(int4_few_kernel<G, ZEROS, LONG>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewShared);
     if (e != cudaSuccess) return (int)e;
-    return launch_early(int4_few_kernel<G, ZEROS>, dim3(blocks), kFewThreads, p.x_bytes + p.stages * F::kStage, stream, p);
+    return launch_early(int4_few_kernel<G, ZEROS, LONG>, dim3(blocks), kFewThreads, p.x_bytes + p.stages * p.stage, stream, p);
 }
 
 template <int N, bool ZEROS>
@@ -681,8 +694,7 @@ extern "C" int32_t glm53f_kda_proj_int4(const uint16_t* x, int64_t ldx, const vo
     int* status = status_word();
     if (status == nullptr) return (int)cudaErrorUnknown;
     const cudaStream_t on = reinterpret_cast<cudaStream_t>(stream);
-    const int x_bytes = (int)(((long long)(rows < kFewRows ? rows : kFewRows) * (k + kRowPad) * 2 + 127) / 128 * 128);
-    if (rows > kFewRows || x_bytes > kFewX) {
+    if (rows > kFewRows) {
         ManyParams m{};
         m.out = out, m.ldo = ldo, m.rows = rows, m.n = n, m.k = k, m.out_f32 = out_f32 != 0, m.group = group;
         m.scales = reinterpret_cast<const uint16_t*>(w + at.scales);
@@ -700,15 +712,20 @@ extern "C" int32_t glm53f_kda_proj_int4(const uint16_t* x, int64_t ldx, const vo
     Int4Params p{};
     p.x = x, p.ldx = ldx, p.out = out, p.ldo = ldo, p.rows = rows, p.n = n, p.k = k, p.out_f32 = out_f32 != 0;
     p.codes = reinterpret_cast<const uint4*>(w), p.scales = reinterpret_cast<const uint32_t*>(w + at.scales), p.zeros = reinterpret_cast<const uint16_t*>(w + at.zeros);
-    p.tiles = (int)at.tiles, p.pieces = (int)at.pieces, p.x_bytes = x_bytes, p.status = status;
+    p.tiles = (int)at.tiles, p.pieces = (int)at.pieces, p.status = status;
     p.split = 1;
     while (p.split < kFewWarps && p.split * 4 <= p.pieces) p.split *= 2;
+    const int x_bytes = (rows * (k + kRowPad) * 2 + 127) / 128 * 128;
+    static_assert(kFewX / (2 * kFewRows) - kRowPad >= 2 * kFewWarps * kPiece, "rows that do not fit are long enough for all warps to share a tile");
+    const bool longer = x_bytes > kFewX;
+    p.x_bytes = longer ? 0 : x_bytes;
     const int abreast = kFewWarps / p.split, sms = sm_count();
     const long long want = (at.tiles + abreast - 1) / abreast;
     const unsigned blocks = (unsigned)(want < sms ? want : sms);
     auto launch = [&](auto g) {
         constexpr int G = decltype(g)::value;
-        return zeros ? few_launch<G, true>(p, blocks, on) : few_launch<G, false>(p, blocks, on);
+        if (longer) return zeros ? few_launch<G, true, true>(p, blocks, on) : few_launch<G, false, true>(p, blocks, on);
+        return zeros ? few_launch<G, true, false>(p, blocks, on) : few_launch<G, false, false>(p, blocks, on);
     };
     return group == 32   ? launch(std::integral_constant<int, 32>{})
            : group == 64 ? launch(std::integral_constant<int, 64>{})

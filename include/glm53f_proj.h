@@ -93,7 +93,7 @@ int32_t glm53f_kda_int4_pack(const uint8_t* codes, const uint16_t* scales, const
 
 /* out[m][o] = sum_i x[m][i] * w[o][i] for rows m < rows: x bf16 at x + m * ldx (16-byte aligned, ldx >= k a multiple of 8), out at out + m * ldo (ldo >= n), bf16 or, with
  * out_f32 != 0, f32, memory of its own.  x times code is exact, a group's sum f32, multiplied by its scale in f32: no weight is rounded; the result is rounded once.  rows == 0
- * launches nothing.  Status codes as glm53f_kda_proj_bf16. */
+ * launches nothing.  Up to eight rows have the bits that each has alone; with more, the order of a row's sums depends on how many there are.  Status codes as glm53f_kda_proj_bf16. */
 int32_t glm53f_kda_proj_int4(const uint16_t* x, int64_t ldx, const void* packed, int32_t n, int32_t k, int32_t group, int32_t zeros, int32_t rows,
                              void* out, int32_t out_f32, int64_t ldo, glm53f_stream_t stream);
 
