@@ -431,88 +431,166 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 2) logprob_kernel
     if (p.blocks > 1) cluster_sync();  // nobody leaves while its results may be read
 }
 
-// A block takes kBackThreads x kBackAtOnce pieces of 16 bytes of the gradient's row.  (Plain loads: the gradient may take the logits' place, each thread's pieces its own.)
-constexpr int kBackThreads = 256, kBackAtOnce = 4;
+// Backwards, log p = x / T - lse, whose parts are rounded at their size: p is off by at most 2 |lse| u of itself (u = 2^-24), 128 u for f32 logits up to kOrdinary, less than what a row's sum may be
+// off by, and 512 u, a hundredth of the gradient's own rounding, for bf16.  Beyond it (low temperatures, logits far from 0, rows of nothing but a mask's lowest value) the row's maximum and sum are
+// formed again and log p is (x - max) / T - log S as forwards: no size of x or T does harm, and lse may have overflowed.  Such a row is read twice, by its first block alone; the others leave.  Nothing is
+// asked of other blocks, so the gradient may take the logits' place, each thread's pieces its own (plain loads).
+constexpr int kBackThreads = 256, kBackAtOnce = 4, kBackWarps = kBackThreads / 32;
 template <bool BF16>
-__global__ void __launch_bounds__(kBackThreads) logprob_backward_kernel(const LogprobParams p) {
-    constexpr int E = Row<BF16>::E;
-    grid_ready();
-    const long long row = blockIdx.x / p.blocks;
-    const long long first = (long long)(blockIdx.x % p.blocks) * kBackThreads * kBackAtOnce + threadIdx.x;
-    const Row<BF16> d(p.dlogits, row * p.dld, p.vocab);  // pieces by the gradient's boundaries
-    const Row<BF16> x(p.logits, row * p.ld, p.vocab);
-    const bool same = d.skip == x.skip;
-    const float heat = heat_of(p.temperature, row), inv = 1.0f / heat, lse = __ldg(p.lse + row);
-    const int token = __ldg(p.tokens + row);
-    const bool named = token >= 0 && token < p.vocab;
-    const bool none = lse == -INFINITY;  // a row that masks everything: no gradient
-    const float l = named && !none && p.dlogprob != nullptr ? __ldg(p.dlogprob + row) * inv : 0.0f;
-    const float n = !none && p.dentropy != nullptr ? __ldg(p.dentropy + row) * inv : 0.0f, entropy = n != 0.0f ? __ldg(p.entropy + row) : 0.0f;
-    // -p (n (log p + H) + l), in pairs; the token's value in its piece only.
-    const float from = none ? 0.0f : -lse, minus_l = -fmaf(n, entropy, l);
-    const float2 inv2 = make_float2(inv, inv), from2 = make_float2(from, from), n2 = make_float2(-n, -n), l2 = make_float2(minus_l, minus_l), log2e2 = make_float2(kLog2e, kLog2e);
-    const long long token_piece = named ? ((long long)token + d.skip) / E : -1;
-    const int token_at = named ? (token + d.skip) % E : 0;
-    uint4 r[kBackAtOnce];
+constexpr float kOrdinary = BF16 ? 256.0f : 64.0f;
+
+// A row's gradient by pieces of 16 bytes, as the gradient's row lies on them.
+template <bool BF16>
+struct Gradient {
+    static constexpr int E = Row<BF16>::E;
+    const Row<BF16> d, x;
+    const LogprobParams& p;
+    const long long row;
+    float minus = 0.0f, from;  // log p = (x + minus) / T + from
+    int token;                 // -1: none
+    float inv, l, n, entropy;  // 1 / T, and the gradients / T
+    __device__ __forceinline__ Gradient(const LogprobParams& q, long long r, float lse) : d(q.dlogits, r * q.dld, q.vocab), x(q.logits, r * q.ld, q.vocab), p(q), row(r), from(-lse) {
+        token = __ldg(p.tokens + row);
+        if (token < 0 || token >= p.vocab) token = -1;
+        inv = 1.0f / heat_of(p.temperature, row);
+        l = token >= 0 && p.dlogprob != nullptr ? __ldg(p.dlogprob + row) * inv : 0.0f;
+        n = p.dentropy != nullptr ? __ldg(p.dentropy + row) * inv : 0.0f;
+        entropy = n != 0.0f ? __ldg(p.entropy + row) : 0.0f;
+    }
+    __device__ __forceinline__ long long pieces() const { return (d.end + E - 1) / E; }
+    __device__ __forceinline__ uint4 load(long long i) const {  // what is not the row's -inf
+        if (d.skip == x.skip) return x.load(i);
+        uint4 r;  // (rows that lie differently on their 16 bytes)
+        uint32_t* w = reinterpret_cast<uint32_t*>(&r);
 #pragma unroll
-    for (int u = 0; u < kBackAtOnce; ++u) {
-        const long long i = first + u * kBackThreads;
-        if (i * E >= d.end) continue;
-        if (same) {
-            r[u] = x.load(i);
-        } else {  // (rows that lie differently on their 16 bytes)
-            uint32_t* w = reinterpret_cast<uint32_t*>(&r[u]);
+        for (int j = 0; j < 4; ++j) w[j] = BF16 ? 0xff80ff80u : 0xff800000u;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = 0u;
-#pragma unroll
-            for (int j = 0; j < E; ++j) {
-                const long long at = i * E + j - d.skip;
-                if (at < 0 || at >= p.vocab) continue;
-                if constexpr (BF16) w[j / 2] |= (uint32_t) static_cast<const uint16_t*>(p.logits)[row * p.ld + at] << (j % 2 * 16);
-                else w[j] = static_cast<const uint32_t*>(p.logits)[row * p.ld + at];
+        for (int j = 0; j < E; ++j) {
+            const long long at = i * E + j - d.skip;
+            if (at < 0 || at >= p.vocab) continue;
+            if constexpr (BF16) {
+                const uint32_t v = static_cast<const uint16_t*>(p.logits)[row * p.ld + at];
+                w[j / 2] = j % 2 ? (w[j / 2] & 0xffffu) | v << 16 : (w[j / 2] & 0xffff0000u) | v;
+            } else {
+                w[j] = static_cast<const uint32_t*>(p.logits)[row * p.ld + at];
             }
         }
+        return r;
     }
+    // The pieces from `first` on that r holds, kBackThreads apart, up to `end` values.  SHIFT: `minus` is not 0.
+    template <bool SHIFT, int N>
+    __device__ __forceinline__ void store(const uint4 (&r)[N], long long first, long long end) const {
+        // -p (n (log p + H) + l), in pairs; the token's value in its piece only.
+        const float minus_l = -fmaf(n, entropy, l);
+        const float2 inv2 = make_float2(inv, inv), from2 = make_float2(from, from), n2 = make_float2(-n, -n), l2 = make_float2(minus_l, minus_l), log2e2 = make_float2(kLog2e, kLog2e);
+        const long long token_piece = token >= 0 ? ((long long)token + d.skip) / E : -1;
+        const int token_at = token >= 0 ? (token + d.skip) % E : 0;
 #pragma unroll
-    for (int u = 0; u < kBackAtOnce; ++u) {
-        const long long i = first + u * kBackThreads;
-        if (i * E >= d.end) continue;
-        float y[E];
+        for (int u = 0; u < N; ++u) {
+            const long long i = first + u * kBackThreads;
+            if (i * E >= end) continue;
+            float y[E];
 #pragma unroll
-        for (int j = 0; j < E; j += 2) {
-            float2 lp = fma2(make_float2(value<BF16>(r[u], j), value<BF16>(r[u], j + 1)), inv2, from2);
-            lp = make_float2(max_nan(lp.x, -1000.0f), max_nan(lp.y, -1000.0f));
-            const float2 t = mul2(lp, log2e2), v = mul2(make_float2(ex2_ftz(t.x), ex2_ftz(t.y)), fma2(n2, lp, l2));
-            y[j] = v.x, y[j + 1] = v.y;
-        }
-        if (i == token_piece) {
+            for (int j = 0; j < E; j += 2) {
+                float2 v = make_float2(value<BF16>(r[u], j), value<BF16>(r[u], j + 1));
+                if constexpr (SHIFT) v = add2(v, make_float2(minus, minus));
+                float2 lp = fma2(v, inv2, from2);
+                lp = make_float2(max_nan(lp.x, -1000.0f), max_nan(lp.y, -1000.0f));
+                const float2 t = mul2(lp, log2e2);
+                v = mul2(make_float2(ex2_ftz(t.x), ex2_ftz(t.y)), fma2(n2, lp, l2));
+                y[j] = v.x, y[j + 1] = v.y;
+            }
+            if (i == token_piece) {
 #pragma unroll
-            for (int j = 0; j < E; ++j)
-                if (j == token_at) y[j] += l;
-        }
-        unsigned char* to = const_cast<unsigned char*>(d.base) + i * 16;
-        if (i * E >= d.skip && i * E + E <= d.end) {
-            uint4 o;
-            uint32_t* w = reinterpret_cast<uint32_t*>(&o);
+                for (int j = 0; j < E; ++j)
+                    if (j == token_at) y[j] += l;
+            }
+            unsigned char* to = const_cast<unsigned char*>(d.base) + i * 16;
+            if (i * E >= d.skip && i * E + E <= d.end) {
+                uint4 o;
+                uint32_t* w = reinterpret_cast<uint32_t*>(&o);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if constexpr (BF16) {
-                    const __nv_bfloat162 two = __floats2bfloat162_rn(y[2 * j], y[2 * j + 1]);
-                    w[j] = *reinterpret_cast<const uint32_t*>(&two);
-                } else {
-                    w[j] = __float_as_uint(y[j]);
+                for (int j = 0; j < 4; ++j) {
+                    if constexpr (BF16) {
+                        const __nv_bfloat162 two = __floats2bfloat162_rn(y[2 * j], y[2 * j + 1]);
+                        w[j] = *reinterpret_cast<const uint32_t*>(&two);
+                    } else {
+                        w[j] = __float_as_uint(y[j]);
+                    }
+                }
+                *reinterpret_cast<uint4*>(to) = o;
+            } else {
+#pragma unroll
+                for (int j = 0; j < E; ++j) {
+                    if (i * E + j < d.skip || i * E + j >= d.end) continue;
+                    if constexpr (BF16) reinterpret_cast<uint16_t*>(to)[j] = f32_to_bf16_bits(y[j]);
+                    else reinterpret_cast<float*>(to)[j] = y[j];
                 }
             }
-            *reinterpret_cast<uint4*>(to) = o;
-        } else {
-#pragma unroll
-            for (int j = 0; j < E; ++j) {
-                if (i * E + j < d.skip || i * E + j >= d.end) continue;
-                if constexpr (BF16) reinterpret_cast<uint16_t*>(to)[j] = f32_to_bf16_bits(y[j]);
-                else reinterpret_cast<float*>(to)[j] = y[j];
-            }
         }
     }
+};
+
+// A whole row by one block, N pieces of a thread in flight: its maximum and sum, then its gradient.
+template <bool BF16, int N>
+__device__ __forceinline__ void whole_row(const LogprobParams& p, long long row) {
+    __shared__ float wmax[kBackWarps], wsum[kBackWarps];
+    Gradient<BF16> g(p, row, 0.0f);
+    const long long pieces = g.pieces();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const float c = kLog2e / heat_of(p.temperature, row);
+    uint4 r[N];
+    LaneSums mine;  // m: the warp's
+    for (long long i = warp * 32; i < pieces; i += kBackThreads * N) {
+        float up = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < N; ++u) r[u] = g.load(i + u * kBackThreads + lane);  // (past the end: all -inf)
+#pragma unroll
+        for (int u = 0; u < N; ++u) up = fmaxf(up, largest<BF16>(r[u]));
+        up = warp_max(up);
+        if (up > mine.m) mine.raise(up, c);
+#pragma unroll
+        for (int u = 0; u < N; ++u) mine.add<BF16>(r[u], c);
+    }
+    const float s = warp_sum(mine.s.x + mine.s.y);
+    if (lane == 0) wmax[warp] = mine.m, wsum[warp] = s;
+    __syncthreads();
+    Sums all;
+    if (lane < kBackWarps) all.m = wmax[lane], all.s = wsum[lane];
+    join_lanes(all, kBackWarps, c);
+    if (all.m == -INFINITY && all.s == 0.0f) g.l = g.n = g.entropy = 0.0f;  // a row that masks everything: no gradient
+    else g.minus = -all.m, g.from = -kLn2 * log2f(all.s);
+    for (long long i = threadIdx.x; i < pieces; i += kBackThreads * N) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) r[u] = g.load(i + u * kBackThreads);
+        g.template store<true>(r, i, g.d.end);
+    }
+}
+
+template <bool BF16>
+__device__ __noinline__ void whole_row_apart(const LogprobParams& p, long long row) { whole_row<BF16, 2>(p, row); }
+
+// A block takes kBackThreads x kBackAtOnce pieces of the gradient's row.  ALL: rows that are read twice too, by a function, whose registers cost blocks beside one another; large calls leave these
+// rows to the kernel behind this one.  (us, bf16 and f32 logits: one row of 131,072 2.4 and 2.4; 2,048 and 1,024 of them 191 and 178 so, 178 and 167 and a launch the other way.)
+template <bool BF16, bool ALL>
+__global__ void __launch_bounds__(kBackThreads, ALL ? (BF16 ? 5 : 6) : 0) logprob_backward_kernel(const __grid_constant__ LogprobParams p) {
+    grid_ready();
+    const long long row = blockIdx.x / p.blocks, first = (long long)(blockIdx.x % p.blocks) * kBackThreads * kBackAtOnce + threadIdx.x;
+    const float lse = __ldg(p.lse + row);
+    const Gradient<BF16> g(p, row, lse);
+    uint4 r[kBackAtOnce];  // (asked for before anything is known of the row: a block lives for little more than a trip to memory)
+#pragma unroll
+    for (int u = 0; u < kBackAtOnce; ++u)
+        if ((first + u * kBackThreads) * Row<BF16>::E < g.d.end) r[u] = g.load(first + u * kBackThreads);
+    const bool ordinary = fabsf(lse) <= kOrdinary<BF16>;
+    g.template store<false>(r, first, ordinary ? g.d.end : 0);
+    if (ALL && !ordinary && blockIdx.x % p.blocks == 0) whole_row_apart<BF16>(p, row);
+}
+// A row a block.
+template <bool BF16>
+__global__ void __launch_bounds__(kBackThreads) logprob_backward_rest_kernel(const __grid_constant__ LogprobParams p) {
+    grid_ready();
+    if (!(fabsf(__ldg(p.lse + blockIdx.x)) <= kOrdinary<BF16>)) whole_row<BF16, kBackAtOnce>(p, blockIdx.x);
 }
 
 // Blocks that share a row: enough that a small call fills the GPU, while each still has a piece a warp.  (Up to two blocks an SM; 131,072 bf16 logits with five alternatives, us: 200 rows 21.5 with two
@@ -589,7 +667,11 @@ extern "C" int glm53f_kda_logprobs_backward(int32_t rows, int32_t vocab, const v
     p.tokens = tokens, p.temperature = temperature, p.lse = const_cast<float*>(lse), p.entropy = const_cast<float*>(entropy);
     p.dlogprob = dlogprob, p.dentropy = dentropy, p.dlogits = dlogits, p.dld = dld;
     if ((long long)rows * p.blocks > 0x7fffffff) return kInvalid;
+    const cudaStream_t on = reinterpret_cast<cudaStream_t>(stream);
     const dim3 grid((unsigned)(rows * p.blocks));
-    if (bf16) return launch_early(logprob_backward_kernel<true>, grid, kBackThreads, 0, reinterpret_cast<cudaStream_t>(stream), p);
-    return launch_early(logprob_backward_kernel<false>, grid, kBackThreads, 0, reinterpret_cast<cudaStream_t>(stream), p);
+    if ((long long)rows * vocab * size < 128ll << 20)
+        return bf16 ? launch_early(logprob_backward_kernel<true, true>, grid, kBackThreads, 0, on, p) : launch_early(logprob_backward_kernel<false, true>, grid, kBackThreads, 0, on, p);
+    const int rc = bf16 ? launch_early(logprob_backward_kernel<true, false>, grid, kBackThreads, 0, on, p) : launch_early(logprob_backward_kernel<false, false>, grid, kBackThreads, 0, on, p);
+    if (rc != 0) return rc;
+    return bf16 ? launch_early(logprob_backward_rest_kernel<true>, dim3((unsigned)rows), kBackThreads, 0, on, p) : launch_early(logprob_backward_rest_kernel<false>, dim3((unsigned)rows), kBackThreads, 0, on, p);
 }
