@@ -142,7 +142,7 @@ class Int4Mat:
         if w.dim() != 2 or group not in INT4_GROUPS or w.shape[1] % group or w.shape[1] % 64:
             raise Invalid(f"a weight [n][k], k a multiple of 64 and of the group (32, 64 or 128), got {tuple(w.shape)}")
         n, k = w.shape
-        g = w.float().view(n, k // group, group)
+        g = w.float().contiguous().view(n, k // group, group)
         if zeros:
             low, high = g.amin(-1).clamp(max=0), g.amax(-1).clamp(min=0)
             scales = ((high - low) / 15).bfloat16()
