@@ -191,7 +191,8 @@ __device__ __forceinline__ float min_nan(float a, float b) {
     return r;
 }
 // a, and with REST 1 - a without the cancellation where a is near one.  Below 2^-126: 0.
-//   e^g: the exponent's rounding costs |g| 2^-24 of a, nothing where a is near one; 1 - a by the exponential's series where a > 1/2.
+//   e^g: the exponent's rounding costs |g| 2^-24 of a, beside the instruction's own error: 1.4 u measured where a is near one (u = 2^-24; -0.1 u on average, so that it does not grow with what
+//     a channel remembers), 2.6 u for a > 1/2, 8.4 u at g = -10.  1 - a by the exponential's series where a > 1/2.
 //   sigmoid: both from e^-|g|, whose exponent's rounding is made good, so that the smaller one keeps its digits: no overflow either.
 template <bool SIGMOID, bool REST>
 __device__ __forceinline__ void gate(float2 g, float2& a, float2& rest) {
@@ -822,7 +823,8 @@ struct Layout {  // of the workspace: bytes from its start
 // 1.3 us a tile of an SM's share and 5 us more where tiles look back; without tensor copies 1.3 to 3.1 us against 1.9 to 3.5.  A walk takes as long as its
 // busiest block.  Measured, us walked and divided (f32 g, bf16 x): 4,096 channels 100 rows 4.0 and 6.4, 2,000 rows 22.6 and 23.6, 4,000 rows 39.9 and 38.1, 8,192 rows 76 and 69;
 // 1,024 channels 1,000 rows 11.6 and 9.2, 16 x 1,000 rows 27 and 43; 64 channels 300 rows 5.4 and 5.8, 3,000 rows 29 and 7.6; there and back 2,048 channels, 16,289 rows in four sequences 163 and 200;
-// 1,001 channels (no tensor copies) 1,000 rows 41 and 13.
+// 1,001 channels (no tensor copies) 1,000 rows 41 and 13.  Backwards alone: 4,096 channels 100 rows 4.4 and 7.0, 8,192 rows 138 and 109; 1,024 channels 1,000 rows 18 and 12, 16 x 1,000 rows 47 and 65, 65,536 rows
+// 989 and 241; 64 channels 3,000 rows 43 and 8; four sequences as above 87 and 116; the rule's losses: 4,096 channels 2,000 rows 38 and 33, 64 channels 300 rows 6.8 and 6.3, both walked.
 bool divide(const Layout& at, int batch, int max_len, bool boxes) {
     if (max_len <= kRows) return false;
     const long long items = at.stripes * batch, sms = sm_count(), longest = (max_len + kRows - 1) / kRows, tiles = at.slots * at.stripes;

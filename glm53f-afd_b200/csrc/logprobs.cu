@@ -6,7 +6,7 @@
 // Bound by HBM and the operations next to it: a row is read once (one exponential, 2/3 of what the units give at bf16 logits, and five or six instructions a value, in pairs).  Every warp keeps
 // its running maximum, its lanes their sums against it, so that the maxima need no pass of their own; blocks of a cluster that share a row meet
 // in distributed shared memory.  No scratch in global memory; the same bits every time.  336 rows of 131,072 bf16 logits take 25.9 us, 3.4 TB/s (1,000 rows
-// 3.8), with five alternatives 30.6; one f32 row 4.6 us, with twenty 12.2: the rounds that find them, one after another.  Backwards 2,048 rows take 206 us, 5.2 TB/s.
+// 3.8), with five alternatives 30.6; one f32 row 4.6 us, with twenty 12.2: the rounds that find them, one after another.  Backwards 2,048 rows take 181 us, 5.9 TB/s.
 //
 // The alternatives need no second pass either.  Each thread knows the largest value it met; 128 groups of threads are 128 disjoint parts of the row, so the
 // k-th largest of the groups' maxima is no larger than the row's k-th largest value.  Of the row's pieces of 32 x 16 bytes, whose
@@ -146,8 +146,9 @@ __device__ __forceinline__ float largest(const uint4& r) {  // (of numbers; NaN 
 }
 
 // t = (x - m) log2(e) / T: the difference first, so that the largest logit's t is 0 itself, and no size of x or T does harm.
-// Stands for -inf where maximum and temperature are ordinary (`plain`): finite times finite, so that no 0 meets an infinity.  (A bf16 value.)
-constexpr float kFloor = -9.969209968386869e29f;
+// Stands for -inf where maximum and temperature are ordinary (`plain`): finite times finite, so that no 0 meets an infinity.  (About -1e30, a bf16 value: for pairs of them kFloorPair.)
+constexpr float kFloor = -0x1.92p99f;
+constexpr uint32_t kFloorPair = 0xf149f149u;
 __device__ __forceinline__ bool plain(float m, float c) { return c >= 1e-6f && c <= 1e6f && (m == -INFINITY || fabsf(m) <= 1e29f); }
 
 // Sums of e^t and e^t t against the maximum m, in powers of two.
@@ -187,7 +188,7 @@ struct LaneSums {
         for (int j = 0; j < Row<BF16>::E / 2; ++j) {
             float2 x;
             if constexpr (BF16) {
-                asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(u[j]) : "r"(0xf149f149u));
+                asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(u[j]) : "r"(kFloorPair));
                 x = make_float2(__uint_as_float(u[j] << 16), __uint_as_float(u[j] & 0xffff0000u));
             } else {
                 x = make_float2(max_nan(__uint_as_float(u[2 * j]), kFloor), max_nan(__uint_as_float(u[2 * j + 1]), kFloor));

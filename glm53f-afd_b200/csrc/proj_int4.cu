@@ -31,8 +31,8 @@ constexpr int kTile = 16;        // weight rows of a tile
 constexpr int kPiece = 64;       // k of a piece
 constexpr int kFewWarps = 16, kFewThreads = 32 * (kFewWarps + 1);  // the last warp loads
 constexpr int kFewRows = 8;
-constexpr int kFewStages = 16;   // of the ring, at most
 constexpr int kFewX = 150 * 1024, kFewShared = 208 * 1024;  // bytes for the rows of x, and with the ring
+constexpr int kFewStages = 12;   // of the ring, at most
 constexpr int kRowPad = 8;       // bf16 between them: the eight rows that one load of fragments reads lie in different banks
 
 struct Int4Layout {  // bytes from the packed weight's start
@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Para
 //
 // N is the smallest that holds the rows, 128 at most (64 for more than 64 rows: 100 rows x 4,096 x 8,192 23.5 us against 20.8, 400 rows 76 against 58, 2,048 rows 202 against 145; only
 // 500 x 512 is faster, 6.6 against 8.9).  Bound by the issue of widening and summing and by the chain from words to sums: 2,048 rows x 4,096 x 8,192 in groups of 128 take
-// 145 to 159 us, 0.5 of the measured bf16 rate (their products alone 83); groups of 64 217, of 32 384, a fetch of the accumulator for each.  40 rows in groups of 64 with zero points 14.9 us.
+// 141 to 159 us, 0.5 of the measured bf16 rate (their products alone 83); groups of 64 217, of 32 367, a fetch of the accumulator for each.  40 rows in groups of 64 with zero points 14.9 us.
 // (Scales and zero points fetched a few groups ahead, without L2 asked before: 154 and 21.3 us.)
 
 enum : int { kStatusInt4Empty = 170, kStatusInt4Full = 171, kStatusInt4AEmpty = 172, kStatusInt4AFull = 173, kStatusInt4AccEmpty = 174, kStatusInt4AccFull = 175, kStatusInt4Words = 176, kStatusInt4WordsFull = 177 };
@@ -567,7 +567,7 @@ __global__ void __launch_bounds__(Many<N>::kThreads, Many<N>::kBlocks) int4_many
     }
 }
 
-// A thread a word of the packed weight, or a group's pair of scales and zero points.
+// A thread a word of the packed weight, or a group's pair of scales and zero points.  Once a weight: 24,640 x 4,096 99 us (15.9 for the bytes: the codes are read a byte at a time), 4,096 x 8,192 36.
 __global__ void int4_pack_kernel(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int n, int k, int group, uint32_t* to, uint32_t* to_scales,
                                  uint16_t* to_zeros) {
     const long long tiles = (n + kTile - 1) / kTile, words = tiles * (k / kPiece) * 128, pairs = tiles * (k / group) * 8;
@@ -610,8 +610,8 @@ template <int G, bool ZEROS, bool LONG>
 int few_launch(Int4Params& p, unsigned blocks, cudaStream_t stream) {
     using F = Few<G, ZEROS>;
     p.stage = LONG ? (F::kStage + p.rows * F::kLongPitch + 127) / 128 * 128 : F::kStage;
-    const int stages = (kFewShared - p.x_bytes) / p.stage;
-    p.stages = stages < kFewStages ? stages : kFewStages;
+    static_assert(kFewShared / F::kStage <= kFewStages && (kFewShared - kFewX) / F::kStage >= 2 && kFewShared / (F::kStage + kFewRows * F::kLongPitch + 127) >= 2, "the ring's barriers, and two stages at least");
+    p.stages = (kFewShared - p.x_bytes) / p.stage;
     const cudaError_t e = cudaFuncSetAttribute(int4_few_kernel<G, ZEROS, LONG>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewShared);
     if (e != cudaSuccess) return (int)e;
     return launch_early(int4_few_kernel<G, ZEROS, LONG>, dim3(blocks), kFewThreads, p.x_bytes + p.stages * p.stage, stream, p);
