@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 2) logprob_kernel
                 join_lanes(all, p.blocks, c);
             }
             const bool none = all.m == -INFINITY && all.s == 0.0f;  // a row whose mask leaves nothing
-            const float l2 = log2f(all.s);
+            const float l2 = log2f(all.s), log_s = kLn2 * l2;
             if (lane == 0) {
                 const int token = p.tokens == nullptr ? -1 : __ldg(p.tokens + row);
                 if (p.logprob != nullptr) {
@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 2) logprob_kernel
                         float v;
                         if constexpr (BF16) v = bf16_bits_to_f32(__ldg(static_cast<const uint16_t*>(p.logits) + row * p.ld + token));
                         else v = __ldg(static_cast<const float*>(p.logits) + row * p.ld + token);
-                        lp = none ? -INFINITY : kLn2 * ((v - all.m) * c - l2);
+                        lp = none ? -INFINITY : (v - all.m) / heat - log_s;  // (not in powers of two: a mask's lowest value would overflow)
                     }
                     p.logprob[row] = lp;
                 }
@@ -425,7 +425,7 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 2) logprob_kernel
             if (lane < p.top) {
                 const Entry e = sh.best[lane];
                 p.top_ids[row * p.top + lane] = e.id;
-                p.top_values[row * p.top + lane] = e.id < 0 ? -INFINITY : kLn2 * ((e.v - all.m) * c - l2);
+                p.top_values[row * p.top + lane] = e.id < 0 ? -INFINITY : (e.v - all.m) / heat - log_s;
             }
         }
     }
