@@ -594,8 +594,8 @@ int glm53f_kda_logprobs(int32_t rows, int32_t vocab, const void* logits, int32_t
 
 /* The logits' gradient, of their type, row r at + r * dld: dlogits_j = (dlogprob [j = token] - dlogprob p_j - dentropy p_j (log p_j + entropy)) / temperature from the
  * gradients dlogprob and dentropy (f32 [rows]; one of them may be NULL) of a call that gave lse and, where dentropy is not NULL, entropy.  A row without a
- * token takes nothing from dlogprob; a row that masks everything gets 0.  p is that of the logits at any temperature and any size of logits: f32, to 1e-5 of itself (bf16 logits 4e-5), where the
- * sum that lse was formed from is.  Rows whose lse is beyond 64 (bf16 logits: 256) in size are read twice, by one block each: 131,072 logits take 40 to 60 us.  dlogits may be `logits` itself (with dld = ld), and otherwise has no byte in common with it. */
+ * token takes nothing from dlogprob; a row that masks everything gets 0.  At any temperature and size of logits p is within 1e-5 of itself (bf16 logits 4e-5),
+ * beside what a row's sum is off by.  Rows whose lse is beyond 64 (bf16 logits: 256) in size are read twice, by a block each: one of 131,072 logits takes 40 to 60 us.  dlogits may be `logits` itself (with dld = ld), and otherwise has no byte in common with it. */
 int glm53f_kda_logprobs_backward(int32_t rows, int32_t vocab, const void* logits, int32_t kind, int64_t ld, const int32_t* tokens,
                                  const float* temperature, const float* lse, const float* entropy, const float* dlogprob, const float* dentropy,
                                  void* dlogits, int64_t dld, glm53f_stream_t stream);
