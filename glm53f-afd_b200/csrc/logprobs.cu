@@ -397,6 +397,7 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 2) logprob_kernel
             __syncthreads();
         }
         if (warp == 0) {
+            const float inv = 1.0f / heat;
             Sums all;
             if (p.blocks == 1) {
                 all.m = sh.max, all.s = sh.sum, all.w = sh.sum_t;
@@ -415,7 +416,7 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 2) logprob_kernel
                         float v;
                         if constexpr (BF16) v = bf16_bits_to_f32(__ldg(static_cast<const uint16_t*>(p.logits) + row * p.ld + token));
                         else v = __ldg(static_cast<const float*>(p.logits) + row * p.ld + token);
-                        lp = none ? -INFINITY : (v - all.m) / heat - log_s;  // (not in powers of two: a mask's lowest value would overflow)
+                        lp = none ? -INFINITY : fmaf(v - all.m, inv, -log_s);  // (not in powers of two: a mask's lowest value would overflow)
                     }
                     p.logprob[row] = lp;
                 }
@@ -425,7 +426,7 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 2) logprob_kernel
             if (lane < p.top) {
                 const Entry e = sh.best[lane];
                 p.top_ids[row * p.top + lane] = e.id;
-                p.top_values[row * p.top + lane] = e.id < 0 ? -INFINITY : (e.v - all.m) / heat - log_s;
+                p.top_values[row * p.top + lane] = e.id < 0 ? -INFINITY : fmaf(e.v - all.m, inv, -log_s);
             }
         }
     }
